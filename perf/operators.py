@@ -313,7 +313,8 @@ def _plain_plan(s: dict) -> dict:
     need = torch.where(valid, (cached + new + BS - 1) // BS - have, 0)
     taken = torch.cumsum(need, 0)
     tokens = torch.cumsum(torch.where(valid, new, 0), 0)
-    fits = valid & ((need == 0) | (taken <= s["nfree"])) & (tokens <= T)
+    fits = (valid & ((need == 0) | (taken <= s["nfree"]))
+            & ((new == 0) | (tokens <= T)))
     new, need = torch.where(fits, new, 0), torch.where(fits, need, 0)
     end = torch.cumsum(new, 0)
     first = torch.where(need > 0, taken - need, 0)
