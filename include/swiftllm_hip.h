@@ -436,7 +436,73 @@ int swiftllm_hip_wave_reduce_check(const float* x, const int32_t* xi,
                                    hipStream_t stream);
 
 /* ------------------------------------------------------------------------ */
-/* 6. Host-side metadata (no device work).                                   */
+/* 6. The attention step around the cache. The reference plans a step on the */
+/*    host (BlockManager, KvCache::get_slot_mapping), declares rotary         */
+/*    embeddings (crates/swiftllm-models/src/layers/attention.rs:297-353) and */
+/*    ALiBi / sliding-window options that no kernel of it implements          */
+/*    (memory/paged_attention.rs:39-43, 111-135). These entry points do all   */
+/*    of it on the device, without a synchronisation, so that a step can be   */
+/*    captured in a graph. Values are fp16 (SWIFTLLM_HIP_F16) or bfloat16     */
+/*    (SWIFTLLM_HIP_BF16) throughout a call; the cache layout is the one      */
+/*    above, block_size 16, head_dim 64 or 128.                               */
+/* ------------------------------------------------------------------------ */
+#define SWIFTLLM_HIP_F16 0
+#define SWIFTLLM_HIP_BF16 1
+
+/* Block tables and slot maps of one step, from request lengths. Sequence s
+ * has cached_lens[s] tokens in the cache, in the first ceil(cached / 16)
+ * entries of its row of block_tables, and brings new_lens[s] tokens. Its
+ * missing blocks are taken from free_blocks in order (sequence by sequence),
+ * of which the first min(num_free[0], free_capacity) are there; num_free is
+ * device memory. Writes
+ *   block_tables[s, ...]   the taken blocks (other entries stay)
+ *   context_lens[s]        = cached + new
+ *   query_offsets[S + 1]   exclusive sums of the new tokens
+ *   positions[t], slot_mapping[t]  of packed token t: its position in its
+ *                          sequence and its cache slot (-1 for a block outside
+ *                          [0, num_blocks), num_blocks <= 0: no upper bound);
+ *                          -1 and -1 for the rows from the last token up to
+ *                          num_tokens (padding)
+ *   counts[3]              blocks taken, tokens placed, sequences refused
+ * A sequence is refused where a length is negative, cached + new does not fit
+ * its table, its blocks are missing from the free list or its tokens from
+ * num_tokens (both sums run over all sequences before it): it keeps
+ * context_lens = cached_lens and no token of it is placed. Blocks past
+ * counts[0] were not taken. No output may overlap another argument. */
+int swiftllm_hip_plan_step(int32_t* block_tables, const int32_t* cached_lens,
+                           const int32_t* new_lens, const int32_t* free_blocks,
+                           const int32_t* num_free, int free_capacity,
+                           int num_seqs, int max_num_blocks_per_seq,
+                           int block_size, int num_tokens, int num_blocks,
+                           int32_t* context_lens, int32_t* query_offsets,
+                           int32_t* positions, int32_t* slot_mapping,
+                           int32_t* counts, hipStream_t stream);
+
+/* Rotary positions of queries and keys, and the cache write of the rotated
+ * keys and the values, in one launch. Pair i < rotary_dim / 2 of a head,
+ * elements (i, i + rotary_dim / 2) or, interleaved != 0, (2 i, 2 i + 1), turns
+ * by positions[t] * inv_freq[i] and is scaled by attn_factor; elements past
+ * rotary_dim (even, 0 to head_dim) stay. inv_freq: double
+ * [rotary_dim / 2] in device memory, radians per position. query, key and
+ * value [T, heads * head_dim] with a stride in elements between tokens (a
+ * fused projection is three such views); query_out [T, num_heads, head_dim]
+ * packed, which may be query itself where query_stride is num_heads *
+ * head_dim and may overlap no input otherwise. Angles are reduced in 64 bits.
+ * A token with a negative position is padding: no row of it is written. One
+ * whose slot is negative or outside [0, num_blocks * 16) (num_blocks <= 0: no
+ * upper bound) has its queries written and nothing else. The slots of a call
+ * are distinct. */
+int swiftllm_hip_rotary_and_cache(
+    void* query_out, const void* query, const void* key, const void* value,
+    void* key_cache, void* value_cache, const int32_t* positions,
+    const int32_t* slot_mapping, const void* inv_freq, float attn_factor,
+    int interleaved, int dtype, int num_tokens, int num_heads,
+    int num_kv_heads, int head_dim, int rotary_dim, int block_size,
+    long long query_stride, long long key_stride, long long value_stride,
+    int num_blocks, hipStream_t stream);
+
+/* ------------------------------------------------------------------------ */
+/* 7. Host-side metadata (no device work).                                   */
 /* ------------------------------------------------------------------------ */
 
 /* KvCache::get_slot_mapping (crates/swiftllm-core/src/memory/kv_cache.rs:

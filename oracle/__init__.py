@@ -337,3 +337,104 @@ def moe_route_dispatch_serial(logits: np.ndarray, x: np.ndarray, top_k: int):
                                            offsets.ctypes.data, x_perm.ctypes.data,
                                            inverse.ctypes.data, sorted_ids.ctypes.data)
     return ids, w, counts, offsets, x_perm.view(np.float16), inverse, sorted_ids
+
+
+def plan_step(block_tables, cached, new, free_blocks, num_tokens, num_blocks=0):
+    """Block tables, slot maps and positions of one step, sequence by sequence
+    in Python integers: what swiftllm_hip_plan_step documents. Returns
+    (block_tables, context_lens, query_offsets, positions, slots, counts)."""
+    bt = np.array(block_tables, dtype=np.int64)
+    S, MB = bt.shape
+    free = [int(b) for b in free_blocks]
+    ctx, offsets, positions, slots = [], [0], [], []
+    wanted_blocks = wanted_rows = taken = refused = 0
+    for s in range(S):
+        c, n = int(cached[s]), int(new[s])
+        ok = c >= 0 and n >= 0 and c + n <= 16 * MB
+        need = -(-(c + n) // 16) - -(-c // 16) if ok else 0
+        first = wanted_blocks
+        wanted_blocks += need
+        wanted_rows += n if ok else 0
+        ok = ok and (need == 0 or wanted_blocks <= len(free)) and (n == 0 or wanted_rows <= num_tokens)
+        if not ok:
+            refused += 1
+            ctx.append(c)
+            offsets.append(offsets[-1])
+            continue
+        have = -(-c // 16)
+        for b in range(need):
+            bt[s, have + b] = free[first + b]
+        if need:
+            taken = wanted_blocks
+        for pos in range(c, c + n):
+            b = int(bt[s, pos // 16])
+            known = 0 <= b < (num_blocks if num_blocks > 0 else 1 << 27) and b < 1 << 27
+            positions.append(pos)
+            slots.append(16 * b + pos % 16 if known else -1)
+        ctx.append(c + n)
+        offsets.append(offsets[-1] + n)
+    pad = num_tokens - len(positions)
+    counts = [taken, len(positions), refused]
+    return (bt.astype(np.int32), np.array(ctx, np.int32), np.array(offsets, np.int32),
+            np.array(positions + [-1] * pad, np.int32), np.array(slots + [-1] * pad, np.int32),
+            np.array(counts, np.int32))
+
+
+def rotary(x, positions, inv_freq, rotary_dim: int, interleaved: bool, attn_factor: float = 1.0):
+    """Rotary positions in float64: x [T, heads, D], pair i of the first
+    rotary_dim elements as a complex number times
+    attn_factor * exp(1j * position * inv_freq[i])."""
+    y = np.array(x, dtype=np.float64)
+    i = np.arange(rotary_dim // 2)
+    a, b = (2 * i, 2 * i + 1) if interleaved else (i, i + rotary_dim // 2)
+    angle = np.asarray(positions, np.float64)[:, None] * np.asarray(inv_freq, np.float64)[None]
+    z = (y[:, :, a] + 1j * y[:, :, b]) * (attn_factor * np.exp(1j * angle))[:, None]
+    y[:, :, a], y[:, :, b] = z.real, z.imag
+    return y
+
+
+def scored_attention(q, kc, vc, bt, ctx, query_offsets, scale, softcap=0.0, slopes=None, window=0,
+                     prefix=None, num_blocks=None):
+    """Paged attention with shaped scores in float64. Rows query_offsets[s] ..
+    query_offsets[s + 1] - 1 of q are the last tokens of sequence s; a query at
+    position p sees key j < ctx[s] where j <= p and, with a window, p - j <
+    window, or where j < prefix[s]; its score is softcap * tanh(scale q.k /
+    softcap) (softcap 0: scale q.k) minus slopes[h] * |p - j|. Blocks outside
+    [0, num_blocks) hold no key; a row that sees none is zero."""
+    T, H, D = q.shape
+    NB, Hkv = kc.shape[0], kc.shape[1]
+    num_blocks = NB if num_blocks is None else num_blocks
+    out = np.zeros((T, H, D), np.float64)
+    for s in range(len(ctx)):
+        t0, t1 = int(query_offsets[s]), int(query_offsets[s + 1])
+        L = min(max(int(ctx[s]), 0), bt.shape[1] * 16)
+        if t1 <= t0 or L == 0:
+            continue
+        ids = np.asarray(bt[s, :(L + 15) // 16], np.int64)
+        real = np.repeat((ids >= 0) & (ids < num_blocks), 16)[:L]
+        ids = np.where((ids >= 0) & (ids < num_blocks), ids, 0)
+        K = kc[ids].transpose(1, 0, 3, 2).reshape(Hkv, -1, D)[:, :L].astype(np.float64)
+        V = vc[ids].transpose(1, 0, 3, 2).reshape(Hkv, -1, D)[:, :L].astype(np.float64)
+        p = np.arange(int(ctx[s]) - (t1 - t0), int(ctx[s]))[:, None]
+        j = np.arange(L)[None]
+        seen = j <= p
+        if window > 0:
+            seen &= p - j < window
+        if prefix is not None:
+            seen |= j < int(prefix[s])
+        seen &= (p >= 0) & real[None]
+        for h in range(H):
+            x = q[t0:t1, h].astype(np.float64) @ np.where(real[:, None], K[h * Hkv // H], 0.0).T
+            x = x * scale
+            if softcap > 0:
+                x = softcap * np.tanh(x / softcap)
+            if slopes is not None:
+                x = x - float(slopes[h]) * np.abs(p - j)
+            x = np.where(seen, x, -np.inf)
+            top = x.max(axis=1, keepdims=True)
+            w = np.where(seen, np.exp(x - np.where(np.isfinite(top), top, 0.0)), 0.0)
+            total = w.sum(axis=1, keepdims=True)
+            # keys that no row sees may hold anything
+            v = np.where(seen.any(axis=0)[:, None], V[h * Hkv // H], 0.0)
+            out[t0:t1, h] = np.where(total > 0, w @ v / np.where(total > 0, total, 1.0), 0.0)
+    return out

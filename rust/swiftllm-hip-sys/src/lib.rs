@@ -37,6 +37,10 @@ pub const SWIFTLLM_ERR_NOT_SUPPORTED: c_int = -6;
 /// SWIFTLLM_HIP_NOALLOC_SCRATCH_BYTES: the static split-K scratch per device.
 pub const SWIFTLLM_HIP_NOALLOC_SCRATCH_BYTES: usize = 64 << 20;
 
+/// Value types of the attention step's entry points.
+pub const SWIFTLLM_HIP_F16: i32 = 0;
+pub const SWIFTLLM_HIP_BF16: i32 = 1;
+
 /// C twin of `PagedAttentionParams` (crates/swiftllm-cuda/src/bindings.rs:8-30).
 #[repr(C)]
 #[derive(Debug, Clone, Copy)]
@@ -233,6 +237,24 @@ extern "C" {
     pub fn swiftllm_hip_wave_reduce_check(
         x: *const c_float, xi: *const i32, num_rows: c_int, out: *mut c_float, scan: *mut i32,
         stream: hipStream_t,
+    ) -> c_int;
+
+    // -- the attention step around the cache; dtype is SWIFTLLM_HIP_F16 / _BF16 ---
+    pub fn swiftllm_hip_plan_step(
+        block_tables: *mut i32, cached_lens: *const i32, new_lens: *const i32,
+        free_blocks: *const i32, num_free: *const i32, free_capacity: c_int, num_seqs: c_int,
+        max_num_blocks_per_seq: c_int, block_size: c_int, num_tokens: c_int,
+        num_blocks: c_int, context_lens: *mut i32, query_offsets: *mut i32,
+        positions: *mut i32, slot_mapping: *mut i32, counts: *mut i32, stream: hipStream_t,
+    ) -> c_int;
+    pub fn swiftllm_hip_rotary_and_cache(
+        query_out: *mut c_void, query: *const c_void, key: *const c_void,
+        value: *const c_void, key_cache: *mut c_void, value_cache: *mut c_void,
+        positions: *const i32, slot_mapping: *const i32, inv_freq: *const c_void,
+        attn_factor: c_float, interleaved: c_int, dtype: c_int, num_tokens: c_int,
+        num_heads: c_int, num_kv_heads: c_int, head_dim: c_int, rotary_dim: c_int,
+        block_size: c_int, query_stride: c_longlong, key_stride: c_longlong,
+        value_stride: c_longlong, num_blocks: c_int, stream: hipStream_t,
     ) -> c_int;
 
     // -- host metadata: kv_cache.rs:186-216, 250-286 ------------------------------

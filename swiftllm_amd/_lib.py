@@ -92,6 +92,11 @@ SIGNATURES = {
     "swiftllm_hip_gather_kv": (
         i32, [vp, vp, vp, vp, i32, i32, i32, i32, i32, i32, i32, vp, vp, vp]),
     "swiftllm_hip_wave_reduce_check": (i32, [vp, vp, i32, vp, vp, vp]),
+    "swiftllm_hip_plan_step": (
+        i32, [vp, vp, vp, vp, vp, i32, i32, i32, i32, i32, i32, vp, vp, vp, vp, vp, vp]),
+    "swiftllm_hip_rotary_and_cache": (
+        i32, [vp, vp, vp, vp, vp, vp, vp, vp, vp, f32, i32, i32, i32, i32, i32, i32, i32, i32,
+              i64, i64, i64, i32, vp]),
     "swiftllm_hip_slot_mapping": (i32, [vp, sz, sz, sz, sz, vp]),
     "swiftllm_hip_pack_block_tables": (i32, [vp, vp, vp, sz, sz, sz, vp, vp]),
 }

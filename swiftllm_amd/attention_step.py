@@ -1,0 +1,135 @@
+"""One attention step around the paged cache, all of it on the device.
+
+    plan_step           block tables, slot maps and positions from request lengths
+    rotary_and_cache    rotary positions of q and k, and the cache write of k and v
+
+Reference (paths relative to the swiftllm repository): the host routines and
+options these stand for are
+  crates/swiftllm-core/src/memory/block_manager.rs, kv_cache.rs:186-216
+                                               block allocation, get_slot_mapping
+  crates/swiftllm-models/src/layers/attention.rs:297-353
+                                               RoPE and its long-context scaling
+Device tensors are DeviceArrays or raw device pointers (ints); values are fp16
+("f16") or bfloat16 ("bf16"). Nothing here synchronises or allocates, so every
+call may be captured in a graph.
+"""
+
+from __future__ import annotations
+
+import math
+from typing import Optional
+
+import numpy as np
+
+from . import _lib
+from ._hip import Stream
+from .paged_attention import InvalidParameter, NotSupported, Ptr, _p, _s, check_status
+
+DTYPES = {"f16": 0, "bf16": 1}   # SWIFTLLM_HIP_F16, SWIFTLLM_HIP_BF16
+
+
+def _dtype(name: str) -> int:
+    if name not in DTYPES:
+        raise NotSupported(f"dtype {name!r} (supported: {', '.join(DTYPES)})")
+    return DTYPES[name]
+
+
+# ---------------------------------------------------------------------------
+# Plan
+# ---------------------------------------------------------------------------
+def plan_step(block_tables: Ptr, cached_lens: Ptr, new_lens: Ptr, free_blocks: Ptr,
+              num_free: Ptr, free_capacity: int, num_seqs: int, max_num_blocks_per_seq: int,
+              block_size: int, num_tokens: int, context_lens: Ptr, query_offsets: Ptr,
+              positions: Ptr, slot_mapping: Ptr, counts: Ptr, num_blocks: int = 0,
+              stream: Optional[Stream] = None) -> None:
+    """Block tables and slot maps of one step from the requests' lengths
+    (swiftllm_hip_plan_step): takes the missing blocks of every sequence from
+    free_blocks in order, and writes context_lens [S], query_offsets [S + 1],
+    positions and slot_mapping [num_tokens] (-1 behind the last token) and
+    counts [3] = (blocks taken, tokens placed, sequences refused)."""
+    check_status(_lib.lib().swiftllm_hip_plan_step(
+        _p(block_tables), _p(cached_lens), _p(new_lens), _p(free_blocks), _p(num_free),
+        free_capacity, num_seqs, max_num_blocks_per_seq, block_size, num_tokens, num_blocks,
+        _p(context_lens), _p(query_offsets), _p(positions), _p(slot_mapping), _p(counts),
+        _s(stream)))
+
+
+# ---------------------------------------------------------------------------
+# Rotary positions
+# ---------------------------------------------------------------------------
+def rotary_inv_freq(rotary_dim: int, base: float = 10000.0, scaling: str = "none",
+                    factor: float = 1.0, original_context: int = 8192, beta_fast: float = 32.0,
+                    beta_slow: float = 1.0, low_factor: float = 1.0,
+                    high_factor: float = 4.0) -> tuple[np.ndarray, float]:
+    """(inv_freq, attn_factor) of rotary_and_cache: the float64 radians per
+    position of the rotary_dim / 2 pairs, and the factor of the rotated values.
+
+    scaling, for contexts `factor` times the `original_context` trained on:
+      "none"     base^(-2 i / rotary_dim)
+      "linear"   positions interpolated: every frequency / factor
+      "ntk"      a larger base, base * factor^(d / (d - 2)), d = rotary_dim: the
+                 slowest pair is interpolated, the fastest stays
+      "yarn"     by wavelength: pairs that turn more than beta_fast times in
+                 the original context stay, those of less than beta_slow are
+                 interpolated, a ramp over the pair's index between; values
+                 times 0.1 ln(factor) + 1
+      "banded"   pairs of more than high_factor turns stay, those of less than
+                 low_factor are interpolated, a ramp in turns between
+    """
+    if rotary_dim < 0 or rotary_dim % 2:
+        raise InvalidParameter(f"rotary_dim {rotary_dim} (even)")
+    if not base > 0 or not factor > 0 or not original_context > 0:
+        raise InvalidParameter(f"base {base} factor {factor} original_context {original_context}")
+    i = np.arange(rotary_dim // 2, dtype=np.float64)
+    freq = float(base) ** (-2.0 * i / max(rotary_dim, 1))
+    if scaling == "none":
+        return freq, 1.0
+    if scaling == "linear":
+        return freq / factor, 1.0
+    if scaling == "ntk":
+        if rotary_dim <= 2:
+            return freq, 1.0
+        wide = base * factor ** (rotary_dim / (rotary_dim - 2.0))
+        return wide ** (-2.0 * i / rotary_dim), 1.0
+    turns = original_context * freq / (2.0 * math.pi)
+    if scaling == "yarn":
+        if not beta_fast > beta_slow > 0:
+            raise InvalidParameter(f"beta_fast {beta_fast} beta_slow {beta_slow}")
+
+        def pair_of(n: float) -> float:   # the (fractional) pair that turns n times
+            return (rotary_dim * math.log(original_context / (2.0 * math.pi * n))
+                    / (2.0 * math.log(base)))
+
+        low = max(math.floor(pair_of(beta_fast)), 0)
+        high = min(math.ceil(pair_of(beta_slow)), rotary_dim - 1)
+        keep = 1.0 - np.clip((i - low) / max(high - low, 1e-3), 0.0, 1.0)
+        return freq / factor * (1.0 - keep) + freq * keep, 0.1 * math.log(max(factor, 1.0)) + 1.0
+    if scaling == "banded":
+        if not high_factor > low_factor:
+            raise InvalidParameter(f"low_factor {low_factor} high_factor {high_factor}")
+        keep = np.clip((turns - low_factor) / (high_factor - low_factor), 0.0, 1.0)
+        return freq / factor * (1.0 - keep) + freq * keep, 1.0
+    raise NotSupported(f"rotary scaling {scaling!r}")
+
+
+def rotary_and_cache(query_out: Ptr, query: Ptr, key: Ptr, value: Ptr, key_cache: Ptr,
+                     value_cache: Ptr, positions: Ptr, slot_mapping: Ptr, inv_freq: Ptr,
+                     num_tokens: int, num_heads: int, num_kv_heads: int, head_dim: int,
+                     rotary_dim: int, block_size: int, dtype: str = "f16",
+                     attn_factor: float = 1.0, interleaved: bool = False,
+                     query_stride: Optional[int] = None, key_stride: Optional[int] = None,
+                     value_stride: Optional[int] = None, num_blocks: int = 0,
+                     stream: Optional[Stream] = None) -> None:
+    """Rotates the queries into query_out and the keys into the cache, and
+    writes the values there (swiftllm_hip_rotary_and_cache). Strides are
+    elements between tokens, packed rows by default; inv_freq is float64
+    [rotary_dim / 2] on the device (rotary_inv_freq). Tokens with a negative
+    position are padding."""
+    check_status(_lib.lib().swiftllm_hip_rotary_and_cache(
+        _p(query_out), _p(query), _p(key), _p(value), _p(key_cache), _p(value_cache),
+        _p(positions), _p(slot_mapping), _p(inv_freq), attn_factor, int(interleaved),
+        _dtype(dtype), num_tokens, num_heads, num_kv_heads, head_dim, rotary_dim, block_size,
+        num_heads * head_dim if query_stride is None else query_stride,
+        num_kv_heads * head_dim if key_stride is None else key_stride,
+        num_kv_heads * head_dim if value_stride is None else value_stride, num_blocks,
+        _s(stream)))
