@@ -501,6 +501,42 @@ int swiftllm_hip_rotary_and_cache(
     long long query_stride, long long key_stride, long long value_stride,
     int num_blocks, hipStream_t stream);
 
+/* Paged attention with shaped scores. A query at position p of sequence s
+ * sees key j < context_lens[s] where j <= p and (window == 0 or p - j <
+ * window), or where j < prefix_lens[s] (NULL: no prefix): a sliding window of
+ * `window` keys, the query's own included, and a prefix that every query
+ * sees, in both directions. Its score is
+ *   softcap > 0: softcap * tanh(scale q.k / softcap), else scale q.k,
+ *   minus alibi_slopes[h] * |p - j| (float [num_heads]; NULL: none).
+ * Outputs are the softmax-weighted sums of the seen values with kv head
+ * h / (num_heads / num_kv_heads), 32-bit sums rounded once. Blocks whose id is
+ * outside [0, num_blocks) (num_blocks <= 0: no upper bound) hold no key;
+ * context lengths are cut at max_num_blocks_per_seq * 16. A query that sees no
+ * key writes zeros. Cache slots that no query of the call sees may hold
+ * anything, NaN included. A key that is not finite makes the outputs of the
+ * queries that see it NaN or unspecified, a value that is not finite one
+ * element of them not finite; other queries are not touched by either. dtype is that of query,
+ * caches and output; scale and softcap are finite, softcap >= 0. */
+
+/* One new token per sequence: query and output [num_seqs, num_heads,
+ * head_dim], the query of sequence s at position context_lens[s] - 1
+ * (context_lens[s] <= 0: zeros). `workspace` holds
+ * swiftllm_hip_scored_decode_workspace_size() bytes, 256-byte aligned, plain
+ * scratch; calls that share one must be ordered on one stream. */
+int swiftllm_hip_scored_decode(
+    void* output, void* workspace, size_t workspace_bytes, const void* query,
+    const void* key_cache, const void* value_cache,
+    const int32_t* block_tables, const int32_t* context_lens,
+    const float* alibi_slopes, const int32_t* prefix_lens, float scale,
+    float softcap, int window, int dtype, int num_seqs, int num_heads,
+    int num_kv_heads, int head_dim, int block_size,
+    int max_num_blocks_per_seq, int num_blocks, hipStream_t stream);
+
+/* Bytes of workspace it needs for these sizes; 0 where it would refuse them. */
+size_t swiftllm_hip_scored_decode_workspace_size(
+    int num_seqs, int num_heads, int num_kv_heads, int head_dim,
+    int block_size, int max_num_blocks_per_seq);
+
 /* ------------------------------------------------------------------------ */
 /* 7. Host-side metadata (no device work).                                   */
 /* ------------------------------------------------------------------------ */

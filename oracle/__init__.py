@@ -433,8 +433,7 @@ def scored_attention(q, kc, vc, bt, ctx, query_offsets, scale, softcap=0.0, slop
             x = np.where(seen, x, -np.inf)
             top = x.max(axis=1, keepdims=True)
             w = np.where(seen, np.exp(x - np.where(np.isfinite(top), top, 0.0)), 0.0)
-            total = w.sum(axis=1, keepdims=True)
-            # keys that no row sees may hold anything
-            v = np.where(seen.any(axis=0)[:, None], V[h * Hkv // H], 0.0)
-            out[t0:t1, h] = np.where(total > 0, w @ v / np.where(total > 0, total, 1.0), 0.0)
+            v = V[h * Hkv // H]
+            for i in np.flatnonzero(seen.any(axis=1)):   # keys that a row does not see may hold anything
+                out[t0 + i, h] = w[i, seen[i]] @ v[seen[i]] / w[i].sum()
     return out

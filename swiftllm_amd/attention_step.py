@@ -2,6 +2,8 @@
 
     plan_step           block tables, slot maps and positions from request lengths
     rotary_and_cache    rotary positions of q and k, and the cache write of k and v
+    scored_decode       paged attention of one new token, its scores shaped: soft cap,
+                        distance bias (ALiBi), sliding window, prefix
 
 Reference (paths relative to the swiftllm repository): the host routines and
 options these stand for are
@@ -9,6 +11,8 @@ options these stand for are
                                                block allocation, get_slot_mapping
   crates/swiftllm-models/src/layers/attention.rs:297-353
                                                RoPE and its long-context scaling
+  crates/swiftllm-core/src/memory/paged_attention.rs:39-43, 111-135
+                                               sliding window and ALiBi options
 Device tensors are DeviceArrays or raw device pointers (ints); values are fp16
 ("f16") or bfloat16 ("bf16"). Nothing here synchronises or allocates, so every
 call may be captured in a graph.
@@ -17,13 +21,15 @@ call may be captured in a graph.
 from __future__ import annotations
 
 import math
+from dataclasses import dataclass
 from typing import Optional
 
 import numpy as np
 
 from . import _lib
 from ._hip import Stream
-from .paged_attention import InvalidParameter, NotSupported, Ptr, _p, _s, check_status
+from .paged_attention import (CudaError, InvalidParameter, NotSupported, Ptr, _p, _s,
+                              check_status)
 
 DTYPES = {"f16": 0, "bf16": 1}   # SWIFTLLM_HIP_F16, SWIFTLLM_HIP_BF16
 
@@ -133,3 +139,59 @@ def rotary_and_cache(query_out: Ptr, query: Ptr, key: Ptr, value: Ptr, key_cache
         num_kv_heads * head_dim if key_stride is None else key_stride,
         num_kv_heads * head_dim if value_stride is None else value_stride, num_blocks,
         _s(stream)))
+
+
+# ---------------------------------------------------------------------------
+# Attention with shaped scores
+# ---------------------------------------------------------------------------
+@dataclass
+class ScoreParams:
+    """How raw products become scores, and what a query at position p sees.
+
+    score of key j = softcap * tanh(scale q.k / softcap), scale q.k where
+    softcap is 0, minus alibi_slopes[h] * |p - j|; seen where j <= p and
+    (window 0 or p - j < window), or j < prefix_lens[s]. alibi_slopes is
+    float32 [num_heads], prefix_lens int32 [num_seqs], both on the device."""
+    scale: float
+    softcap: float = 0.0
+    window: int = 0
+    alibi_slopes: Ptr = None
+    prefix_lens: Ptr = None
+
+
+def alibi_slopes(num_heads: int) -> np.ndarray:
+    """The usual slopes of a distance bias, float32 [num_heads]: the powers
+    2^(-8 i / n), i = 1 .. n, for n heads a power of two; for other counts
+    those of the next lower power of two, then every other one of twice as
+    many."""
+    if num_heads < 1:
+        raise InvalidParameter(f"num_heads {num_heads}")
+    n = 1 << (num_heads.bit_length() - 1)
+    first = 2.0 ** (-8.0 * np.arange(1, n + 1) / n)
+    more = 2.0 ** (-4.0 * np.arange(1, 2 * n, 2) / n)
+    return np.concatenate([first, more])[:num_heads].astype(np.float32)
+
+
+def scored_decode_workspace_size(num_seqs: int, num_heads: int, num_kv_heads: int, head_dim: int,
+                                 block_size: int, max_num_blocks_per_seq: int) -> int:
+    n = _lib.lib().swiftllm_hip_scored_decode_workspace_size(
+        num_seqs, num_heads, num_kv_heads, head_dim, block_size, max_num_blocks_per_seq)
+    if n == 0:
+        check_status(_lib.lib().swiftllm_hip_last_error() or CudaError.code)
+    return int(n)
+
+
+def scored_decode(output: Ptr, workspace: Ptr, workspace_bytes: int, query: Ptr, key_cache: Ptr,
+                  value_cache: Ptr, block_tables: Ptr, context_lens: Ptr, score: ScoreParams,
+                  num_seqs: int, num_heads: int, num_kv_heads: int, head_dim: int,
+                  block_size: int, max_num_blocks_per_seq: int, dtype: str = "f16",
+                  num_blocks: int = 0, stream: Optional[Stream] = None) -> None:
+    """Paged attention of the last token of every sequence with shaped scores
+    (swiftllm_hip_scored_decode). `workspace` is plain scratch of
+    scored_decode_workspace_size(...) bytes; calls that share one are ordered
+    on one stream."""
+    check_status(_lib.lib().swiftllm_hip_scored_decode(
+        _p(output), _p(workspace), workspace_bytes, _p(query), _p(key_cache), _p(value_cache),
+        _p(block_tables), _p(context_lens), _p(score.alibi_slopes), _p(score.prefix_lens),
+        score.scale, score.softcap, score.window, _dtype(dtype), num_seqs, num_heads,
+        num_kv_heads, head_dim, block_size, max_num_blocks_per_seq, num_blocks, _s(stream)))

@@ -9,7 +9,8 @@ namespace swiftllm {
 
 typedef short s4 __attribute__((ext_vector_type(4)));
 typedef short s8 __attribute__((ext_vector_type(8)));
-typedef unsigned u2v __attribute__((ext_vector_type(2)));
+typedef unsigned u2 __attribute__((ext_vector_type(2)));
+typedef unsigned u4 __attribute__((ext_vector_type(4)));
 typedef float f16x __attribute__((ext_vector_type(16)));
 
 __device__ __forceinline__ s8 join8(s4 lo, s4 hi) {

@@ -1,0 +1,102 @@
+"""The scored attention's entry points without a GPU: argument checks and the
+distance bias's slopes."""
+
+import math
+
+import numpy as np
+import pytest
+
+import oracle
+from swiftllm_amd import _lib
+from swiftllm_amd import attention_step as step
+from swiftllm_amd import paged_attention as pa
+
+INVALID, UNSUP = -4, -6
+P = 1 << 20   # never dereferenced: validation fails first
+
+
+def _decode(**kw):
+    a = dict(output=P, workspace=P, workspace_bytes=1 << 40, query=P, key_cache=P, value_cache=P,
+             block_tables=P, context_lens=P, alibi_slopes=0, prefix_lens=0, scale=0.1, softcap=0.0,
+             window=0, dtype=0, num_seqs=3, num_heads=8, num_kv_heads=2, head_dim=64, block_size=16,
+             max_num_blocks_per_seq=4, num_blocks=0)
+    a.update(kw)
+    return _lib.lib().swiftllm_hip_scored_decode(*a.values(), None)
+
+
+SHARED = [
+    (dict(num_seqs=-1), INVALID),
+    (dict(num_heads=0), INVALID),
+    (dict(num_heads=9), INVALID),
+    (dict(head_dim=96), UNSUP),
+    (dict(head_dim=0), INVALID),
+    (dict(block_size=32), UNSUP),
+    (dict(max_num_blocks_per_seq=-1), INVALID),
+    (dict(max_num_blocks_per_seq=1 << 27), UNSUP),
+    (dict(num_seqs=65536), UNSUP),
+    (dict(num_seqs=65535, max_num_blocks_per_seq=1 << 20), UNSUP),
+    (dict(dtype=2), UNSUP),
+    (dict(scale=math.nan), INVALID),
+    (dict(scale=math.inf), INVALID),
+    (dict(softcap=-1.0), INVALID),
+    (dict(softcap=math.nan), INVALID),
+    (dict(softcap=math.inf), INVALID),
+    (dict(softcap=1e-30, scale=1e30), INVALID),     # scale / softcap is no finite number
+    (dict(window=-1), INVALID),
+    (dict(query=0), INVALID),
+    (dict(context_lens=0), INVALID),
+    (dict(block_tables=0), INVALID),
+    (dict(query=P + 4), INVALID),
+    (dict(key_cache=P + 2), INVALID),
+    (dict(output=P + 1), INVALID),
+    (dict(alibi_slopes=P + 2), INVALID),
+    (dict(prefix_lens=P + 2), INVALID),
+]
+
+
+@pytest.mark.parametrize("kw,code", SHARED + [
+    (dict(workspace=P + 128), INVALID),
+    (dict(workspace=0), INVALID),
+    (dict(workspace_bytes=1000), INVALID),
+])
+def test_decode_refuses(kw, code):
+    assert _decode(**kw) == code
+    assert _lib.last_error()[0] == code and _lib.last_error()[1]
+
+
+def test_decode_workspace_size():
+    n = step.scored_decode_workspace_size(8, 64, 8, 128, 16, 2048)
+    # two fragments of 16-byte aligned heads for each of the ranges
+    assert 768 * 2 * 8 * (128 + 2) * 4 <= n < 64 << 20
+    with pytest.raises(pa.NotSupported):
+        step.scored_decode_workspace_size(8, 64, 8, 96, 16, 2048)
+    with pytest.raises(pa.InvalidParameter):
+        step.scored_decode_workspace_size(8, 9, 8, 64, 16, 2048)
+
+
+def test_alibi_slopes():
+    assert step.alibi_slopes(8).tolist() == [2.0 ** -i for i in range(1, 9)]
+    s = step.alibi_slopes(12)
+    assert s[:8].tolist() == step.alibi_slopes(8).tolist()
+    assert np.allclose(s[8:], [2.0 ** -(i / 2) for i in (1, 3, 5, 7)], rtol=1e-7)
+    assert step.alibi_slopes(1).tolist() == [2.0 ** -8]
+    for n in (1, 3, 16, 40, 64):
+        assert step.alibi_slopes(n).shape == (n,) and step.alibi_slopes(n).dtype == np.float32
+    with pytest.raises(pa.InvalidParameter):
+        step.alibi_slopes(0)
+
+
+def test_oracle_without_shaping_is_plain_attention():
+    """The shaped oracle at cap 0, no bias and no window gives the decode and
+    prefill oracles' values."""
+    rng = np.random.default_rng(1)
+    kc, vc = rng.standard_normal((2, 9, 2, 64, 16)).astype(np.float16)
+    bt = rng.permutation(9)[:8].reshape(2, 4).astype(np.int32)
+    q = rng.standard_normal((2, 8, 64)).astype(np.float16)
+    ctx = np.array([50, 17], np.int32)
+    got = oracle.scored_attention(q, kc, vc, bt, ctx, [0, 1, 2], 0.125)
+    assert np.allclose(got, oracle.decode_numpy(q, kc, vc, bt, ctx, 0.125), rtol=1e-12, atol=1e-14)
+    qp = rng.standard_normal((67, 8, 64)).astype(np.float16)
+    slots = np.concatenate([pa.get_slot_mapping(bt[0], 16, 0, 50), pa.get_slot_mapping(bt[1], 16, 0, 17)])
+    got = oracle.scored_attention(qp, kc, vc, bt, ctx, [0, 50, 67], 0.125)
+    assert np.allclose(got, oracle.prefill_numpy(qp, kc, vc, slots, ctx, 0.125), rtol=1e-12, atol=1e-14)
