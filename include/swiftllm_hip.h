@@ -515,7 +515,7 @@ int swiftllm_hip_rotary_and_cache(
  * key writes zeros. Cache slots that no query of the call sees may hold
  * anything, NaN included. A key that is not finite makes the outputs of the
  * queries that see it NaN or unspecified, a value that is not finite one
- * element of them not finite; other queries are not touched by either. dtype is that of query,
+ * element of them, or all, not finite; other queries are not touched. dtype is that of query,
  * caches and output; scale and softcap are finite, softcap >= 0. */
 
 /* One new token per sequence: query and output [num_seqs, num_heads,
@@ -536,6 +536,23 @@ int swiftllm_hip_scored_decode(
 size_t swiftllm_hip_scored_decode_workspace_size(
     int num_seqs, int num_heads, int num_kv_heads, int head_dim,
     int block_size, int max_num_blocks_per_seq);
+
+/* Packed query tokens: rows query_offsets[s] .. query_offsets[s + 1] - 1 of
+ * query and output [num_tokens, num_heads, head_dim] are the last tokens of
+ * sequence s, at positions up to context_lens[s] - 1, and their keys are in
+ * the cache already: whole prompts, or chunks on top of what is cached (the
+ * arrays that swiftllm_hip_plan_step writes). query_offsets has num_seqs + 1
+ * entries within [0, num_tokens]; a sequence whose offsets are not ascending
+ * within it has no rows. Rows of no sequence are left as they were; a row at a
+ * negative position is zero. The caches are 16-byte aligned. */
+int swiftllm_hip_scored_prefill(
+    void* output, const void* query, const void* key_cache,
+    const void* value_cache, const int32_t* block_tables,
+    const int32_t* context_lens, const int32_t* query_offsets,
+    const float* alibi_slopes, const int32_t* prefix_lens, float scale,
+    float softcap, int window, int dtype, int num_tokens, int num_seqs,
+    int num_heads, int num_kv_heads, int head_dim, int block_size,
+    int max_num_blocks_per_seq, int num_blocks, hipStream_t stream);
 
 /* ------------------------------------------------------------------------ */
 /* 7. Host-side metadata (no device work).                                   */

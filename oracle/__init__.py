@@ -408,7 +408,7 @@ def scored_attention(q, kc, vc, bt, ctx, query_offsets, scale, softcap=0.0, slop
     for s in range(len(ctx)):
         t0, t1 = int(query_offsets[s]), int(query_offsets[s + 1])
         L = min(max(int(ctx[s]), 0), bt.shape[1] * 16)
-        if t1 <= t0 or L == 0:
+        if not 0 <= t0 < t1 <= T or L == 0:
             continue
         ids = np.asarray(bt[s, :(L + 15) // 16], np.int64)
         real = np.repeat((ids >= 0) & (ids < num_blocks), 16)[:L]
@@ -433,7 +433,11 @@ def scored_attention(q, kc, vc, bt, ctx, query_offsets, scale, softcap=0.0, slop
             x = np.where(seen, x, -np.inf)
             top = x.max(axis=1, keepdims=True)
             w = np.where(seen, np.exp(x - np.where(np.isfinite(top), top, 0.0)), 0.0)
-            v = V[h * Hkv // H]
-            for i in np.flatnonzero(seen.any(axis=1)):   # keys that a row does not see may hold anything
+            v = np.where(seen.any(axis=0)[:, None], V[h * Hkv // H], 0.0)
+            rows = np.flatnonzero(seen.any(axis=1))
+            if np.isfinite(v).all():
+                out[t0 + rows, h] = w[rows] @ v / w[rows].sum(axis=1, keepdims=True)
+                continue
+            for i in rows:   # keys that a row does not see may hold anything
                 out[t0 + i, h] = w[i, seen[i]] @ v[seen[i]] / w[i].sum()
     return out

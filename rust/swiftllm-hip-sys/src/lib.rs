@@ -270,6 +270,15 @@ extern "C" {
         num_seqs: c_int, num_heads: c_int, num_kv_heads: c_int, head_dim: c_int,
         block_size: c_int, max_num_blocks_per_seq: c_int,
     ) -> usize;
+    pub fn swiftllm_hip_scored_prefill(
+        output: *mut c_void, query: *const c_void, key_cache: *const c_void,
+        value_cache: *const c_void, block_tables: *const i32, context_lens: *const i32,
+        query_offsets: *const i32, alibi_slopes: *const c_float, prefix_lens: *const i32,
+        scale: c_float, softcap: c_float, window: c_int, dtype: c_int, num_tokens: c_int,
+        num_seqs: c_int, num_heads: c_int, num_kv_heads: c_int, head_dim: c_int,
+        block_size: c_int, max_num_blocks_per_seq: c_int, num_blocks: c_int,
+        stream: hipStream_t,
+    ) -> c_int;
 
     // -- host metadata: kv_cache.rs:186-216, 250-286 ------------------------------
     pub fn swiftllm_hip_slot_mapping(

@@ -101,6 +101,9 @@ SIGNATURES = {
         i32, [vp, vp, sz, vp, vp, vp, vp, vp, vp, vp, f32, f32, i32, i32, i32, i32, i32, i32, i32,
               i32, i32, vp]),
     "swiftllm_hip_scored_decode_workspace_size": (sz, [i32, i32, i32, i32, i32, i32]),
+    "swiftllm_hip_scored_prefill": (
+        i32, [vp, vp, vp, vp, vp, vp, vp, vp, vp, f32, f32, i32, i32, i32, i32, i32, i32, i32, i32,
+              i32, i32, vp]),
     "swiftllm_hip_slot_mapping": (i32, [vp, sz, sz, sz, sz, vp]),
     "swiftllm_hip_pack_block_tables": (i32, [vp, vp, vp, sz, sz, sz, vp, vp]),
 }

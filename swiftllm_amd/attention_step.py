@@ -4,6 +4,7 @@
     rotary_and_cache    rotary positions of q and k, and the cache write of k and v
     scored_decode       paged attention of one new token, its scores shaped: soft cap,
                         distance bias (ALiBi), sliding window, prefix
+    scored_prefill      the same of packed prompts or chunks of them
 
 Reference (paths relative to the swiftllm repository): the host routines and
 options these stand for are
@@ -194,4 +195,19 @@ def scored_decode(output: Ptr, workspace: Ptr, workspace_bytes: int, query: Ptr,
         _p(output), _p(workspace), workspace_bytes, _p(query), _p(key_cache), _p(value_cache),
         _p(block_tables), _p(context_lens), _p(score.alibi_slopes), _p(score.prefix_lens),
         score.scale, score.softcap, score.window, _dtype(dtype), num_seqs, num_heads,
+        num_kv_heads, head_dim, block_size, max_num_blocks_per_seq, num_blocks, _s(stream)))
+
+
+def scored_prefill(output: Ptr, query: Ptr, key_cache: Ptr, value_cache: Ptr, block_tables: Ptr,
+                   context_lens: Ptr, query_offsets: Ptr, score: ScoreParams, num_tokens: int,
+                   num_seqs: int, num_heads: int, num_kv_heads: int, head_dim: int,
+                   block_size: int, max_num_blocks_per_seq: int, dtype: str = "f16",
+                   num_blocks: int = 0, stream: Optional[Stream] = None) -> None:
+    """Paged attention of packed query tokens with shaped scores
+    (swiftllm_hip_scored_prefill): rows query_offsets[s] .. query_offsets[s + 1]
+    - 1 are the last tokens of sequence s, whose keys are in the cache."""
+    check_status(_lib.lib().swiftllm_hip_scored_prefill(
+        _p(output), _p(query), _p(key_cache), _p(value_cache), _p(block_tables),
+        _p(context_lens), _p(query_offsets), _p(score.alibi_slopes), _p(score.prefix_lens),
+        score.scale, score.softcap, score.window, _dtype(dtype), num_tokens, num_seqs, num_heads,
         num_kv_heads, head_dim, block_size, max_num_blocks_per_seq, num_blocks, _s(stream)))

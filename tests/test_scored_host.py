@@ -64,6 +64,31 @@ def test_decode_refuses(kw, code):
     assert _lib.last_error()[0] == code and _lib.last_error()[1]
 
 
+def _prefill(**kw):
+    a = dict(output=P, query=P, key_cache=P, value_cache=P, block_tables=P, context_lens=P,
+             query_offsets=P, alibi_slopes=0, prefix_lens=0, scale=0.1, softcap=0.0, window=0,
+             dtype=0, num_tokens=10, num_seqs=3, num_heads=8, num_kv_heads=2, head_dim=64,
+             block_size=16, max_num_blocks_per_seq=4, num_blocks=0)
+    a.update(kw)
+    return _lib.lib().swiftllm_hip_scored_prefill(*a.values(), None)
+
+
+@pytest.mark.parametrize("kw,code", [c for c in SHARED if c[0].get("max_num_blocks_per_seq") != 1 << 20] + [
+    (dict(num_tokens=-1), INVALID),
+    (dict(num_tokens=1 << 30), UNSUP),
+    (dict(max_num_blocks_per_seq=1 << 26), UNSUP),
+    (dict(query_offsets=0), INVALID),
+    (dict(query_offsets=P + 1), INVALID),
+    (dict(key_cache=P + 8), INVALID),
+    (dict(value_cache=P + 8), INVALID),
+    (dict(output=P + 4), INVALID),
+    (dict(num_tokens=(1 << 30) - 1, num_heads=1024, num_kv_heads=1024), UNSUP),
+])
+def test_prefill_refuses(kw, code):
+    assert _prefill(**kw) == code
+    assert _lib.last_error()[0] == code and _lib.last_error()[1]
+
+
 def test_decode_workspace_size():
     n = step.scored_decode_workspace_size(8, 64, 8, 128, 16, 2048)
     # two fragments of 16-byte aligned heads for each of the ranges
