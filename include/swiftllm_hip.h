@@ -518,19 +518,23 @@ int swiftllm_hip_rotary_and_cache(
  * element of them, or all, not finite; other queries are not touched. dtype is that of query,
  * caches and output; scale and softcap are finite, softcap >= 0. */
 
-/* One new token per sequence: query and output [num_seqs, num_heads,
- * head_dim], the query of sequence s at position context_lens[s] - 1
- * (context_lens[s] <= 0: zeros). `workspace` holds
+/* One new token per sequence: the query of sequence s, at position
+ * context_lens[s] - 1 (context_lens[s] <= 0: zeros), is row s of query and
+ * output [num_seqs, num_heads, head_dim]; with query_offsets [num_seqs + 1]
+ * (not NULL, as swiftllm_hip_plan_step writes them) it is the last of the rows
+ * query_offsets[s] .. query_offsets[s + 1] - 1 of num_tokens, and a sequence
+ * without rows there has no output. `workspace` holds
  * swiftllm_hip_scored_decode_workspace_size() bytes, 256-byte aligned, plain
  * scratch; calls that share one must be ordered on one stream. */
 int swiftllm_hip_scored_decode(
     void* output, void* workspace, size_t workspace_bytes, const void* query,
     const void* key_cache, const void* value_cache,
     const int32_t* block_tables, const int32_t* context_lens,
-    const float* alibi_slopes, const int32_t* prefix_lens, float scale,
-    float softcap, int window, int dtype, int num_seqs, int num_heads,
-    int num_kv_heads, int head_dim, int block_size,
-    int max_num_blocks_per_seq, int num_blocks, hipStream_t stream);
+    const int32_t* query_offsets, const float* alibi_slopes,
+    const int32_t* prefix_lens, float scale, float softcap, int window,
+    int dtype, int num_tokens, int num_seqs, int num_heads, int num_kv_heads,
+    int head_dim, int block_size, int max_num_blocks_per_seq, int num_blocks,
+    hipStream_t stream);
 
 /* Bytes of workspace it needs for these sizes; 0 where it would refuse them. */
 size_t swiftllm_hip_scored_decode_workspace_size(

@@ -260,11 +260,11 @@ extern "C" {
     pub fn swiftllm_hip_scored_decode(
         output: *mut c_void, workspace: *mut c_void, workspace_bytes: usize,
         query: *const c_void, key_cache: *const c_void, value_cache: *const c_void,
-        block_tables: *const i32, context_lens: *const i32, alibi_slopes: *const c_float,
-        prefix_lens: *const i32, scale: c_float, softcap: c_float, window: c_int,
-        dtype: c_int, num_seqs: c_int, num_heads: c_int, num_kv_heads: c_int,
-        head_dim: c_int, block_size: c_int, max_num_blocks_per_seq: c_int,
-        num_blocks: c_int, stream: hipStream_t,
+        block_tables: *const i32, context_lens: *const i32, query_offsets: *const i32,
+        alibi_slopes: *const c_float, prefix_lens: *const i32, scale: c_float,
+        softcap: c_float, window: c_int, dtype: c_int, num_tokens: c_int, num_seqs: c_int,
+        num_heads: c_int, num_kv_heads: c_int, head_dim: c_int, block_size: c_int,
+        max_num_blocks_per_seq: c_int, num_blocks: c_int, stream: hipStream_t,
     ) -> c_int;
     pub fn swiftllm_hip_scored_decode_workspace_size(
         num_seqs: c_int, num_heads: c_int, num_kv_heads: c_int, head_dim: c_int,

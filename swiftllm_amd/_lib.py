@@ -98,8 +98,8 @@ SIGNATURES = {
         i32, [vp, vp, vp, vp, vp, vp, vp, vp, vp, f32, i32, i32, i32, i32, i32, i32, i32, i32,
               i64, i64, i64, i32, vp]),
     "swiftllm_hip_scored_decode": (
-        i32, [vp, vp, sz, vp, vp, vp, vp, vp, vp, vp, f32, f32, i32, i32, i32, i32, i32, i32, i32,
-              i32, i32, vp]),
+        i32, [vp, vp, sz, vp, vp, vp, vp, vp, vp, vp, vp, f32, f32, i32, i32, i32, i32, i32, i32,
+              i32, i32, i32, i32, vp]),
     "swiftllm_hip_scored_decode_workspace_size": (sz, [i32, i32, i32, i32, i32, i32]),
     "swiftllm_hip_scored_prefill": (
         i32, [vp, vp, vp, vp, vp, vp, vp, vp, vp, f32, f32, i32, i32, i32, i32, i32, i32, i32, i32,

@@ -28,7 +28,7 @@ from typing import Optional
 import numpy as np
 
 from . import _lib
-from ._hip import Stream
+from ._hip import DeviceArray, Stream
 from .paged_attention import (CudaError, InvalidParameter, NotSupported, Ptr, _p, _s,
                               check_status)
 
@@ -186,16 +186,19 @@ def scored_decode(output: Ptr, workspace: Ptr, workspace_bytes: int, query: Ptr,
                   value_cache: Ptr, block_tables: Ptr, context_lens: Ptr, score: ScoreParams,
                   num_seqs: int, num_heads: int, num_kv_heads: int, head_dim: int,
                   block_size: int, max_num_blocks_per_seq: int, dtype: str = "f16",
-                  num_blocks: int = 0, stream: Optional[Stream] = None) -> None:
+                  num_blocks: int = 0, query_offsets: Ptr = None, num_tokens: int = 0,
+                  stream: Optional[Stream] = None) -> None:
     """Paged attention of the last token of every sequence with shaped scores
-    (swiftllm_hip_scored_decode). `workspace` is plain scratch of
-    scored_decode_workspace_size(...) bytes; calls that share one are ordered
-    on one stream."""
+    (swiftllm_hip_scored_decode): row s of query and output, or with
+    query_offsets the last of the sequence's rows of num_tokens. `workspace` is
+    plain scratch of scored_decode_workspace_size(...) bytes; calls that share
+    one are ordered on one stream."""
     check_status(_lib.lib().swiftllm_hip_scored_decode(
         _p(output), _p(workspace), workspace_bytes, _p(query), _p(key_cache), _p(value_cache),
-        _p(block_tables), _p(context_lens), _p(score.alibi_slopes), _p(score.prefix_lens),
-        score.scale, score.softcap, score.window, _dtype(dtype), num_seqs, num_heads,
-        num_kv_heads, head_dim, block_size, max_num_blocks_per_seq, num_blocks, _s(stream)))
+        _p(block_tables), _p(context_lens), _p(query_offsets), _p(score.alibi_slopes),
+        _p(score.prefix_lens), score.scale, score.softcap, score.window, _dtype(dtype),
+        num_tokens, num_seqs, num_heads, num_kv_heads, head_dim, block_size,
+        max_num_blocks_per_seq, num_blocks, _s(stream)))
 
 
 def scored_prefill(output: Ptr, query: Ptr, key_cache: Ptr, value_cache: Ptr, block_tables: Ptr,
@@ -211,3 +214,87 @@ def scored_prefill(output: Ptr, query: Ptr, key_cache: Ptr, value_cache: Ptr, bl
         _p(context_lens), _p(query_offsets), _p(score.alibi_slopes), _p(score.prefix_lens),
         score.scale, score.softcap, score.window, _dtype(dtype), num_tokens, num_seqs, num_heads,
         num_kv_heads, head_dim, block_size, max_num_blocks_per_seq, num_blocks, _s(stream)))
+
+
+class AttentionStep:
+    """A layer's share of a serving step: rotary positions and the cache write,
+    then attention with shaped scores, over the arrays that plan() makes once
+    per step for all layers. Calls are asynchronous on `stream`, and the arrays
+    are the object's own, so a step of fixed capacities can be captured in a
+    graph; steps that overlap take an object each.
+
+        step = AttentionStep(num_seqs, num_tokens, max_blocks, H, Hkv, D, score, inv_freq)
+        step.plan(tables, cached, new, free, num_free)     # once per step
+        step.layer(q, k, v, key_cache, value_cache, out)   # every layer
+
+    num_seqs and num_tokens are capacities: sequences past a batch have
+    cached and new lengths of 0, rows past its tokens are left as they are.
+    The rows of a step whose every sequence brings at most one token go through
+    scored_decode (decode=True), all others through scored_prefill."""
+
+    def __init__(self, num_seqs: int, num_tokens: int, max_num_blocks_per_seq: int,
+                 num_heads: int, num_kv_heads: int, head_dim: int, score: ScoreParams,
+                 inv_freq: np.ndarray, attn_factor: float = 1.0, interleaved: bool = False,
+                 dtype: str = "f16", block_size: int = 16):
+        _dtype(dtype)
+        inv = np.ascontiguousarray(inv_freq, dtype=np.float64)
+        if inv.ndim != 1 or 2 * inv.size > head_dim:
+            raise InvalidParameter(f"inv_freq of shape {inv.shape} for head_dim {head_dim}")
+        self.num_seqs, self.num_tokens = num_seqs, num_tokens
+        self.max_num_blocks_per_seq, self.block_size = max_num_blocks_per_seq, block_size
+        self.num_heads, self.num_kv_heads, self.head_dim = num_heads, num_kv_heads, head_dim
+        self.score, self.dtype = score, dtype
+        self.rotary_dim, self.attn_factor, self.interleaved = 2 * inv.size, attn_factor, interleaved
+        self.inv_freq = DeviceArray.from_numpy(inv if inv.size else np.zeros(1))
+        n = scored_decode_workspace_size(num_seqs, num_heads, num_kv_heads, head_dim, block_size,
+                                         max_num_blocks_per_seq)
+        self.workspace = DeviceArray((n,), np.uint8)
+        self.context_lens = DeviceArray((max(num_seqs, 1),), np.int32)
+        self.query_offsets = DeviceArray((num_seqs + 1,), np.int32)
+        self.positions = DeviceArray((max(num_tokens, 1),), np.int32)
+        self.slot_mapping = DeviceArray((max(num_tokens, 1),), np.int32)
+        self.counts = DeviceArray((3,), np.int32)
+        self.query = DeviceArray((max(num_tokens, 1), num_heads, head_dim), np.uint16)
+        self._tables: Ptr = None
+
+    def plan(self, block_tables: Ptr, cached_lens: Ptr, new_lens: Ptr, free_blocks: Ptr,
+             num_free: Ptr, free_capacity: int, num_blocks: int = 0,
+             stream: Optional[Stream] = None) -> None:
+        """plan_step into this object's arrays; block_tables is completed in place."""
+        plan_step(block_tables, cached_lens, new_lens, free_blocks, num_free, free_capacity,
+                  self.num_seqs, self.max_num_blocks_per_seq, self.block_size, self.num_tokens,
+                  self.context_lens, self.query_offsets, self.positions, self.slot_mapping,
+                  self.counts, num_blocks=num_blocks, stream=stream)
+        self._tables = block_tables
+
+    def layer(self, query: Ptr, key: Ptr, value: Ptr, key_cache: Ptr, value_cache: Ptr,
+              output: Ptr, query_stride: Optional[int] = None, key_stride: Optional[int] = None,
+              value_stride: Optional[int] = None, num_blocks: int = 0, decode: bool = False,
+              stream: Optional[Stream] = None) -> None:
+        """Rotates the step's queries and keys, writes keys and values to this
+        layer's cache and attends over it. query, key and value hold num_tokens
+        rows; output is [num_tokens, num_heads, head_dim]. decode: the caller
+        knows that no sequence brings more than one token (of more, only the
+        last would be attended)."""
+        if self._tables is None:
+            raise InvalidParameter("layer() before plan()")
+        H, Hkv, D = self.num_heads, self.num_kv_heads, self.head_dim
+        rotary_and_cache(self.query, query, key, value, key_cache, value_cache, self.positions,
+                         self.slot_mapping, self.inv_freq, self.num_tokens, H, Hkv, D,
+                         self.rotary_dim, self.block_size, dtype=self.dtype,
+                         attn_factor=self.attn_factor, interleaved=self.interleaved,
+                         query_stride=query_stride, key_stride=key_stride,
+                         value_stride=value_stride, num_blocks=num_blocks, stream=stream)
+        if decode:
+            scored_decode(output, self.workspace, self.workspace.nbytes, self.query, key_cache,
+                          value_cache, self._tables, self.context_lens, self.score, self.num_seqs,
+                          H, Hkv, D, self.block_size, self.max_num_blocks_per_seq,
+                          dtype=self.dtype, num_blocks=num_blocks,
+                          query_offsets=self.query_offsets, num_tokens=self.num_tokens,
+                          stream=stream)
+        else:
+            scored_prefill(output, self.query, key_cache, value_cache, self._tables,
+                           self.context_lens, self.query_offsets, self.score, self.num_tokens,
+                           self.num_seqs, H, Hkv, D, self.block_size,
+                           self.max_num_blocks_per_seq, dtype=self.dtype, num_blocks=num_blocks,
+                           stream=stream)

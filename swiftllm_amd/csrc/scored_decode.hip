@@ -1,7 +1,7 @@
 // Paged attention of one new token with shaped scores (gfx950): soft cap,
 // distance bias, sliding window, and a prefix that stays in sight
 // (scored_core.hpp). The query of sequence s is its last token, at position
-// context_lens[s] - 1.
+// context_lens[s] - 1: row s, or the last of its rows of a packed step.
 //
 // Bound: HBM, one read of the visible K and V: blocks that a window hides are
 // never touched. Per 16-token block a wave has 8 KB to read at D = 128 and
@@ -39,6 +39,8 @@ struct ScoredDecodeArgs {
     const uint16_t* vc;
     const int* bt;
     const int* ctx;
+    const int* qoff;       // [S + 1] or null: row s
+    int T;                 // rows, where qoff is given
     int4* info;            // [ranges]: sequence that is cut at the range's end, its last range
     float* frag_ml;        // [ranges][2][HC][2][gs]
     float* frag_o;         // [ranges][2][HC][gs][D], normalised
@@ -59,6 +61,13 @@ constexpr int kPieceCost = 4;
 // Shortest range, in blocks: two per wave.
 constexpr int kLeastRange = 8;
 
+// The row of a sequence's query and output; negative: it has none.
+__device__ __forceinline__ int row_of(const ScoredDecodeArgs& a, int s) {
+    if (a.qoff == nullptr) return s;
+    const int b = a.qoff[s], e = a.qoff[s + 1];
+    return b >= 0 && e > b && e <= a.T ? e - 1 : -1;
+}
+
 // What the query of a sequence sees, in blocks: the walk takes blocks 0 ..
 // before - 1 (the prefix) and then those from `low / 16` on.
 struct Sight {
@@ -73,7 +82,7 @@ struct Sight {
 
 __device__ __forceinline__ Sight sight_of(const ScoredDecodeArgs& a, int s) {
     Sight v;
-    v.L = min(max(a.ctx[s], 0), a.MB * kBlockTokens);
+    v.L = row_of(a, s) < 0 ? 0 : min(max(a.ctx[s], 0), a.MB * kBlockTokens);
     v.low = a.shape.window > 0 ? max(v.L - a.shape.window, 0) : 0;
     v.pre = a.shape.prefix != nullptr ? min(max(a.shape.prefix[s], 0), v.L) : 0;
     const int first = v.low >> kBlockShift;
@@ -188,10 +197,10 @@ __host__ __device__ constexpr int merge_floats(int gs) {
 }
 
 // Blocks i0 .. i1 - 1 of a sequence's walk for one kv head and chunk of query
-// heads, by the whole workgroup. emit(g, d, o, m, l): normalised output d of
+// heads, by the whole workgroup. at: the query's row. emit(g, d, o, m, l): normalised output d of
 // head g, and its maximum and sum.
 template <typename T, int D, typename Emit>
-__device__ __forceinline__ void run_piece(const ScoredDecodeArgs& a, const Sight& sight, int s, int kvh, int hc, int i0,
+__device__ __forceinline__ void run_piece(const ScoredDecodeArgs& a, const Sight& sight, int s, int at, int kvh, int hc, int i0,
                                           int i1, Emit emit) {
     constexpr int NJ = D / 16;
     // Worked out per piece behind an empty asm: kept over the pieces, what
@@ -218,7 +227,7 @@ __device__ __forceinline__ void run_piece(const ScoredDecodeArgs& a, const Sight
         auto ids_from = [&](int c) { return row[sight.block(min(i0 + w + kWaves * (64 * c + lane), i1 - 1))]; };
         int ids = ids_from(0);
         s8 q[NJ / 2];
-        const uint16_t* const qp = a.q + (static_cast<size_t>(s) * a.H + h0 + min(r, gn - 1)) * D + 4 * kg;
+        const uint16_t* const qp = a.q + (static_cast<size_t>(at) * a.H + h0 + min(r, gn - 1)) * D + 4 * kg;
 #pragma unroll
         for (int J = 0; J < NJ; J += 2) {
             const s8 x = join8(*reinterpret_cast<const s4*>(qp + 16 * J), *reinterpret_cast<const s4*>(qp + 16 * J + 16));
@@ -237,11 +246,11 @@ __device__ __forceinline__ void run_piece(const ScoredDecodeArgs& a, const Sight
             j = sight.block(i0 + w + kWaves * k);
             seen = known ? sight.tokens(j) & 0xffffu : 0u;
             // A block outside the pool is read as block 0 and hidden.
-            const size_t at = kv_tile_offset(known ? b : 0, kvh, a.Hkv, D) + loff;
+            const size_t tile = kv_tile_offset(known ? b : 0, kvh, a.Hkv, D) + loff;
 #pragma unroll
-            for (int J = 0; J < NJ; ++J) kk[J] = load4(a.kc + at + kv_elem_offset(16 * J, 0));
+            for (int J = 0; J < NJ; ++J) kk[J] = load4(a.kc + tile + kv_elem_offset(16 * J, 0));
 #pragma unroll
-            for (int J = 0; J < NJ; ++J) vv[J] = load4(a.vc + at + kv_elem_offset(16 * J, 0));
+            for (int J = 0; J < NJ; ++J) vv[J] = load4(a.vc + tile + kv_elem_offset(16 * J, 0));
         };
         auto take = [&](s4 (&kk)[NJ], s4 (&vv)[NJ], int j, unsigned seen) {
             attend<T, D>(st, seen, j * kBlockTokens - (sight.L - 1), kg, kk, vv, q, ident, a.shape, slope);
@@ -367,9 +376,10 @@ void scored_decode_kernel(const ScoredDecodeArgs a) {
         const int slot = begin < start ? 0 : 1;
         if (!whole && slot == 1) cut = int4{s, (stop - 1) / len, 0, 0};
         const size_t f = static_cast<size_t>(2 * range + slot) * HC + sub;
-        run_piece<T, D>(a, sight, s, kvh, hc, i0, i1, [&](int g, int d, float o, float m, float l) {
+        const int row = row_of(a, s);
+        run_piece<T, D>(a, sight, s, row, kvh, hc, i0, i1, [&](int g, int d, float o, float m, float l) {
             if (whole) {
-                a.out[(static_cast<size_t>(s) * a.H + h0 + g) * D + d] = T::down(o);
+                if (row >= 0) a.out[(static_cast<size_t>(row) * a.H + h0 + g) * D + d] = T::down(o);
                 return;
             }
             a.frag_o[(f * gs + g) * D + d] = o;
@@ -449,7 +459,8 @@ __global__ __launch_bounds__(64 * kWaves) void scored_decode_join_kernel(const S
         num += f * s_o[x][d];
         den += f * s_ml[x][1];
     }
-    a.out[(static_cast<size_t>(cut.x) * a.H + h) * D + d] = T::down(den == 0.0f ? 0.0f : num / den);
+    const int row = row_of(a, cut.x);
+    if (row >= 0) a.out[(static_cast<size_t>(row) * a.H + h) * D + d] = T::down(den == 0.0f ? 0.0f : num / den);
 }
 
 // Workgroups of the kernel that fit an MI355X at once: 256 CUs, three each.
@@ -512,8 +523,9 @@ size_t swiftllm_hip_scored_decode_workspace_size(int num_seqs, int num_heads, in
 
 int swiftllm_hip_scored_decode(void* output, void* workspace, size_t workspace_bytes, const void* query,
                                const void* key_cache, const void* value_cache, const int32_t* block_tables,
-                               const int32_t* context_lens, const float* alibi_slopes, const int32_t* prefix_lens,
-                               float scale, float softcap, int window, int dtype, int num_seqs, int num_heads,
+                               const int32_t* context_lens, const int32_t* query_offsets, const float* alibi_slopes,
+                               const int32_t* prefix_lens, float scale, float softcap, int window, int dtype,
+                               int num_tokens, int num_seqs, int num_heads,
                                int num_kv_heads, int head_dim, int block_size, int max_num_blocks_per_seq,
                                int num_blocks, hipStream_t stream) {
     const char* who = "swiftllm_hip_scored_decode";
@@ -526,13 +538,16 @@ int swiftllm_hip_scored_decode(void* output, void* workspace, size_t workspace_b
     if (!scored::make_shape(a.shape, scale, softcap, window, prefix_lens, alibi_slopes)) {
         return fail(SWIFTLLM_ERR_INVALID_PARAMETER, "%s: scale=%g softcap=%g window=%d", who, scale, softcap, window);
     }
+    if (query_offsets && num_tokens < 0) {
+        return fail(SWIFTLLM_ERR_INVALID_PARAMETER, "%s: num_tokens=%d", who, num_tokens);
+    }
     if (num_seqs > 0 && (!output || !query || !key_cache || !value_cache || !context_lens || !workspace ||
                          (max_num_blocks_per_seq > 0 && !block_tables))) {
         return fail(SWIFTLLM_ERR_INVALID_PARAMETER, "%s: null pointer", who);
     }
     if (!aligned(output, 2) || !aligned(query, 8) || !aligned(key_cache, 8) || !aligned(value_cache, 8) ||
-        !aligned(block_tables, 4) || !aligned(context_lens, 4) || !aligned(alibi_slopes, 4) ||
-        !aligned(prefix_lens, 4) || !aligned(workspace, 256)) {
+        !aligned(block_tables, 4) || !aligned(context_lens, 4) || !aligned(query_offsets, 4) ||
+        !aligned(alibi_slopes, 4) || !aligned(prefix_lens, 4) || !aligned(workspace, 256)) {
         return fail(SWIFTLLM_ERR_INVALID_PARAMETER, "%s: misaligned pointer", who);
     }
     const Layout l = layout_of(num_heads, num_kv_heads, head_dim);
@@ -555,6 +570,8 @@ int swiftllm_hip_scored_decode(void* output, void* workspace, size_t workspace_b
     a.vc = static_cast<const uint16_t*>(value_cache);
     a.bt = block_tables;
     a.ctx = context_lens;
+    a.qoff = query_offsets;
+    a.T = num_tokens;
     char* const ws = static_cast<char*>(workspace);
     a.info = reinterpret_cast<int4*>(ws);
     a.frag_ml = reinterpret_cast<float*>(ws + l.ml);

@@ -282,3 +282,28 @@ def test_decode_in_a_captured_graph(dev):
             s.synchronize()
         for c in cs:
             c.check(f"replay {step_}")
+
+
+@pytest.mark.parametrize("wide", [False, True])
+def test_decode_rows_of_a_packed_step(dev, wide):
+    """With offsets: the last row of each sequence, none for one without rows
+    or with offsets out of range; other rows are left as they were."""
+    rng = np.random.default_rng(15)
+    d = Decode(rng, [40, 700, 33, 5, 64, 20], 8, 2, 64, "f16", cap=20.0, MB=300 if wide else 44)
+    off = np.array([2, 3, 6, 6, 7, 40, 41], np.int32)     # 0, 1 and 3 have rows; 5's lie past them
+    T = 12
+    q = normal(rng, (T, 8, 64), "f16", 3.0)
+    rows = {0: 2, 1: 5, 3: 6}
+    for s in range(6):
+        d.q[s] = q[rows.get(s, 0)]
+    out, d_q, d_off = DeviceArray((T, 8, 64), np.uint16), DeviceArray.from_numpy(q), DeviceArray.from_numpy(off)
+    out.fill_byte(0x7F)
+    p = step.ScoreParams(d.score["scale"], 20.0)
+    step.scored_decode(out, d.ws, d.ws.nbytes, d_q, d.d["kc"], d.d["vc"], d.d["bt"], d.d["ctx"], p, 6, 8, 2,
+                       64, 16, d.MB, num_blocks=d.NB, query_offsets=d_off, num_tokens=T)
+    synchronize()
+    got = out.numpy()
+    want, bound = d.want()
+    for s, r in rows.items():
+        assert (np.abs(to_float(got[r], "f16") - want[s]) <= bound[s]).all()
+    assert (np.delete(got, list(rows.values()), axis=0) == 0x7F7F).all()

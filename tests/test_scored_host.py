@@ -17,8 +17,8 @@ P = 1 << 20   # never dereferenced: validation fails first
 
 def _decode(**kw):
     a = dict(output=P, workspace=P, workspace_bytes=1 << 40, query=P, key_cache=P, value_cache=P,
-             block_tables=P, context_lens=P, alibi_slopes=0, prefix_lens=0, scale=0.1, softcap=0.0,
-             window=0, dtype=0, num_seqs=3, num_heads=8, num_kv_heads=2, head_dim=64, block_size=16,
+             block_tables=P, context_lens=P, query_offsets=0, alibi_slopes=0, prefix_lens=0, scale=0.1,
+             softcap=0.0, window=0, dtype=0, num_tokens=-1, num_seqs=3, num_heads=8, num_kv_heads=2, head_dim=64, block_size=16,
              max_num_blocks_per_seq=4, num_blocks=0)
     a.update(kw)
     return _lib.lib().swiftllm_hip_scored_decode(*a.values(), None)
@@ -58,6 +58,8 @@ SHARED = [
     (dict(workspace=P + 128), INVALID),
     (dict(workspace=0), INVALID),
     (dict(workspace_bytes=1000), INVALID),
+    (dict(query_offsets=P), INVALID),               # and num_tokens below 0
+    (dict(query_offsets=P + 2, num_tokens=5), INVALID),
 ])
 def test_decode_refuses(kw, code):
     assert _decode(**kw) == code
