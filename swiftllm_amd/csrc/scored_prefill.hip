@@ -274,7 +274,8 @@ __device__ __forceinline__ float add_pair(F16, unsigned p, float a) {
     return __builtin_amdgcn_fdot2(__builtin_bit_cast(v2, p), v2{1, 1}, a, false);
 }
 __device__ __forceinline__ float add_pair(BF16, unsigned p, float a) {
-    return a + (__builtin_bit_cast(float, p << 16) + __builtin_bit_cast(float, p & 0xffff0000u));
+    typedef __bf16 v2 __attribute__((ext_vector_type(2)));
+    return __builtin_amdgcn_fdot2_f32_bf16(__builtin_bit_cast(v2, p), __builtin_bit_cast(v2, 0x3f803f80u), a, false);
 }
 
 template <typename T, int D, bool CAP, bool BIAS>
@@ -424,11 +425,11 @@ void scored_prefill_kernel(const ScoredPrefillArgs a) {
         return block_known(b, a.num_blocks) ? b : 0;
     };
     // This wave's block of stage t of the walk has landed in its V buffer.
-    auto landed = [&](int t) {
+    auto landed = [&](int t, int ok4) {
         const int base = kStage * stage_of(t);
         const int end = base + kStage - 1;
         unsigned bad = 0;
-        if (tp0 < end || end >= L || (end >= pre && tp1 - base >= window)) bad = clean_v<T, D>(s_v[t & 1], w, lane);
+        if (tp0 < end || end >= L || ok4 != 15 || (end >= pre && tp1 - base >= window)) bad = clean_v<T, D>(s_v[t & 1], w, lane);
         if (lane == 0) s_bad[t & 1][w] = bad;
     };
     int ok_t, ok_1 = 15, ok_2 = 15;  // of stages t, t + 1 and t + 2
@@ -442,7 +443,7 @@ void scored_prefill_kernel(const ScoredPrefillArgs a) {
             stage_k<D>(a, s_k[1], w, b_1, kvh, lane);
         }
         wait_vm<0>();
-        landed(0);
+        landed(0, ok_t);
     }
     __syncthreads();
     f16x sc[2];
@@ -483,29 +484,30 @@ void scored_prefill_kernel(const ScoredPrefillArgs a) {
         }
         const float scale = a.shape.scale;
         const float cap = a.shape.cap;
-        if constexpr (BIAS) {
-            const float d0 = static_cast<float>(base + 8 * h - pos);  // the first key's place from the row
-            // -slope * |d| of key i; d <= 0 in a whole stage.
-            const float b0 = __builtin_fmaf(slope, d0, CAP ? cap : 0.0f);
-            auto scored = [&](float v, float bias) {
-                if constexpr (CAP) {
-                    return __builtin_fmaf(__builtin_amdgcn_rcpf(__builtin_amdgcn_exp2f(v * scale) + 1.0f), -2.0f * cap, bias);
-                } else {
-                    return __builtin_fmaf(v, scale, bias);
+        if constexpr (CAP || BIAS) {
+            // Scores in the products' place: key i lies d0 + off from the row, and
+            // d0 + off <= 0 in a whole stage.
+            const float d0 = static_cast<float>(base + 8 * h - pos);
+            const float b0 = BIAS ? __builtin_fmaf(slope, d0, CAP ? cap : 0.0f) : cap;
+            auto score = [&](auto bias_of) {
+#pragma unroll
+                for (int i = 0; i < 32; ++i) {
+                    const float x = sc[i >> 4][i & 15];
+                    const float bias = bias_of(static_cast<float>(16 * (i >> 3) + (i & 7)));
+                    if constexpr (CAP) {
+                        const float u = __builtin_amdgcn_rcpf(__builtin_amdgcn_exp2f(x * scale) + 1.0f);
+                        sc[i >> 4][i & 15] = __builtin_fmaf(u, -2.0f * cap, bias);
+                    } else {
+                        sc[i >> 4][i & 15] = __builtin_fmaf(x, scale, bias);
+                    }
                 }
             };
-            if (whole) {
-#pragma unroll
-                for (int i = 0; i < 32; ++i) {
-                    const float off = static_cast<float>(16 * (i >> 3) + (i & 7));
-                    sc[i >> 4][i & 15] = scored(sc[i >> 4][i & 15], __builtin_fmaf(slope, off, b0));
-                }
+            if constexpr (!BIAS) {
+                score([&](float) { return cap; });
+            } else if (whole) {
+                score([&](float off) { return __builtin_fmaf(slope, off, b0); });
             } else {
-#pragma unroll
-                for (int i = 0; i < 32; ++i) {
-                    const float off = static_cast<float>(16 * (i >> 3) + (i & 7));
-                    sc[i >> 4][i & 15] = scored(sc[i >> 4][i & 15], __builtin_fmaf(-slope, __builtin_fabsf(d0 + off), CAP ? cap : 0.0f));
-                }
+                score([&](float off) { return __builtin_fmaf(-slope, __builtin_fabsf(d0 + off), CAP ? cap : 0.0f); });
             }
         }
         if (!whole) {
@@ -525,14 +527,7 @@ void scored_prefill_kernel(const ScoredPrefillArgs a) {
             const auto y = __builtin_amdgcn_permlane32_swap(__builtin_bit_cast(unsigned, bm), __builtin_bit_cast(unsigned, bm), false, false);
             bm = fmaxf(__builtin_bit_cast(float, static_cast<unsigned>(y[0])), __builtin_bit_cast(float, static_cast<unsigned>(y[1])));
         }
-        if constexpr (!BIAS) {
-            // A row that sees nothing yet keeps -inf, which the cap would lift.
-            if constexpr (CAP) {
-                bm = bm == -INFINITY ? bm : capped_score(bm, scale, cap);
-            } else {
-                bm *= scale;
-            }
-        }
+        if constexpr (!CAP && !BIAS) bm *= scale;
         if (__any(bm > m + kLag)) {
             const float m_new = fmaxf(m, bm);
             const float alpha = m_new == -INFINITY ? 1.0f : __builtin_amdgcn_exp2f(m - m_new);
@@ -549,51 +544,35 @@ void scored_prefill_kernel(const ScoredPrefillArgs a) {
             for (int b = 0; b < 4; ++b) keys |= ((bad[b] >> (8 * h)) & 0xffu) << (8 * b);
             if (seen & keys) l = __builtin_nanf("");
         }
+        // Weights, O^T += V P^T, and the next stage's scores in the place of the
+        // pair's that are used up, without a branch, so that the products run
+        // among the weights. (Behind the last stage they are made of what lies in
+        // the buffer, and not used.)
         const uint16_t* const next = s_k[(t + 1) & 1] + koff;
 #pragma unroll
         for (int b = 0; b < 4; ++b) {
-            // (unless no row of the wave sees a key of the block)
-            if (whole || __ballot((seen >> (8 * b)) & 0xffu) != 0) {
-                float p[8];
+            u4 pp;
 #pragma unroll
-                for (int i = 0; i < 8; ++i) {
-                    const float v = sc[b >> 1][8 * (b & 1) + i];
-                    if constexpr (BIAS) {
-                        p[i] = __builtin_amdgcn_exp2f(v - c);
-                    } else if constexpr (CAP) {
-                        const float u = __builtin_amdgcn_rcpf(__builtin_amdgcn_exp2f(v * scale) + 1.0f);
-                        p[i] = __builtin_amdgcn_exp2f(__builtin_fmaf(u, -2.0f * cap, cap - c));
-                    } else {
-                        p[i] = __builtin_amdgcn_exp2f(__builtin_fmaf(v, scale, -c));
-                    }
-                }
-                if constexpr (CAP && !BIAS) {
-                    if (!whole) {   // the cap of a hidden score is no -inf
+            for (int i = 0; i < 4; ++i) {
+                float p[2];
 #pragma unroll
-                        for (int i = 0; i < 8; ++i) {
-                            p[i] = __builtin_bit_cast(float, __builtin_bit_cast(int, p[i]) &
-                                                                 __builtin_amdgcn_sbfe(static_cast<int>(seen), 8 * b + i, 1));
-                        }
-                    }
+                for (int z = 0; z < 2; ++z) {
+                    const float v = sc[b >> 1][8 * (b & 1) + 2 * i + z];
+                    p[z] = __builtin_amdgcn_exp2f(CAP || BIAS ? v - c : __builtin_fmaf(v, scale, -c));
                 }
-                u4 pp;
-#pragma unroll
-                for (int i = 0; i < 4; ++i) {
-                    pp[i] = T::down2(p[2 * i], p[2 * i + 1]);
-                    l = add_pair(T{}, pp[i], l);
-                }
-                const uint16_t* const vl = s_v[t & 1] + b * St::kTile + 8 * lane;
-#pragma unroll
-                for (int i = 0; i < ND; ++i) {
-                    acc[i] = T::mfma32(*reinterpret_cast<const s8*>(vl + 512 * i), __builtin_bit_cast(s8, pp), acc[i]);
-                }
+                pp[i] = T::down2(p[0], p[1]);
+                l = add_pair(T{}, pp[i], l);
             }
-            // The pair's scores are used up: the next stage's take their place.
-            if ((b & 1) && more) qk_pair<T, D>(sc[b >> 1], next + (b >> 1) * St::kPair, q);
+            const uint16_t* const vl = s_v[t & 1] + b * St::kTile + 8 * lane;
+#pragma unroll
+            for (int i = 0; i < ND; ++i) {
+                acc[i] = T::mfma32(*reinterpret_cast<const s8*>(vl + 512 * i), __builtin_bit_cast(s8, pp), acc[i]);
+            }
+            if (b & 1) qk_pair<T, D>(sc[b >> 1], next + (b >> 1) * St::kPair, q);
         }
         if (more) {
             wait_vm<0>();
-            landed(t + 1);
+            landed(t + 1, ok_1);
             ok_t = ok_1;
             ok_1 = ok_2;
             b_1 = b_2;
