@@ -89,6 +89,7 @@ struct CopySrc {
     const uint16_t* rows;     // row0 of the slice
     long long stride;
     __device__ __forceinline__ int slot(int t) const { return slots[t]; }
+    __device__ __forceinline__ void before(int) const {}
     __device__ __forceinline__ uint16_t one(int t, int i) const { return rows[t * stride + i]; }
     __device__ __forceinline__ u4v eight(int t, int c) const {
         return *reinterpret_cast<const u4v*>(rows + t * stride + c);

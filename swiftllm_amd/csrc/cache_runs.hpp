@@ -47,7 +47,8 @@ constexpr int kWinStride = kWinRows + 16;      // halves per token in LDS (544 b
 // (one lane of 32 looks at each of the W + 15 tokens those runs can span).
 // tile: (W + 15) * kWinStride halves of LDS. n: rows of a block. src gives the
 // slot of token t (negative: none), and of row0's slice of it the 8 values
-// from c or the one at i.
+// from c or the one at i; before(k) comes ahead of the 8 values of token t0 + k,
+// with every lane active.
 template <int W, typename Src>
 __device__ __forceinline__ void write_runs(const Src& src, uint16_t* const cache, uint16_t* const tile, int t0,
                                            int row0, int n, int T, long long num_slots) {
@@ -101,6 +102,7 @@ __device__ __forceinline__ void write_runs(const Src& src, uint16_t* const cache
 #pragma unroll
     for (int i = 0; i < kLoads; ++i) {
         const int k = first + 8 * i + (tid >> 5);
+        src.before(k);
         if (k < end && row0 + c < n) {
             buf[i] = src.eight(t0 + k, c);
         }

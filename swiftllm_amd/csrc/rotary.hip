@@ -17,9 +17,7 @@
 //
 // Bound: HBM, one read of q, k and v and one write of q and of the blocks.
 // One launch: a workgroup takes either a window of tokens of 256 rows of K or
-// of V (see cache_runs.hpp), or a piece of the queries: there a thread owns 8
-// values of a head at one token and walks the heads, so that its 8 angles are
-// made once.
+// of V (see cache_runs.hpp), or the queries of four tokens.
 
 #include <algorithm>
 #include <cmath>
@@ -54,8 +52,9 @@ struct RotaryArgs {
     int rot;                 // rotary_dim
     int windows;             // windows of tokens of K and V
     int slices;              // of kWinRows rows
-    int each;                // query heads a thread walks
-    int groups;              // of tokens, of the queries
+    int each;                // query heads a wave takes of a token
+    int parts;               // waves per token
+    bool whole;              // rotary_dim is a multiple of 16
     bool wide_q;             // 16-byte accesses of q and out, whole pieces of 8 rotated alike
     bool wide_k;
     bool wide_v;
@@ -87,34 +86,68 @@ __device__ __forceinline__ void pair_of(int d, int half, int& i, int& other, flo
     }
 }
 
-// The cosines and signed sines of elements d .. d + 7 at a position: 1 and 0
-// past rotary_dim.
+// The cosines and sines of a token's pairs, one pair a lane, in LDS of the
+// wave: an angle costs some 20 operations, and every head needs it.
+struct TurnLds {
+    float c[64], s[64];
+    __device__ __forceinline__ void make(const RotaryArgs& a, int pos) {
+        const int i = threadIdx.x & 63;
+        float cc = 1.0f, ss = 0.0f;
+        if (i < a.rot >> 1) turn(a, pos, i, cc, ss);
+        __builtin_amdgcn_wave_barrier();   // after the reads of the one before
+        c[i] = cc;
+        s[i] = ss;
+        __builtin_amdgcn_wave_barrier();
+    }
+};
+
+// The cosines and signed sines of elements d .. d + 7: 1 and 0 past rotary_dim.
 template <bool INTER>
 struct Turn8 {
     float c[8], s[8];
-    __device__ __forceinline__ void make(const RotaryArgs& a, int pos, int d) {
-        const int half = a.rot >> 1;
-        if constexpr (INTER) {
+    __device__ __forceinline__ void take(const TurnLds& l, int d, int rot, bool whole) {
+        const int half = rot >> 1;
+        if (whole) {   // (rotary_dim a multiple of 16: 8 elements lie in one half)
+            if (d >= rot) {
 #pragma unroll
-            for (int e = 0; e < 8; e += 2) {
-                float cc = 1.0f, ss = 0.0f;
-                if (d + e < a.rot) turn(a, pos, (d + e) >> 1, cc, ss);
-                c[e] = c[e + 1] = cc;
-                s[e] = -ss;
-                s[e + 1] = ss;
-            }
-        } else {
-#pragma unroll
-            for (int e = 0; e < 8; ++e) {
-                c[e] = 1.0f;
-                s[e] = 0.0f;
-                if (d + e < a.rot) {
-                    int i, other;
-                    float sign;
-                    pair_of<false>(d + e, half, i, other, sign);
-                    turn(a, pos, i, c[e], s[e]);
-                    s[e] *= sign;
+                for (int e = 0; e < 8; ++e) {
+                    c[e] = 1.0f;
+                    s[e] = 0.0f;
                 }
+            } else if constexpr (INTER) {
+                const f4 cc = *reinterpret_cast<const f4*>(l.c + (d >> 1));
+                const f4 ss = *reinterpret_cast<const f4*>(l.s + (d >> 1));
+#pragma unroll
+                for (int e = 0; e < 8; ++e) {
+                    c[e] = cc[e >> 1];
+                    s[e] = e & 1 ? ss[e >> 1] : -ss[e >> 1];
+                }
+            } else {
+                const bool up = d >= half;
+                const int i = up ? d - half : d;
+#pragma unroll
+                for (int e = 0; e < 8; e += 4) {
+                    const f4 cc = *reinterpret_cast<const f4*>(l.c + i + e);
+                    const f4 ss = *reinterpret_cast<const f4*>(l.s + i + e);
+#pragma unroll
+                    for (int z = 0; z < 4; ++z) {
+                        c[e + z] = cc[z];
+                        s[e + z] = up ? ss[z] : -ss[z];
+                    }
+                }
+            }
+            return;
+        }
+#pragma unroll
+        for (int e = 0; e < 8; ++e) {
+            c[e] = 1.0f;
+            s[e] = 0.0f;
+            if (d + e < rot) {
+                int i, other;
+                float sign;
+                pair_of<INTER>(d + e, half, i, other, sign);
+                c[e] = l.c[i];
+                s[e] = l.s[i] * sign;
             }
         }
     }
@@ -171,7 +204,14 @@ struct RowSrc {
     int row0;
     bool is_v;
     bool wide;
+    TurnLds* lds;             // two of this wave: the tokens of its lower and upper lanes
+    int pos;                  // of token t0 + lane
     __device__ __forceinline__ int slot(int t) const { return a.positions[t] < 0 ? -1 : a.slots[t]; }
+    __device__ __forceinline__ void before(int k) const {
+        if (is_v) return;
+        lds[0].make(a, __builtin_amdgcn_readlane(pos, __builtin_amdgcn_readlane(k, 0) & 63));
+        lds[1].make(a, __builtin_amdgcn_readlane(pos, __builtin_amdgcn_readlane(k, 63) & 63));
+    }
     __device__ __forceinline__ uint16_t one(int t, int i) const {
         const uint16_t* const p = rows + t * stride + row0 + i;
         const int d = (row0 + i) & (a.D - 1);
@@ -195,7 +235,7 @@ struct RowSrc {
         }
         const int d = (row0 + i) & (a.D - 1);
         Turn8<INTER> r;
-        r.make(a, a.positions[t], d);
+        r.take(lds[(threadIdx.x >> 5) & 1], d, a.rot, a.whole);
         load8<INTER>(p - d, d, a.rot, wide, x, y);
         return rotate8<T, INTER>(r, x, y, d, a.rot);
     }
@@ -204,46 +244,56 @@ struct RowSrc {
 template <typename T, bool INTER, int W>
 __global__ __launch_bounds__(256) void rotary_and_cache_kernel(const RotaryArgs a) {
     __shared__ __align__(16) uint16_t tile[(W + kBlockTokens - 1) * kWinStride];
-    const int kv = a.windows * a.slices;
-    if (blockIdx.x < 2u * kv) {
-        const bool is_v = blockIdx.x >= static_cast<unsigned>(kv);
-        const int i = blockIdx.x - (is_v ? kv : 0);
-        const int slice = i / a.windows;
-        const int row0 = slice * kWinRows;
+    __shared__ __align__(16) TurnLds s_turn[4][2];
+    TurnLds* const lds = s_turn[__builtin_amdgcn_readfirstlane(threadIdx.x >> 6)];
+    const int lane = threadIdx.x & 63;
+    const int pieces = 2 * a.slices;   // of a window: its slices of K, then of V
+    const int kv = a.windows * pieces;
+    if (blockIdx.x < static_cast<unsigned>(kv)) {
+        const int piece = blockIdx.x / a.windows;
+        const int t0 = (blockIdx.x - piece * a.windows) * W;
+        const bool is_v = piece >= a.slices;
+        const int row0 = (is_v ? piece - a.slices : piece) * kWinRows;
+        const int pos = a.positions[min(t0 + lane, a.T - 1)];
         const RowSrc<T, INTER> src{a, is_v ? a.v : a.k, is_v ? a.v_stride : a.k_stride, row0, is_v,
-                                   is_v ? a.wide_v : a.wide_k};
-        write_runs<W>(src, is_v ? a.vc : a.kc, tile, (i - slice * a.windows) * W, row0, a.Hkv * a.D, a.T, a.num_slots);
+                                   is_v ? a.wide_v : a.wide_k, lds, pos};
+        write_runs<W>(src, is_v ? a.vc : a.kc, tile, t0, row0, a.Hkv * a.D, a.T, a.num_slots);
         return;
     }
-    // Queries. The lanes of one head at one token are lanes of one wave, and
-    // each has its loads back before any stores: query_out may be query.
-    const int i = blockIdx.x - 2 * kv;
-    const int part = i / a.groups;
-    const int pieces = a.D >> 3;
-    const int t = (i - part * a.groups) * (256 / pieces) + threadIdx.x / pieces;
+    // Queries. A wave takes `each` heads of one token, 1 KB of its row at a
+    // time. The lanes of one head are lanes of one wave, and each has its loads
+    // back before any stores: query_out may be query.
+    const int unit = (blockIdx.x - kv) * 4 + __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    const int t = unit / a.parts;
     if (t >= a.T) return;
     const int pos = a.positions[t];
     if (pos < 0) return;
-    const int d = 8 * (threadIdx.x & (pieces - 1));
-    Turn8<INTER> r;
-    r.make(a, pos, d);
-    const int h1 = min(a.H, (part + 1) * a.each);
+    const int lanes = a.D >> 3;                 // of one head
+    const int d = 8 * (lane & (lanes - 1));
+    const int step = 64 / lanes;
+    const int h0 = (unit - t * a.parts) * a.each + lane / lanes;
+    const int h1 = min(a.H, (unit - t * a.parts + 1) * a.each);
     const uint16_t* const src = a.q + t * a.q_stride;
-    uint16_t* const dst = a.out + static_cast<size_t>(t) * a.H * a.D;
-#pragma unroll 4
-    for (int h = part * a.each; h < h1; ++h) {
-        uint16_t x[8], y[8];
-        load8<INTER>(src + h * a.D, d, a.rot, a.wide_q, x, y);
-        const u4v u = rotate8<T, INTER>(r, x, y, d, a.rot);
-        uint16_t* const o = dst + h * a.D + d;
-        if (a.wide_q) {
-            *reinterpret_cast<u4v*>(o) = u;
-        } else {
-            uint16_t w[8];
-            __builtin_memcpy(w, &u, 16);
-#pragma unroll
-            for (int e = 0; e < 8; ++e) o[e] = w[e];
+    uint16_t* const dst = a.out + static_cast<size_t>(t) * a.H * a.D + d;
+    lds->make(a, pos);
+    Turn8<INTER> r;
+    r.take(*lds, d, a.rot, a.whole);
+    if (a.wide_q) {
+#pragma unroll 8
+        for (int h = h0; h < h1; h += step) {
+            uint16_t x[8], y[8];
+            load8<INTER>(src + h * a.D, d, a.rot, true, x, y);
+            *reinterpret_cast<u4v*>(dst + h * a.D) = rotate8<T, INTER>(r, x, y, d, a.rot);
         }
+        return;
+    }
+    for (int h = h0; h < h1; h += step) {
+        uint16_t x[8], y[8], w[8];
+        load8<INTER>(src + h * a.D, d, a.rot, false, x, y);
+        const u4v u = rotate8<T, INTER>(r, x, y, d, a.rot);
+        __builtin_memcpy(w, &u, 16);
+#pragma unroll
+        for (int e = 0; e < 8; ++e) dst[h * a.D + e] = w[e];
     }
 }
 
@@ -336,17 +386,18 @@ int swiftllm_hip_rotary_and_cache(void* query_out, const void* query, const void
     a.Hkv = num_kv_heads;
     a.D = head_dim;
     a.rot = rotary_dim;
-    const bool whole = rotary_dim % 16 == 0;
-    a.wide_q = whole && aligned(query, 16) && aligned(query_out, 16) && query_stride % 8 == 0;
-    a.wide_k = whole && aligned(key, 16) && key_stride % 8 == 0;
+    a.whole = rotary_dim % 16 == 0;
+    a.wide_q = a.whole && aligned(query, 16) && aligned(query_out, 16) && query_stride % 8 == 0;
+    a.wide_k = a.whole && aligned(key, 16) && key_stride % 8 == 0;
     a.wide_v = aligned(value, 16) && value_stride % 8 == 0;
     a.slices = static_cast<int>((Hkv * D + kWinRows - 1) / kWinRows);
     const int W = small_windows(T, a.slices) ? 4 : 16;
     a.windows = static_cast<int>((T + W - 1) / W);
-    a.each = T > 512 ? num_heads : std::min(num_heads, 4);
-    const long long per = 256 / (D / 8);
-    a.groups = static_cast<int>((T + per - 1) / per);
-    const long long grid = 2LL * a.windows * a.slices + static_cast<long long>(a.groups) * ((H + a.each - 1) / a.each);
+    // Long calls have a wave per token; short ones are latency, and split them.
+    const int step = static_cast<int>(512 / D);
+    a.each = T > 512 ? num_heads : std::min(num_heads, step);
+    a.parts = (num_heads + a.each - 1) / a.each;
+    const long long grid = 2LL * a.windows * a.slices + (T * a.parts + 3) / 4;
     if (grid >= (1LL << 24)) {
         return fail(SWIFTLLM_ERR_NOT_SUPPORTED, "%s: num_tokens=%d of %d + 2 * %d heads", who, num_tokens, num_heads,
                     num_kv_heads);
