@@ -41,7 +41,7 @@ struct ScoredDecodeArgs {
     const int* ctx;
     const int* qoff;       // [S + 1] or null: row s
     int T;                 // rows, where qoff is given
-    int4* info;            // [ranges]: sequence that is cut at the range's end, its last range
+    int4* info;            // [min(S, ranges)]: a cut sequence, its first and last range
     float* frag_ml;        // [ranges][2][HC][2][gs]
     float* frag_o;         // [ranges][2][HC][gs][D], normalised
     Shape shape;
@@ -64,7 +64,7 @@ constexpr int kLeastRange = 8;
 // The row of a sequence's query and output; negative: it has none.
 __device__ __forceinline__ int row_of(const ScoredDecodeArgs& a, int s) {
     if (a.qoff == nullptr) return s;
-    const int b = a.qoff[s], e = a.qoff[s + 1];
+    const int b = as_const(a.qoff)[s], e = as_const(a.qoff)[s + 1];
     return b >= 0 && e > b && e <= a.T ? e - 1 : -1;
 }
 
@@ -82,9 +82,9 @@ struct Sight {
 
 __device__ __forceinline__ Sight sight_of(const ScoredDecodeArgs& a, int s) {
     Sight v;
-    v.L = row_of(a, s) < 0 ? 0 : min(max(a.ctx[s], 0), a.MB * kBlockTokens);
+    v.L = row_of(a, s) < 0 ? 0 : min(max(as_const(a.ctx)[s], 0), a.MB * kBlockTokens);
     v.low = a.shape.window > 0 ? max(v.L - a.shape.window, 0) : 0;
-    v.pre = a.shape.prefix != nullptr ? min(max(a.shape.prefix[s], 0), v.L) : 0;
+    v.pre = a.shape.prefix != nullptr ? min(max(as_const(a.shape.prefix)[s], 0), v.L) : 0;
     const int first = v.low >> kBlockShift;
     v.before = min((v.pre + kBlockTokens - 1) >> kBlockShift, first);
     v.skip = first - v.before;
@@ -315,9 +315,9 @@ template <typename T, int D>
 __global__ __launch_bounds__(64 * kWaves) __attribute__((amdgpu_waves_per_eu(3)))
 void scored_decode_kernel(const ScoredDecodeArgs a) {
     const int HC = a.Hkv * a.nhc;
-    const int range = blockIdx.x / HC;     // every sequence whole: the sequence
-    const int sub = blockIdx.x - range * HC;
-    const int kvh = sub / a.nhc;
+    const int range = blockIdx.y;          // every sequence whole: the sequence
+    const int sub = blockIdx.x;
+    const int kvh = a.nhc == 1 ? sub : sub / a.nhc;
     const int hc = sub - kvh * a.nhc;
     const int h0 = kvh * a.G + hc * 16;
     const int gs = min(16, a.G);
@@ -361,6 +361,8 @@ void scored_decode_kernel(const ScoredDecodeArgs a) {
         s = __builtin_amdgcn_readfirstlane(s_at[0]);
         begin = __builtin_amdgcn_readfirstlane(s_at[1]);
     }
+    const bool by_seq = a.S < a.ranges;   // what the entries of info belong to
+    const bool teller = a.ranges > 0 && sub == 0 && threadIdx.x == 0;
     int4 cut = int4{-1, 0, 0, 0};
     for (int at = start; at < end;) {
         const Sight sight = sight_of(a, s);
@@ -374,7 +376,11 @@ void scored_decode_kernel(const ScoredDecodeArgs a) {
         const bool whole = at == begin && e == stop;
         // Slot 0: the sequence began in a range before; 1: it begins here.
         const int slot = begin < start ? 0 : 1;
-        if (!whole && slot == 1) cut = int4{s, (stop - 1) / len, 0, 0};
+        if (slot == 1) {
+            const int4 x = whole ? int4{-1, 0, 0, 0} : int4{s, range, (stop - 1) / len, 0};
+            if (!whole) cut = x;
+            if (teller && by_seq) a.info[s] = x;
+        }
         const size_t f = static_cast<size_t>(2 * range + slot) * HC + sub;
         const int row = row_of(a, s);
         run_piece<T, D>(a, sight, s, row, kvh, hc, i0, i1, [&](int g, int d, float o, float m, float l) {
@@ -388,28 +394,30 @@ void scored_decode_kernel(const ScoredDecodeArgs a) {
                 a.frag_ml[f * 2 * gs + gs + g] = l;
             }
         });
-        __syncthreads();  // the merge's LDS is free again
         at = e;
-        if (e == stop) {
-            ++s;
-            begin = stop;
-        }
+        if (at >= end) break;
+        __syncthreads();  // the merge's LDS is free again
+        ++s;              // a piece that ends inside the range ends its sequence
+        begin = stop;
     }
-    if (a.ranges > 0 && sub == 0 && threadIdx.x == 0) a.info[range] = cut;
+    if (teller && !by_seq) a.info[range] = cut;
 }
 
-// Joins the fragments of the sequence that begins in a range and is cut at its
-// end: one workgroup per (range, query head), its waves take the fragments in
-// turn.
+// Joins the fragments of a cut sequence: one workgroup per (entry of info, query
+// head), its waves take the fragments in turn. A lane holds the maximum and the
+// sum of a fragment, and the first rows are on their way before those are there:
+// a join is bound by latency.
+constexpr int kJoinRows = 8;
+
 template <typename T, int D>
 __global__ __launch_bounds__(64 * kWaves) void scored_decode_join_kernel(const ScoredDecodeArgs a) {
     constexpr int DL = D / 64;
     __shared__ float s_o[kWaves][D];
     __shared__ float s_ml[kWaves][2];
-    const int range = blockIdx.y;
     const int h = blockIdx.x;
-    const int4 cut = a.info[range];
-    if (cut.x < 0) return;
+    const const_int* const cut = as_const(reinterpret_cast<const int*>(a.info + blockIdx.y));
+    const int s = cut[0], first = cut[1], last = cut[2];
+    if (s < 0) return;
     const int kvh = h / a.G;
     const int hg = h - kvh * a.G;
     const int HC = a.Hkv * a.nhc;
@@ -417,28 +425,51 @@ __global__ __launch_bounds__(64 * kWaves) void scored_decode_join_kernel(const S
     const int g = hg % 16;
     const int gs = min(16, a.G);
     const int lane = threadIdx.x & 63;
-    const int w = threadIdx.x >> 6;
+    const int w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    // The wave's i-th fragment.
+    const int count = max((last - first - w + kWaves) / kWaves, 0);
+    auto place = [&](int i) {
+        const int x = first + w + kWaves * i;
+        return static_cast<size_t>(2 * x + (x == first)) * HC + sub;
+    };
     float m = -INFINITY, l = 0.0f, o[DL];
 #pragma unroll
     for (int j = 0; j < DL; ++j) o[j] = 0.0f;
-#pragma unroll 4
-    for (int x = range + w; x <= cut.y; x += kWaves) {
-        const size_t f = static_cast<size_t>(2 * x + (x == range)) * HC + sub;
-        const float fm = a.frag_ml[f * 2 * gs + g];
-        const float fl = a.frag_ml[f * 2 * gs + gs + g];
-        const float* const fo = a.frag_o + (f * gs + g) * D + lane * DL;
-        float v[DL];
+    for (int c = 0; c < count; c += 64) {
+        const int n = min(count - c, 64);
+        float v[kJoinRows][DL];
+        auto rows = [&](int i) {
 #pragma unroll
-        for (int j = 0; j < DL; ++j) v[j] = fo[j];
-        // An empty fragment weighs nothing (its output is zero); one of NaN
-        // scores alone has a sum that is NaN.
-        const float mn = fmaxf(m, fm);
-        const float fa = m == -INFINITY ? 1.0f : __builtin_amdgcn_exp2f(m - mn);
-        const float fb = (fm == -INFINITY ? 1.0f : __builtin_amdgcn_exp2f(fm - mn)) * fl;
-        l = l * fa + fb;
+            for (int k = 0; k < kJoinRows; ++k) {
+                if (i + k >= n) break;
+                const float* const p = a.frag_o + (place(c + i + k) * gs + g) * D + lane * DL;
 #pragma unroll
-        for (int j = 0; j < DL; ++j) o[j] = o[j] * fa + v[j] * fb;
-        m = mn;
+                for (int j = 0; j < DL; ++j) v[k][j] = p[j];
+            }
+        };
+        rows(0);
+        const float* const ml = a.frag_ml + place(c + min(lane, n - 1)) * 2 * gs + g;
+        const float fm = lane < n ? ml[0] : -INFINITY;
+        const float fl = lane < n ? ml[gs] : 0.0f;
+        const float top = fmaxf(m, wave_max(fm));
+        const float keep = m == -INFINITY ? 1.0f : __builtin_amdgcn_exp2f(m - top);
+        // An empty fragment has a sum of 0; one of NaN scores alone has NaN.
+        const float weight = (fm == -INFINITY ? 1.0f : __builtin_amdgcn_exp2f(fm - top)) * fl;
+        l = l * keep + wave_sum(weight);
+#pragma unroll
+        for (int j = 0; j < DL; ++j) o[j] *= keep;
+        m = top;
+        for (int i = 0; i < n; i += kJoinRows) {
+            if (i > 0) rows(i);
+#pragma unroll
+            for (int k = 0; k < kJoinRows; ++k) {
+                const float x = __builtin_bit_cast(float, __builtin_amdgcn_readlane(__builtin_bit_cast(int, weight), (i + k) & 63));
+                if (i + k < n) {
+#pragma unroll
+                    for (int j = 0; j < DL; ++j) o[j] += x * v[k][j];
+                }
+            }
+        }
     }
 #pragma unroll
     for (int j = 0; j < DL; ++j) s_o[w][lane * DL + j] = o[j];
@@ -459,7 +490,7 @@ __global__ __launch_bounds__(64 * kWaves) void scored_decode_join_kernel(const S
         num += f * s_o[x][d];
         den += f * s_ml[x][1];
     }
-    const int row = row_of(a, cut.x);
+    const int row = row_of(a, s);
     if (row >= 0) a.out[(static_cast<size_t>(row) * a.H + h) * D + d] = T::down(den == 0.0f ? 0.0f : num / den);
 }
 
@@ -595,10 +626,9 @@ int swiftllm_hip_scored_decode(void* output, void* workspace, size_t workspace_b
     static const K join_kernel[2][2] = {{scored_decode_join_kernel<F16, 64>, scored_decode_join_kernel<F16, 128>},
                                         {scored_decode_join_kernel<BF16, 64>, scored_decode_join_kernel<BF16, 128>}};
     const int t = dtype == SWIFTLLM_HIP_BF16;
-    const long long grid = a.ranges > 0 ? a.ranges * HC : items;
-    rc = launched(launch(main_kernel[t][D == 128], dim3(static_cast<unsigned>(grid)), dim3(64 * kWaves), lds, stream, a), who);
+    rc = launched(launch(main_kernel[t][D == 128], dim3(static_cast<unsigned>(HC), a.ranges > 0 ? a.ranges : S), dim3(64 * kWaves), lds, stream, a), who);
     if (rc != SWIFTLLM_OK || a.ranges == 0) return rc;
-    return launched(launch(join_kernel[t][D == 128], dim3(num_heads, a.ranges), dim3(64 * kWaves), 0, stream, a), who);
+    return launched(launch(join_kernel[t][D == 128], dim3(num_heads, std::min(S, a.ranges)), dim3(64 * kWaves), 0, stream, a), who);
 }
 
 }  // extern "C"
