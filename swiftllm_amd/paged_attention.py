@@ -83,8 +83,8 @@ def check_status(status: int) -> None:
 
 
 def _p(x: Ptr) -> Optional[int]:
-    if x is None:
-        return None
+    if x is None or type(x) is int:
+        return x
     if isinstance(x, (DeviceArray, HostArray)):
         return x.ptr
     return int(x)

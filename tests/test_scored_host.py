@@ -94,7 +94,7 @@ def test_prefill_refuses(kw, code):
 def test_decode_workspace_size():
     n = step.scored_decode_workspace_size(8, 64, 8, 128, 16, 2048)
     # two fragments of 16-byte aligned heads for each of the ranges
-    assert 768 * 2 * 8 * (128 + 2) * 4 <= n < 64 << 20
+    assert 512 * 2 * 8 * (128 + 2) * 4 <= n < 64 << 20
     with pytest.raises(pa.NotSupported):
         step.scored_decode_workspace_size(8, 64, 8, 96, 16, 2048)
     with pytest.raises(pa.InvalidParameter):
