@@ -114,36 +114,16 @@ __device__ __forceinline__ void stage_v(const ScoredPrefillArgs& a, uint16_t* vs
     }
 }
 
-// The K operands of a stage's pair of blocks, and S^T of its 32 keys.
-template <int D>
-__device__ __forceinline__ void read_k(s8 (&k)[D / 16], const uint16_t* kl) {
+// S^T of the 32 keys of a stage's pair of blocks.
+template <typename T, int D>
+__device__ __forceinline__ void qk_pair(f16x& sc, const uint16_t* kl, const s8 (&q)[D / 16]) {
+    sc = f16x{};
 #pragma unroll
     for (int J = 0; J < D / 16; ++J) {
         const uint16_t* p = kl + 256 * J;
-        k[J] = join8(__builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s4*)(const_cast<uint16_t*>(p))),
-                     __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s4*)(const_cast<uint16_t*>(p + 64))));
-    }
-}
-template <typename T, int D>
-__device__ __forceinline__ void qk_pair(f16x& sc, const s8 (&k)[D / 16], const s8 (&q)[D / 16]) {
-    sc = f16x{};
-#pragma unroll
-    for (int J = 0; J < D / 16; ++J) sc = T::mfma32(k[J], q[J], sc);
-}
-template <int D>
-__device__ __forceinline__ void read_v(s8 (&v)[D / 32], const uint16_t* vl) {
-#pragma unroll
-    for (int i = 0; i < D / 32; ++i) v[i] = *reinterpret_cast<const s8*>(vl + 512 * i);
-}
-// The order of the instructions of a stage: nothing crosses a fence, and `among`
-// puts N products between groups of EACH other vector operations.
-__device__ __forceinline__ void fence() { __builtin_amdgcn_sched_barrier(0); }
-template <int N, int EACH>
-__device__ __forceinline__ void among() {
-#pragma unroll
-    for (int i = 0; i < N; ++i) {
-        __builtin_amdgcn_sched_group_barrier(0x8, 1, 0);
-        __builtin_amdgcn_sched_group_barrier(0x402, EACH, 0);
+        const s4 x = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s4*)(const_cast<uint16_t*>(p)));
+        const s4 y = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s4*)(const_cast<uint16_t*>(p + 64)));
+        sc = T::mfma32(join8(x, y), q[J], sc);
     }
 }
 
@@ -467,11 +447,8 @@ void scored_prefill_kernel(const ScoredPrefillArgs a) {
     }
     __syncthreads();
     f16x sc[2];
-    s8 kr[NJ], vr[2][ND];   // operands on their way from LDS
-    read_k<D>(kr, s_k[0] + koff);
-    qk_pair<T, D>(sc[0], kr, q);
-    read_k<D>(kr, s_k[0] + koff + St::kPair);
-    qk_pair<T, D>(sc[1], kr, q);
+    qk_pair<T, D>(sc[0], s_k[0] + koff, q);
+    qk_pair<T, D>(sc[1], s_k[0] + koff + St::kPair, q);
     __syncthreads();
     for (int t = 0; t < nsteps; ++t) {
         const bool more = t + 1 < nsteps;
@@ -482,12 +459,6 @@ void scored_prefill_kernel(const ScoredPrefillArgs a) {
                 stage_k<D>(a, s_k[t & 1], w, b_2, kvh, lane);
             }
         }
-        const uint16_t* const next = s_k[(t + 1) & 1] + koff;
-        const uint16_t* const vl = s_v[t & 1] + 8 * lane;
-        const u4 bad = *reinterpret_cast<const u4*>(s_bad[t & 1]);
-        read_v<D>(vr[0], vl);
-        read_k<D>(kr, next);
-        fence();
         const int base = kStage * stage_of(t);
         const int end = base + kStage - 1;
         // Whether every row of the wave sees every key of the stage, none of them
@@ -566,6 +537,7 @@ void scored_prefill_kernel(const ScoredPrefillArgs a) {
             m = m_new;
         }
         const float c = ((m == -INFINITY) ? 0.0f : m) - kWeightExp;
+        const u4 bad = *reinterpret_cast<const u4*>(s_bad[t & 1]);
         if (__builtin_amdgcn_readfirstlane(bad[0] | bad[1] | bad[2] | bad[3]) != 0) [[unlikely]] {
             unsigned keys = 0;   // this lane's, as `seen`
 #pragma unroll
@@ -573,10 +545,12 @@ void scored_prefill_kernel(const ScoredPrefillArgs a) {
             if (seen & keys) l = __builtin_nanf("");
         }
         // Weights, O^T += V P^T, and the next stage's scores in the place of the
-        // pair's that are used up, without a branch: the products of a block run
-        // among the weights of the next, their operands read a block ahead. (Behind
-        // the last stage scores are made of what lies in the buffer, and not used.)
-        auto weights = [&](int b) {
+        // pair's that are used up, without a branch, so that the products run
+        // among the weights. (Behind the last stage they are made of what lies in
+        // the buffer, and not used.)
+        const uint16_t* const next = s_k[(t + 1) & 1] + koff;
+#pragma unroll
+        for (int b = 0; b < 4; ++b) {
             u4 pp;
 #pragma unroll
             for (int i = 0; i < 4; ++i) {
@@ -589,35 +563,13 @@ void scored_prefill_kernel(const ScoredPrefillArgs a) {
                 pp[i] = T::down2(p[0], p[1]);
                 l = add_pair(T{}, pp[i], l);
             }
-            return __builtin_bit_cast(s8, pp);
-        };
-        auto weigh = [&](int b, s8 p) {
+            const uint16_t* const vl = s_v[t & 1] + b * St::kTile + 8 * lane;
 #pragma unroll
-            for (int i = 0; i < ND; ++i) acc[i] = T::mfma32(vr[b & 1][i], p, acc[i]);
-        };
-        s8 p0 = weights(0);
-        read_v<D>(vr[1], vl + St::kTile);
-        fence();
-        weigh(0, p0);
-        s8 p1 = weights(1);
-        among<ND, 24 / ND>();
-        fence();
-        read_v<D>(vr[0], vl + 2 * St::kTile);
-        fence();
-        weigh(1, p1);
-        qk_pair<T, D>(sc[0], kr, q);
-        p0 = weights(2);
-        among<ND + NJ, 24 / (ND + NJ)>();
-        fence();
-        read_v<D>(vr[1], vl + 3 * St::kTile);
-        read_k<D>(kr, next + St::kPair);
-        fence();
-        weigh(2, p0);
-        p1 = weights(3);
-        among<ND, 24 / ND>();
-        fence();
-        weigh(3, p1);
-        qk_pair<T, D>(sc[1], kr, q);
+            for (int i = 0; i < ND; ++i) {
+                acc[i] = T::mfma32(*reinterpret_cast<const s8*>(vl + 512 * i), __builtin_bit_cast(s8, pp), acc[i]);
+            }
+            if (b & 1) qk_pair<T, D>(sc[b >> 1], next + (b >> 1) * St::kPair, q);
+        }
         if (more) {
             wait_vm<0>();
             landed(t + 1, ok_1);
