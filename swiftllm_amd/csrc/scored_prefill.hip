@@ -87,14 +87,15 @@ struct Stage {
     static constexpr int kV = 4 * kTile;
 };
 
-__device__ __forceinline__ __amdgpu_buffer_rsrc_t tile_rsrc(const uint16_t* cache, int b, int kvh, int Hkv, int D) {
-    return __builtin_amdgcn_make_buffer_rsrc(const_cast<uint16_t*>(cache + kv_tile_offset(b, kvh, Hkv, D)), 0,
-                                             D * kBlockTokens * 2, kRsrcWord3);
+// A block's tile of one kv head, `off` elements into its cache; with no bytes
+// there is nothing to load.
+__device__ __forceinline__ __amdgpu_buffer_rsrc_t tile_rsrc(const uint16_t* cache, size_t off, int bytes) {
+    return __builtin_amdgcn_make_buffer_rsrc(const_cast<uint16_t*>(cache + off), 0, bytes, kRsrcWord3);
 }
 
 template <int D>
-__device__ __forceinline__ void stage_k(const ScoredPrefillArgs& a, uint16_t* ks, int w, int b, int kvh, int lane) {
-    const __amdgpu_buffer_rsrc_t rk = tile_rsrc(a.kc, b, kvh, a.Hkv, D);
+__device__ __forceinline__ void stage_k(const ScoredPrefillArgs& a, uint16_t* ks, int w, size_t off, int bytes, int lane) {
+    const __amdgpu_buffer_rsrc_t rk = tile_rsrc(a.kc, off, bytes);
     uint16_t* const k = ks + (w >> 1) * Stage<D>::kPair + (w & 1) * Stage<D>::kOdd;
 #pragma unroll
     for (int i = 0; i < D / 32; ++i) {
@@ -104,8 +105,8 @@ __device__ __forceinline__ void stage_k(const ScoredPrefillArgs& a, uint16_t* ks
 
 // Each 32-row piece's 16-byte chunks: the rows' first 8 tokens, then their last 8.
 template <int D>
-__device__ __forceinline__ void stage_v(const ScoredPrefillArgs& a, uint16_t* vs, int w, int b, int kvh, int lane) {
-    const __amdgpu_buffer_rsrc_t rv = tile_rsrc(a.vc, b, kvh, a.Hkv, D);
+__device__ __forceinline__ void stage_v(const ScoredPrefillArgs& a, uint16_t* vs, int w, size_t off, int bytes, int lane) {
+    const __amdgpu_buffer_rsrc_t rv = tile_rsrc(a.vc, off, bytes);
     uint16_t* const v = vs + w * Stage<D>::kTile;
     const unsigned vo = 32u * (lane & 31) + 16u * (lane >> 5);
 #pragma unroll
@@ -375,6 +376,16 @@ void scored_prefill_kernel(const ScoredPrefillArgs a) {
     const int skip = low - before;
     const int nsteps = tp1 < 0 || last < 0 ? 0 : before + max(last / kStage - low + 1, 0);
     auto stage_of = [&](int t) { return t < before ? t : t + skip; };
+    // First keys of the stages that every row of the wave sees whole, none of
+    // them ahead of the row where the distance counts: from w0 to w1, and to w2
+    // in the prefix. The same for the tile's rows.
+    const bool wave_rows = wp0 >= 0 && wp0 <= wp1;
+    const int w0 = max(wp1 - min(window, wp1 + 1) + 1, 0);
+    const int w1 = wave_rows ? min(wp0, L - 1) - (kStage - 1) : -1;
+    const int w2 = wave_rows ? (BIAS ? min(pre, wp0 + 1) : pre) - kStage : -1;
+    const int t0 = max(tp1 - min(window, tp1 + 1) + 1, 0);
+    const int t1 = tp0 >= 0 ? min(tp0, L - 1) - (kStage - 1) : -1;
+    const int t2 = tp0 >= 0 ? pre - kStage : -1;
 
     // (zeros behind an empty asm: 16 of them would be kept over the tiles)
     float zero = 0.0f;
@@ -411,62 +422,47 @@ void scored_prefill_kernel(const ScoredPrefillArgs a) {
             q[J] = __builtin_bit_cast(s8, (v & keep) ^ flip);
         }
     }
-    // Block of this wave in stage t of the walk (asked for in order) and, in
-    // ok4, which of the stage's four blocks are in the pool.
-    auto block_of = [&](int t, int& ok4) {
-        if (t > 0 && (t & 15) == 0) {
-            ids = ids_next;
-            ids_next = chunk_ids((t >> 4) + 1);
-        }
+    // Tile of this wave in stage t of the walk (16 stages per load of ids) and,
+    // in ok4, which of the stage's four blocks are in the pool.
+    auto tile_of = [&](int t, int& ok4) {
         const unsigned long long okm = __ballot(block_known(ids, a.num_blocks));
         const int at = 4 * (t & 15);
         ok4 = static_cast<int>((okm >> at) & 15ull);
-        const int b = __builtin_amdgcn_readlane(ids, at + w);
-        return block_known(b, a.num_blocks) ? b : 0;
+        const int b = (ok4 >> w) & 1 ? __builtin_amdgcn_readlane(ids, at + w) : 0;
+        return kv_tile_offset(b, kvh, a.Hkv, D);
     };
-    // This wave's block of stage t of the walk has landed in its V buffer.
+    auto bytes_of = [&](int t) { return t < nsteps ? D * kBlockTokens * 2 : 0; };
+    // This wave's block of stage t of the walk has landed in its V buffer: true
+    // if some row of the tile may not see the stage whole.
     auto landed = [&](int t, int ok4) {
         const int base = kStage * stage_of(t);
-        const int end = base + kStage - 1;
-        unsigned bad = 0;
-        if (tp0 < end || end >= L || ok4 != 15 || (end >= pre && tp1 - base >= window)) bad = clean_v<T, D>(s_v[t & 1], w, lane);
+        if (t >= nsteps || (ok4 == 15 && ((base >= t0 && base <= t1) || base <= t2))) return false;
+        const unsigned bad = clean_v<T, D>(s_v[t & 1], w, lane);
         if (lane == 0) s_bad[t & 1][w] = bad;
+        return true;
     };
-    int ok_t, ok_1 = 15, ok_2 = 15;  // of stages t, t + 1 and t + 2
-    int b_1 = 0, b_2 = 0;
-    {
-        const int b = block_of(0, ok_t);
-        stage_k<D>(a, s_k[0], w, b, kvh, lane);
-        stage_v<D>(a, s_v[0], w, b, kvh, lane);
-        if (nsteps > 1) {
-            b_1 = block_of(1, ok_1);
-            stage_k<D>(a, s_k[1], w, b_1, kvh, lane);
-        }
-        wait_vm<0>();
-        landed(0, ok_t);
-    }
+    int ok_t, ok_1;                  // of stages t and t + 1
+    const size_t off = tile_of(0, ok_t);
+    stage_k<D>(a, s_k[0], w, off, bytes_of(0), lane);
+    stage_v<D>(a, s_v[0], w, off, bytes_of(0), lane);
+    size_t off_1 = tile_of(1, ok_1);
+    stage_k<D>(a, s_k[1], w, off_1, bytes_of(1), lane);
+    wait_vm<0>();
+    bool cleaned = landed(0, ok_t);  // stage t
     __syncthreads();
     f16x sc[2];
     qk_pair<T, D>(sc[0], s_k[0] + koff, q);
     qk_pair<T, D>(sc[1], s_k[0] + koff + St::kPair, q);
     __syncthreads();
     for (int t = 0; t < nsteps; ++t) {
-        const bool more = t + 1 < nsteps;
-        if (more) {
-            stage_v<D>(a, s_v[(t + 1) & 1], w, b_1, kvh, lane);
-            if (t + 2 < nsteps) {
-                b_2 = block_of(t + 2, ok_2);
-                stage_k<D>(a, s_k[t & 1], w, b_2, kvh, lane);
-            }
-        }
+        int ok_2;
+        stage_v<D>(a, s_v[(t + 1) & 1], w, off_1, bytes_of(t + 1), lane);
+        off_1 = tile_of(t + 2, ok_2);
+        stage_k<D>(a, s_k[t & 1], w, off_1, bytes_of(t + 2), lane);
         const int base = kStage * stage_of(t);
-        const int end = base + kStage - 1;
-        // Whether every row of the wave sees every key of the stage, none of them
-        // ahead of the row where the distance counts. (One copy of the stage with
-        // scalar branches: two copies, with and without masks, took 100 more
-        // registers for the sums that they hand each other.)
-        const bool behind = end <= wp0 && (end < pre || wp1 - base < window);
-        const bool whole = wp0 >= 0 && wp0 <= wp1 && ok_t == 15 && end < L && (behind || (!BIAS && end < pre));
+        // (One copy of the stage with scalar branches: two copies, with and without
+        // masks, took 100 more registers for the sums that they hand each other.)
+        const bool whole = ok_t == 15 && ((base >= w0 && base <= w1) || base <= w2);
         // Score i of pair p: key base + 32 p + 16 (i / 8) + 8 h + i % 8; bit
         // 16 p + i of `seen` whether this row sees it.
         unsigned seen = ~0u;
@@ -537,8 +533,8 @@ void scored_prefill_kernel(const ScoredPrefillArgs a) {
             m = m_new;
         }
         const float c = ((m == -INFINITY) ? 0.0f : m) - kWeightExp;
-        const u4 bad = *reinterpret_cast<const u4*>(s_bad[t & 1]);
-        if (__builtin_amdgcn_readfirstlane(bad[0] | bad[1] | bad[2] | bad[3]) != 0) [[unlikely]] {
+        if (cleaned) {
+            const u4 bad = *reinterpret_cast<const u4*>(s_bad[t & 1]);
             unsigned keys = 0;   // this lane's, as `seen`
 #pragma unroll
             for (int b = 0; b < 4; ++b) keys |= ((bad[b] >> (8 * h)) & 0xffu) << (8 * b);
@@ -546,8 +542,7 @@ void scored_prefill_kernel(const ScoredPrefillArgs a) {
         }
         // Weights, O^T += V P^T, and the next stage's scores in the place of the
         // pair's that are used up, without a branch, so that the products run
-        // among the weights. (Behind the last stage they are made of what lies in
-        // the buffer, and not used.)
+        // among the weights. (Behind the last stage they are not used.)
         const uint16_t* const next = s_k[(t + 1) & 1] + koff;
 #pragma unroll
         for (int b = 0; b < 4; ++b) {
@@ -570,14 +565,15 @@ void scored_prefill_kernel(const ScoredPrefillArgs a) {
             }
             if (b & 1) qk_pair<T, D>(sc[b >> 1], next + (b >> 1) * St::kPair, q);
         }
-        if (more) {
-            wait_vm<0>();
-            landed(t + 1, ok_1);
-            ok_t = ok_1;
-            ok_1 = ok_2;
-            b_1 = b_2;
-            __syncthreads();
+        wait_vm<0>();
+        cleaned = landed(t + 1, ok_1);
+        ok_t = ok_1;
+        ok_1 = ok_2;
+        if (((t + 3) & 15) == 0) {
+            ids = ids_next;
+            ids_next = chunk_ids(((t + 3) >> 4) + 1);
         }
+        __syncthreads();
     }
     }
 
