@@ -115,16 +115,20 @@ __device__ __forceinline__ void stage_v(const ScoredPrefillArgs& a, uint16_t* vs
     }
 }
 
+// Row operand of K: 16 rows of a pair of blocks.
+__device__ __forceinline__ s8 k_rows(const uint16_t* p) {
+    const s4 x = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s4*)(const_cast<uint16_t*>(p)));
+    const s4 y = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s4*)(const_cast<uint16_t*>(p + 64)));
+    return join8(x, y);
+}
+
 // S^T of the 32 keys of a stage's pair of blocks.
 template <typename T, int D>
 __device__ __forceinline__ void qk_pair(f16x& sc, const uint16_t* kl, const s8 (&q)[D / 16]) {
     sc = f16x{};
 #pragma unroll
     for (int J = 0; J < D / 16; ++J) {
-        const uint16_t* p = kl + 256 * J;
-        const s4 x = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s4*)(const_cast<uint16_t*>(p)));
-        const s4 y = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s4*)(const_cast<uint16_t*>(p + 64)));
-        sc = T::mfma32(join8(x, y), q[J], sc);
+        sc = T::mfma32(k_rows(kl + 256 * J), q[J], sc);
     }
 }
 
@@ -383,6 +387,7 @@ void scored_prefill_kernel(const ScoredPrefillArgs a) {
     const int w0 = max(wp1 - min(window, wp1 + 1) + 1, 0);
     const int w1 = wave_rows ? min(wp0, L - 1) - (kStage - 1) : -1;
     const int w2 = wave_rows ? (BIAS ? min(pre, wp0 + 1) : pre) - kStage : -1;
+    const int last_seen = max(wp1 < wp0 ? -1 : min(wp1, L - 1), pre - 1);
     const int t0 = max(tp1 - min(window, tp1 + 1) + 1, 0);
     const int t1 = tp0 >= 0 ? min(tp0, L - 1) - (kStage - 1) : -1;
     const int t2 = tp0 >= 0 ? pre - kStage : -1;
@@ -454,12 +459,21 @@ void scored_prefill_kernel(const ScoredPrefillArgs a) {
     qk_pair<T, D>(sc[0], s_k[0] + koff, q);
     qk_pair<T, D>(sc[1], s_k[0] + koff + St::kPair, q);
     __syncthreads();
+    const float scale = a.shape.scale;
+    const float cap = a.shape.cap;
+    auto cap_part = [&](float x) { return __builtin_amdgcn_rcpf(__builtin_amdgcn_exp2f(x * scale) + 1.0f); };
+    if constexpr (CAP) {
+#pragma unroll
+        for (int i = 0; i < 16; ++i) sc[0][i] = cap_part(sc[0][i]);
+    }
     for (int t = 0; t < nsteps; ++t) {
         int ok_2;
         stage_v<D>(a, s_v[(t + 1) & 1], w, off_1, bytes_of(t + 1), lane);
         off_1 = tile_of(t + 2, ok_2);
         stage_k<D>(a, s_k[t & 1], w, off_1, bytes_of(t + 2), lane);
         const int base = kStage * stage_of(t);
+        // (The walk's stages behind the wave's last row are hidden from it.)
+        if (base <= last_seen) {
         // (One copy of the stage with scalar branches: two copies, with and without
         // masks, took 100 more registers for the sums that they hand each other.)
         const bool whole = ok_t == 15 && ((base >= w0 && base <= w1) || base <= w2);
@@ -478,8 +492,6 @@ void scored_prefill_kernel(const ScoredPrefillArgs a) {
                 if ((ok_t >> b) & 1) seen |= bits << (8 * b);
             }
         }
-        const float scale = a.shape.scale;
-        const float cap = a.shape.cap;
         if constexpr (CAP || BIAS) {
             // Scores in the products' place: key i lies d0 + off from the row, and
             // d0 + off <= 0 in a whole stage.
@@ -491,8 +503,7 @@ void scored_prefill_kernel(const ScoredPrefillArgs a) {
                     const float x = sc[i >> 4][i & 15];
                     const float bias = bias_of(static_cast<float>(16 * (i >> 3) + (i & 7)));
                     if constexpr (CAP) {
-                        const float u = __builtin_amdgcn_rcpf(__builtin_amdgcn_exp2f(x * scale) + 1.0f);
-                        sc[i >> 4][i & 15] = __builtin_fmaf(u, -2.0f * cap, bias);
+                        sc[i >> 4][i & 15] = __builtin_fmaf(i < 16 ? x : cap_part(x), -2.0f * cap, bias);
                     } else {
                         sc[i >> 4][i & 15] = __builtin_fmaf(x, scale, bias);
                     }
@@ -541,29 +552,62 @@ void scored_prefill_kernel(const ScoredPrefillArgs a) {
             if (seen & keys) l = __builtin_nanf("");
         }
         // Weights, O^T += V P^T, and the next stage's scores in the place of the
-        // pair's that are used up, without a branch, so that the products run
-        // among the weights. (Behind the last stage they are not used.)
+        // pair's that are used up: two blocks' products, a pair's scores, and both
+        // again, in this order, so that nothing waits for its operands or leaves
+        // the matrix unit alone. A product's operand is read kAhead products
+        // before, and among the products go the weights of the blocks to come and
+        // what a cap makes of the next stage's first pair. (Behind the last stage
+        // the scores are not used.)
         const uint16_t* const next = s_k[(t + 1) & 1] + koff;
+        const uint16_t* const vl = s_v[t & 1] + 8 * lane;
+        u4 pw[4];
+        auto weights = [&](int k) {   // the k-th pair of them
+            const int b = k >> 2, i = k & 3;
+            float p[2];
 #pragma unroll
-        for (int b = 0; b < 4; ++b) {
-            u4 pp;
+            for (int z = 0; z < 2; ++z) {
+                const float v = sc[b >> 1][8 * (b & 1) + 2 * i + z];
+                p[z] = __builtin_amdgcn_exp2f(CAP || BIAS ? v - c : __builtin_fmaf(v, scale, -c));
+            }
+            pw[b][i] = T::down2(p[0], p[1]);
+            l = add_pair(T{}, pw[b][i], l);
+        };
+        constexpr int kHalf = 2 * ND + NJ;
+        constexpr int kAhead = 4;
+        auto operand = [&](int n) {
+            const int half = n / kHalf, k = n % kHalf;
+            if (k < 2 * ND) return *reinterpret_cast<const s8*>(vl + (2 * half + k / ND) * St::kTile + 512 * (k % ND));
+            return k_rows(next + half * St::kPair + 256 * (k - 2 * ND));
+        };
+        s8 ring[kAhead];
 #pragma unroll
-            for (int i = 0; i < 4; ++i) {
-                float p[2];
+        for (int n = 0; n < kAhead; ++n) ring[n] = operand(n);
 #pragma unroll
-                for (int z = 0; z < 2; ++z) {
-                    const float v = sc[b >> 1][8 * (b & 1) + 2 * i + z];
-                    p[z] = __builtin_amdgcn_exp2f(CAP || BIAS ? v - c : __builtin_fmaf(v, scale, -c));
+        for (int k = 0; k < 4; ++k) weights(k);
+        __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+        for (int n = 0; n < 2 * kHalf; ++n) {
+            const int half = n / kHalf, k = n % kHalf;
+            const s8 x = ring[n % kAhead];
+            if (n + kAhead < 2 * kHalf) ring[n % kAhead] = operand(n + kAhead);
+            if (k < 2 * ND) {
+                const int b = 2 * half + k / ND;
+                acc[k % ND] = T::mfma32(x, __builtin_bit_cast(s8, pw[b]), acc[k % ND]);
+            } else {
+                sc[half] = T::mfma32(x, q[k - 2 * ND], k == 2 * ND ? f16x{} : sc[half]);
+            }
+            if (half == 0) {
+#pragma unroll
+                for (int i = 4 + k * 4 / ND; i < 4 + (k + 1) * 4 / ND; ++i) {
+                    if (i < 12) weights(i);
                 }
-                pp[i] = T::down2(p[0], p[1]);
-                l = add_pair(T{}, pp[i], l);
-            }
-            const uint16_t* const vl = s_v[t & 1] + b * St::kTile + 8 * lane;
+                if (k >= 2 * ND && k < 2 * ND + 4) weights(12 + k - 2 * ND);
+            } else if (CAP) {
 #pragma unroll
-            for (int i = 0; i < ND; ++i) {
-                acc[i] = T::mfma32(*reinterpret_cast<const s8*>(vl + 512 * i), __builtin_bit_cast(s8, pp), acc[i]);
+                for (int i = k * 16 / kHalf; i < (k + 1) * 16 / kHalf; ++i) sc[0][i] = cap_part(sc[0][i]);
             }
-            if (b & 1) qk_pair<T, D>(sc[b >> 1], next + (b >> 1) * St::kPair, q);
+            __builtin_amdgcn_sched_barrier(0);
+        }
         }
         wait_vm<0>();
         cleaned = landed(t + 1, ok_1);
