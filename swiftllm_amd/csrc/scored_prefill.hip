@@ -16,13 +16,21 @@
 // XCD its own kv heads, so that a kv head's K and V are read through one L2.
 //
 // Scores. The masks and the two-sided distance are worked out only in stages
-// that some row of the wave does not see whole. A capped score is
-// c - 2 c / (1 + e^y) with y = 2 x / c: its maximum is that of x, so the
-// running maximum is found on the raw products and costs one capped score a
-// row; three transcendental operations a score (exp2, rcp, exp2) and the
-// subtraction of the maximum folded into the last multiply-add.
+// that some row of the wave does not see whole, and a wave leaves out the
+// stages behind its last row. A capped score is c - 2 c u with
+// u = 1 / (1 + e^y), y = 2 x / c: two transcendental operations, a third for
+// the weight. Without a bias the score itself is not made: the largest comes
+// from the least u, and the weight is exp2 of one multiply-add of u.
 // Weights are rounded to 16 bits, to nearest, and summed as rounded: the
 // output's error is that of its own rounding and one of the same size.
+//
+// Order. What a stage costs a wave beside its 32 products (D = 128) is 70 to
+// 130 vector operations for its 32 scores a lane, so the order of both is
+// fixed: products of two blocks' values, both pairs' next scores, the other
+// two blocks' values, each operand read two products ahead (2, 3, 4, 6 and 8
+// took the same time, left to the compiler 8 x 2048 tokens with a cap took 4 %
+// longer and 2048 tokens alone 14 %), with the weights still to come and the
+// caps' parts of the next scores among them.
 //
 // A weight of 0 times a value that is not finite is NaN. So in a stage that
 // some row of the tile does not see whole, such values become zeros in LDS, and
@@ -462,9 +470,15 @@ void scored_prefill_kernel(const ScoredPrefillArgs a) {
     const float scale = a.shape.scale;
     const float cap = a.shape.cap;
     auto cap_part = [&](float x) { return __builtin_amdgcn_rcpf(__builtin_amdgcn_exp2f(x * scale) + 1.0f); };
+    // Without a bias what scores are made of keeps its place: they are it times
+    // mul, plus add. They fall as a cap's part grows.
+    constexpr float kHidden = CAP && !BIAS ? INFINITY : -INFINITY;
+    const float mul = CAP ? -2.0f * cap : scale;
+    const float add = CAP ? cap : 0.0f;
+    auto most = [](float x, float y) { return CAP && !BIAS ? fminf(x, y) : fmaxf(x, y); };
     if constexpr (CAP) {
 #pragma unroll
-        for (int i = 0; i < 16; ++i) sc[0][i] = cap_part(sc[0][i]);
+        for (int i = 0; i < 32; ++i) sc[i >> 4][i & 15] = cap_part(sc[i >> 4][i & 15]);
     }
     for (int t = 0; t < nsteps; ++t) {
         int ok_2;
@@ -492,26 +506,19 @@ void scored_prefill_kernel(const ScoredPrefillArgs a) {
                 if ((ok_t >> b) & 1) seen |= bits << (8 * b);
             }
         }
-        if constexpr (CAP || BIAS) {
-            // Scores in the products' place: key i lies d0 + off from the row, and
-            // d0 + off <= 0 in a whole stage.
+        if constexpr (BIAS) {
+            // Scores in the place of what they are made of: key i lies d0 + off from
+            // the row, and d0 + off <= 0 in a whole stage.
             const float d0 = static_cast<float>(base + 8 * h - pos);
-            const float b0 = BIAS ? __builtin_fmaf(slope, d0, CAP ? cap : 0.0f) : cap;
+            const float b0 = __builtin_fmaf(slope, d0, CAP ? cap : 0.0f);
             auto score = [&](auto bias_of) {
 #pragma unroll
                 for (int i = 0; i < 32; ++i) {
-                    const float x = sc[i >> 4][i & 15];
                     const float bias = bias_of(static_cast<float>(16 * (i >> 3) + (i & 7)));
-                    if constexpr (CAP) {
-                        sc[i >> 4][i & 15] = __builtin_fmaf(i < 16 ? x : cap_part(x), -2.0f * cap, bias);
-                    } else {
-                        sc[i >> 4][i & 15] = __builtin_fmaf(x, scale, bias);
-                    }
+                    sc[i >> 4][i & 15] = __builtin_fmaf(sc[i >> 4][i & 15], CAP ? -2.0f * cap : scale, bias);
                 }
             };
-            if constexpr (!BIAS) {
-                score([&](float) { return cap; });
-            } else if (whole) {
+            if (whole) {
                 score([&](float off) { return __builtin_fmaf(slope, off, b0); });
             } else {
                 score([&](float off) { return __builtin_fmaf(-slope, __builtin_fabsf(d0 + off), CAP ? cap : 0.0f); });
@@ -523,18 +530,18 @@ void scored_prefill_kernel(const ScoredPrefillArgs a) {
                 const int keep = __builtin_amdgcn_sbfe(static_cast<int>(seen), i, 1);  // 0 or -1
                 const float x = sc[i >> 4][i & 15];   // (a bit cast of the element itself takes element 0)
                 const int v = __builtin_bit_cast(int, x);
-                sc[i >> 4][i & 15] = __builtin_bit_cast(float, (v & keep) | (__builtin_bit_cast(int, -INFINITY) & ~keep));
+                sc[i >> 4][i & 15] = __builtin_bit_cast(float, (v & keep) | (__builtin_bit_cast(int, kHidden) & ~keep));
             }
         }
-        float bm = fmaxf(fmaxf(sc[0][0], sc[0][1]), sc[0][2]);
+        float bm = most(most(sc[0][0], sc[0][1]), sc[0][2]);
 #pragma unroll
-        for (int i = 3; i < 31; i += 2) bm = fmaxf(fmaxf(bm, sc[i >> 4][i & 15]), sc[(i + 1) >> 4][(i + 1) & 15]);
-        bm = fmaxf(bm, sc[1][15]);
+        for (int i = 3; i < 31; i += 2) bm = most(most(bm, sc[i >> 4][i & 15]), sc[(i + 1) >> 4][(i + 1) & 15]);
+        bm = most(bm, sc[1][15]);
         {
             const auto y = __builtin_amdgcn_permlane32_swap(__builtin_bit_cast(unsigned, bm), __builtin_bit_cast(unsigned, bm), false, false);
-            bm = fmaxf(__builtin_bit_cast(float, static_cast<unsigned>(y[0])), __builtin_bit_cast(float, static_cast<unsigned>(y[1])));
+            bm = most(__builtin_bit_cast(float, static_cast<unsigned>(y[0])), __builtin_bit_cast(float, static_cast<unsigned>(y[1])));
         }
-        if constexpr (!CAP && !BIAS) bm *= scale;
+        if constexpr (!BIAS) bm = __builtin_fmaf(bm, mul, add);
         if (__any(bm > m + kLag)) {
             const float m_new = fmaxf(m, bm);
             const float alpha = m_new == -INFINITY ? 1.0f : __builtin_amdgcn_exp2f(m - m_new);
@@ -544,6 +551,7 @@ void scored_prefill_kernel(const ScoredPrefillArgs a) {
             m = m_new;
         }
         const float c = ((m == -INFINITY) ? 0.0f : m) - kWeightExp;
+        const float add_c = add - c;
         if (cleaned) {
             const u4 bad = *reinterpret_cast<const u4*>(s_bad[t & 1]);
             unsigned keys = 0;   // this lane's, as `seen`
@@ -551,13 +559,9 @@ void scored_prefill_kernel(const ScoredPrefillArgs a) {
             for (int b = 0; b < 4; ++b) keys |= ((bad[b] >> (8 * h)) & 0xffu) << (8 * b);
             if (seen & keys) l = __builtin_nanf("");
         }
-        // Weights, O^T += V P^T, and the next stage's scores in the place of the
-        // pair's that are used up: two blocks' products, a pair's scores, and both
-        // again, in this order, so that nothing waits for its operands or leaves
-        // the matrix unit alone. A product's operand is read kAhead products
-        // before, and among the products go the weights of the blocks to come and
-        // what a cap makes of the next stage's first pair. (Behind the last stage
-        // the scores are not used.)
+        // Weights, O^T += V P^T, and the next stage's scores in the place of those
+        // that are used up, in a fixed order. (Behind the last stage the scores are
+        // not used.)
         const uint16_t* const next = s_k[(t + 1) & 1] + koff;
         const uint16_t* const vl = s_v[t & 1] + 8 * lane;
         u4 pw[4];
@@ -567,17 +571,20 @@ void scored_prefill_kernel(const ScoredPrefillArgs a) {
 #pragma unroll
             for (int z = 0; z < 2; ++z) {
                 const float v = sc[b >> 1][8 * (b & 1) + 2 * i + z];
-                p[z] = __builtin_amdgcn_exp2f(CAP || BIAS ? v - c : __builtin_fmaf(v, scale, -c));
+                p[z] = __builtin_amdgcn_exp2f(BIAS ? v - c : __builtin_fmaf(v, mul, add_c));
             }
             pw[b][i] = T::down2(p[0], p[1]);
             l = add_pair(T{}, pw[b][i], l);
         };
-        constexpr int kHalf = 2 * ND + NJ;
-        constexpr int kAhead = 4;
+        constexpr int kScores = 2 * ND, kBack = 2 * ND + 2 * NJ, kProducts = 4 * ND + 2 * NJ;
+        constexpr int kAhead = 2;
         auto operand = [&](int n) {
-            const int half = n / kHalf, k = n % kHalf;
-            if (k < 2 * ND) return *reinterpret_cast<const s8*>(vl + (2 * half + k / ND) * St::kTile + 512 * (k % ND));
-            return k_rows(next + half * St::kPair + 256 * (k - 2 * ND));
+            if (n >= kScores && n < kBack) {
+                const int k = n - kScores;
+                return k_rows(next + k / NJ * St::kPair + 256 * (k % NJ));
+            }
+            const int k = n < kScores ? n : n - 2 * NJ;
+            return *reinterpret_cast<const s8*>(vl + k / ND * St::kTile + 512 * (k % ND));
         };
         s8 ring[kAhead];
 #pragma unroll
@@ -586,25 +593,26 @@ void scored_prefill_kernel(const ScoredPrefillArgs a) {
         for (int k = 0; k < 4; ++k) weights(k);
         __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
-        for (int n = 0; n < 2 * kHalf; ++n) {
-            const int half = n / kHalf, k = n % kHalf;
+        for (int n = 0; n < kProducts; ++n) {
             const s8 x = ring[n % kAhead];
-            if (n + kAhead < 2 * kHalf) ring[n % kAhead] = operand(n + kAhead);
-            if (k < 2 * ND) {
-                const int b = 2 * half + k / ND;
-                acc[k % ND] = T::mfma32(x, __builtin_bit_cast(s8, pw[b]), acc[k % ND]);
+            if (n + kAhead < kProducts) ring[n % kAhead] = operand(n + kAhead);
+            if (n >= kScores && n < kBack) {
+                const int k = n - kScores;
+                sc[k / NJ] = T::mfma32(x, q[k % NJ], k % NJ == 0 ? f16x{} : sc[k / NJ]);
             } else {
-                sc[half] = T::mfma32(x, q[k - 2 * ND], k == 2 * ND ? f16x{} : sc[half]);
+                const int k = n < kScores ? n : n - 2 * NJ;
+                acc[k % ND] = T::mfma32(x, __builtin_bit_cast(s8, pw[k / ND]), acc[k % ND]);
             }
-            if (half == 0) {
+            if (n < kScores) {
 #pragma unroll
-                for (int i = 4 + k * 4 / ND; i < 4 + (k + 1) * 4 / ND; ++i) {
-                    if (i < 12) weights(i);
-                }
-                if (k >= 2 * ND && k < 2 * ND + 4) weights(12 + k - 2 * ND);
-            } else if (CAP) {
+                for (int i = 4 + n * 4 / ND; i < 4 + (n + 1) * 4 / ND; ++i) weights(i);
+            } else if (n < kScores + 4) {
+                weights(12 + n - kScores);
+            } else if (CAP && n >= kScores + NJ) {
+                constexpr int kSlots = 2 * ND + NJ;
+                const int k = n - kScores - NJ;
 #pragma unroll
-                for (int i = k * 16 / kHalf; i < (k + 1) * 16 / kHalf; ++i) sc[0][i] = cap_part(sc[0][i]);
+                for (int i = k * 32 / kSlots; i < (k + 1) * 32 / kSlots; ++i) sc[i >> 4][i & 15] = cap_part(sc[i >> 4][i & 15]);
             }
             __builtin_amdgcn_sched_barrier(0);
         }
