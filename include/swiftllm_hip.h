@@ -515,8 +515,9 @@ int swiftllm_hip_rotary_and_cache(
  * key writes zeros. Cache slots that no query of the call sees may hold
  * anything, NaN included. A key that is not finite makes the outputs of the
  * queries that see it NaN or unspecified, a value that is not finite one
- * element of them, or all, not finite; other queries are not touched. dtype is that of query,
- * caches and output; scale and softcap are finite, softcap >= 0. */
+ * element of them, or all, not finite; other queries are not touched. dtype is
+ * that of query, caches and output; scale and softcap are finite, softcap 0 to
+ * 1024. output may be query itself and overlaps no other argument. */
 
 /* One new token per sequence: the query of sequence s, at position
  * context_lens[s] - 1 (context_lens[s] <= 0: zeros), is row s of query and
@@ -547,7 +548,7 @@ size_t swiftllm_hip_scored_decode_workspace_size(
  * the cache already: whole prompts, or chunks on top of what is cached (the
  * arrays that swiftllm_hip_plan_step writes). query_offsets has num_seqs + 1
  * entries within [0, num_tokens]; a sequence whose offsets are not ascending
- * within it has no rows. Rows of no sequence are left as they were; a row at a
+ * within it has no rows. If sequences share rows the output is unspecified. Rows of no sequence are left as they were; a row at a
  * negative position is zero. The caches are 16-byte aligned. */
 int swiftllm_hip_scored_prefill(
     void* output, const void* query, const void* key_cache,

@@ -9,7 +9,8 @@
 // Scores are kept in units of log2(e), so that weights are exp2. The cap costs
 // two transcendental operations: c * tanh(x / c) = c - 2 c / (1 + e^(2 x / c)),
 // whose error for small x is that of the subtraction from c, 2^-24 c absolute,
-// which moves a weight by under 10^-5 of itself for a cap of 50.
+// which moves a weight by under 10^-5 of itself for a cap of 50. A cap past
+// kMostCap is refused: its error would pass the output's rounding (10^-4 there).
 #pragma once
 
 #include <cmath>
@@ -20,6 +21,8 @@ namespace swiftllm {
 namespace scored {
 
 constexpr float kLog2e = 1.4426950408889634f;
+
+constexpr float kMostCap = 1024.0f;
 
 struct Shape {
     float scale;         // no cap: scale * log2(e); cap: 2 log2(e) scale / cap

@@ -574,6 +574,9 @@ int swiftllm_hip_scored_decode(void* output, void* workspace, size_t workspace_b
     if (!scored::make_shape(a.shape, scale, softcap, window, prefix_lens, alibi_slopes)) {
         return fail(SWIFTLLM_ERR_INVALID_PARAMETER, "%s: scale=%g softcap=%g window=%d", who, scale, softcap, window);
     }
+    if (softcap > scored::kMostCap) {
+        return fail(SWIFTLLM_ERR_NOT_SUPPORTED, "%s: softcap=%g (at most %g)", who, softcap, scored::kMostCap);
+    }
     if (query_offsets && num_tokens < 0) {
         return fail(SWIFTLLM_ERR_INVALID_PARAMETER, "%s: num_tokens=%d", who, num_tokens);
     }
@@ -596,6 +599,14 @@ int swiftllm_hip_scored_decode(void* output, void* workspace, size_t workspace_b
     const long long HC = static_cast<long long>(num_kv_heads) * nhc;
     if (S * HC >= (1LL << 24)) {
         return fail(SWIFTLLM_ERR_NOT_SUPPORTED, "%s: num_seqs=%d num_heads=%d", who, num_seqs, num_heads);
+    }
+    // A workgroup has read its queries before it or a later kernel writes their
+    // rows; rows of others must not be among them.
+    const size_t rows = static_cast<size_t>(query_offsets ? num_tokens : num_seqs);
+    const size_t values = rows * num_heads * head_dim * 2;
+    if ((output != query && overlap(output, values, query, values)) || overlap(workspace, l.bytes, output, values) ||
+        overlap(workspace, l.bytes, query, values)) {
+        return fail(SWIFTLLM_ERR_INVALID_PARAMETER, "%s: output or workspace overlaps another argument", who);
     }
     rc = require_device();
     if (rc != SWIFTLLM_OK) return rc;

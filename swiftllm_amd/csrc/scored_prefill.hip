@@ -73,6 +73,9 @@ struct ScoredPrefillArgs {
 constexpr int kWaves = 4;
 constexpr int kStage = 64;             // keys
 constexpr int kListSeqs = 1024;        // sequences of the longest-first list
+// Tiles of a lane's sequences: memory holds the rows of fewer, and sums over a
+// wave stay in range where sequences share rows.
+constexpr int kMostTiles = 1 << 24;
 constexpr long long kCUs = 256;        // MI355X; any grid is correct, this one is resident
 template <int D>
 constexpr int kPerCU = D == 128 ? 2 : 3;
@@ -179,7 +182,7 @@ struct List {
         for (int s0 = 0; s0 < S; s0 += 64) {
             int n, f;
             get(s0, lane, n, f);
-            sum += max(min(n, f + n - i), 0);
+            sum = min(sum + max(min(n, f + n - i), 0), kMostTiles);
         }
         return wave_total(sum);
     }
@@ -206,7 +209,7 @@ struct List {
             if (k < here || s0 + 64 >= S) {
                 const int rank = __popcll(mask & ((1ull << lane) - 1ull));
                 const int at = __ffsll(static_cast<long long>(__ballot(has && rank == k))) - 1;
-                seq = s0 + at;
+                seq = max(s0 + at, 0);  // (there is one, unless sequences share rows)
                 tile = lo - __builtin_amdgcn_readlane(f, at);
                 return;
             }
@@ -315,7 +318,9 @@ void scored_prefill_kernel(const ScoredPrefillArgs a) {
     const unsigned heads = a.Hkv * a.nhc / a.xcds;
     // Past kListSeqs sequences the tiles go in order: sequence s has the
     // entries from query_offsets[s] / per_wg + s on, at least one per tile.
-    const unsigned entries = listed ? list.count(0, threadIdx.x & 63) : a.T / per_wg + a.S;
+    // (More entries than of separate rows come of sequences that share some.)
+    const int most_entries = a.T / per_wg + a.S;
+    const unsigned entries = listed ? max(min(list.count(0, threadIdx.x & 63), most_entries), 0) : most_entries;
     const unsigned total = entries * heads;  // below 2^31 (host)
     auto item_of = [&](unsigned round) { return round * wgs + ((round & 1) ? wgs - 1 - l0 : l0); };
     for (unsigned round = 0; item_of(round) < total; ++round) {
@@ -713,6 +718,9 @@ int swiftllm_hip_scored_prefill(void* output, const void* query, const void* key
     if (!scored::make_shape(a.shape, std::fabs(scale), softcap, window, prefix_lens, alibi_slopes)) {
         return fail(SWIFTLLM_ERR_INVALID_PARAMETER, "%s: scale=%g softcap=%g window=%d", who, scale, softcap, window);
     }
+    if (softcap > scored::kMostCap) {
+        return fail(SWIFTLLM_ERR_NOT_SUPPORTED, "%s: softcap=%g (at most %g)", who, softcap, scored::kMostCap);
+    }
     if (T > 0 && S > 0 && (!output || !query || !key_cache || !value_cache || !context_lens || !query_offsets ||
                            (MB > 0 && !block_tables))) {
         return fail(SWIFTLLM_ERR_INVALID_PARAMETER, "%s: null pointer", who);
@@ -721,6 +729,12 @@ int swiftllm_hip_scored_prefill(void* output, const void* query, const void* key
         !aligned(block_tables, 4) || !aligned(context_lens, 4) || !aligned(query_offsets, 4) ||
         !aligned(alibi_slopes, 4) || !aligned(prefix_lens, 4)) {
         return fail(SWIFTLLM_ERR_INVALID_PARAMETER, "%s: misaligned pointer", who);
+    }
+    // A wave has read its queries before it writes their rows; rows of others
+    // must not be among them.
+    const size_t values = static_cast<size_t>(T) * H * D * 2;
+    if (output != query && overlap(output, values, query, values)) {
+        return fail(SWIFTLLM_ERR_INVALID_PARAMETER, "%s: output overlaps query", who);
     }
     a.S = num_seqs;
     a.T = num_tokens;

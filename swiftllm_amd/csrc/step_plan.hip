@@ -235,11 +235,6 @@ __global__ __launch_bounds__(kPlanThreads) void step_plan_kernel(const PlanArgs 
     }
 }
 
-bool overlap(const void* p, size_t n, const void* q, size_t m) {
-    const uintptr_t a = reinterpret_cast<uintptr_t>(p), b = reinterpret_cast<uintptr_t>(q);
-    return n > 0 && m > 0 && a < b + m && b < a + n;
-}
-
 }  // namespace
 }  // namespace swiftllm
 

@@ -254,6 +254,18 @@ def test_decode_leaves_no_trace_between_calls(dev):
     assert np.array_equal(first, a.out.numpy())
 
 
+@pytest.mark.parametrize("ctx,H,Hkv", [([33, 1, 16, 0, 300], 8, 2), ([5000, 9, 700], 40, 2)])
+def test_decode_into_the_queries(dev, ctx, H, Hkv):
+    """output may be query: sequences taken whole, and cut ones that a join writes."""
+    d = Decode(np.random.default_rng(16), ctx, H, Hkv, 64, "f16", cap=20.0)
+    d.run()
+    synchronize()
+    d.out.upload(np.concatenate([d.q, np.full((1, H, 64), 0x7F7F, np.uint16)]))
+    d.d["q"] = d.out
+    d.run()
+    d.check("in place")
+
+
 def test_decode_in_a_captured_graph(dev):
     """Replays follow the lengths and tables in the buffers; two graphs with a
     workspace each on two streams at once."""

@@ -269,6 +269,37 @@ def test_prefill_query_and_output_8_byte_aligned(dev):
     p.check(got=out.download_at(8, p.q.shape, np.uint16))
 
 
+@pytest.mark.parametrize("H,Hkv,D", [(8, 2, 64), (40, 1, 128)])
+def test_prefill_into_the_queries(dev, H, Hkv, D):
+    """output may be query; rows of no sequence stay."""
+    p = Prefill(np.random.default_rng(13), [1, 150, 33], H, Hkv, D, "f16", cached=[40, 3, 0], cap=20.0, tail=0)
+    p.out.upload(p.q)
+    p.run(q=p.out)
+    p.check("in place")
+    p = Prefill(np.random.default_rng(14), [5], H, Hkv, D, "f16", lead=4, tail=7)
+    p.run(q=p.d["q"], out=p.d["q"])
+    synchronize()
+    got = p.d["q"].numpy()
+    assert np.array_equal(got[:4], p.q[:4]) and np.array_equal(got[9:], p.q[9:])
+
+
+def test_prefill_rows_that_sequences_share(dev):
+    """Offsets that run back and forth make rows of several sequences: the
+    output is unspecified, but the call ends and writes within its rows."""
+    p = Prefill(np.random.default_rng(15), [7] * 70, 8, 2, 64, "f16", cached=[9] * 70)
+    good = p.off.copy()
+    p.off[1:40] = [0, 200] * 19 + [0]
+    p.upload()
+    p.run()
+    synchronize()
+    assert (p.out.numpy()[490:] == 0x7F7F).all()
+    p.off = good
+    p.d["off"].upload(good)
+    p.out.fill_byte(0x7F)
+    p.run()
+    p.check("separate rows")
+
+
 def test_prefill_nothing_to_do(dev):
     p = Prefill(np.random.default_rng(12), [0, 0], 8, 2, 64, "f16", tail=20)
     p.run()

@@ -91,6 +91,26 @@ def test_prefill_refuses(kw, code):
     assert _lib.last_error()[0] == code and _lib.last_error()[1]
 
 
+@pytest.mark.parametrize("call", [_decode, _prefill])
+def test_a_cap_has_an_upper_bound(call):
+    """The capped score is off by 2^-24 of its cap."""
+    assert call(softcap=1024.5) == UNSUP
+    assert "at most 1024" in _lib.last_error()[1]
+
+
+def test_outputs_that_overlap_are_refused():
+    far = 1 << 40   # of the other arguments
+    for d in (-64, 64, 3 * 8 * 64 * 2 - 16):        # of 3 rows of 8 heads x 64 values
+        assert _decode(workspace=far, output=P + d) == INVALID
+        assert "overlaps" in _lib.last_error()[1]
+    assert _decode(workspace=far, output=P + 64, query_offsets=P, num_tokens=1) == INVALID
+    assert _decode(output=far) == INVALID            # workspace on the queries
+    assert _decode(query=far) == INVALID             # and on the output
+    for d in (-64, 64, 10 * 8 * 64 * 2 - 16):
+        assert _prefill(output=P + d) == INVALID
+        assert "overlaps" in _lib.last_error()[1]
+
+
 def test_decode_workspace_size():
     n = step.scored_decode_workspace_size(8, 64, 8, 128, 16, 2048)
     # two fragments of 16-byte aligned heads for each of the ranges
