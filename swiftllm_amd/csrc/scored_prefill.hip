@@ -11,9 +11,8 @@
 // LDS once for the four waves by direct loads, two stages deep, one barrier a
 // stage; V lies in the cache as the product's row operand, K comes back turned
 // by ds_read_b64_tr_b16. The walk takes the stages of the prefix, then those
-// from the tile's window on: hidden stages are not read. A resident grid goes
-// through one list of query tiles, longest walk first over all sequences, each
-// XCD its own kv heads, so that a kv head's K and V are read through one L2.
+// from the tile's window on: hidden stages are not read. The tiles of all
+// sequences are one list, longest walk first.
 //
 // Scores. The masks and the two-sided distance are worked out only in stages
 // that some row of the wave does not see whole, and a wave leaves out the
@@ -77,7 +76,8 @@ constexpr int kListSeqs = 1024;
 // Tiles of a lane's sequences: memory holds the rows of fewer, and sums over a
 // wave stay in range where sequences share rows.
 constexpr int kMostTiles = 1 << 24;
-constexpr long long kCUs = 256;        // MI355X; any grid is correct, this one is resident
+constexpr long long kCUs = 256;        // MI355X; any grid is correct
+constexpr long long kMostGroups = 1LL << 22;   // 2^30 threads
 // Workgroups of a CU: as registers allow. (At D = 64 two, not three: 40 ragged
 // prompts up to 1500 tokens of 8/8 heads 72 us, not 65.)
 template <int D>
@@ -772,8 +772,13 @@ int swiftllm_hip_scored_prefill(void* output, const void* query, const void* key
     a.num_blocks = num_blocks;
     a.q16 = aligned(query, 16);
     a.out16 = aligned(output, 16);
-    const long long resident = kCUs * (D == 128 ? kPerCU<128> : kPerCU<64>);
-    const long long grid = std::min<long long>((items + 7) / 8 * 8, resident);
+    // A list in registers is made in no time, so a tile gets a workgroup of its own
+    // and goes where one ended; a longer one is made once per resident workgroup.
+    // Of their own / resident: 8 x 2048 tokens with a cap 378 / 388 us, 40 ragged
+    // prompts of 8/8 heads x 64 with a cap 79 / 85, without 62 / 64, 700 of 1-60
+    // tokens 190 / 159.
+    const long long resident = S <= 64 ? kMostGroups : kCUs * (D == 128 ? kPerCU<128> : kPerCU<64>);
+    const long long grid = (std::min(items, resident) + 7) / 8 * 8;
     using K = void (*)(ScoredPrefillArgs);
 #define SCORED_PREFILL(T_) \
     {{{scored_prefill_kernel<T_, 64, false, false>, scored_prefill_kernel<T_, 64, false, true>}, \
