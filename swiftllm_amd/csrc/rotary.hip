@@ -17,7 +17,11 @@
 //
 // Bound: HBM, one read of q, k and v and one write of q and of the blocks.
 // One launch: a workgroup takes either a window of tokens of 256 rows of K or
-// of V (see cache_runs.hpp), or the queries of four tokens.
+// of V (see cache_runs.hpp), or the queries of four tokens. An angle's 20
+// operations are made once per wave and token (per element: 123 us, not 91).
+// Measured: 16384 tokens of prompts, 32/8 heads x 128, 91 us (4.4 TB/s read and
+// written); 64 lone tokens of that layer 6.1 us; 2013 tokens of 8/8 x 64 7.2 us.
+// 4096 lone tokens of 32/8 x 128 take 125 us: 2 bytes per 32-byte row each.
 
 #include <algorithm>
 #include <cmath>

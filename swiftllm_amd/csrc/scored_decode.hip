@@ -22,6 +22,10 @@
 // with the identity (exact), S^T = K Q^T and O^T = V P^T as in paged decode,
 // with P in two 16-bit parts (about 20 bits for fp16, 16 for bfloat16), so
 // that only the output is rounded.
+//
+// Measured, with a cap: 64 contexts of 512-4096 tokens, 32/8 heads x 128, 96 us
+// (6.2 TB/s, 4.7 us of it the join), 8 x 32768 of 64/8 166 us (6.5 TB/s); 4 chats
+// of 8/8 x 64 in one launch 6.1 us.
 
 #include <algorithm>
 

@@ -20,6 +20,8 @@
 // them find in the L2) 1024 at a time, keeps the ends of those in LDS and
 // finds a row's sequence by bisection. A block's first row writes its table
 // entry: entries that a row reads are never written in the same call.
+// Measured: 64 sequences of one token each 4.8 us of the kernel, 5.4 us a call;
+// 64 sequences of 169000 rows 5.4 us, the call's floor being a launch's 4.3.
 
 #include "common.hpp"
 
