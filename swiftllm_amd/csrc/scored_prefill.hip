@@ -23,8 +23,8 @@
 // Weights are rounded to 16 bits, to nearest, and summed as rounded: the
 // output's error is that of its own rounding and one of the same size.
 //
-// Order. What a stage costs a wave beside its 32 products (D = 128) is 70 to
-// 130 vector operations for its 32 scores a lane, so the order of both is
+// Order. What a stage costs a wave beside its 32 products (D = 128) is 115 to
+// 250 vector operations for its 32 scores a lane, so the order of both is
 // fixed: products of two blocks' values, both pairs' next scores, the other
 // two blocks' values, each operand read two products ahead (2, 3, 4, 6 and 8
 // took the same time, left to the compiler 8 x 2048 tokens with a cap took 4 %
