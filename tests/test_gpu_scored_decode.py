@@ -204,6 +204,48 @@ def test_decode_values_that_are_not_finite(dev, dtype, wide):
 
 
 @pytest.mark.parametrize("dtype", ["f16", "bf16"])
+@pytest.mark.parametrize("kw", [dict(), dict(cap=1000.0)])
+def test_decode_sums_small_weights(dev, dtype, kw):
+    """20000 keys 22 binary places below the largest count; of values of 1 the
+    output is 1 (powers of two and exact sums, but for a cap's, which are off
+    alike), and of a 0 for the largest it is their share, off by a step of their
+    weight in fp16 (2^-9 of it), half a step of the output and the cap's 2^-11."""
+    d = Decode(np.random.default_rng(17), [20010, 40], 2, 1, 64, dtype, scale=1.0, **kw)
+    d.kc[:], d.vc[:], d.q[:] = 0, to_half(np.ones(1), dtype)[0], 0
+    d.kc[d.bt[0, 0], 0, 0, 0] = to_half(np.array([15.25]), dtype)[0]     # 22 / log2(e)
+    d.q[:, :, 0] = to_half(np.ones(1), dtype)[0]
+    d.upload()
+    d.run()
+    synchronize()
+    got = to_float(d.out.numpy()[:2], dtype)
+    assert (np.abs(got - 1.0) <= 2.0 ** (-11 if dtype == "f16" else -8)).all(), np.abs(got - 1).max()
+    d.vc[d.bt[0, 0], 0, :, 0] = 0
+    d.d["vc"].upload(d.vc)
+    d.run()
+    synchronize()
+    got = to_float(d.out.numpy()[:1], dtype)
+    want = 20009 / (20009 + np.exp(1000 * np.tanh(0.01525) if kw else 15.25))
+    assert (np.abs(got / want - 1) <= 2.0 ** (-8 if dtype == "f16" else -7)).all(), np.abs(got / want - 1).max()
+
+
+@pytest.mark.parametrize("dtype", ["f16", "bf16"])
+@pytest.mark.parametrize("wide", [False, True])
+def test_decode_a_query_that_is_not_finite(dev, dtype, wide):
+    """It makes NaN of its own head and of no other."""
+    d = Decode(np.random.default_rng(18), [40, 3000 if wide else 40], 8, 2, 64, dtype, alibi=True)
+    want, bound = d.want()
+    d.q[0, 1, 7] = d.q[1, 6, 63] = NAN16
+    d.upload()
+    d.run()
+    synchronize()
+    got = to_float(d.out.numpy()[:2], dtype)
+    fine = np.ones((2, 8), bool)
+    fine[0, 1] = fine[1, 6] = False
+    assert np.isnan(got[~fine]).all()
+    assert (np.abs(got - want)[fine] <= bound[fine]).all()
+
+
+@pytest.mark.parametrize("dtype", ["f16", "bf16"])
 def test_decode_large_scores(dev, dtype):
     """Scores of hundreds, far above and below each other; a cap bounds them."""
     for cap in (0.0, 50.0):

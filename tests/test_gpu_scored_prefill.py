@@ -300,6 +300,55 @@ def test_prefill_rows_that_sequences_share(dev):
     p.check("separate rows")
 
 
+@pytest.mark.parametrize("dtype", ["f16", "bf16"])
+@pytest.mark.parametrize("kw", [dict(), dict(cap=1000.0), dict(window=30000)])
+def test_prefill_sums_small_weights(dev, dtype, kw):
+    """Some 20000 keys 22 binary places below the largest: their weights are
+    below fp16's normal range and count, in the sum as in the output. Of values
+    of 1 the output is 1: every weight is rounded to a power of two and every sum
+    exact (with a cap the scores are off by under 2^-11, the same for all of
+    those keys), so only the last division and the rounding to the type are left.
+    Of a 0 for the largest it is their share: off by half a step of their weight
+    (2^-10 of it in fp16, 2^-9 in bf16), of the output's, and of the cap."""
+    p = Prefill(np.random.default_rng(16), [40], 2, 1, 64, dtype, cached=[19970], scale=1.0, tail=0, **kw)
+    p.kc[:], p.vc[:], p.q[:] = 0, to_half(np.ones(1), dtype)[0], 0
+    p.kc[p.bt[0, 0], 0, 0, 0] = to_half(np.array([15.25]), dtype)[0]     # 22 / log2(e)
+    p.q[:, :, 0] = to_half(np.ones(1), dtype)[0]
+    p.upload()
+    p.run()
+    synchronize()
+    got = to_float(p.out.numpy(), dtype)
+    assert (np.abs(got - 1.0) <= 2.0 ** (-11 if dtype == "f16" else -8)).all(), np.abs(got - 1).max()
+    p.vc[p.bt[0, 0], 0, :, 0] = 0
+    p.d["vc"].upload(p.vc)
+    p.run()
+    synchronize()
+    got = to_float(p.out.numpy(), dtype)
+    top = 1000 * np.tanh(0.01525) if "cap" in kw else 15.25
+    n = 19970 + np.arange(40)[:, None, None]      # keys behind the first that row t sees
+    want = n / (n + np.exp(top))
+    assert (np.abs(got / want - 1) <= 2.0 ** (-8 if dtype == "f16" else -7)).all(), np.abs(got / want - 1).max()
+
+
+@pytest.mark.parametrize("dtype", ["f16", "bf16"])
+@pytest.mark.parametrize("kw", [dict(), dict(cap=20.0), dict(alibi=True)])
+def test_prefill_a_query_that_is_not_finite(dev, dtype, kw):
+    """It makes NaN of its own row and head and of no other."""
+    p = Prefill(np.random.default_rng(17), [70, 20], 8, 2, 64, dtype, **kw)
+    want, bound = p.want()
+    for t, h in ((0, 0), (33, 5), (75, 7)):
+        p.q[t, h, 11] = NAN16
+    p.upload()
+    p.run()
+    synchronize()
+    got, mine = to_float(p.out.numpy(), dtype), p.rows()
+    bad = np.zeros(got.shape[:2], bool)
+    bad[0, 0] = bad[33, 5] = bad[75, 7] = True
+    assert np.isnan(got[bad]).all()
+    fine = mine[:, None] & ~bad
+    assert (np.abs(got - want)[fine] <= bound[fine]).all()
+
+
 def test_prefill_nothing_to_do(dev):
     p = Prefill(np.random.default_rng(12), [0, 0], 8, 2, 64, "f16", tail=20)
     p.run()
