@@ -403,15 +403,15 @@ void scored_prefill_kernel(const ScoredPrefillArgs a) {
     const int nsteps = tp1 < 0 || last < 0 ? 0 : before + max(last / kStage - low + 1, 0);
     auto stage_of = [&](int t) { return t < before ? t : t + skip; };
     // First keys of the stages that every row of the wave sees whole, none of
-    // them ahead of the row where the distance counts: from w0 to w1, and to w2
+    // them ahead of the row where the distance counts: w_span from w0 on, and to w2
     // in the prefix. The same for the tile's rows.
     const bool wave_rows = wp0 >= 0 && wp0 <= wp1;
     const int w0 = max(wp1 - min(window, wp1 + 1) + 1, 0);
-    const int w1 = wave_rows ? min(wp0, L - 1) - (kStage - 1) : -1;
+    const unsigned w_span = wave_rows ? max(min(wp0, L - 1) - (kStage - 1) - w0 + 1, 0) : 0;
     const int w2 = wave_rows ? (BIAS ? min(pre, wp0 + 1) : pre) - kStage : -1;
     const int last_seen = max(wp1 < wp0 ? -1 : min(wp1, L - 1), pre - 1);
     const int t0 = max(tp1 - min(window, tp1 + 1) + 1, 0);
-    const int t1 = tp0 >= 0 ? min(tp0, L - 1) - (kStage - 1) : -1;
+    const unsigned t_span = tp0 >= 0 ? max(min(tp0, L - 1) - (kStage - 1) - t0 + 1, 0) : 0;
     const int t2 = tp0 >= 0 ? pre - kStage : -1;
 
     // (zeros behind an empty asm: 16 of them would be kept over the tiles)
@@ -429,7 +429,7 @@ void scored_prefill_kernel(const ScoredPrefillArgs a) {
     const int* const row = a.bt + static_cast<size_t>(s) * a.MB;
     // Ids of 16 stages of the walk, four lanes each.
     auto chunk_ids = [&](int c) { return row[min(4 * stage_of(16 * c + (lane >> 2)) + (lane & 3), nblk - 1)]; };
-    int ids = chunk_ids(0);
+    const int ids_first = chunk_ids(0);
     int ids_next = chunk_ids(1);
     // Q^T operand: lane (r, h) holds q[r][16 J + 8 h .. + 7].
     s8 q[NJ];
@@ -449,21 +449,28 @@ void scored_prefill_kernel(const ScoredPrefillArgs a) {
             q[J] = __builtin_bit_cast(s8, (v & keep) ^ flip);
         }
     }
+    // The chunk at hand, unknown blocks as block 0 and their bits in `known` clear.
+    int ids;
+    unsigned long long known;
+    auto take_chunk = [&](int x) {
+        const bool k = block_known(x, a.num_blocks);
+        known = __ballot(k);
+        ids = k ? x : 0;
+    };
+    take_chunk(ids_first);
     // Tile of this wave in stage t of the walk (16 stages per load of ids) and,
     // in ok4, which of the stage's four blocks are in the pool.
     auto tile_of = [&](int t, int& ok4) {
-        const unsigned long long okm = __ballot(block_known(ids, a.num_blocks));
         const int at = 4 * (t & 15);
-        ok4 = static_cast<int>((okm >> at) & 15ull);
-        const int b = (ok4 >> w) & 1 ? __builtin_amdgcn_readlane(ids, at + w) : 0;
-        return kv_tile_offset(b, kvh, a.Hkv, D);
+        ok4 = static_cast<int>((known >> at) & 15ull);
+        return kv_tile_offset(__builtin_amdgcn_readlane(ids, at + w), kvh, a.Hkv, D);
     };
     auto bytes_of = [&](int t) { return t < nsteps ? D * kBlockTokens * 2 : 0; };
     // This wave's block of stage t of the walk has landed in its V buffer: true
     // if some row of the tile may not see the stage whole.
     auto landed = [&](int t, int ok4) {
         const int base = kStage * stage_of(t);
-        if (t >= nsteps || (ok4 == 15 && ((base >= t0 && base <= t1) || base <= t2))) return false;
+        if (t >= nsteps || (ok4 == 15 && (static_cast<unsigned>(base - t0) < t_span || base <= t2))) return false;
         const unsigned bad = clean_v<T, D>(s_v[t & 1], w, lane);
         if (lane == 0) s_bad[t & 1][w] = bad;
         return true;
@@ -504,7 +511,7 @@ void scored_prefill_kernel(const ScoredPrefillArgs a) {
         if (base <= last_seen) {
         // (One copy of the stage with scalar branches: two copies, with and without
         // masks, took 100 more registers for the sums that they hand each other.)
-        const bool whole = ok_t == 15 && ((base >= w0 && base <= w1) || base <= w2);
+        const bool whole = ok_t == 15 && (static_cast<unsigned>(base - w0) < w_span || base <= w2);
         // Score i of pair p: key base + 32 p + 16 (i / 8) + 8 h + i % 8; bit
         // 16 p + i of `seen` whether this row sees it.
         unsigned seen = ~0u;
@@ -636,7 +643,7 @@ void scored_prefill_kernel(const ScoredPrefillArgs a) {
         ok_t = ok_1;
         ok_1 = ok_2;
         if (((t + 3) & 15) == 0) {
-            ids = ids_next;
+            take_chunk(ids_next);
             ids_next = chunk_ids(((t + 3) >> 4) + 1);
         }
         __syncthreads();
