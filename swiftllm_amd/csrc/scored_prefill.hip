@@ -156,7 +156,7 @@ struct Rows {
     int start, n;
 };
 __device__ __forceinline__ Rows rows_of(const ScoredPrefillArgs& a, int s) {
-    const int b = a.qoff[s], e = a.qoff[s + 1];
+    const int b = as_const(a.qoff)[s], e = as_const(a.qoff)[s + 1];
     // Offsets that run backwards or out of the rows have no rows.
     return b >= 0 && e > b && e <= a.T ? Rows{b, e - b} : Rows{0, 0};
 }
@@ -374,9 +374,9 @@ void scored_prefill_kernel(const ScoredPrefillArgs a) {
     const int yy = static_cast<int>(item - e * heads);
     const int kvh = yy / a.nhc;
     const int hc = yy - kvh * a.nhc;
-    const int ctx = a.ctx[s];
+    const int ctx = as_const(a.ctx)[s];
     const int L = min(max(ctx, 0), a.MB * kBlockTokens);
-    const int pre = a.shape.prefix != nullptr ? min(max(a.shape.prefix[s], 0), L) : 0;
+    const int pre = a.shape.prefix != nullptr ? min(max(as_const(a.shape.prefix)[s], 0), L) : 0;
     // A window of every key is the same as none.
     const int window = a.shape.window > 0 ? a.shape.window : 0x7fffffff;
     const int pos0 = ctx - rows.n;                       // of the sequence's first row
