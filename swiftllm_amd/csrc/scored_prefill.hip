@@ -33,9 +33,9 @@
 //
 // Measured: 8 x 2048 tokens, 32/8 heads x 128, with a cap 380 us (720 TFLOP/s;
 // bound by the vector operations), without 314; chunks in a window 280 us (970
-// TFLOP/s; bound by power, 1.6 GHz, and LDS, about 76 % of the cycles); 24 prompts
-// of 52-912 tokens, 16/16 heads, with a bias and prefixes 56 us (short walks, bound
-// by latency).
+// TFLOP/s; bound by power: 1.6 GHz, matrix unit 58 % and LDS 30 % of the cycles); 24
+// prompts of 52-912 tokens, 16/16 heads, with a bias and prefixes 56 us (short walks,
+// bound by latency).
 //
 // A weight of 0 times a value that is not finite is NaN. So in a stage that
 // some row of the tile does not see whole, such values become zeros in LDS, and
