@@ -19,8 +19,8 @@
 // One launch: a workgroup takes either a window of tokens of 256 rows of K or
 // of V (see cache_runs.hpp), or the queries of four tokens. An angle's 20
 // operations are made once per wave and token (per element: 123 us, not 91).
-// Measured: 16384 tokens of prompts, 32/8 heads x 128, 91 us (4.4 TB/s read and
-// written); 64 lone tokens of that layer 6.1 us; 2013 tokens of 8/8 x 64 7.2 us.
+// Measured: 16384 tokens of prompts, 32/8 heads x 128, 87 us (4.6 TB/s read and
+// written); 64 lone tokens of that layer 6.2 us; 2013 tokens of 8/8 x 64 6.4 us.
 // 4096 lone tokens of 32/8 x 128 take 125 us: 2 bytes per 32-byte row each.
 
 #include <algorithm>
@@ -66,9 +66,9 @@ struct RotaryArgs {
 
 constexpr double kPerTurn = 0.15915494309189533577;  // 1 / (2 pi)
 
-// Cosine and sine, times the factor, of pair i at a position.
-__device__ __forceinline__ void turn(const RotaryArgs& a, int pos, int i, float& c, float& s) {
-    const double t = static_cast<double>(pos) * a.inv_freq[i] * kPerTurn;
+// Cosine and sine, times the factor, of a pair at a position.
+__device__ __forceinline__ void turn(const RotaryArgs& a, int pos, double freq, float& c, float& s) {
+    const double t = static_cast<double>(pos) * freq * kPerTurn;
     const float f = static_cast<float>(__builtin_amdgcn_fract(t));
     c = __builtin_amdgcn_cosf(f) * a.factor;
     s = __builtin_amdgcn_sinf(f) * a.factor;
@@ -94,10 +94,15 @@ __device__ __forceinline__ void pair_of(int d, int half, int& i, int& other, flo
 // wave: an angle costs some 20 operations, and every head needs it.
 struct TurnLds {
     float c[64], s[64];
-    __device__ __forceinline__ void make(const RotaryArgs& a, int pos) {
+    // The frequency of this lane's pair.
+    static __device__ __forceinline__ double freq(const RotaryArgs& a) {
         const int i = threadIdx.x & 63;
-        float cc = 1.0f, ss = 0.0f;
-        if (i < a.rot >> 1) turn(a, pos, i, cc, ss);
+        return i < a.rot >> 1 ? a.inv_freq[i] : 0.0;
+    }
+    __device__ __forceinline__ void make(const RotaryArgs& a, int pos, double f) {
+        const int i = threadIdx.x & 63;
+        float cc, ss;
+        turn(a, pos, f, cc, ss);
         __builtin_amdgcn_wave_barrier();   // after the reads of the one before
         c[i] = cc;
         s[i] = ss;
@@ -210,11 +215,12 @@ struct RowSrc {
     bool wide;
     TurnLds* lds;             // two of this wave: the tokens of its lower and upper lanes
     int pos;                  // of token t0 + lane
+    double freq;              // of pair `lane`
     __device__ __forceinline__ int slot(int t) const { return a.positions[t] < 0 ? -1 : a.slots[t]; }
     __device__ __forceinline__ void before(int k) const {
         if (is_v) return;
-        lds[0].make(a, __builtin_amdgcn_readlane(pos, __builtin_amdgcn_readlane(k, 0) & 63));
-        lds[1].make(a, __builtin_amdgcn_readlane(pos, __builtin_amdgcn_readlane(k, 63) & 63));
+        lds[0].make(a, __builtin_amdgcn_readlane(pos, __builtin_amdgcn_readlane(k, 0) & 63), freq);
+        lds[1].make(a, __builtin_amdgcn_readlane(pos, __builtin_amdgcn_readlane(k, 63) & 63), freq);
     }
     __device__ __forceinline__ uint16_t one(int t, int i) const {
         const uint16_t* const p = rows + t * stride + row0 + i;
@@ -223,7 +229,7 @@ struct RowSrc {
         int pair, other;
         float sign, c, s;
         pair_of<INTER>(d, a.rot >> 1, pair, other, sign);
-        turn(a, a.positions[t], pair, c, s);
+        turn(a, a.positions[t], a.inv_freq[pair], c, s);
         return T::down(__builtin_fmaf(T::up(*p), c, T::up(p[other - d]) * (s * sign)));
     }
     __device__ __forceinline__ u4v eight(int t, int i) const {
@@ -260,7 +266,7 @@ __global__ __launch_bounds__(256) void rotary_and_cache_kernel(const RotaryArgs 
         const int row0 = (is_v ? piece - a.slices : piece) * kWinRows;
         const int pos = a.positions[min(t0 + lane, a.T - 1)];
         const RowSrc<T, INTER> src{a, is_v ? a.v : a.k, is_v ? a.v_stride : a.k_stride, row0, is_v,
-                                   is_v ? a.wide_v : a.wide_k, lds, pos};
+                                   is_v ? a.wide_v : a.wide_k, lds, pos, is_v ? 0.0 : TurnLds::freq(a)};
         write_runs<W>(src, is_v ? a.vc : a.kc, tile, t0, row0, a.Hkv * a.D, a.T, a.num_slots);
         return;
     }
@@ -271,7 +277,7 @@ __global__ __launch_bounds__(256) void rotary_and_cache_kernel(const RotaryArgs 
     const int t = unit / a.parts;
     if (t >= a.T) return;
     const int pos = a.positions[t];
-    if (pos < 0) return;
+    const double freq = TurnLds::freq(a);
     const int lanes = a.D >> 3;                 // of one head
     const int d = 8 * (lane & (lanes - 1));
     const int step = 64 / lanes;
@@ -279,8 +285,20 @@ __global__ __launch_bounds__(256) void rotary_and_cache_kernel(const RotaryArgs 
     const int h1 = min(a.H, (unit - t * a.parts + 1) * a.each);
     const uint16_t* const src = a.q + t * a.q_stride;
     uint16_t* const dst = a.out + static_cast<size_t>(t) * a.H * a.D + d;
-    lds->make(a, pos);
     Turn8<INTER> r;
+    if (a.wide_q && a.each <= step) {
+        // One row a lane, on its way with the position (a lane without a head reads
+        // the token's last one): 2013 tokens of 8/8 heads x 64 6.3 us, not 6.9.
+        uint16_t x[8], y[8];
+        load8<INTER>(src + min(h0, a.H - 1) * a.D, d, a.rot, true, x, y);
+        if (pos < 0) return;
+        lds->make(a, pos, freq);
+        r.take(*lds, d, a.rot, a.whole);
+        if (h0 < h1) *reinterpret_cast<u4v*>(dst + h0 * a.D) = rotate8<T, INTER>(r, x, y, d, a.rot);
+        return;
+    }
+    if (pos < 0) return;
+    lds->make(a, pos, freq);
     r.take(*lds, d, a.rot, a.whole);
     if (a.wide_q) {
 #pragma unroll 8
@@ -397,12 +415,12 @@ int swiftllm_hip_rotary_and_cache(void* query_out, const void* query, const void
     a.slices = static_cast<int>((Hkv * D + kWinRows - 1) / kWinRows);
     const int W = small_windows(T, a.slices) ? 4 : 16;
     a.windows = static_cast<int>((T + W - 1) / W);
-    // Long calls have a wave per token, which makes its angles once; short ones
-    // are latency, and a wave takes 1 KB of it. Split / whole, 64/8 heads x 128:
-    // 64 tokens 5.9 / 9.2 us, 600 8.0 / 10.4, 1024 10.3 / 12.4, 2048 17.8 / 16.8,
-    // 4096 31.9 / 29.8; 32/8: 64 6.0 / 6.8, 1024 7.9 / 8.1, 2048 11.9 / 11.3.
+    // Long calls have a wave per token, which makes its angles once; in others a
+    // wave takes 1 KB of it, one row a lane. Split / whole: 64/8 heads x 128 64 tokens
+    // 6.4 / 9.1 us, 1024 9.1 / 12.4, 4096 27.8 / 29.3, 8192 69.6 / 65.7; 32/8 1024
+    // 7.3 / 7.4, 4096 18.8 / 19.0, 8192 35.3 / 34.4, 16384 91 / 87.
     const int step = static_cast<int>(512 / D);
-    a.each = T > 1024 ? num_heads : std::min(num_heads, step);
+    a.each = T > 4096 ? num_heads : std::min(num_heads, step);
     a.parts = (num_heads + a.each - 1) / a.each;
     const long long grid = 2LL * a.windows * a.slices + (T * a.parts + 3) / 4;
     if (grid >= (1LL << 24)) {
