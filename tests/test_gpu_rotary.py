@@ -163,6 +163,19 @@ def test_rotary_prompts(dev, lens, interleaved):
     c.check()
 
 
+@pytest.mark.parametrize("H,D,extra,interleaved", [(24, 64, 0, False), (9, 128, 0, True), (20, 64, 3, False)])
+def test_rotary_long_calls(dev, H, D, extra, interleaved):
+    """Thousands of tokens, more query heads than a wave takes at once, aligned
+    and not, padding among them."""
+    rng = np.random.default_rng(H)
+    pos, slots = _runs(rng, [4000, 1, 150, 30], 4096, 300)
+    pos = np.array(pos)
+    pos[[0, 77, 4100, 4180]] = -1
+    c = Case(rng, pos, slots, H, 1, D, D, "bf16", interleaved, extra=extra, NB=300)
+    c.run()
+    c.check()
+
+
 @pytest.mark.parametrize("dtype", ["f16", "bf16"])
 def test_rotary_far_positions(dev, dtype):
     """Angles of positions up to 2^31 - 1: 32-bit angles would be wrong by turns."""
@@ -192,6 +205,14 @@ def test_rotary_in_place(dev, dtype, rot, interleaved):
     pos, slots = _runs(rng, [50, 1, 20], 900, 12)
     pos[3] = -1
     c = Case(rng, pos, slots, 8, 4, 64, rot, dtype, interleaved, fused=False)
+    c.run(out=c.device[0])
+    c.check(out=c.device[0])
+
+
+def test_rotary_in_place_of_a_long_call(dev):
+    rng = np.random.default_rng(12)
+    pos, slots = _runs(rng, [4090, 60], 900, 280)
+    c = Case(rng, pos, slots, 17, 1, 64, 64, "f16", fused=False, NB=280)
     c.run(out=c.device[0])
     c.check(out=c.device[0])
 
