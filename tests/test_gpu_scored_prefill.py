@@ -157,6 +157,17 @@ def test_prefill_many_sequences(dev, S):
     p.check(f"S {S}")
 
 
+@pytest.mark.parametrize("D", [64, 128])
+@pytest.mark.parametrize("kw", [dict(), dict(cap=20.0), dict(alibi=True), dict(cap=20.0, alibi=True, window=50)])
+def test_prefill_workgroups_of_many_tiles(dev, D, kw):
+    """More tiles of more sequences than stay on the GPU at once: a workgroup's
+    next tile is another sequence's, shorter or longer."""
+    rng = np.random.default_rng(D)
+    p = Prefill(rng, rng.integers(0, 150, 90), 16, 16, D, "f16", cached=rng.integers(0, 70, 90), **kw)
+    p.run()
+    p.check(str(kw))
+
+
 @pytest.mark.parametrize("S", [3, 1100])
 def test_prefill_malformed_offsets_and_lengths(dev, S):
     """Offsets that run backwards or out of the rows have no rows; contexts
