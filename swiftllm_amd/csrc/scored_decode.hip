@@ -637,11 +637,12 @@ int swiftllm_hip_scored_decode(void* output, void* workspace, size_t workspace_b
     // A sequence per workgroup, in one launch, up to `line` blocks: the longest
     // walk as far as the host knows. Whole / cut, 32/8 heads x 128: 1 sequence up
     // to 512 tokens 8.4 / 9.8 us, 1024 11.9 / 9.8; 16 up to 768 12.4 / 15.0, 1024
-    // 16.4 / 16.2, 1280 19.5 / 18.6; 64 up to 1024 34.9 / 39.1; 200 up to 1024
-    // 100.8 / 103.6, 2048 197.5 / 195.2.
+    // 16.4 / 16.2, 1280 19.5 / 18.6; 64 up to 1024 34.9 / 39.1, 1536 50.8 / 54.4;
+    // 200 up to 1536 152.8 / 151.9, 2048 197.5 / 195.2; of 64/8 1536 155.6 / 162.3;
+    // 128 ragged ones in a window of 1024 54.1 / 54.4, of 2048 77.7 / 65.9.
     const int most = window > 0 && !prefix_lens ? std::min(a.MB, window / kBlockTokens + 2) : a.MB;
     const long long items = S * HC;
-    const int line = items > kResident ? 64 : static_cast<int>(std::min<long long>(32 + items / 4, 96));
+    const int line = static_cast<int>(std::min<long long>(32 + items / 4, 96));
     a.ranges = most <= line || l.ranges < 4 ? 0 : l.ranges;
     const size_t lds = sizeof(float) * (D == 128 ? merge_floats<128>(std::min(G, 16)) : merge_floats<64>(std::min(G, 16)));
     using K = void (*)(ScoredDecodeArgs);
