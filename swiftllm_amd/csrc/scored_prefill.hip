@@ -31,11 +31,11 @@
 // longer and 2048 tokens alone 14 %), with the weights still to come and the
 // caps' parts of the next scores among them.
 //
-// Measured: 8 x 2048 tokens, 32/8 heads x 128, with a cap 380 us (720 TFLOP/s;
-// bound by the vector operations), without 314; chunks in a window 280 us (970
-// TFLOP/s; bound by power: 1.6 GHz, matrix unit 58 % and LDS 30 % of the cycles); 24
-// prompts of 52-912 tokens, 16/16 heads, with a bias and prefixes 56 us (short walks,
-// bound by latency).
+// Measured: 8 x 2048 tokens, 32/8 heads x 128, with a cap 368 us (750 TFLOP/s; bound
+// by the vector operations), without 312; chunks in a window 275 us (990 TFLOP/s;
+// bound by power: 1.6 GHz, matrix unit 60 % and LDS 30 % of the cycles); 24 prompts of
+// 52-912 tokens, 16/16 heads, with a bias and prefixes 57 us (short walks, bound by
+// latency).
 //
 // A weight of 0 times a value that is not finite is NaN. So in a stage that
 // some row of the tile does not see whole, such values become zeros in LDS, and
