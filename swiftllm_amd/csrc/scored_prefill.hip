@@ -19,7 +19,9 @@
 // stages behind its last row. A capped score is c - 2 c u with
 // u = 1 / (1 + e^y), y = 2 x / c: two transcendental operations, a third for
 // the weight. Without a bias the score itself is not made: the largest comes
-// from the least u, and the weight is exp2 of one multiply-add of u.
+// from the least u, and the weight is exp2 of one multiply-add of u. A bias in a
+// stage that is seen whole is its first key's, the same for a pair's scores, and
+// a rise over them that 16 registers keep: one operation a score less, 2-4 %.
 // Weights are rounded to 16 bits, to nearest, and summed as rounded: the
 // output's error is that of its own rounding and one of the same size.
 //
@@ -497,6 +499,9 @@ void scored_prefill_kernel(const ScoredPrefillArgs a) {
     constexpr float kHidden = CAP && !BIAS ? INFINITY : -INFINITY;
     const float mul = CAP ? -2.0f * cap : scale;
     const float add = CAP ? cap : 0.0f;
+    float rise[16];   // of the bias over a pair's scores
+#pragma unroll
+    for (int i = 0; i < 16; ++i) rise[i] = BIAS ? slope * static_cast<float>(16 * (i >> 3) + (i & 7)) : 0.0f;
     auto most = [](float x, float y) { return CAP && !BIAS ? fminf(x, y) : fmaxf(x, y); };
     if constexpr (CAP) {
 #pragma unroll
@@ -528,22 +533,25 @@ void scored_prefill_kernel(const ScoredPrefillArgs a) {
                 if ((ok_t >> b) & 1) seen |= bits << (8 * b);
             }
         }
+        // What a pair's scores lack: in a whole stage the bias of its first key.
+        float lack[2] = {add, add};
         if constexpr (BIAS) {
             // Scores in the place of what they are made of: key i lies d0 + off from
             // the row, and d0 + off <= 0 in a whole stage.
             const float d0 = static_cast<float>(base + 8 * h - pos);
-            const float b0 = __builtin_fmaf(slope, d0, CAP ? cap : 0.0f);
-            auto score = [&](auto bias_of) {
+            if (whole) {
+                lack[0] = __builtin_fmaf(slope, d0, add);
+                lack[1] = __builtin_fmaf(slope, d0 + 32.0f, add);
 #pragma unroll
                 for (int i = 0; i < 32; ++i) {
-                    const float bias = bias_of(static_cast<float>(16 * (i >> 3) + (i & 7)));
-                    sc[i >> 4][i & 15] = __builtin_fmaf(sc[i >> 4][i & 15], CAP ? -2.0f * cap : scale, bias);
+                    sc[i >> 4][i & 15] = __builtin_fmaf(sc[i >> 4][i & 15], mul, rise[i & 15]);
                 }
-            };
-            if (whole) {
-                score([&](float off) { return __builtin_fmaf(slope, off, b0); });
             } else {
-                score([&](float off) { return __builtin_fmaf(-slope, __builtin_fabsf(d0 + off), CAP ? cap : 0.0f); });
+#pragma unroll
+                for (int i = 0; i < 32; ++i) {
+                    const float bias = -slope * __builtin_fabsf(d0 + static_cast<float>(16 * (i >> 3) + (i & 7)));
+                    sc[i >> 4][i & 15] = __builtin_fmaf(sc[i >> 4][i & 15], mul, bias);
+                }
             }
         }
         if (!whole) {
@@ -555,15 +563,22 @@ void scored_prefill_kernel(const ScoredPrefillArgs a) {
                 sc[i >> 4][i & 15] = __builtin_bit_cast(float, (v & keep) | (__builtin_bit_cast(int, kHidden) & ~keep));
             }
         }
-        float bm = most(most(sc[0][0], sc[0][1]), sc[0][2]);
+        auto most_of = [&](const f16x& x) {
+            float y = most(most(x[0], x[1]), x[2]);
 #pragma unroll
-        for (int i = 3; i < 31; i += 2) bm = most(most(bm, sc[i >> 4][i & 15]), sc[(i + 1) >> 4][(i + 1) & 15]);
-        bm = most(bm, sc[1][15]);
+            for (int i = 3; i < 15; i += 2) y = most(most(y, x[i]), x[i + 1]);
+            return most(y, x[15]);
+        };
+        float bm;
+        if constexpr (BIAS) {
+            bm = fmaxf(most_of(sc[0]) + lack[0], most_of(sc[1]) + lack[1]);
+        } else {
+            bm = __builtin_fmaf(most(most_of(sc[0]), most_of(sc[1])), mul, add);
+        }
         {
             const auto y = __builtin_amdgcn_permlane32_swap(__builtin_bit_cast(unsigned, bm), __builtin_bit_cast(unsigned, bm), false, false);
-            bm = most(__builtin_bit_cast(float, static_cast<unsigned>(y[0])), __builtin_bit_cast(float, static_cast<unsigned>(y[1])));
+            bm = fmaxf(__builtin_bit_cast(float, static_cast<unsigned>(y[0])), __builtin_bit_cast(float, static_cast<unsigned>(y[1])));
         }
-        if constexpr (!BIAS) bm = __builtin_fmaf(bm, mul, add);
         if (__any(bm > m + kLag)) {
             const float m_new = fmaxf(m, bm);
             const float alpha = m_new == -INFINITY ? 1.0f : __builtin_amdgcn_exp2f(m - m_new);
@@ -573,7 +588,7 @@ void scored_prefill_kernel(const ScoredPrefillArgs a) {
             m = m_new;
         }
         const float c = ((m == -INFINITY) ? 0.0f : m) - kWeightExp;
-        const float add_c = add - c;
+        const float lack_c[2] = {lack[0] - c, lack[1] - c};
         if (cleaned) {
             const u4 bad = *reinterpret_cast<const u4*>(s_bad[t & 1]);
             unsigned keys = 0;   // this lane's, as `seen`
@@ -593,7 +608,7 @@ void scored_prefill_kernel(const ScoredPrefillArgs a) {
 #pragma unroll
             for (int z = 0; z < 2; ++z) {
                 const float v = sc[b >> 1][8 * (b & 1) + 2 * i + z];
-                p[z] = __builtin_amdgcn_exp2f(BIAS ? v - c : __builtin_fmaf(v, mul, add_c));
+                p[z] = __builtin_amdgcn_exp2f(BIAS ? v + lack_c[b >> 1] : __builtin_fmaf(v, mul, lack_c[0]));
             }
             pw[b][i] = T::down2(p[0], p[1]);
             l = add_pair(T{}, pw[b][i], l);
