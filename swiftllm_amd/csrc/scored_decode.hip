@@ -57,6 +57,7 @@ struct ScoredDecodeArgs {
     int MB;
     int num_blocks;
     int ranges;            // 0: every sequence whole
+    bool out8;             // out is 8-byte aligned
 };
 
 constexpr int kWaves = 4;
@@ -203,8 +204,8 @@ __host__ __device__ constexpr int merge_floats(int gs) {
 }
 
 // Blocks i0 .. i1 - 1 of a sequence's walk for one kv head and chunk of query
-// heads, by the whole workgroup. at: the query's row. emit(g, d, o, m, l): normalised output d of
-// head g, and its maximum and sum.
+// heads, by the whole workgroup. at: the query's row. emit(g, d, o, m, l): normalised outputs d ..
+// d + 3 of head g, and its maximum and sum.
 template <typename T, int D, typename Emit>
 __device__ __forceinline__ void run_piece(const ScoredDecodeArgs& a, const Sight& sight, int s, int at, int kvh, int hc, int i0,
                                           int i1, Emit emit) {
@@ -298,22 +299,26 @@ __device__ __forceinline__ void run_piece(const ScoredDecodeArgs& a, const Sight
         }
     }
     __syncthreads();
-    for (int i = tid; i < gn * D; i += 64 * kWaves) {
-        const int g = i / D;
-        const int d = i - g * D;
-        float m = -INFINITY;
+    for (int i = tid; i < gn * (D / 4); i += 64 * kWaves) {
+        const int g = i / (D / 4);
+        const int d = 4 * (i - g * (D / 4));
+        float mx[kWaves], m = -INFINITY;
 #pragma unroll
-        for (int x = 0; x < kWaves; ++x) m = fmaxf(m, sm_m[x * 16 + g]);
-        float num = 0.0f, den = 0.0f;
+        for (int x = 0; x < kWaves; ++x) {
+            mx[x] = sm_m[x * 16 + g];
+            m = fmaxf(m, mx[x]);
+        }
+        f4 num = f4{0, 0, 0, 0};
+        float den = 0.0f;
 #pragma unroll
         for (int x = 0; x < kWaves; ++x) {
             // A wave that saw no key has zeros; one of NaN scores alone a NaN sum.
-            const float mx = sm_m[x * 16 + g];
-            const float f = mx == -INFINITY ? 1.0f : __builtin_amdgcn_exp2f(mx - m);
-            num += f * sm_o[static_cast<size_t>(x * gs + g) * D + d];
+            const float f = mx[x] == -INFINITY ? 1.0f : __builtin_amdgcn_exp2f(mx[x] - m);
+            num += f * *reinterpret_cast<const f4*>(sm_o + static_cast<size_t>(x * gs + g) * D + d);
             den += f * sm_l[x * 16 + g];
         }
-        emit(g, d, den == 0.0f ? 0.0f : num / den, m, den);
+        const float inv = den == 0.0f ? 0.0f : 1.0f / den;
+        emit(g, d, num * inv, m, den);
     }
 }
 
@@ -389,12 +394,19 @@ void scored_decode_kernel(const ScoredDecodeArgs a) {
         }
         const size_t f = static_cast<size_t>(2 * range + slot) * HC + sub;
         const int row = row_of(a, s);
-        run_piece<T, D>(a, sight, s, row, kvh, hc, i0, i1, [&](int g, int d, float o, float m, float l) {
+        run_piece<T, D>(a, sight, s, row, kvh, hc, i0, i1, [&](int g, int d, f4 o, float m, float l) {
             if (whole) {
-                if (row >= 0) a.out[(static_cast<size_t>(row) * a.H + h0 + g) * D + d] = T::down(o);
+                if (row < 0) return;
+                uint16_t* const p = a.out + (static_cast<size_t>(row) * a.H + h0 + g) * D + d;
+                if (a.out8) {
+                    *reinterpret_cast<u2*>(p) = u2{T::down2(o[0], o[1]), T::down2(o[2], o[3])};
+                } else {
+#pragma unroll
+                    for (int z = 0; z < 4; ++z) p[z] = T::down(o[z]);
+                }
                 return;
             }
-            a.frag_o[(f * gs + g) * D + d] = o;
+            *reinterpret_cast<f4*>(a.frag_o + (f * gs + g) * D + d) = o;
             if (d == 0) {
                 a.frag_ml[f * 2 * gs + g] = m;
                 a.frag_ml[f * 2 * gs + gs + g] = l;
@@ -634,6 +646,7 @@ int swiftllm_hip_scored_decode(void* output, void* workspace, size_t workspace_b
     a.nhc = nhc;
     a.MB = max_num_blocks_per_seq;
     a.num_blocks = num_blocks;
+    a.out8 = aligned(output, 8);
     // A sequence per workgroup, in one launch, up to `line` blocks: the longest
     // walk as far as the host knows. Whole / cut, 32/8 heads x 128: 1 sequence up
     // to 512 tokens 8.4 / 9.8 us, 1024 11.9 / 9.8; 16 up to 768 12.4 / 15.0, 1024

@@ -281,6 +281,23 @@ def test_decode_block_offsets_past_32_bits(dev):
     d.check()
 
 
+@pytest.mark.parametrize("ctx", [[33, 1, 300], [4000, 16, 700]])
+@pytest.mark.parametrize("shift", [1, 2, 3])
+def test_decode_output_2_byte_aligned(dev, ctx, shift):
+    """Any alignment of the output gives the same bits, and nothing beside it is written."""
+    d = Decode(np.random.default_rng(19), ctx, 6, 2, 128, "f16", cap=20.0)
+    d.run()
+    d.check()
+    n = d.S * d.H * d.D
+    buf = DeviceArray((n + 8,), np.uint16)
+    buf.fill_byte(0x7F)
+    d.run(out=buf.ptr + 2 * shift)
+    synchronize()
+    got = buf.numpy()
+    assert np.array_equal(got[shift:shift + n], d.out.numpy()[:d.S].ravel())
+    assert (got[:shift] == 0x7F7F).all() and (got[shift + n:] == 0x7F7F).all()
+
+
 def test_decode_leaves_no_trace_between_calls(dev):
     """One workspace for calls of other shapes in turn, and the same call twice: the same bits."""
     a = Decode(np.random.default_rng(12), [3000, 1, 500], 8, 2, 64, "f16", alibi=True)
