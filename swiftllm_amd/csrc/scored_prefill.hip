@@ -85,7 +85,6 @@ constexpr int kListSeqs = 1024;
 // wave stay in range where sequences share rows.
 constexpr int kMostTiles = 1 << 24;
 constexpr long long kCUs = 256;        // MI355X; any grid is correct
-constexpr long long kMostGroups = 1LL << 22;   // 2^30 threads
 // Workgroups of a CU: as registers allow. (At D = 64 two, not three: 40 ragged
 // prompts up to 1500 tokens of 8/8 heads 72 us, not 65.)
 template <int D>
@@ -806,12 +805,13 @@ int swiftllm_hip_scored_prefill(void* output, const void* query, const void* key
     a.num_blocks = num_blocks;
     a.q16 = aligned(query, 16);
     a.out16 = aligned(output, 16);
-    // A list in registers is made in no time, so a tile gets a workgroup of its own
-    // and goes where one ended; a longer one is made once per resident workgroup.
-    // Of their own / resident: 8 x 2048 tokens with a cap 378 / 388 us, 40 ragged
-    // prompts of 8/8 heads x 64 with a cap 79 / 85, without 62 / 64, 700 of 1-60
-    // tokens 190 / 159.
-    const long long resident = S <= 64 ? kMostGroups : kCUs * (D == 128 ? kPerCU<128> : kPerCU<64>);
+    // A list in registers is made in no time, so up to four tiles per resident
+    // workgroup each have one of their own, which goes where another ended; a longer
+    // list is made once per resident workgroup. Four / one: 8 x 2048 tokens with a cap
+    // 378 / 388 us, 40 ragged prompts of 8/8 heads x 64 with a cap 71 / 75, 700 of 1-60
+    // tokens 190 / 159. (One for every tile that num_tokens has room for: 2000 tokens
+    // in 65536 rows 33.5 us, not 17.6.)
+    const long long resident = (S <= 64 ? 4 : 1) * kCUs * (D == 128 ? kPerCU<128> : kPerCU<64>);
     const long long grid = (std::min(items, resident) + 7) / 8 * 8;
     using K = void (*)(ScoredPrefillArgs);
 #define SCORED_PREFILL(T_) \
