@@ -286,17 +286,6 @@ __global__ __launch_bounds__(256) void rotary_and_cache_kernel(const RotaryArgs 
     const uint16_t* const src = a.q + t * a.q_stride;
     uint16_t* const dst = a.out + static_cast<size_t>(t) * a.H * a.D + d;
     Turn8<INTER> r;
-    if (a.wide_q && a.each <= step) {
-        // One row a lane, on its way with the position (a lane without a head reads
-        // the token's last one): 2013 tokens of 8/8 heads x 64 6.3 us, not 6.9.
-        uint16_t x[8], y[8];
-        load8<INTER>(src + min(h0, a.H - 1) * a.D, d, a.rot, true, x, y);
-        if (pos < 0) return;
-        lds->make(a, pos, freq);
-        r.take(*lds, d, a.rot, a.whole);
-        if (h0 < h1) *reinterpret_cast<u4v*>(dst + h0 * a.D) = rotate8<T, INTER>(r, x, y, d, a.rot);
-        return;
-    }
     if (pos < 0) return;
     lds->make(a, pos, freq);
     r.take(*lds, d, a.rot, a.whole);
@@ -416,11 +405,12 @@ int swiftllm_hip_rotary_and_cache(void* query_out, const void* query, const void
     const int W = small_windows(T, a.slices) ? 4 : 16;
     a.windows = static_cast<int>((T + W - 1) / W);
     // Long calls have a wave per token, which makes its angles once; in others a
-    // wave takes 1 KB of it, one row a lane. Split / whole: 64/8 heads x 128 64 tokens
-    // 6.4 / 9.1 us, 1024 9.1 / 12.4, 4096 27.8 / 29.3, 8192 69.6 / 65.7; 32/8 1024
-    // 7.3 / 7.4, 4096 18.8 / 19.0, 8192 35.3 / 34.4, 16384 91 / 87.
+    // wave takes 1 KB of it. Split / whole: 64/8 heads x 128 64 tokens 6.4 / 9.1 us,
+    // 1024 9.1 / 12.4, 2048 15.4 / 16.7, 8192 69.6 / 65.7; 32/8 1024 7.3 / 7.4, 2048
+    // 10.4 / 11.1, 8192 35.3 / 34.4, 16384 91 / 87; but 64 tokens in 4096 rows of
+    // padding 19.7 / 11.
     const int step = static_cast<int>(512 / D);
-    a.each = T > 4096 ? num_heads : std::min(num_heads, step);
+    a.each = T > 1024 ? num_heads : std::min(num_heads, step);
     a.parts = (num_heads + a.each - 1) / a.each;
     const long long grid = 2LL * a.windows * a.slices + (T * a.parts + 3) / 4;
     if (grid >= (1LL << 24)) {
