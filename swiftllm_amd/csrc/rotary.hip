@@ -405,10 +405,11 @@ int swiftllm_hip_rotary_and_cache(void* query_out, const void* query, const void
     const int W = small_windows(T, a.slices) ? 4 : 16;
     a.windows = static_cast<int>((T + W - 1) / W);
     // Long calls have a wave per token, which makes its angles once; in others a
-    // wave takes 1 KB of it. Split / whole: 64/8 heads x 128 64 tokens 6.4 / 9.1 us,
-    // 1024 9.1 / 12.4, 2048 15.4 / 16.7, 8192 69.6 / 65.7; 32/8 1024 7.3 / 7.4, 2048
-    // 10.4 / 11.1, 8192 35.3 / 34.4, 16384 91 / 87; but 64 tokens in 4096 rows of
-    // padding 19.7 / 11.
+    // wave takes 1 KB of it. Split / whole: 64/8 heads x 128 64 tokens 5.8 / 9.0 us,
+    // 1024 10.1 / 12.4, 2048 16.9 / 16.8, 4096 30.3 / 29.1; 32/8 512 6.1 / 7.6, 1024
+    // 7.4 / 7.3, 2048 11.3 / 11.0, 4096 20.1 / 19.0. (A first row asked for with the
+    // position, so that padding is read too: 2048 tokens 10.4 and 15.5 us, 64 in 1024
+    // rows 11.5, not 9.9.)
     const int step = static_cast<int>(512 / D);
     a.each = T > 1024 ? num_heads : std::min(num_heads, step);
     a.parts = (num_heads + a.each - 1) / a.each;
