@@ -80,7 +80,10 @@ constexpr int kWaves = 4;
 constexpr int kStage = 64;             // keys
 // Sequences of the longest-first list, whose lengths fit LDS. In sequence order 8 x
 // 2048 tokens of 32/8 heads x 128 take 413 us, not 319, 700 of 1-60 184, not 159.
+// More sequences go in order, by the tiles of each 64 of them (at most 65535, host).
 constexpr int kListSeqs = 1024;
+constexpr int kCountChunks = 1024;
+static_assert(kCountChunks <= kListSeqs && 64 * kCountChunks >= 65535, "their sums take the list's place");
 // Tiles of a lane's sequences: memory holds the rows of fewer, and sums over a
 // wave stay in range where sequences share rows.
 constexpr int kMostTiles = 1 << 24;
@@ -256,6 +259,60 @@ __device__ __forceinline__ List make_list(const ScoredPrefillArgs& a, int per_wg
     return l;
 }
 
+// Past kListSeqs: the tiles up to and with every 64 sequences, in lds->first. Sums
+// stop above any tile of separate rows, so sequences that share rows, or have
+// none, change nothing for the others. (Found from query_offsets[s] / per_wg + s
+// by bisection, where one offset out of order hides the tiles of others, 2500
+// sequences of 1-30 tokens of 8/2 heads x 64 take 74 us, not 44, 1100 of 1-60 of
+// 32/8 x 128 281, not 215.)
+constexpr int kMostEntries = (1 << 30) - 1;   // (entries are below it, host)
+
+__device__ __forceinline__ int capped_scan(int x) {
+    return dpp_scan(x, 0, [](int a, int b) { return min(a + b, kMostEntries); });
+}
+
+__device__ __forceinline__ int tiles_at(const ScoredPrefillArgs& a, int s, int per_wg) {
+    return s < a.S ? (rows_of(a, s).n + per_wg - 1) / per_wg : 0;
+}
+
+// The number of tiles.
+__device__ __forceinline__ int make_counts(const ScoredPrefillArgs& a, int per_wg, ListLds* lds) {
+    const int lane = threadIdx.x & 63;
+    const int w = threadIdx.x >> 6;
+    const int chunks = (a.S + 63) / 64;
+    for (int c = w; c < chunks; c += kWaves) {
+        const int sum = capped_scan(tiles_at(a, 64 * c + lane, per_wg));
+        if (lane == 63) lds->tiles[c] = sum;
+    }
+    __syncthreads();
+    if (w == 0) {
+        int before = 0;
+        for (int c = 0; c < chunks; c += 64) {
+            const int sum = min(capped_scan(c + lane < chunks ? lds->tiles[c + lane] : 0) + before, kMostEntries);
+            if (c + lane < chunks) lds->first[c + lane] = sum;
+            before = __builtin_amdgcn_readlane(sum, 63);
+        }
+    }
+    __syncthreads();
+    return lds->first[chunks - 1];
+}
+
+// Entry e, below the number of tiles.
+__device__ __forceinline__ void counted_entry(const ScoredPrefillArgs& a, int per_wg, const ListLds* lds, int e, int lane,
+                                              int& tile, int& seq) {
+    constexpr int kEach = kCountChunks / 64;
+    const int last = (a.S + 63) / 64 - 1;
+    // The sums ascend: the first above e, among every 16th and then among 16.
+    const int g = kEach * __popcll(__ballot(lds->first[min(kEach * lane + kEach - 1, last)] <= e));
+    const int c = g + __popcll(__ballot(lane < kEach && lds->first[min(g + lane, last)] <= e));
+    const int k = e - (c > 0 ? lds->first[c - 1] : 0);
+    const int n = tiles_at(a, 64 * c + lane, per_wg);
+    const int upto = capped_scan(n);
+    const int at = __popcll(__ballot(upto <= k));
+    seq = 64 * c + at;
+    tile = k - __builtin_amdgcn_readlane(upto - n, at);
+}
+
 // Bits 0 .. n - 1 of 8.
 __device__ __forceinline__ unsigned low8(int n) { return (1u << min(max(n, 0), 8)) - 1u; }
 
@@ -324,11 +381,10 @@ void scored_prefill_kernel(const ScoredPrefillArgs a) {
     // Workgroups go to the XCDs round-robin, and items are heads-fastest: where
     // the heads are a multiple of 8, an XCD reads the K and V of its own ones.
     const unsigned heads = a.Hkv * a.nhc;
-    // Past kListSeqs sequences the tiles go in order: sequence s has the
-    // entries from query_offsets[s] / per_wg + s on, at least one per tile.
     // (More entries than of separate rows come of sequences that share some.)
     const int most_entries = a.T / per_wg + a.S;
-    const unsigned entries = listed ? max(min(list.count(0, threadIdx.x & 63), most_entries), 0) : most_entries;
+    const int tiles = listed ? list.count(0, threadIdx.x & 63) : make_counts(a, per_wg, &s_list);
+    const unsigned entries = max(min(tiles, most_entries), 0);
     const unsigned total = entries * heads;  // below 2^31 (host)
     // Every other round backwards: who had the longest tile gets the shortest.
     auto item_of = [&](unsigned round) {
@@ -360,14 +416,7 @@ void scored_prefill_kernel(const ScoredPrefillArgs a) {
     if (listed) {
         list.entry(static_cast<int>(e), lane, tile, s);
     } else {
-        int lo = 0, hi = a.S;  // entry lo's first <= e < hi's
-        while (hi - lo > 1) {
-            const int mid = (lo + hi) >> 1;
-            const int at = min(max(a.qoff[mid], 0), a.T) / per_wg + mid;
-            if (at <= static_cast<int>(e)) lo = mid; else hi = mid;
-        }
-        s = lo;
-        tile = static_cast<int>(e) - (min(max(a.qoff[lo], 0), a.T) / per_wg + lo);
+        counted_entry(a, per_wg, &s_list, static_cast<int>(e), lane, tile, s);
     }
     s = __builtin_amdgcn_readfirstlane(s);
     tile = __builtin_amdgcn_readfirstlane(tile);

@@ -389,3 +389,53 @@ def test_prefill_in_a_captured_graph(dev):
         g.launch(stream)
         stream.synchronize()
         p.check(f"{new}")
+
+
+def _with_offsets(rng, S, off, T, **kw):
+    """S sequences of rows off[s] .. off[s + 1] - 1 of T, their whole contexts in the cache."""
+    off = np.asarray(off)
+    n = off[1:] - off[:-1]
+    n[(off[:-1] < 0) | (off[1:] > T)] = 0
+    p = Prefill(rng, np.maximum(n, 0), 8, 8, 64, "f16", tail=0, **kw)
+    p.off, p.T = off.astype(np.int32), T
+    p.q = normal(rng, (T, 8, 64), "f16", 3.0)
+    p.upload()
+    return p
+
+
+def test_prefill_offsets_in_any_order(dev):
+    """More than 1024 sequences whose offsets go back and forth within the rows:
+    the rows of two of them, and a sequence between without any."""
+    S = 1100
+    off = np.full(S + 1, 1280)
+    off[:4] = [1280, 2560, 0, 1280]
+    p = _with_offsets(np.random.default_rng(18), S, off, 2560, window=50)
+    p.run()
+    assert p.rows().all()
+    p.check()
+
+
+@pytest.mark.parametrize("S", [1000, 1100])
+@pytest.mark.parametrize("at", [275, 550, 825])
+@pytest.mark.parametrize("bad", [-1, -(1 << 31), 1109, 10 ** 6, 2 ** 31 - 1])
+def test_prefill_one_bad_offset_among_many(dev, S, at, bad):
+    """It takes the rows of the two sequences that it belongs to and no other."""
+    off = 3 + np.arange(S + 1)
+    off[at] = bad
+    p = _with_offsets(np.random.default_rng(19), S, off, S + 8)
+    p.run()
+    assert p.rows().sum() == S - 2
+    p.check()
+
+
+@pytest.mark.parametrize("S", [1025, 4096, 4097, 20000, 65535])
+@pytest.mark.parametrize("H,Hkv", [(8, 8), (8, 1), (3, 1)])
+def test_prefill_few_tokens_among_many_sequences(dev, S, H, Hkv):
+    """Mostly sequences without tokens, with one or two tiles or more at either end and at random."""
+    rng = np.random.default_rng(S)
+    new = np.zeros(S, np.int64)
+    new[rng.choice(S, 100, replace=False)] = rng.integers(1, 40, 100)
+    new[[0, 63, 64, S - 1]] = [130, 1, 300, 65]
+    p = Prefill(rng, new, H, Hkv, 64, "bf16", cap=20.0, lead=3)
+    p.run()
+    p.check(f"S {S}")
