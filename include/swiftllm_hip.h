@@ -510,9 +510,9 @@ int swiftllm_hip_rotary_and_cache(
  *   minus alibi_slopes[h] * |p - j| (float [num_heads]; NULL: none).
  * Outputs are the softmax-weighted sums of the seen values with kv head
  * h / (num_heads / num_kv_heads), 32-bit sums rounded once. Blocks whose id is
- * outside [0, num_blocks) (num_blocks <= 0: no upper bound) hold no key;
- * context lengths are cut at max_num_blocks_per_seq * 16. A query that sees no
- * key writes zeros. Cache slots that no query of the call sees may hold
+ * outside [0, num_blocks) (num_blocks <= 0: no upper bound) hold no key, and
+ * there are none past max_num_blocks_per_seq * 16: of a longer context the
+ * queries keep their positions. A query that sees no key writes zeros. Cache slots that no query of the call sees may hold
  * anything, NaN included. A key that is not finite makes the outputs of the
  * queries that see it NaN or unspecified, a value that is not finite one
  * element of them, or all, not finite; other queries are not touched. dtype is

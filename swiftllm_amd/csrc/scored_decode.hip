@@ -76,7 +76,10 @@ __device__ __forceinline__ int row_of(const ScoredDecodeArgs& a, int s) {
 }
 
 // What the query of a sequence sees, in blocks: the walk takes blocks 0 ..
-// before - 1 (the prefix) and then those from `low / 16` on.
+// before - 1 (the prefix) and then those from `low / 16` on. The keys end with
+// the table, at L; of a longer context the query keeps its position, and a window
+// of it may lie past them all (low = L). (A bias's distances are taken from key
+// L - 1: what they lack is the same for every key.)
 struct Sight {
     int L, low, pre, before, skip, n;
     __device__ __forceinline__ int block(int i) const { return i < before ? i : i + skip; }
@@ -89,8 +92,9 @@ struct Sight {
 
 __device__ __forceinline__ Sight sight_of(const ScoredDecodeArgs& a, int s) {
     Sight v;
-    v.L = row_of(a, s) < 0 ? 0 : min(max(as_const(a.ctx)[s], 0), a.MB * kBlockTokens);
-    v.low = a.shape.window > 0 ? max(v.L - a.shape.window, 0) : 0;
+    const int ctx = row_of(a, s) < 0 ? 0 : max(as_const(a.ctx)[s], 0);
+    v.L = min(ctx, a.MB * kBlockTokens);
+    v.low = a.shape.window > 0 ? min(max(ctx - a.shape.window, 0), v.L) : 0;
     v.pre = a.shape.prefix != nullptr ? min(max(as_const(a.shape.prefix)[s], 0), v.L) : 0;
     const int first = v.low >> kBlockShift;
     v.before = min((v.pre + kBlockTokens - 1) >> kBlockShift, first);
