@@ -14,6 +14,7 @@
 #pragma once
 
 #include <cmath>
+#include <type_traits>
 
 #include "half_types.hpp"
 
@@ -23,6 +24,15 @@ namespace scored {
 constexpr float kLog2e = 1.4426950408889634f;
 
 constexpr float kMostCap = 1024.0f;
+
+// Weights are 2^weight_exp * exp2(score - m): m may lag the maximum by kLag
+// (log2 units) before the sums are rescaled. In fp16 they stay below 2^15, so
+// that small ones are as far from its subnormals as can be; bfloat16 reaches as
+// far down as 32 bits do, and there they stay at 1 and below: a weight times the
+// type's largest value is still a number.
+constexpr float kLag = 8.0f;
+template <typename T>
+constexpr float weight_exp = std::is_same<T, F16>::value ? 7.0f : -kLag;
 
 struct Shape {
     float scale;         // no cap: scale * log2(e); cap: 2 log2(e) scale / cap

@@ -127,11 +127,6 @@ __device__ __forceinline__ float sum_over_groups(float v) {
     return __builtin_bit_cast(float, static_cast<unsigned>(b[0])) + __builtin_bit_cast(float, static_cast<unsigned>(b[1]));
 }
 
-// Weights are 2^kWeightExp * exp2(score - m): m may lag the maximum by
-// kLag (log2 units) before the sums are rescaled, so they stay below 2^15.
-constexpr float kWeightExp = 7.0f;
-constexpr float kLag = 8.0f;
-
 // One block for the wave's 16 query heads. Lane (r, kg) has rows 16 J + r,
 // tokens 4 kg .. + 3 of K and V. seen: the block's visible tokens; from:
 // its first token's position minus the query's.
@@ -184,7 +179,7 @@ __device__ __forceinline__ void attend(State<D>& st, unsigned seen, int from, in
         st.l *= alpha;
         st.m = m_new;
     }
-    const float c = (st.m == -INFINITY ? 0.0f : st.m) - kWeightExp;
+    const float c = (st.m == -INFINITY ? 0.0f : st.m) - weight_exp<T>;
     float p[4];
 #pragma unroll
     for (int i = 0; i < 4; ++i) p[i] = __builtin_amdgcn_exp2f(sv[i] - c);

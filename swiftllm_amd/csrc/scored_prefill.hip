@@ -92,10 +92,6 @@ constexpr long long kCUs = 256;        // MI355X; any grid is correct
 // prompts up to 1500 tokens of 8/8 heads 72 us, not 65.)
 template <int D>
 constexpr int kPerCU = D == 128 ? 2 : 3;
-// Weights are 2^kWeightExp * exp2(score - m): m may lag the maximum by kLag
-// (log2 units) before the sums are rescaled, so they stay below 2^15.
-constexpr float kWeightExp = 7.0f;
-constexpr float kLag = 8.0f;
 
 typedef __attribute__((address_space(3))) s4 lds_s4;
 
@@ -635,7 +631,7 @@ void scored_prefill_kernel(const ScoredPrefillArgs a) {
             l *= alpha;
             m = m_new;
         }
-        const float c = ((m == -INFINITY) ? 0.0f : m) - kWeightExp;
+        const float c = ((m == -INFINITY) ? 0.0f : m) - weight_exp<T>;
         const float lack_c[2] = {lack[0] - c, lack[1] - c};
         if (cleaned) {
             const u4 bad = *reinterpret_cast<const u4*>(s_bad[t & 1]);

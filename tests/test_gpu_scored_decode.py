@@ -378,3 +378,32 @@ def test_decode_rows_of_a_packed_step(dev, wide):
     for s, r in rows.items():
         assert (np.abs(to_float(got[r], "f16") - want[s]) <= bound[s]).all()
     assert (np.delete(got, list(rows.values()), axis=0) == 0x7F7F).all()
+
+
+@pytest.mark.parametrize("ctx", [[1, 20, 64, 100], [3000, 40, 7]])
+@pytest.mark.parametrize("kw", [dict(), dict(cap=20.0, alibi=True)])
+def test_decode_of_large_values(dev, ctx, kw):
+    """bfloat16 has values near 2^128: a weighted mean of values of 2^116, at
+    most 2^121 of them, is a number like any other."""
+    d = Decode(np.random.default_rng(20), ctx, 8, 2, 64, "bf16", **kw)
+    for s, n in enumerate(ctx):
+        for i in range(-(-n // 16)):
+            t = np.arange(min(n - 16 * i, 16))
+            b = d.bt[s, i]
+            d.vc[b][:, :, t] = normal(np.random.default_rng(i), (2, 64, t.size), "bf16", 2.0 ** 116)
+    d.upload()
+    d.run()
+    d.check()
+
+
+def test_decode_of_the_largest_value(dev):
+    """One key: its value, whatever it is."""
+    d = Decode(np.random.default_rng(21), [1, 1], 8, 2, 64, "bf16")
+    top = to_half(np.array([2.0 ** 127 * (2 - 2.0 ** -7)]), "bf16")[0]
+    for s in range(2):
+        d.vc[d.bt[s, 0], :, :, 0] = top if s == 0 else top | 0x8000
+    d.upload()
+    d.run()
+    synchronize()
+    got = d.out.numpy()
+    assert (got[0] == top).all() and (got[1] == (top | 0x8000)).all()

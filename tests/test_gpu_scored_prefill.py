@@ -439,3 +439,29 @@ def test_prefill_few_tokens_among_many_sequences(dev, S, H, Hkv):
     p = Prefill(rng, new, H, Hkv, 64, "bf16", cap=20.0, lead=3)
     p.run()
     p.check(f"S {S}")
+
+
+@pytest.mark.parametrize("kw", [dict(), dict(cap=20.0), dict(alibi=True), dict(window=70, prefix=[40, 3, 1])])
+@pytest.mark.parametrize("D", [64, 128])
+def test_prefill_of_large_values(dev, kw, D):
+    """bfloat16 has values near 2^128: a weighted mean of values of 2^116, at
+    most 2^121 of them, is a number like any other."""
+    p = Prefill(np.random.default_rng(20), [150, 64, 1], 8, 2, D, "bf16", cached=[70, 0, 0], **kw)
+    hidden = p.vc == NAN16
+    p.vc = np.where(hidden, p.vc, normal(np.random.default_rng(21), p.vc.shape, "bf16", 2.0 ** 116))
+    p.upload()
+    p.run()
+    p.check()
+
+
+def test_prefill_of_the_largest_value(dev):
+    """One key: its value, whatever it is."""
+    p = Prefill(np.random.default_rng(22), [1, 1], 8, 2, 64, "bf16", tail=0)
+    top = to_half(np.array([2.0 ** 127 * (2 - 2.0 ** -7)]), "bf16")[0]
+    for s in range(2):
+        p.vc[p.bt[s, 0], :, :, 0] = top if s == 0 else top | 0x8000
+    p.upload()
+    p.run()
+    synchronize()
+    got = p.out.numpy()
+    assert (got[0] == top).all() and (got[1] == (top | 0x8000)).all()
