@@ -836,9 +836,10 @@ int swiftllm_hip_scored_prefill(void* output, const void* query, const void* key
     if (T == 0 || S == 0) return ok();
     // The sign of the scale goes into the query, and a scale of zero makes it
     // zero: the kernel's scale is positive, so that raw products order as scores.
+    // (Of products of zero any finite one does; 1 / softcap may be none.)
     a.q_and = scale == 0.0f ? 0u : 0xffffffffu;
     a.q_xor = scale < 0.0f ? 0x80008000u : 0u;
-    if (scale == 0.0f) scored::make_shape(a.shape, 1.0f, softcap, window, prefix_lens, alibi_slopes);
+    if (scale == 0.0f) a.shape.scale = 1.0f;
     a.out = static_cast<uint16_t*>(output);
     a.q = static_cast<const uint16_t*>(query);
     a.kc = static_cast<const uint16_t*>(key_cache);

@@ -407,3 +407,12 @@ def test_decode_of_the_largest_value(dev):
     synchronize()
     got = d.out.numpy()
     assert (got[0] == top).all() and (got[1] == (top | 0x8000)).all()
+
+
+@pytest.mark.parametrize("cap", [0.0, 1e-39, 20.0])
+def test_decode_scale_of_zero(dev, cap):
+    """Every key counts the same, whatever the cap."""
+    d = Decode(np.random.default_rng(22), [70, 5], 8, 2, 64, "f16", scale=0.0, cap=cap)
+    d.run()
+    d.score["softcap"] = 0.0
+    d.check()

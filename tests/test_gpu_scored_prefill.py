@@ -465,3 +465,12 @@ def test_prefill_of_the_largest_value(dev):
     synchronize()
     got = p.out.numpy()
     assert (got[0] == top).all() and (got[1] == (top | 0x8000)).all()
+
+
+@pytest.mark.parametrize("kw", [dict(cap=0.0), dict(cap=1e-39), dict(cap=1e-39, alibi=True), dict(cap=20.0)])
+def test_prefill_scale_of_zero(dev, kw):
+    """Every key counts the same but for its bias, whatever the cap."""
+    p = Prefill(np.random.default_rng(23), [90, 5], 8, 2, 64, "f16", scale=0.0, **kw)
+    p.run()
+    p.score["softcap"] = 0.0
+    p.check()
