@@ -233,7 +233,7 @@ __device__ __forceinline__ List make_list(const ScoredPrefillArgs& a, int per_wg
     const auto tiles_of = [&](int s, int& n, int& f) {
         const Rows r = rows_of(a, s);
         n = (r.n + per_wg - 1) / per_wg;
-        f = max(a.ctx[s] - r.n, 0) / per_wg;
+        f = (max(a.ctx[s], r.n) - r.n) / per_wg;
     };
     if (a.S <= 64) {
         if (lane < a.S) tiles_of(lane, l.tiles, l.first);
@@ -421,8 +421,8 @@ void scored_prefill_kernel(const ScoredPrefillArgs a) {
     const int yy = static_cast<int>(item - e * heads);
     const int kvh = yy / a.nhc;
     const int hc = yy - kvh * a.nhc;
-    const int ctx = as_const(a.ctx)[s];
-    const int L = min(max(ctx, 0), a.MB * kBlockTokens);
+    const int ctx = max(as_const(a.ctx)[s], 0);          // (below 0 as 0: no position either way)
+    const int L = min(ctx, a.MB * kBlockTokens);
     const int pre = a.shape.prefix != nullptr ? min(max(as_const(a.shape.prefix)[s], 0), L) : 0;
     // A window of every key is the same as none.
     const int window = a.shape.window > 0 ? a.shape.window : 0x7fffffff;

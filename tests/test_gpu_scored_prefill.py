@@ -474,3 +474,16 @@ def test_prefill_scale_of_zero(dev, kw):
     p.run()
     p.score["softcap"] = 0.0
     p.check()
+
+
+@pytest.mark.parametrize("S", [3, 70, 1100])
+@pytest.mark.parametrize("ctx", [-(1 << 31), -(1 << 31) + 20, -1])
+def test_prefill_lengths_far_below_zero(dev, S, ctx):
+    """Their rows are zero, and the sum of a length and a row count stays a number."""
+    p = Prefill(np.random.default_rng(24), [40, 300] + [2] * (S - 2), 8, 2, 64, "f16", alibi=True, window=9,
+                prefix=[4] * S)
+    p.ctx[[1, S - 1]] = ctx
+    p.upload()
+    p.run()
+    p.check()
+    assert (p.out.numpy()[p.off[1]:p.off[2]] == 0).all()
