@@ -485,7 +485,8 @@ int swiftllm_hip_plan_step(int32_t* block_tables, const int32_t* cached_lens,
  * rotary_dim (even, 0 to head_dim) stay. inv_freq: double
  * [rotary_dim / 2] in device memory, radians per position. query, key and
  * value [T, heads * head_dim] with a stride in elements between tokens (a
- * fused projection is three such views); query_out [T, num_heads, head_dim]
+ * fused projection is three such views), at most 2^40, and from the first
+ * token to the last at most 2^46; query_out [T, num_heads, head_dim]
  * packed, which may be query itself where query_stride is num_heads *
  * head_dim and may overlap no input otherwise. Angles are reduced in 64 bits.
  * A token with a negative position is padding: no row of it is written. One

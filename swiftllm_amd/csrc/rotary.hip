@@ -353,11 +353,14 @@ int swiftllm_hip_rotary_and_cache(void* query_out, const void* query, const void
     if (H > 65535 || Hkv > 65535) {
         return fail(SWIFTLLM_ERR_NOT_SUPPORTED, "%s: num_heads=%d num_kv_heads=%d", who, num_heads, num_kv_heads);
     }
-    const long long most = 1LL << 40;  // elements; a token's offset in bytes stays far below 2^63
+    // Elements between tokens, and from the first to the last: 2^47 bytes hold any
+    // tensor, so offsets and the sums of one with a pointer stay below 2^63.
+    const long long most = 1LL << 40, most_all = 1LL << 46;
     if (query_stride < H * D || key_stride < Hkv * D || value_stride < Hkv * D || query_stride > most ||
-        key_stride > most || value_stride > most) {
-        return fail(SWIFTLLM_ERR_INVALID_PARAMETER, "%s: query_stride=%lld key_stride=%lld value_stride=%lld", who,
-                    query_stride, key_stride, value_stride);
+        key_stride > most || value_stride > most ||
+        (T > 1 && std::max({query_stride, key_stride, value_stride}) > most_all / (T - 1))) {
+        return fail(SWIFTLLM_ERR_INVALID_PARAMETER, "%s: num_tokens=%d query_stride=%lld key_stride=%lld value_stride=%lld",
+                    who, num_tokens, query_stride, key_stride, value_stride);
     }
     if (T > 0 && (!query_out || !query || !key || !value || !key_cache || !value_cache || !positions ||
                   !slot_mapping || (rotary_dim > 0 && !inv_freq))) {

@@ -155,3 +155,12 @@ def test_inv_freq_kinds():
         step.rotary_inv_freq(3)
     with pytest.raises(pa.InvalidParameter):
         step.rotary_inv_freq(64, factor=0.0)
+
+
+@pytest.mark.parametrize("name", ["query_stride", "key_stride", "value_stride"])
+def test_rotary_refuses_strides_past_any_memory(name):
+    """Each within its bound, but not the last token's offset."""
+    far = dict(query_out=1 << 44, query=2 << 44, key=3 << 44, value=4 << 44)
+    for T, stride in ((1 << 24, 1 << 40), ((1 << 23) + 1, 1 << 40), (66, 1 << 40), ((1 << 20) + 2, 1 << 26)):
+        assert _rotary(num_tokens=T, **far, **{name: stride}) == INVALID, (T, stride, _lib.last_error())
+        assert f"num_tokens={T}" in _lib.last_error()[1]
