@@ -488,7 +488,8 @@ int swiftllm_hip_plan_step(int32_t* block_tables, const int32_t* cached_lens,
  * fused projection is three such views), at most 2^40, and from the first
  * token to the last at most 2^46; query_out [T, num_heads, head_dim]
  * packed, which may be query itself where query_stride is num_heads *
- * head_dim and may overlap no input otherwise. Angles are reduced in 64 bits.
+ * head_dim and may overlap no other argument otherwise. Angles are reduced in
+ * 64 bits.
  * A token with a negative position is padding: no row of it is written. One
  * whose slot is negative or outside [0, num_blocks * 16) (num_blocks <= 0: no
  * upper bound) has its queries written and nothing else. The slots of a call
@@ -518,7 +519,8 @@ int swiftllm_hip_rotary_and_cache(
  * queries that see it NaN or unspecified, a value that is not finite one
  * element of them, or all, not finite; other queries are not touched. dtype is
  * that of query, caches and output; scale and softcap are finite, softcap 0 to
- * 1024. output may be query itself and overlaps no other argument. */
+ * 1024. output may be query itself and overlaps no other argument (of caches
+ * that is checked where num_blocks is given). */
 
 /* One new token per sequence: the query of sequence s, at position
  * context_lens[s] - 1 (context_lens[s] <= 0: zeros), is row s of query and

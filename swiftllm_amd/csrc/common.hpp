@@ -5,6 +5,7 @@
 
 #include <cstddef>
 #include <cstdint>
+#include <initializer_list>
 
 #include "swiftllm_hip.h"
 
@@ -60,6 +61,22 @@ __device__ __forceinline__ void wait_vm() {
 inline bool overlap(const void* p, size_t n, const void* q, size_t m) {
     const uintptr_t a = reinterpret_cast<uintptr_t>(p), b = reinterpret_cast<uintptr_t>(q);
     return n > 0 && m > 0 && a < b + m && b < a + n;
+}
+
+// The bytes of an argument; none where it is null or its size is not known.
+struct Bytes {
+    const void* p;
+    size_t n;
+};
+inline bool overlap_any(Bytes x, std::initializer_list<Bytes> others) {
+    for (const Bytes& o : others) {
+        if (x.p && o.p && overlap(x.p, x.n, o.p, o.n)) return true;
+    }
+    return false;
+}
+// Of a paged cache of 16-bit values.
+inline size_t cache_bytes(long long num_blocks, long long num_kv_heads, long long head_dim) {
+    return num_blocks > 0 ? static_cast<size_t>(num_blocks) * num_kv_heads * head_dim * 16 * 2 : 0;
 }
 
 inline bool aligned(const void* p, size_t bytes) {

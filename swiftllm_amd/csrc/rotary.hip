@@ -308,15 +308,10 @@ __global__ __launch_bounds__(256) void rotary_and_cache_kernel(const RotaryArgs 
     }
 }
 
-// [first, last) bytes of `tokens` rows of n values, `stride` values apart.
-struct Span {
-    uintptr_t first, last;
-};
-Span span_of(const void* p, long long tokens, long long n, long long stride) {
-    const uintptr_t b = reinterpret_cast<uintptr_t>(p);
-    return Span{b, b + 2 * static_cast<uintptr_t>((tokens - 1) * stride + n)};
+// The bytes of `tokens` rows of n values, `stride` values apart.
+Bytes rows_of(const void* p, long long tokens, long long n, long long stride) {
+    return Bytes{p, 2 * static_cast<size_t>((tokens - 1) * stride + n)};
 }
-bool meet(Span a, Span b) { return a.first < b.last && b.first < a.last; }
 
 }  // namespace
 }  // namespace swiftllm
@@ -372,12 +367,16 @@ int swiftllm_hip_rotary_and_cache(void* query_out, const void* query, const void
         return fail(SWIFTLLM_ERR_INVALID_PARAMETER, "%s: misaligned pointer", who);
     }
     if (T > 0) {
-        // In place is fine; any other overlap would be read after it is written.
-        const Span o = span_of(query_out, T, H * D, H * D);
+        // In place is fine; any other overlap would be read, or written again, after
+        // it is written. (Of caches, where their size is known.)
+        const Bytes o = rows_of(query_out, T, H * D, H * D), q = rows_of(query, T, H * D, query_stride);
+        const Bytes k = rows_of(key, T, Hkv * D, key_stride), v = rows_of(value, T, Hkv * D, value_stride);
+        const Bytes pos{positions, 4 * static_cast<size_t>(T)}, slots{slot_mapping, 4 * static_cast<size_t>(T)};
+        const Bytes freq{inv_freq, 4 * static_cast<size_t>(rotary_dim)};
+        const Bytes kc{key_cache, cache_bytes(num_blocks, Hkv, D)}, vc{value_cache, kc.n};
         const bool in_place = query_out == query && query_stride == H * D;
-        if ((!in_place && meet(o, span_of(query, T, H * D, query_stride))) ||
-            meet(o, span_of(key, T, Hkv * D, key_stride)) || meet(o, span_of(value, T, Hkv * D, value_stride))) {
-            return fail(SWIFTLLM_ERR_INVALID_PARAMETER, "%s: query_out overlaps an input", who);
+        if ((!in_place && overlap_any(o, {q})) || overlap_any(o, {k, v, pos, slots, freq, kc, vc})) {
+            return fail(SWIFTLLM_ERR_INVALID_PARAMETER, "%s: query_out overlaps another argument", who);
         }
     }
     RotaryArgs a{};

@@ -616,12 +616,18 @@ int swiftllm_hip_scored_decode(void* output, void* workspace, size_t workspace_b
         return fail(SWIFTLLM_ERR_NOT_SUPPORTED, "%s: num_seqs=%d num_heads=%d", who, num_seqs, num_heads);
     }
     // A workgroup has read its queries before it or a later kernel writes their
-    // rows; rows of others must not be among them.
-    const size_t rows = static_cast<size_t>(query_offsets ? num_tokens : num_seqs);
-    const size_t values = rows * num_heads * head_dim * 2;
-    if ((output != query && overlap(output, values, query, values)) || overlap(workspace, l.bytes, output, values) ||
-        overlap(workspace, l.bytes, query, values)) {
-        return fail(SWIFTLLM_ERR_INVALID_PARAMETER, "%s: output or workspace overlaps another argument", who);
+    // rows; rows of others, and what every workgroup reads, must not be among them.
+    if (num_seqs > 0) {
+        const size_t n = num_seqs, rows = query_offsets ? static_cast<size_t>(num_tokens) : n;
+        const Bytes out{output, rows * num_heads * head_dim * 2}, q{query, out.n}, ws{workspace, l.bytes};
+        const Bytes kc{key_cache, cache_bytes(num_blocks, num_kv_heads, head_dim)}, vc{value_cache, kc.n};
+        const Bytes bt{block_tables, 4 * n * max_num_blocks_per_seq}, ctx{context_lens, 4 * n};
+        const Bytes off{query_offsets, 4 * (n + 1)}, pre{prefix_lens, 4 * n};
+        const Bytes slopes{alibi_slopes, 4 * static_cast<size_t>(num_heads)};
+        if ((output != query && overlap_any(out, {q})) || overlap_any(out, {kc, vc, bt, ctx, off, pre, slopes}) ||
+            overlap_any(ws, {out, q, kc, vc, bt, ctx, off, pre, slopes})) {
+            return fail(SWIFTLLM_ERR_INVALID_PARAMETER, "%s: output or workspace overlaps another argument", who);
+        }
     }
     rc = require_device();
     if (rc != SWIFTLLM_OK) return rc;

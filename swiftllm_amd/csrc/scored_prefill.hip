@@ -812,12 +812,6 @@ int swiftllm_hip_scored_prefill(void* output, const void* query, const void* key
         !aligned(alibi_slopes, 4) || !aligned(prefix_lens, 4)) {
         return fail(SWIFTLLM_ERR_INVALID_PARAMETER, "%s: misaligned pointer", who);
     }
-    // A wave has read its queries before it writes their rows; rows of others
-    // must not be among them.
-    const size_t values = static_cast<size_t>(T) * H * D * 2;
-    if (output != query && overlap(output, values, query, values)) {
-        return fail(SWIFTLLM_ERR_INVALID_PARAMETER, "%s: output overlaps query", who);
-    }
     a.S = num_seqs;
     a.T = num_tokens;
     a.H = num_heads;
@@ -830,6 +824,19 @@ int swiftllm_hip_scored_prefill(void* output, const void* query, const void* key
     const long long items = (T / (kWaves * a.tpw) + S) * heads;
     if (items >= (1LL << 30)) {
         return fail(SWIFTLLM_ERR_NOT_SUPPORTED, "%s: num_tokens=%lld of %lld kv heads", who, T, Hkv);
+    }
+    // A wave has read its queries before it writes their rows; rows of others, and
+    // what every workgroup reads, must not be among them.
+    if (T > 0 && S > 0) {
+        const size_t n = num_seqs;
+        const Bytes out{output, static_cast<size_t>(T) * H * D * 2}, q{query, out.n};
+        const Bytes kc{key_cache, cache_bytes(num_blocks, Hkv, D)}, vc{value_cache, kc.n};
+        const Bytes bt{block_tables, 4 * n * max_num_blocks_per_seq}, ctx{context_lens, 4 * n};
+        const Bytes off{query_offsets, 4 * (n + 1)}, pre{prefix_lens, 4 * n};
+        const Bytes slopes{alibi_slopes, 4 * static_cast<size_t>(H)};
+        if ((output != query && overlap_any(out, {q})) || overlap_any(out, {kc, vc, bt, ctx, off, pre, slopes})) {
+            return fail(SWIFTLLM_ERR_INVALID_PARAMETER, "%s: output overlaps another argument", who);
+        }
     }
     const int rc = require_device();
     if (rc != SWIFTLLM_OK) return rc;

@@ -147,3 +147,29 @@ def test_oracle_without_shaping_is_plain_attention():
     slots = np.concatenate([pa.get_slot_mapping(bt[0], 16, 0, 50), pa.get_slot_mapping(bt[1], 16, 0, 17)])
     got = oracle.scored_attention(qp, kc, vc, bt, ctx, [0, 50, 67], 0.125)
     assert np.allclose(got, oracle.prefill_numpy(qp, kc, vc, slots, ctx, 0.125), rtol=1e-12, atol=1e-14)
+
+
+_SIZES = dict(num_seqs=3, num_heads=8, num_kv_heads=2, head_dim=64, max_num_blocks_per_seq=4, num_blocks=5)
+
+
+@pytest.mark.parametrize("name,nbytes", [
+    ("key_cache", 5 * 2 * 64 * 16 * 2), ("value_cache", 5 * 2 * 64 * 16 * 2), ("block_tables", 3 * 4 * 4),
+    ("context_lens", 3 * 4), ("query_offsets", 4 * 4), ("alibi_slopes", 8 * 4), ("prefix_lens", 3 * 4)])
+def test_outputs_on_any_other_argument_are_refused(name, nbytes):
+    """The output, and the decode's workspace, from the argument's first byte to its last."""
+    M = 1 << 32
+    names = ["query", "key_cache", "value_cache", "block_tables", "context_lens", "query_offsets", "alibi_slopes",
+             "prefix_lens"]
+    at = {n: (i + 2) * M for i, n in enumerate(names)}
+    ws = step.scored_decode_workspace_size(3, 8, 2, 64, 16, 4)
+    out = 10 * 8 * 64 * 2
+    last = at[name] + (nbytes - 1) // 16 * 16
+    for where in (at[name] - out + 16, at[name], last):
+        assert _prefill(output=where, **at, **_SIZES) == INVALID
+        assert "overlaps" in _lib.last_error()[1]
+        assert _decode(output=where, workspace=M, num_tokens=10, **at, **_SIZES) == INVALID
+        assert "overlaps" in _lib.last_error()[1]
+    for where in (at[name] - (ws - 1) // 256 * 256, at[name]):
+        assert _decode(output=1 << 20, workspace=where, workspace_bytes=1 << 40, num_tokens=10, **at,
+                       **_SIZES) == INVALID
+        assert "overlaps" in _lib.last_error()[1]

@@ -164,3 +164,15 @@ def test_rotary_refuses_strides_past_any_memory(name):
     for T, stride in ((1 << 24, 1 << 40), ((1 << 23) + 1, 1 << 40), (66, 1 << 40), ((1 << 20) + 2, 1 << 26)):
         assert _rotary(num_tokens=T, **far, **{name: stride}) == INVALID, (T, stride, _lib.last_error())
         assert f"num_tokens={T}" in _lib.last_error()[1]
+
+
+@pytest.mark.parametrize("name,nbytes", [
+    ("positions", 5 * 4), ("slot_mapping", 5 * 4), ("inv_freq", 32 * 8), ("key_cache", 3 * 2 * 64 * 16 * 2),
+    ("value_cache", 3 * 2 * 64 * 16 * 2), ("key", 5 * 128 * 2), ("value", 5 * 128 * 2)])
+def test_rotary_refuses_queries_out_on_any_other_argument(name, nbytes):
+    at = {"positions": 7 * P, "slot_mapping": 8 * P, "inv_freq": 9 * P, "key_cache": 5 * P, "value_cache": 6 * P,
+          "key": 3 * P, "value": 4 * P}[name]
+    out = 5 * 512 * 2
+    for where in (at - out + 8, at, at + nbytes - 2):
+        assert _rotary(query_out=where, num_blocks=3) == INVALID
+        assert "overlaps" in _lib.last_error()[1]
