@@ -224,8 +224,8 @@ class AttentionStep:
     graph; steps that overlap take an object each.
 
         step = AttentionStep(num_seqs, num_tokens, max_blocks, H, Hkv, D, score, inv_freq)
-        step.plan(tables, cached, new, free, num_free)     # once per step
-        step.layer(q, k, v, key_cache, value_cache, out)   # every layer
+        step.plan(tables, cached, new, free, num_free, free_capacity)   # once per step
+        step.layer(q, k, v, key_cache, value_cache, out)                # every layer
 
     num_seqs and num_tokens are capacities: sequences past a batch have
     cached and new lengths of 0, rows past its tokens are left as they are.

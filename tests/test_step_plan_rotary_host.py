@@ -2,7 +2,10 @@
 checks, the rotary frequencies, and the oracle's plan against the host routine
 that it generalises."""
 
+import ast
+import inspect
 import math
+import re
 
 import numpy as np
 import pytest
@@ -176,3 +179,16 @@ def test_rotary_refuses_queries_out_on_any_other_argument(name, nbytes):
     for where in (at - out + 8, at, at + nbytes - 2):
         assert _rotary(query_out=where, num_blocks=3) == INVALID
         assert "overlaps" in _lib.last_error()[1]
+
+
+def test_documented_calls_of_a_step_are_calls():
+    """The example of AttentionStep's docstring: every call fits its signature."""
+    doc = inspect.getdoc(step.AttentionStep)
+    lines = re.findall(r"^ +(?:step = AttentionStep|step\.\w+)\(.*?\)(?= *(?:#|$))", doc, flags=re.M)
+    assert len(lines) == 3
+    for line in lines:
+        call = ast.walk(ast.parse(line.strip()))
+        call = next(n for n in call if isinstance(n, ast.Call))
+        f = step.AttentionStep if isinstance(call.func, ast.Name) else getattr(step.AttentionStep, call.func.attr)
+        args = [None] * (len(call.args) + (f is not step.AttentionStep))
+        inspect.signature(f).bind(*args, **{k.arg: None for k in call.keywords})
