@@ -85,7 +85,7 @@ def rotary_inv_freq(rotary_dim: int, base: float = 10000.0, scaling: str = "none
     """
     if rotary_dim < 0 or rotary_dim % 2:
         raise InvalidParameter(f"rotary_dim {rotary_dim} (even)")
-    if not base > 0 or not factor > 0 or not original_context > 0:
+    if not all(0 < x < math.inf for x in (base, factor, original_context)):
         raise InvalidParameter(f"base {base} factor {factor} original_context {original_context}")
     i = np.arange(rotary_dim // 2, dtype=np.float64)
     freq = float(base) ** (-2.0 * i / max(rotary_dim, 1))
@@ -100,8 +100,8 @@ def rotary_inv_freq(rotary_dim: int, base: float = 10000.0, scaling: str = "none
         return wide ** (-2.0 * i / rotary_dim), 1.0
     turns = original_context * freq / (2.0 * math.pi)
     if scaling == "yarn":
-        if not beta_fast > beta_slow > 0:
-            raise InvalidParameter(f"beta_fast {beta_fast} beta_slow {beta_slow}")
+        if not math.inf > beta_fast > beta_slow > 0 or not base > 1:
+            raise InvalidParameter(f"beta_fast {beta_fast} beta_slow {beta_slow} base {base} (above 1)")
 
         def pair_of(n: float) -> float:   # the (fractional) pair that turns n times
             return (rotary_dim * math.log(original_context / (2.0 * math.pi * n))
@@ -112,7 +112,7 @@ def rotary_inv_freq(rotary_dim: int, base: float = 10000.0, scaling: str = "none
         keep = 1.0 - np.clip((i - low) / max(high - low, 1e-3), 0.0, 1.0)
         return freq / factor * (1.0 - keep) + freq * keep, 0.1 * math.log(max(factor, 1.0)) + 1.0
     if scaling == "banded":
-        if not high_factor > low_factor:
+        if not math.inf > high_factor > low_factor > -math.inf:
             raise InvalidParameter(f"low_factor {low_factor} high_factor {high_factor}")
         keep = np.clip((turns - low_factor) / (high_factor - low_factor), 0.0, 1.0)
         return freq / factor * (1.0 - keep) + freq * keep, 1.0

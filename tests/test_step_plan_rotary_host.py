@@ -192,3 +192,24 @@ def test_documented_calls_of_a_step_are_calls():
         f = step.AttentionStep if isinstance(call.func, ast.Name) else getattr(step.AttentionStep, call.func.attr)
         args = [None] * (len(call.args) + (f is not step.AttentionStep))
         inspect.signature(f).bind(*args, **{k.arg: None for k in call.keywords})
+
+
+@pytest.mark.parametrize("kw", [
+    dict(scaling="yarn", base=1.0), dict(scaling="yarn", base=0.5), dict(scaling="yarn", beta_fast=math.inf),
+    dict(scaling="yarn", beta_fast=math.nan), dict(scaling="yarn", beta_slow=0.0),
+    dict(scaling="yarn", original_context=math.inf), dict(base=math.inf), dict(base=math.nan), dict(base=0.0),
+    dict(scaling="linear", factor=math.inf), dict(scaling="ntk", factor=math.nan),
+    dict(scaling="banded", low_factor=4.0), dict(scaling="banded", high_factor=math.inf),
+    dict(scaling="banded", low_factor=-math.inf)])
+def test_inv_freq_refuses(kw):
+    """Numbers that leave no frequencies are refused, not divided by."""
+    with pytest.raises(pa.InvalidParameter):
+        step.rotary_inv_freq(64, **kw)
+
+
+@pytest.mark.parametrize("base", [0.5, 1.0])
+@pytest.mark.parametrize("kind", ["none", "linear", "ntk", "banded"])
+def test_inv_freq_of_small_bases(kind, base):
+    """Only the ramp over pairs needs frequencies that fall."""
+    f, _ = step.rotary_inv_freq(64, base, kind, factor=2.0)
+    assert f.shape == (32,) and np.isfinite(f).all()
