@@ -178,3 +178,62 @@ def test_step_refuses(dev):
     s = step.AttentionStep(2, 4, 4, 4, 2, 64, step.ScoreParams(0.1), np.ones(32))
     with pytest.raises(pa.InvalidParameter):
         s.layer(0, 0, 0, 0, 0, 0)
+
+
+def _check_layers(s, decode):
+    """Layer after layer: the rotated queries against the oracle's of the host's
+    inputs, and the outputs against the oracle's of those queries and the
+    layer's own cache; then the whole step once more, to the same bits."""
+    d, st = s.d, s.step
+    f = lambda x: to_float(x, s.dtype)  # noqa: E731
+    st.plan(d["bt"], d["cached"], d["new"], d["free"], d["num_free"], s.cap, num_blocks=s.NB)
+    bt, ctx, off, pos, _, _ = oracle.plan_step(s.bt, s.cached, s.new, s.free, s.T, s.NB)
+    n, half = int(off[-1]), len(s.inv)
+    i = np.arange(half)
+    first, second = (2 * i, 2 * i + 1) if s.inter else (i, i + half)
+    last = np.zeros(s.T, bool)
+    last[off[1:][off[1:] > off[:-1]] - 1] = True
+    outs = []
+    for (kc, vc), x, dx, out in zip(s.caches, s.qkv, d["qkv"], s.out):
+        q, k, v = (dx.ptr + 2 * s.D * h for h in (0, s.H, s.H + s.Hkv))
+        st.layer(q, k, v, kc, vc, out, query_stride=s.row, key_stride=s.row, value_stride=s.row,
+                 num_blocks=s.NB, decode=decode)
+        synchronize()
+        mine = x[:n, :s.H * s.D].reshape(n, s.H, s.D)
+        want = oracle.rotary(f(mine), pos[:n], s.inv, 2 * half, s.inter, s.factor)
+        size = np.zeros((n, s.H, s.D))
+        size[..., first] = size[..., second] = np.abs(f(mine))[..., first] + np.abs(f(mine))[..., second]
+        q = st.query.numpy().reshape(s.T, s.H, s.D)
+        err = np.abs(f(q[:n]) - want)
+        assert (err <= HALF_STEP[s.dtype] * np.abs(want) + 2.0 ** -19 * s.factor * size).all(), "queries"
+        a = (f(q[:n]), f(kc.numpy()), f(vc.numpy()), bt, ctx, off)
+        want = oracle.scored_attention(*a, **s.score)
+        bound = scored_bound(*a, s.dtype, 2 if decode else 1, want, **s.score)
+        got = out.numpy()
+        err = np.abs(f(got[:n]) - want)
+        rows = last[:n] if decode else np.ones(n, bool)
+        assert (err <= bound)[rows].all(), f"{(err / bound)[rows].max():.2f} of the bound"
+        outs.append(got)
+    for o in s.out:
+        o.fill_byte(0x7F)
+    s.enqueue(decode)
+    synchronize()
+    for o, want in zip(s.out, outs):
+        assert np.array_equal(o.numpy(), want)
+
+
+@pytest.mark.parametrize("score", SCORES)
+@pytest.mark.parametrize("H,Hkv,D,rot,dtype,inter", [(8, 2, 128, 128, "bf16", False), (4, 4, 64, 32, "f16", True),
+                                                     (6, 1, 64, 64, "bf16", False), (16, 2, 128, 64, "f16", True)])
+def test_every_layer_of_a_step(dev, H, Hkv, D, rot, dtype, inter, score):
+    """Queries and outputs of all three layers, in mixed steps and in decode
+    steps, one of them with long contexts beside short ones. (The second step has
+    614 tokens for 600 rows: its last sequence is refused.)"""
+    rng = np.random.default_rng(H + rot)
+    S = 6
+    s = Server(rng, S, 600, 80, 420, H, Hkv, D, dtype, _score(rng, S, H, score), rot, layers=3, interleaved=inter)
+    for new, decode, refused in (([500, 1, 33, 0, 16, 0], False, 0), ([1, 64, 31, 500, 1, 17], False, 1),
+                                 ([1, 1, 40, 1, 1, 0], False, 0), ([1] * 6, True, 0), ([1, 0, 1, 1, 0, 1], True, 0)):
+        s.inputs(new)
+        _check_layers(s, decode)
+        assert s.check()[2] == refused
