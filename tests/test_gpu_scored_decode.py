@@ -416,3 +416,29 @@ def test_decode_scale_of_zero(dev, cap):
     d.run()
     d.score["softcap"] = 0.0
     d.check()
+
+
+def test_decode_weights_in_two_parts(dev):
+    """bfloat16 weights are kept in two parts, each rounded to nearest: off by
+    2^-8 and then by 2^-9 of that, 2^-17 of the weight. Seen where a block's 15
+    equal weights of values of 1 are taken against one of 1 of a value of some
+    -15 of them; the exponent, exp2, sums and the quotient add less than 2^-20."""
+    x = to_float(np.arange(0x3F80, 0x4040, dtype=np.uint16), "bf16").astype(np.float64)   # 1 .. 3
+    p = np.exp(-x)
+    v = to_float(to_half(-15 * p, "bf16"), "bf16").astype(np.float64)
+    want = (15 * p + v) / (15 * p + 1)
+    best = np.argsort(np.abs(want))[:16]        # near 0, so that their rounding is small
+    x, p, v, want = x[best], p[best], v[best], want[best]
+    d = Decode(np.random.default_rng(23), [16], 16, 16, 64, "bf16", scale=1.0)
+    one = to_half(np.ones(1), "bf16")[0]
+    d.q[:], d.kc[:], d.vc[:] = 0, 0, one
+    d.q[0, :, 0] = to_half(x, "bf16")
+    d.kc[d.bt[0, 0], :, 0, :] = one | 0x8000    # scores of -x
+    d.kc[d.bt[0, 0], :, 0, 5] = 0               # but one of 0
+    d.vc[d.bt[0, 0], :, :, 5] = to_half(v, "bf16")[:, None]
+    d.upload()
+    d.run()
+    synchronize()
+    err = np.abs(to_float(d.out.numpy()[0], "bf16") - want[:, None]).max(axis=1)
+    bound = 2.0 ** -17 * 15 * p / (15 * p + 1) + 2.0 ** -20 + 2.0 ** -8 * np.abs(want)
+    assert (err <= bound).all(), (err / bound).max()
