@@ -20,7 +20,7 @@
 // of V (see cache_runs.hpp), or the queries of four tokens. An angle's 20
 // operations are made once per wave and token (per element: 123 us, not 91).
 // Measured: 16384 tokens of prompts, 32/8 heads x 128, 87 us (4.6 TB/s read and
-// written); 64 lone tokens of that layer 6.2 us; 2013 tokens of 8/8 x 64 6.4 us.
+// written); 64 lone tokens of that layer 6.2 us; 2013 tokens of 8/8 x 64 6.5 us.
 // 4096 lone tokens of 32/8 x 128 take 125 us: 2 bytes per 32-byte row each.
 
 #include <algorithm>

@@ -23,7 +23,10 @@
 // stage that is seen whole is its first key's, the same for a pair's scores, and
 // a rise over them that 16 registers keep: one operation a score less, 2-4 %.
 // Weights are rounded to 16 bits, to nearest, and summed as rounded: the
-// output's error is that of its own rounding and one of the same size.
+// output's error is that of its own rounding and a smaller one, 1.05 to 1.15
+// times that of the rounding alone (8 x 2048 tokens in fp16 2.32e-4 of the
+// output, not 2.07e-4). A second 16-bit part of the weights, as in decode, would
+// add 16 products to a stage's 32 (D = 128).
 //
 // Order. What a stage costs a wave beside its 32 products (D = 128) is 115 to
 // 250 vector operations for its 32 scores a lane, so the order of both is
@@ -33,11 +36,11 @@
 // longer and 2048 tokens alone 14 %), with the weights still to come and the
 // caps' parts of the next scores among them.
 //
-// Measured: 8 x 2048 tokens, 32/8 heads x 128, with a cap 368 us (750 TFLOP/s; bound
-// by the vector operations), without 312; chunks in a window 275 us (990 TFLOP/s;
-// bound by power: 1.6 GHz, matrix unit 60 % and LDS 30 % of the cycles); 24 prompts of
-// 52-912 tokens, 16/16 heads, with a bias and prefixes 57 us (short walks, bound by
-// latency).
+// Measured: 8 x 2048 tokens, 32/8 heads x 128, bfloat16, with a cap 378 us (730
+// TFLOP/s; vector operations 68 % of the cycles, matrix unit 38 %, waits 23 %),
+// without 308 (890; in fp16 51 %, 51 %, 31 %); chunks in a window 276 us (985 TFLOP/s;
+// 1.6 GHz, matrix unit 60 % and LDS 30 % of the cycles); 24 prompts of 52-912
+// tokens, 16/16 heads, with a bias and prefixes 56 us (short walks: waits 41 %).
 //
 // A weight of 0 times a value that is not finite is NaN. So in a stage that
 // some row of the tile does not see whole, such values become zeros in LDS, and
@@ -78,9 +81,13 @@ struct ScoredPrefillArgs {
 
 constexpr int kWaves = 4;
 constexpr int kStage = 64;             // keys
-// Sequences of the longest-first list, whose lengths fit LDS. In sequence order 8 x
-// 2048 tokens of 32/8 heads x 128 take 413 us, not 319, 700 of 1-60 184, not 159.
-// More sequences go in order, by the tiles of each 64 of them (at most 65535, host).
+// Sequences of the longest-first list, whose lengths fit LDS; more go in sequence
+// order, by the tiles of each 64 of them (at most 65535, host). Longest first / in
+// order, 32/8 heads x 128 unless said: batches that few rounds of workgroups take
+// gain by the list, 2 x 2048 tokens 82 / 101 us, 40 of 1-1500 of 8/8 x 64 with a cap
+// 108 / 126, 6 chunks of 1000 on up to 8000 435 / 473; those of many tiles, where an
+// entry's search costs more than an even end saves, do not, 8 x 2048 320 / 312, 700 of
+// 1-60 with a cap 167 / 145, 900 lognormal ones up to 4096 3950 / 3000.
 constexpr int kListSeqs = 1024;
 constexpr int kCountChunks = 1024;
 static_assert(kCountChunks <= kListSeqs && 64 * kCountChunks >= 65535, "their sums take the list's place");
