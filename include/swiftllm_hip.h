@@ -514,13 +514,14 @@ int swiftllm_hip_rotary_and_cache(
  * h / (num_heads / num_kv_heads), 32-bit sums rounded once. Blocks whose id is
  * outside [0, num_blocks) (num_blocks <= 0: no upper bound) hold no key, and
  * there are none past max_num_blocks_per_seq * 16: of a longer context the
- * queries keep their positions. A query that sees no key writes zeros. Cache slots that no query of the call sees may hold
- * anything, NaN included. A key that is not finite makes the outputs of the
- * queries that see it NaN or unspecified, a value that is not finite one
- * element of them, or all, not finite; other queries are not touched. dtype is
- * that of query, caches and output; scale and softcap are finite, softcap 0 to
- * 1024. output may be query itself and overlaps no other argument (of caches
- * that is checked where num_blocks is given). */
+ * queries keep their positions. A query that sees no key writes zeros. Cache
+ * slots that no query of the call sees may hold anything, NaN included. A key
+ * that is not finite makes the outputs of the queries that see it NaN or
+ * unspecified, a value that is not finite one element of them, or all, not
+ * finite; other queries are not touched. dtype is that of query, caches and
+ * output; scale and softcap are finite, softcap 0 to 1024. output may be query
+ * itself and overlaps no other argument (of caches that is checked where
+ * num_blocks is given). */
 
 /* One new token per sequence: the query of sequence s, at position
  * context_lens[s] - 1 (context_lens[s] <= 0: zeros), is row s of query and

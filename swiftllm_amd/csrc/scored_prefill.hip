@@ -262,9 +262,10 @@ __device__ __forceinline__ List make_list(const ScoredPrefillArgs& a, int per_wg
     return l;
 }
 
-// Past kListSeqs: the tiles up to and with every 64 sequences, in lds->first. Sums
-// stop above any tile of separate rows, so sequences that share rows, or have
-// none, change nothing for the others. (Found from query_offsets[s] / per_wg + s
+// Past kListSeqs: the tiles up to and with every 64 sequences, in lds->first. A
+// sequence without rows, wherever its offsets lie, has no tile and changes nothing
+// for the others; sums stop above the tiles of any separate rows, so those of
+// shared ones do not overflow. (Found from query_offsets[s] / per_wg + s
 // by bisection, where one offset out of order hides the tiles of others, 2500
 // sequences of 1-30 tokens of 8/2 heads x 64 take 74 us, not 44, 1100 of 1-60 of
 // 32/8 x 128 281, not 215.)
