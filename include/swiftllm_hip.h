@@ -552,8 +552,9 @@ size_t swiftllm_hip_scored_decode_workspace_size(
  * the cache already: whole prompts, or chunks on top of what is cached (the
  * arrays that swiftllm_hip_plan_step writes). query_offsets has num_seqs + 1
  * entries within [0, num_tokens]; a sequence whose offsets are not ascending
- * within it has no rows. If sequences share rows the output is unspecified. Rows of no sequence are left as they were; a row at a
- * negative position is zero. The caches are 16-byte aligned. */
+ * within it has no rows. If sequences share rows the output is unspecified.
+ * Rows of no sequence are left as they were; a row at a negative position is
+ * zero. The caches are 16-byte aligned. */
 int swiftllm_hip_scored_prefill(
     void* output, const void* query, const void* key_cache,
     const void* value_cache, const int32_t* block_tables,
