@@ -565,7 +565,97 @@ int swiftllm_hip_scored_prefill(
     int max_num_blocks_per_seq, int num_blocks, hipStream_t stream);
 
 /* ------------------------------------------------------------------------ */
-/* 7. Host-side metadata (no device work).                                   */
+/* 7. Sequences that come of one another: beams, parallel samples, chats on   */
+/*    one prompt. The reference counts references and forks blocks on the     */
+/*    host (crates/swiftllm-core/src/memory/block_manager.rs) and has no beam  */
+/*    search. As in section 6 nothing synchronises or allocates, all state is  */
+/*    device memory, and every call can be captured.                          */
+/* ------------------------------------------------------------------------ */
+#define SWIFTLLM_HIP_F32 2
+
+/* A beam search's selection. Row r * beam_width + w of logits (dtype F16, BF16
+ * or F32; `vocab` values, logits_stride between rows) belongs to beam w of
+ * request r, whose sum of log probabilities is beam_scores[row]. The score of
+ * going on with token v is beam_scores[row] + log softmax(logits[row])[v], in
+ * 64 bits. Writes, for every request,
+ *   cand_scores, cand_rows, cand_tokens [R, num_candidates]: the largest scores
+ *     in descending order (rounded to 32 bits), their rows and tokens; ties go to
+ *     the lower beam, then the larger logit, then the lower token
+ *   next_scores, next_rows, next_tokens [R, beam_width]: the first of the
+ *     candidates whose token is not eos_id (below 0: all go on)
+ * Places without a candidate hold -infinity, -1 and -1. A score of -infinity is
+ * no candidate: banned tokens (a logit of -infinity, or NaN) and beams without a
+ * score (-infinity or NaN; at a request's first step all but one). Where a logit
+ * is +infinity, its like share the row. beam_width <= num_candidates <= 64;
+ * twice the width leaves every beam a candidate that goes on. next_scores may be
+ * beam_scores. `workspace`: plain scratch, 256-byte aligned, of
+ * swiftllm_hip_beam_select_workspace_size() bytes. */
+int swiftllm_hip_beam_select(
+    const void* logits, const float* beam_scores, float* cand_scores,
+    int32_t* cand_rows, int32_t* cand_tokens, float* next_scores,
+    int32_t* next_rows, int32_t* next_tokens, void* workspace,
+    size_t workspace_bytes, int dtype, int num_requests, int beam_width,
+    int vocab, int num_candidates, long long logits_stride, int eos_id,
+    hipStream_t stream);
+
+/* Bytes of workspace it needs for these sizes; 0 where it would refuse them. */
+size_t swiftllm_hip_beam_select_workspace_size(int num_requests,
+                                               int beam_width, int vocab,
+                                               int num_candidates);
+
+/* Tables and references of rows that go on from others. Row i of
+ * block_tables_out and context_lens_out continues row parents[i] of
+ * block_tables and context_lens (any number that is no row: it ends, with a
+ * context of 0). ref_counts[b] is how many rows hold block b, in all tables of
+ * the pool; it loses the old rows' holds and gains the new ones'. A partly
+ * filled last block is about to be written: of the rows with the same parent,
+ * the r-th (from 0) gets a block of its own where r < ref_counts[b] - 1, the
+ * holds before any copy, so that one child keeps it unless others hold it. Copies take
+ * the lowest blocks that nothing refers to, rows in order; copy_pairs int64
+ * [num_seqs][2] holds their (source, destination) for swiftllm_hip_copy_blocks,
+ * which has to run before the next token is written, and -1 behind them. A row
+ * that finds none loses its last, partly filled block: its context ends with
+ * the whole ones. Writes free_blocks[0 .. num_free) = the blocks that nothing
+ * refers to then, in ascending order (room for num_blocks; entries behind stay),
+ * and counts[2] = copies, rows cut. taken (NULL: none): the first taken[0] of
+ * free_blocks as they come in were taken since (counts of
+ * swiftllm_hip_plan_step) and get their first reference here. Entries of a row
+ * behind its context stay as they were; ids outside [0, num_blocks) are carried
+ * along and not counted. No output may overlap another argument. */
+int swiftllm_hip_fork_pages(
+    int32_t* block_tables_out, int32_t* context_lens_out,
+    const int32_t* block_tables, const int32_t* context_lens,
+    const int32_t* parents, int32_t* ref_counts, int32_t* free_blocks,
+    int32_t* num_free, const int32_t* taken, int64_t* copy_pairs,
+    int32_t* counts, void* workspace, size_t workspace_bytes, int num_seqs,
+    int max_num_blocks_per_seq, int block_size, int num_blocks,
+    hipStream_t stream);
+
+/* Brings a pool together: the highest block that something refers to moves to
+ * the lowest that nothing does, and so on while it lies above it, at most
+ * max_moves of them. copy_pairs int64 [max_moves][2] holds the moves for
+ * swiftllm_hip_copy_blocks, -1 behind them; new_ids[num_blocks] every block's
+ * new id (its own where it stays), block_tables_out the tables with those, which
+ * may be block_tables itself, ref_counts_out the references by the new ids,
+ * free_blocks[0 .. num_free) the free blocks in ascending order, counts[2] =
+ * moves, blocks in use. ref_counts are up to date: blocks that a plan took since
+ * have had their reference (swiftllm_hip_fork_pages). Every other holder of a
+ * block takes its new id from new_ids. No other output may overlap an argument. */
+int swiftllm_hip_compact_pages(
+    int32_t* block_tables_out, int32_t* ref_counts_out,
+    const int32_t* block_tables, const int32_t* context_lens,
+    const int32_t* ref_counts, int32_t* free_blocks, int32_t* num_free,
+    int64_t* copy_pairs, int32_t* new_ids, int32_t* counts, void* workspace,
+    size_t workspace_bytes, int num_seqs, int max_num_blocks_per_seq,
+    int block_size, int num_blocks, int max_moves, hipStream_t stream);
+
+/* Bytes of workspace (plain scratch, 256-byte aligned) that
+ * swiftllm_hip_fork_pages and swiftllm_hip_compact_pages need; 0 where they
+ * would refuse the sizes. */
+size_t swiftllm_hip_pages_workspace_size(int num_seqs, int num_blocks);
+
+/* ------------------------------------------------------------------------ */
+/* 8. Host-side metadata (no device work).                                   */
 /* ------------------------------------------------------------------------ */
 
 /* KvCache::get_slot_mapping (crates/swiftllm-core/src/memory/kv_cache.rs:

@@ -441,3 +441,123 @@ def scored_attention(q, kc, vc, bt, ctx, query_offsets, scale, softcap=0.0, slop
             for i in rows:   # keys that a row does not see may hold anything
                 out[t0 + i, h] = w[i, seen[i]] @ v[seen[i]] / w[i].sum()
     return out
+
+
+def beam_select(logits, beam_scores, num_candidates: int, eos_id: int = -1):
+    """A beam search's selection in float64, request by request, as
+    swiftllm_hip_beam_select documents it: logits [R, W, V] and beam_scores [R, W]
+    -> (cand_scores, cand_rows, cand_tokens, next_scores, next_rows, next_tokens),
+    the scores in float64."""
+    x = np.array(logits, dtype=np.float64)
+    R, W, V = x.shape
+    C = num_candidates
+    cand = np.full((R, C), -np.inf), np.full((R, C), -1, np.int32), np.full((R, C), -1, np.int32)
+    on = np.full((R, W), -np.inf), np.full((R, W), -1, np.int32), np.full((R, W), -1, np.int32)
+    x[np.isnan(x)] = -np.inf
+    for r in range(R):
+        found = []
+        for w in range(W):
+            c, row = float(beam_scores[r, w]), x[r, w]
+            if not c > -np.inf or not (row > -np.inf).any():
+                continue
+            top = row.max()
+            if top == np.inf:
+                gap = np.where(row == np.inf, 0.0, -np.inf)
+            else:
+                gap = row - top
+            score = c - np.log(np.exp(gap).sum()) + gap
+            best = np.lexsort((np.arange(V), -row))[:C]      # of a beam: by logit, then token
+            found += [(-score[v], w, -row[v], v) for v in best.tolist() if score[v] > -np.inf]
+        found.sort()
+        going = 0
+        for k, (s, w, _, v) in enumerate(found[:C]):
+            cand[0][r, k], cand[1][r, k], cand[2][r, k] = -s, r * W + w, v
+            if v != eos_id and going < W:
+                on[0][r, going], on[1][r, going], on[2][r, going] = -s, r * W + w, v
+                going += 1
+    return (*cand, *on)
+
+
+def fork_pages(block_tables_out, block_tables, context_lens, parents, ref_counts, free_blocks,
+               num_free: int, taken: int = 0):
+    """Rows that go on from others, row by row in Python integers: what
+    swiftllm_hip_fork_pages documents. Returns (tables, contexts, ref_counts,
+    free_blocks, num_free, pairs, counts)."""
+    old, tables = np.asarray(block_tables), np.array(block_tables_out)
+    S, MB = old.shape
+    refs, free = [int(n) for n in ref_counts], np.array(free_blocks)
+    NB = len(refs)
+
+    def used(ctx):
+        return min(-(-max(int(ctx), 0) // 16), MB)
+
+    def count(b, by):
+        if 0 <= b < NB:
+            refs[b] += by
+
+    for b in free[:min(max(taken, 0), max(num_free, 0), NB)]:
+        count(int(b), 1)
+    ctx = [0] * S
+    for i, p in enumerate(parents):
+        for b in old[i, :used(context_lens[i])]:
+            count(int(b), -1)
+        if 0 <= p < S:
+            ctx[i] = max(int(context_lens[p]), 0)
+            n = used(ctx[i])
+            tables[i, :n] = old[p, :n]
+            for b in old[p, :n]:
+                count(int(b), 1)
+    holds = list(refs)
+    spare = [b for b in range(NB) if holds[b] <= 0]
+    pairs, cut, copies, seen = [], 0, 0, {}
+    for i, p in enumerate(parents):
+        older = seen.get(int(p), 0)
+        seen[int(p)] = older + 1
+        j = ctx[i] // 16
+        if ctx[i] % 16 == 0 or j >= MB:
+            continue
+        b = int(tables[i, j])
+        if not 0 <= b < NB or older >= holds[b] - 1:
+            continue
+        refs[b] -= 1
+        if copies < len(spare):
+            new = spare[copies]
+            copies += 1
+            refs[new] = 1
+            tables[i, j] = new
+            pairs.append((b, new))
+        else:
+            cut += 1
+            ctx[i] -= ctx[i] % 16
+    left = spare[copies:]
+    free[:len(left)] = left
+    pairs += [(-1, -1)] * (S - len(pairs))
+    return (tables, np.array(ctx, np.int32), np.array(refs, np.int32), free, len(left),
+            np.array(pairs, np.int64).reshape(S, 2), np.array([copies, cut], np.int32))
+
+
+def compact_pages(block_tables, context_lens, ref_counts, free_blocks, max_moves: int):
+    """The highest blocks in use to the lowest free ones, one by one: what
+    swiftllm_hip_compact_pages documents. Returns (tables, ref_counts, free_blocks,
+    num_free, pairs, new_ids, counts)."""
+    tables, refs = np.array(block_tables), np.array(ref_counts)
+    NB = len(refs)
+    ids = np.arange(NB, dtype=np.int32)
+    used = np.flatnonzero(refs > 0)
+    moves = list(zip(used[::-1].tolist(), np.flatnonzero(refs <= 0).tolist()))
+    moves = [(s, d) for s, d in moves[:max_moves] if s > d]
+    for s, d in moves:
+        ids[s] = d
+        refs[d], refs[s] = refs[s], 0
+    MB = tables.shape[1]
+    for i, c in enumerate(context_lens):
+        n = min(-(-max(int(c), 0) // 16), MB)
+        row = tables[i, :n]
+        known = (row >= 0) & (row < NB)
+        row[known] = ids[row[known]]
+    free = np.array(free_blocks)
+    left = np.flatnonzero(refs <= 0)
+    free[:len(left)] = left
+    pairs = np.full((max_moves, 2), -1, np.int64)
+    pairs[:len(moves)] = np.array(moves, np.int64).reshape(-1, 2)
+    return tables, refs, free, len(left), pairs, ids, np.array([len(moves), len(used)], np.int32)

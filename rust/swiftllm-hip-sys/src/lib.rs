@@ -40,6 +40,7 @@ pub const SWIFTLLM_HIP_NOALLOC_SCRATCH_BYTES: usize = 64 << 20;
 /// Value types of the attention step's entry points.
 pub const SWIFTLLM_HIP_F16: i32 = 0;
 pub const SWIFTLLM_HIP_BF16: i32 = 1;
+pub const SWIFTLLM_HIP_F32: i32 = 2;
 
 /// C twin of `PagedAttentionParams` (crates/swiftllm-cuda/src/bindings.rs:8-30).
 #[repr(C)]
@@ -279,6 +280,36 @@ extern "C" {
         block_size: c_int, max_num_blocks_per_seq: c_int, num_blocks: c_int,
         stream: hipStream_t,
     ) -> c_int;
+
+    // -- sequences that come of one another; logits also SWIFTLLM_HIP_F32 ---------
+    pub fn swiftllm_hip_beam_select(
+        logits: *const c_void, beam_scores: *const c_float, cand_scores: *mut c_float,
+        cand_rows: *mut i32, cand_tokens: *mut i32, next_scores: *mut c_float,
+        next_rows: *mut i32, next_tokens: *mut i32, workspace: *mut c_void,
+        workspace_bytes: usize, dtype: c_int, num_requests: c_int, beam_width: c_int,
+        vocab: c_int, num_candidates: c_int, logits_stride: c_longlong, eos_id: c_int,
+        stream: hipStream_t,
+    ) -> c_int;
+    pub fn swiftllm_hip_beam_select_workspace_size(
+        num_requests: c_int, beam_width: c_int, vocab: c_int, num_candidates: c_int,
+    ) -> usize;
+    pub fn swiftllm_hip_fork_pages(
+        block_tables_out: *mut i32, context_lens_out: *mut i32, block_tables: *const i32,
+        context_lens: *const i32, parents: *const i32, ref_counts: *mut i32,
+        free_blocks: *mut i32, num_free: *mut i32, taken: *const i32, copy_pairs: *mut i64,
+        counts: *mut i32, workspace: *mut c_void, workspace_bytes: usize, num_seqs: c_int,
+        max_num_blocks_per_seq: c_int, block_size: c_int, num_blocks: c_int,
+        stream: hipStream_t,
+    ) -> c_int;
+    pub fn swiftllm_hip_compact_pages(
+        block_tables_out: *mut i32, ref_counts_out: *mut i32, block_tables: *const i32,
+        context_lens: *const i32, ref_counts: *const i32, free_blocks: *mut i32,
+        num_free: *mut i32, copy_pairs: *mut i64, new_ids: *mut i32, counts: *mut i32,
+        workspace: *mut c_void, workspace_bytes: usize, num_seqs: c_int,
+        max_num_blocks_per_seq: c_int, block_size: c_int, num_blocks: c_int,
+        max_moves: c_int, stream: hipStream_t,
+    ) -> c_int;
+    pub fn swiftllm_hip_pages_workspace_size(num_seqs: c_int, num_blocks: c_int) -> usize;
 
     // -- host metadata: kv_cache.rs:186-216, 250-286 ------------------------------
     pub fn swiftllm_hip_slot_mapping(

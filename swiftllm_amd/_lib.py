@@ -104,6 +104,14 @@ SIGNATURES = {
     "swiftllm_hip_scored_prefill": (
         i32, [vp, vp, vp, vp, vp, vp, vp, vp, vp, f32, f32, i32, i32, i32, i32, i32, i32, i32, i32,
               i32, i32, vp]),
+    "swiftllm_hip_beam_select": (
+        i32, [vp, vp, vp, vp, vp, vp, vp, vp, vp, sz, i32, i32, i32, i32, i32, i64, i32, vp]),
+    "swiftllm_hip_beam_select_workspace_size": (sz, [i32, i32, i32, i32]),
+    "swiftllm_hip_fork_pages": (
+        i32, [vp, vp, vp, vp, vp, vp, vp, vp, vp, vp, vp, vp, sz, i32, i32, i32, i32, vp]),
+    "swiftllm_hip_compact_pages": (
+        i32, [vp, vp, vp, vp, vp, vp, vp, vp, vp, vp, vp, sz, i32, i32, i32, i32, i32, vp]),
+    "swiftllm_hip_pages_workspace_size": (sz, [i32, i32]),
     "swiftllm_hip_slot_mapping": (i32, [vp, sz, sz, sz, sz, vp]),
     "swiftllm_hip_pack_block_tables": (i32, [vp, vp, vp, sz, sz, sz, vp, vp]),
 }

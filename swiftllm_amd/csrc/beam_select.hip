@@ -1,0 +1,544 @@
+// A beam search's selection over beams and vocabulary (gfx950).
+//
+// Beam w of a request has the score c_w (a sum of log probabilities) and the
+// logits x_w[v] of its next token:
+//   score(w, v) = c_w + x_w[v] - lse_w,   lse_w = log sum_v exp x_w[v]
+// Candidates are the C largest scores, compared in 64 bits; ties go to the lower
+// beam, then the larger logit, then the lower token. Within a beam that is the
+// order of (logit, token), so its C first by those hold all of its candidates.
+//
+// First kernel, a workgroup per kChunk logits of a row: their sum of exponentials
+// and a list that holds their C largest. The threads' own maxima are 256 of them,
+// so the C-th largest of those is a threshold that at least C logits reach, and few
+// more do: only values in threads above it can. It is found bit by bit, a ballot
+// each, which costs an eighth of what the exponentials do. Second kernel, a
+// workgroup per request: the rows' lse, the same threshold over all lists' scores
+// rounded to 32 bits (which keeps their order), and the few that reach it ranked by
+// counting. Lists that ties fill past their room are cut to C one by one.
+//
+// lse. exp(x - m) = 2^(x L - m L) with L = log2(e) in 32 bits and m the thread's
+// maximum: one multiply-add with r, the rounded m L, and the sum times 2^(r - m L),
+// that difference exact. So the roundings are those of the exponents, of exp2 and
+// of the sums: 32 bits up to a chunk's, 64 bits over chunks. L's own error moves
+// lse by 2e-8 of the distance from the maximum.
+//
+// Bound: HBM for 32-bit logits, for 16-bit ones as much the vector operations, nine
+// per logit of which the exponential is four.
+
+#include <algorithm>
+#include <cmath>
+#include <type_traits>
+
+#include "half_types.hpp"
+
+namespace swiftllm {
+namespace {
+
+constexpr int kThreads = 256;
+constexpr int kWaves = kThreads / 64;
+constexpr int kEach = 32;                  // logits of a thread
+constexpr int kChunk = kThreads * kEach;
+constexpr int kRoom = 128;                 // entries of a chunk's list
+constexpr int kMostCandidates = 64;
+constexpr int kPickThreads = 1024;
+constexpr int kPickWaves = kPickThreads / 64;
+constexpr int kPickRoom = 512;             // candidates that are ranked
+constexpr float kLog2e = 1.4426950408889634f;
+static_assert(kMostCandidates <= kRoom && kMostCandidates <= kThreads, "a list holds the candidates");
+
+struct Entry {
+    float x;
+    int token;
+};
+
+struct SelectArgs {
+    const void* logits;
+    const float* scores;        // [R * W]
+    float* cand_scores;         // [R][C]
+    int* cand_rows;
+    int* cand_tokens;
+    float* next_scores;         // [R][W]
+    int* next_rows;
+    int* next_tokens;
+    // workspace
+    float2* sums;               // [rows][chunks]: the maximum m, the sum of exp(x - m)
+    int* fill;                  // [rows][chunks]
+    Entry* lists;               // [rows][chunks][kRoom]
+    long long stride;
+    int W;
+    int V;
+    int C;
+    int chunks;
+    int eos;
+};
+
+struct F32 {};
+template <typename T>    // the upper bits in which keys differ
+constexpr int key_bits = std::is_same<T, BF16>::value ? 16 : std::is_same<T, F16>::value ? 19 : 32;
+template <typename T>
+constexpr int vec_of = std::is_same<T, F32>::value ? 4 : 8;    // values of 16 bytes
+
+// Orders as the floats do (-0 below 0).
+__device__ __forceinline__ unsigned key_of(float x) {
+    const unsigned u = __builtin_bit_cast(unsigned, x);
+    return u ^ (static_cast<unsigned>(static_cast<int>(u) >> 31) | 0x80000000u);
+}
+__device__ __forceinline__ float of_key(unsigned k) {
+    return __builtin_bit_cast(float, k ^ ((k >> 31) ? 0x80000000u : 0xffffffffu));
+}
+
+// The n-th largest of 256 keys, four of each lane, that differ in their `bits`
+// upper bits alone: the largest number that n of them reach.
+__device__ __forceinline__ unsigned nth_largest(const unsigned (&k)[4], int n, int bits) {
+    unsigned t = 0;
+    for (int b = 31; b >= 32 - bits; --b) {
+        const unsigned c = t | (1u << b);
+        int reach = 0;
+#pragma unroll
+        for (int i = 0; i < 4; ++i) reach += __popcll(__ballot(k[i] >= c));
+        if (reach >= n) t = c;
+    }
+    // A negative value's lower bits are ones in its key.
+    return (t >> 31) || bits == 32 ? t : t | ((1u << (32 - bits)) - 1u);
+}
+
+// A value that is no number counts as one that is banned.
+__device__ __forceinline__ float number(float x) { return x != x ? -INFINITY : x; }
+
+template <typename T>
+__device__ __forceinline__ void unpack(u4 r, float* v) {
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+        if constexpr (std::is_same<T, F32>::value) {
+            const unsigned u = r[i];
+            v[i] = __builtin_bit_cast(float, u);
+        } else {
+            v[2 * i] = T::up(static_cast<uint16_t>(r[i] & 0xffffu));
+            v[2 * i + 1] = T::up(static_cast<uint16_t>(r[i] >> 16));
+        }
+    }
+}
+
+template <typename T>
+__device__ __forceinline__ float load_one(const void* row, long long i) {
+    if constexpr (std::is_same<T, F32>::value) {
+        return static_cast<const float*>(row)[i];
+    } else {
+        return T::up(static_cast<const uint16_t*>(row)[i]);
+    }
+}
+
+// A sum of exp(x - m) as one of exp(x - top), top >= m.
+__device__ __forceinline__ float weighed(float sum, float m, float top) {
+    return m == top ? sum : sum * __builtin_amdgcn_exp2f((m - top) * kLog2e);
+}
+
+// The largest of the workgroup's keys, in every thread. part: kWaves.
+__device__ __forceinline__ unsigned long long block_max(unsigned long long k, unsigned long long* part) {
+#pragma unroll
+    for (int d = 1; d < 64; d <<= 1) {
+        const unsigned lo = __shfl_xor(static_cast<int>(k), d);
+        const unsigned hi = __shfl_xor(static_cast<int>(k >> 32), d);
+        k = std::max(k, static_cast<unsigned long long>(hi) << 32 | lo);
+    }
+    __syncthreads();
+    if ((threadIdx.x & 63) == 0) part[threadIdx.x >> 6] = k;
+    __syncthreads();
+    for (int i = 0; i < kWaves; ++i) k = std::max(k, part[i]);
+    return k;
+}
+
+template <typename T>
+__global__ __launch_bounds__(kThreads) void beam_chunk_kernel(const SelectArgs a) {
+    constexpr int VEC = vec_of<T>;
+    constexpr int NV = kEach / VEC;
+    constexpr int kSize = 16 / VEC;
+    __shared__ __align__(16) unsigned s_key[kThreads];
+    __shared__ float s_f[kWaves], s_sum[kWaves];
+    __shared__ unsigned long long s_best[kWaves];
+    __shared__ Entry s_list[kRoom];
+    __shared__ int s_fill;
+    const int tid = threadIdx.x, lane = tid & 63;
+    const int w = __builtin_amdgcn_readfirstlane(tid >> 6);
+    const int row = blockIdx.x / a.chunks;
+    const int chunk = blockIdx.x - row * a.chunks;
+    const size_t slot = static_cast<size_t>(row) * a.chunks + chunk;
+    const float score = a.scores[row];
+    if (!(score > -INFINITY)) {
+        // Nothing comes of this beam.
+        if (tid == 0) a.fill[slot] = 0;
+        return;
+    }
+    if (tid == 0) s_fill = 0;
+    // Vectors begin at 16-byte addresses, the first of them up to VEC - 1 values
+    // before the row.
+    const char* const base = static_cast<const char*>(a.logits) + static_cast<long long>(row) * a.stride * kSize;
+    const int off = static_cast<int>((reinterpret_cast<uintptr_t>(base) & 15u) / kSize);
+    const int first = chunk * kChunk - off;
+    auto index = [&](int k) { return first + (k * kThreads + tid) * VEC; };
+    float v[kEach];
+#pragma unroll
+    for (int k = 0; k < NV; ++k) {
+        const int i = index(k);
+        if (i >= 0 && i <= a.V - VEC) {
+            const u4 r = __builtin_nontemporal_load(reinterpret_cast<const u4*>(base + static_cast<long long>(i) * kSize));
+            unpack<T>(r, v + k * VEC);
+        } else {
+#pragma unroll
+            for (int j = 0; j < VEC; ++j) {
+                v[k * VEC + j] = i + j >= 0 && i + j < a.V ? load_one<T>(base, i + j) : -INFINITY;
+            }
+        }
+    }
+    // (fmaxf passes over what is no number)
+    float most = -INFINITY;
+#pragma unroll
+    for (int k = 0; k < kEach; ++k) most = fmaxf(most, v[k]);
+    s_key[tid] = key_of(most);
+    const float r = most * kLog2e;
+    float sum = 0.0f;
+#pragma unroll
+    for (int k = 0; k < kEach; ++k) sum += __builtin_amdgcn_exp2f(__builtin_fmaf(v[k], kLog2e, -r));
+    sum *= __builtin_amdgcn_exp2f(-__builtin_fmaf(most, kLog2e, -r));
+    if (__any(!(sum < INFINITY))) {
+        // Values that are no number, nothing but banned ones, a product past the
+        // type's range, or an infinite maximum, which has all the weight.
+#pragma unroll
+        for (int k = 0; k < kEach; ++k) v[k] = number(v[k]);
+        if (!(sum < INFINITY)) {
+            sum = 0.0f;
+#pragma unroll
+            for (int k = 0; k < kEach; ++k) {
+                sum += v[k] == most ? 1.0f : __builtin_amdgcn_exp2f((v[k] - most) * kLog2e);
+            }
+        }
+    }
+    const float wf = wave_max(most);
+    const float ws = wave_sum(weighed(sum, most, wf));
+    if (lane == 0) {
+        s_f[w] = wf;
+        s_sum[w] = ws;
+    }
+    __syncthreads();
+    const u4 ks = *reinterpret_cast<const u4*>(s_key + 4 * lane);
+    const unsigned keys[4] = {ks[0], ks[1], ks[2], ks[3]};
+    // What is banned is no candidate.
+    const float line = fmaxf(of_key(nth_largest(keys, a.C, key_bits<T>)), -3.402823466e38f);
+#pragma unroll
+    for (int k = 0; k < kEach; ++k) {
+        if (v[k] >= line) {
+            const int at = atomicAdd(&s_fill, 1);
+            if (at < kRoom) s_list[at] = Entry{v[k], index(k / VEC) + k % VEC};
+        }
+    }
+    __syncthreads();
+    int n = s_fill;
+    if (n > kRoom) {
+        // Ties: the C largest one by one.
+        n = a.C;
+        for (int c = 0; c < n; ++c) {
+            unsigned long long best = 0;
+#pragma unroll
+            for (int k = 0; k < kEach; ++k) {
+                const unsigned i = index(k / VEC) + k % VEC;
+                const unsigned long long key = static_cast<unsigned long long>(key_of(v[k] + 0.0f)) << 32 | (0xffffffffu - i);
+                if (v[k] >= line) best = std::max(best, key);
+            }
+            best = block_max(best, s_best);
+            const int token = static_cast<int>(0xffffffffu - static_cast<unsigned>(best));
+#pragma unroll
+            for (int k = 0; k < kEach; ++k) {
+                if (index(k / VEC) + k % VEC == token) {
+                    s_list[c] = Entry{v[k], token};
+                    v[k] = -INFINITY;
+                }
+            }
+        }
+        __syncthreads();
+    }
+    if (tid < n) a.lists[slot * kRoom + tid] = s_list[tid];
+    if (tid == 0) {
+        float F = -INFINITY, S = 0.0f;
+        for (int i = 0; i < kWaves; ++i) F = fmaxf(F, s_f[i]);
+        for (int i = 0; i < kWaves; ++i) S += weighed(s_sum[i], s_f[i], F);
+        a.sums[slot] = float2{F, S};
+        a.fill[slot] = n;
+    }
+}
+
+// A candidate, and the order of candidates.
+struct Cand {
+    double score;
+    float x;
+    int beam;
+    int token;
+};
+__device__ __forceinline__ bool before(const Cand& p, const Cand& q) {
+    if (p.score != q.score) return p.score > q.score;
+    if (p.beam != q.beam) return p.beam < q.beam;
+    if (p.x != q.x) return p.x > q.x;
+    return p.token < q.token;
+}
+
+__device__ __forceinline__ double wave_sum64(double x) {
+#pragma unroll
+    for (int d = 1; d < 64; d <<= 1) x += __shfl_xor(x, d);
+    return x;
+}
+
+__global__ __launch_bounds__(kPickThreads) void beam_pick_kernel(const SelectArgs a) {
+    __shared__ double s_base[kMostCandidates];     // of a beam: its score less log sum exp(x - top)
+    __shared__ float s_top[kMostCandidates];
+    __shared__ __align__(16) unsigned s_key[kPickThreads / 4];
+    __shared__ Cand s_cand[kPickRoom];
+    __shared__ Cand s_best[kPickThreads / 64];
+    __shared__ Cand s_order[kMostCandidates];
+    __shared__ int s_fill;
+    __shared__ float s_line;
+    const int tid = threadIdx.x, lane = tid & 63;
+    const int w = __builtin_amdgcn_readfirstlane(tid >> 6);
+    const int r = blockIdx.x;
+    if (tid == 0) s_fill = 0;
+    for (int b = w; b < a.W; b += kPickWaves) {
+        const size_t row = static_cast<size_t>(r) * a.W + b;
+        const float score = a.scores[row];
+        double base = -INFINITY;
+        float top = 0.0f;
+        if (score > -INFINITY) {
+            const float2* const sums = a.sums + row * a.chunks;
+            float F = -INFINITY;
+            for (int c = lane; c < a.chunks; c += 64) F = fmaxf(F, sums[c].x);
+            F = wave_max(F);
+            double S = 0.0;
+            for (int c = lane; c < a.chunks; c += 64) {
+                const float2 x = sums[c];
+                S += x.x == F ? static_cast<double>(x.y) : x.y * exp(static_cast<double>(x.x) - F);
+            }
+            S = wave_sum64(S);
+            base = score - log(S);
+            top = F;
+        }
+        if (lane == 0) {
+            s_base[b] = base;
+            s_top[b] = top;
+        }
+    }
+    __syncthreads();
+    // A list per 16 lanes.
+    const int lists = a.W * a.chunks;
+    auto each = [&](auto take) {
+        for (int i = tid >> 4; i < lists; i += kPickThreads / 16) {
+            const int b = i / a.chunks;
+            const size_t slot = static_cast<size_t>(r) * lists + i;
+            const int n = a.fill[slot];
+            const double base = s_base[b], top = s_top[b];
+            for (int k = tid & 15; k < n; k += 16) {
+                const Entry e = a.lists[slot * kRoom + k];
+                // (beside an infinite logit only others of its kind have a share)
+                const double score = e.x == s_top[b] ? base : base + (e.x - top);
+                if (score > -INFINITY) take(Cand{score, e.x, b, e.token});
+            }
+        }
+    };
+    float most = -INFINITY;
+    each([&](const Cand& c) { most = fmaxf(most, static_cast<float>(c.score)); });
+    most = fmaxf(most, __shfl_xor(most, 1));
+    most = fmaxf(most, __shfl_xor(most, 2));
+    if ((tid & 3) == 0) s_key[tid >> 2] = key_of(most);
+    __syncthreads();
+    if (w == 0) {
+        const u4 ks = *reinterpret_cast<const u4*>(s_key + 4 * lane);
+        const unsigned keys[4] = {ks[0], ks[1], ks[2], ks[3]};
+        const unsigned t = nth_largest(keys, a.C, 32);
+        if (lane == 0) s_line = of_key(t);
+    }
+    __syncthreads();
+    const float line = s_line;
+    each([&](const Cand& c) {
+        if (static_cast<float>(c.score) >= line) {
+            const int at = atomicAdd(&s_fill, 1);
+            if (at < kPickRoom) s_cand[at] = c;
+        }
+    });
+    __syncthreads();
+    int n = s_fill;
+    if (n <= kPickRoom) {
+        for (int i = tid; i < n; i += kPickThreads) {
+            const Cand mine = s_cand[i];
+            int rank = 0;
+            for (int j = 0; j < n; ++j) rank += before(s_cand[j], mine);
+            if (rank < a.C) s_order[rank] = mine;
+        }
+        n = min(n, a.C);
+    } else {
+        // Ties: one by one, each behind the last.
+        const Cand none{-INFINITY, 0.0f, 0x7fffffff, 0x7fffffff};
+        n = a.C;
+        for (int k = 0; k < n; ++k) {
+            Cand best = none;
+            each([&](const Cand& c) {
+                if (k > 0 && !before(s_order[k - 1], c)) return;
+                if (before(c, best)) best = c;
+            });
+#pragma unroll
+            for (int d = 1; d < 64; d <<= 1) {
+                const Cand c{__shfl_xor(best.score, d), __shfl_xor(best.x, d), __shfl_xor(best.beam, d), __shfl_xor(best.token, d)};
+                if (before(c, best)) best = c;
+            }
+            if (lane == 0) s_best[w] = best;
+            __syncthreads();
+            if (tid == 0) {
+                for (int i = 1; i < kPickWaves; ++i) {
+                    if (before(s_best[i], best)) best = s_best[i];
+                }
+                s_order[k] = best;
+            }
+            __syncthreads();
+        }
+    }
+    __syncthreads();
+    if (w > 0) return;
+    // Lane c has candidate c.
+    const bool real = lane < n;
+    const Cand c = real ? s_order[lane] : Cand{-INFINITY, 0.0f, 0, -1};
+    const int row = real ? r * a.W + c.beam : -1;
+    const float score = static_cast<float>(c.score);
+    if (lane < a.C) {
+        const size_t at = static_cast<size_t>(r) * a.C + lane;
+        a.cand_scores[at] = score;
+        a.cand_rows[at] = row;
+        a.cand_tokens[at] = c.token;
+    }
+    const unsigned long long on = __ballot(real && c.token != a.eos);
+    const int place = __popcll(on & ((1ull << lane) - 1ull));
+    const int all = __popcll(on);
+    const size_t at = static_cast<size_t>(r) * a.W;
+    if (((on >> lane) & 1ull) && place < a.W) {
+        a.next_scores[at + place] = score;
+        a.next_rows[at + place] = row;
+        a.next_tokens[at + place] = c.token;
+    }
+    if (lane >= all && lane < a.W) {
+        a.next_scores[at + lane] = -INFINITY;
+        a.next_rows[at + lane] = -1;
+        a.next_tokens[at + lane] = -1;
+    }
+}
+
+struct Space {
+    size_t sums, fill, lists, bytes;
+    int chunks;
+};
+
+// A row that begins off a 16-byte address takes up to 7 values more.
+Space space_of(long long rows, long long V) {
+    const auto up = [](long long n) { return static_cast<size_t>((n + 255) / 256 * 256); };
+    Space s;
+    s.chunks = static_cast<int>((V + 7 + kChunk - 1) / kChunk);
+    const long long slots = rows * s.chunks;
+    s.sums = 0;
+    s.fill = up(8 * slots);
+    s.lists = s.fill + up(4 * slots);
+    s.bytes = s.lists + up(8 * kRoom * slots) + 256;
+    return s;
+}
+
+int check_sizes(const char* who, long long R, long long W, long long V, long long C) {
+    if (R < 0 || W <= 0 || V <= 0 || C < W) {
+        return fail(SWIFTLLM_ERR_INVALID_PARAMETER, "%s: num_requests=%lld beam_width=%lld vocab=%lld num_candidates=%lld",
+                    who, R, W, V, C);
+    }
+    if (C > kMostCandidates || R > (1 << 20) || V > (1 << 27) || R * W * ((V + 7 + kChunk - 1) / kChunk) >= (1 << 24)) {
+        return fail(SWIFTLLM_ERR_NOT_SUPPORTED, "%s: num_requests=%lld beam_width=%lld vocab=%lld num_candidates=%lld (at most %d)",
+                    who, R, W, V, C, kMostCandidates);
+    }
+    return SWIFTLLM_OK;
+}
+
+}  // namespace
+}  // namespace swiftllm
+
+using namespace swiftllm;
+
+extern "C" {
+
+size_t swiftllm_hip_beam_select_workspace_size(int num_requests, int beam_width, int vocab, int num_candidates) {
+    if (check_sizes("swiftllm_hip_beam_select_workspace_size", num_requests, beam_width, vocab, num_candidates) != SWIFTLLM_OK) {
+        return 0;
+    }
+    ok();
+    return space_of(static_cast<long long>(num_requests) * beam_width, vocab).bytes;
+}
+
+int swiftllm_hip_beam_select(const void* logits, const float* beam_scores, float* cand_scores, int32_t* cand_rows,
+                             int32_t* cand_tokens, float* next_scores, int32_t* next_rows, int32_t* next_tokens,
+                             void* workspace, size_t workspace_bytes, int dtype, int num_requests, int beam_width,
+                             int vocab, int num_candidates, long long logits_stride, int eos_id, hipStream_t stream) {
+    const char* who = "swiftllm_hip_beam_select";
+    const long long R = num_requests, W = beam_width, V = vocab, C = num_candidates;
+    int rc = check_sizes(who, R, W, V, C);
+    if (rc != SWIFTLLM_OK) return rc;
+    if (dtype != SWIFTLLM_HIP_F16 && dtype != SWIFTLLM_HIP_BF16 && dtype != SWIFTLLM_HIP_F32) {
+        return fail(SWIFTLLM_ERR_NOT_SUPPORTED, "%s: dtype=%d (supported: 0 fp16, 1 bf16, 2 fp32)", who, dtype);
+    }
+    if (logits_stride < V || logits_stride > (1LL << 40)) {
+        return fail(SWIFTLLM_ERR_INVALID_PARAMETER, "%s: logits_stride=%lld of vocab=%d", who, logits_stride, vocab);
+    }
+    if (R > 0 && (!logits || !beam_scores || !cand_scores || !cand_rows || !cand_tokens || !next_scores || !next_rows ||
+                  !next_tokens || !workspace)) {
+        return fail(SWIFTLLM_ERR_INVALID_PARAMETER, "%s: null pointer", who);
+    }
+    const size_t size = dtype == SWIFTLLM_HIP_F32 ? 4 : 2;
+    const size_t rows = static_cast<size_t>(R * W);
+    const Space space = space_of(R * W, V);
+    const Bytes span[] = {{cand_scores, 4 * static_cast<size_t>(R * C)}, {cand_rows, 4 * static_cast<size_t>(R * C)},
+                          {cand_tokens, 4 * static_cast<size_t>(R * C)}, {next_scores, 4 * rows}, {next_rows, 4 * rows},
+                          {next_tokens, 4 * rows}, {workspace, space.bytes}, {beam_scores, 4 * rows},
+                          {logits, rows == 0 ? 0 : (static_cast<size_t>(logits_stride) * (rows - 1) + V) * size}};
+    for (const Bytes& s : span) {
+        if (!aligned(s.p, s.p == logits ? size : 4)) return fail(SWIFTLLM_ERR_INVALID_PARAMETER, "%s: misaligned pointer", who);
+    }
+    if (!aligned(workspace, 256)) return fail(SWIFTLLM_ERR_INVALID_PARAMETER, "%s: misaligned pointer", who);
+    if (R > 0 && workspace_bytes < space.bytes) {
+        return fail(SWIFTLLM_ERR_INVALID_PARAMETER, "%s: workspace of %zu bytes, %zu needed", who, workspace_bytes, space.bytes);
+    }
+    for (int i = 0; i < 7; ++i) {
+        for (int j = i + 1; j < 9; ++j) {
+            // The next step's beams may take the place of this step's: a workgroup
+            // has read its request's before it writes them.
+            if (i == 3 && j == 7 && next_scores == beam_scores) continue;
+            if (overlap_any(span[i], {span[j]})) {
+                return fail(SWIFTLLM_ERR_INVALID_PARAMETER, "%s: an output overlaps another argument", who);
+            }
+        }
+    }
+    rc = require_device();
+    if (rc != SWIFTLLM_OK) return rc;
+    if (R == 0) return ok();
+    SelectArgs a{};
+    a.logits = logits;
+    a.scores = beam_scores;
+    a.cand_scores = cand_scores;
+    a.cand_rows = cand_rows;
+    a.cand_tokens = cand_tokens;
+    a.next_scores = next_scores;
+    a.next_rows = next_rows;
+    a.next_tokens = next_tokens;
+    char* const ws = static_cast<char*>(workspace);
+    a.sums = reinterpret_cast<float2*>(ws + space.sums);
+    a.fill = reinterpret_cast<int*>(ws + space.fill);
+    a.lists = reinterpret_cast<Entry*>(ws + space.lists);
+    a.stride = logits_stride;
+    a.W = beam_width;
+    a.V = vocab;
+    a.C = num_candidates;
+    a.chunks = space.chunks;
+    a.eos = eos_id >= 0 ? eos_id : -2;
+    using K = void (*)(SelectArgs);
+    static const K kernels[3] = {beam_chunk_kernel<F16>, beam_chunk_kernel<BF16>, beam_chunk_kernel<F32>};
+    rc = launched(launch(kernels[dtype], dim3(static_cast<unsigned>(rows * space.chunks)), dim3(kThreads), 0, stream, a), who);
+    if (rc != SWIFTLLM_OK) return rc;
+    return launched(launch(beam_pick_kernel, dim3(static_cast<unsigned>(R)), dim3(kPickThreads), 0, stream, a), who);
+}
+
+}  // extern "C"

@@ -1,0 +1,544 @@
+// Pages of a cache whose sequences come of one another (gfx950): forking, with
+// the references of every block, and bringing a pool together.
+//
+// fork_pages. Row i of the new batch goes on from row p = parents[i] of the old
+// one, -1 or any other number that is no row: from none. With
+// used_i = ceil(context_i / 16):
+//   tables_out[i, j] = tables[p, j] for j < used_p, context_out[i] = context[p]
+//   refs[b] += (new rows' entries b) - (old rows' entries b)
+// A partly filled last block is written by its row's next token, so that each
+// row that goes on needs one of its own: of the rows with the same parent, the
+// r-th (from 0) takes a copy where r < refs[b] - 1, refs as they are now. So the
+// last child keeps the block, and every child copies one that somebody else
+// holds. Copies go to the free blocks (refs[b] <= 0) in ascending order, rows in
+// order; the free blocks behind those are the new list. A row whose block is
+// missing ends with its whole blocks.
+//
+// compact_pages. The k-th highest block in use moves to the k-th lowest free one
+// while it lies above it, at most max_moves. With L blocks in use, L - M of them
+// stay: those below T, the lowest that moves, and ids from T on are free
+// afterwards, id - L of them before id; below T the free ones but for the M lowest.
+//
+// Bound: latency. A step of 16 requests of 8 beams in 65536 blocks moves 0.9 MB
+// (0.2 us), 1024 beams in 524288 blocks 12 MB. Three launches each, whose ends are
+// the only order between workgroups: what moves references, what counts the free
+// blocks of every 4096 ids (and keeps them as bits), what lists them. Where a row
+// and its parent have the same block in the same place, as in a prompt that both
+// share, nothing is counted: a search's reordering touches few counters.
+
+#include <algorithm>
+
+#include "common.hpp"
+
+namespace swiftllm {
+namespace {
+
+constexpr int kRowThreads = 256;
+constexpr int kScanThreads = 1024;
+constexpr int kScanWaves = kScanThreads / 64;
+constexpr int kIds = 4096;               // ids of a workgroup: 64 words of 64 bits
+constexpr int kWords = kIds / 64;
+constexpr int kEach = kIds / kScanThreads;
+
+struct PagesArgs {
+    const int* tables;
+    const int* ctx;
+    const int* parents;
+    int* tables_out;
+    int* ctx_out;
+    const int* refs;       // compact_pages: as they were
+    int* refs_out;         // fork_pages: the references
+    const int* taken;      // [1] or null
+    int* free_blocks;
+    int* num_free;         // [1]
+    long long* pairs;      // [rooms][2]
+    int* new_ids;
+    int* counts;           // [2]
+    // workspace
+    int* sums;             // [groups]: blocks free (in use: compact) of a group of ids
+    int* num_copies;       // [1]
+    unsigned long long* bits;
+    int* rank;             // [S]: children of the same parent before this one
+    int* copies;           // [S]: rows that take a copy, in order
+    int* from;             // [NB / 2]: compact: the blocks that move, highest first,
+    int* to;               //   the free ones, lowest first,
+    int* order;            // [NB]: and a moving block's place among them
+    int S;
+    int MB;
+    int NB;
+    int groups;            // ceil(NB / kIds)
+    int rooms;             // pairs
+};
+
+__device__ __forceinline__ bool in_pool(int b, int NB) { return b >= 0 && b < NB; }
+
+__device__ __forceinline__ int blocks_of(int ctx, int MB) {
+    return min((max(ctx, 0) >> kBlockShift) + ((ctx & (kBlockTokens - 1)) != 0 && ctx > 0), MB);
+}
+
+__device__ __forceinline__ int parent_of(const PagesArgs& a, int i) {
+    const int p = a.parents[i];
+    return p >= 0 && p < a.S ? p : -1;
+}
+
+// The sum of x over the workgroup, in every thread.
+template <int WAVES>
+__device__ __forceinline__ int block_total(int x, int* part) {
+    const int sum = wave_total(x);
+    if ((threadIdx.x & 63) == 0) part[threadIdx.x >> 6] = sum;
+    __syncthreads();
+    int all = 0;
+#pragma unroll
+    for (int i = 0; i < WAVES; ++i) all += part[i];
+    return all;
+}
+
+__global__ __launch_bounds__(kRowThreads) void fork_rows_kernel(const PagesArgs a) {
+    __shared__ int s_part[kRowThreads / 64];
+    const int i = blockIdx.x, tid = threadIdx.x;
+    if (a.taken != nullptr) {
+        // Blocks that a plan took: of nobody until now.
+        const int n = min(min(max(a.taken[0], 0), max(a.num_free[0], 0)), a.NB);
+        for (int k = i * kRowThreads + tid; k < n; k += gridDim.x * kRowThreads) {
+            const int b = a.free_blocks[k];
+            if (in_pool(b, a.NB)) atomicAdd(a.refs_out + b, 1);
+        }
+    }
+    if (i >= a.S) return;
+    const int p = parent_of(a, i);
+    const int was = blocks_of(a.ctx[i], a.MB);
+    const int ctx = p < 0 ? 0 : max(a.ctx[p], 0);
+    const int is = blocks_of(ctx, a.MB);
+    const int* const old = a.tables + static_cast<size_t>(i) * a.MB;
+    const int* const row = a.tables + static_cast<size_t>(max(p, 0)) * a.MB;
+    int* const out = a.tables_out + static_cast<size_t>(i) * a.MB;
+    for (int j = tid; j < max(was, is); j += kRowThreads) {
+        const int x = j < was ? old[j] : -1;
+        const int y = j < is ? row[j] : -1;
+        if (j < is) out[j] = y;
+        if (x != y) {
+            if (in_pool(y, a.NB)) atomicAdd(a.refs_out + y, 1);
+            if (in_pool(x, a.NB)) atomicAdd(a.refs_out + x, -1);
+        }
+    }
+    int n = 0;
+    if (p >= 0) {
+        for (int k = tid; k < i; k += kRowThreads) n += a.parents[k] == p;
+    }
+    n = block_total<kRowThreads / 64>(n, s_part);
+    if (tid == 0) {
+        a.rank[i] = n;
+        a.ctx_out[i] = ctx;
+    }
+}
+
+// Bit b of word w of the pool: a block that nothing refers to (in use: LIVE).
+template <bool LIVE>
+__device__ __forceinline__ void scan_ids(const PagesArgs& a, const int* refs, int group, int* part) {
+    const int tid = threadIdx.x, lane = tid & 63;
+    const int w = __builtin_amdgcn_readfirstlane(tid >> 6);
+    int r[kEach];
+#pragma unroll
+    for (int k = 0; k < kEach; ++k) {
+        const int id = group * kIds + (w * kEach + k) * 64 + lane;
+        r[k] = id < a.NB ? refs[id] : (LIVE ? 0 : 1);
+    }
+    int n = 0;
+#pragma unroll
+    for (int k = 0; k < kEach; ++k) {
+        const unsigned long long m = __ballot(LIVE ? r[k] > 0 : r[k] <= 0);
+        if (lane == 0) {
+            a.bits[static_cast<size_t>(group) * kWords + w * kEach + k] = m;
+            n += __popcll(m);
+        }
+    }
+    n = block_total<kScanWaves>(n, part);
+    if (tid == 0) a.sums[group] = n;
+}
+
+// The last entry of a row that goes on, where it is partly filled and of the pool; -1: none.
+__device__ __forceinline__ int open_entry(const PagesArgs& a, int ctx) {
+    const int j = ctx >> kBlockShift;
+    return (ctx & (kBlockTokens - 1)) != 0 && j < a.MB ? j : -1;
+}
+
+__global__ __launch_bounds__(kScanThreads) void fork_scan_kernel(const PagesArgs a) {
+    __shared__ int s_part[kScanWaves];
+    const int tid = threadIdx.x;
+    if (static_cast<int>(blockIdx.x) < a.groups) {
+        scan_ids<false>(a, a.refs_out, blockIdx.x, s_part);
+        return;
+    }
+    // The rows that take a copy, in order, four rows a thread at a time.
+    int before = 0;
+    for (int s0 = 0; s0 < a.S; s0 += 4 * kScanThreads) {
+        bool copy[4];
+        int n = 0;
+#pragma unroll
+        for (int k = 0; k < 4; ++k) {
+            const int i = s0 + 4 * tid + k;
+            copy[k] = false;
+            if (i < a.S) {
+                const int j = open_entry(a, a.ctx_out[i]);
+                const int b = j < 0 ? -1 : a.tables_out[static_cast<size_t>(i) * a.MB + j];
+                copy[k] = in_pool(b, a.NB) && a.rank[i] < a.refs_out[b] - 1;
+            }
+            n += copy[k];
+        }
+        const int incl = wave_inclusive_scan(n);
+        if ((tid & 63) == 63) s_part[tid >> 6] = incl;
+        __syncthreads();
+        int at = before + incl - n;
+#pragma unroll
+        for (int w = 0; w < kScanWaves; ++w) {
+            if (w < (tid >> 6)) at += s_part[w];
+            before += s_part[w];
+        }
+        __syncthreads();
+#pragma unroll
+        for (int k = 0; k < 4; ++k) {
+            if (copy[k]) a.copies[at++] = s0 + 4 * tid + k;
+        }
+    }
+    if (tid == 0) a.num_copies[0] = before;
+}
+
+// What lies before this workgroup's ids, and in all: set bits. part: 2 kScanWaves.
+__device__ __forceinline__ void sums_of(const PagesArgs& a, int group, int* part, int& before, int& all) {
+    int x = 0, y = 0;
+    for (int k = threadIdx.x; k < a.groups; k += kScanThreads) {
+        const int n = a.sums[k];
+        y += n;
+        if (k < group) x += n;
+    }
+    before = block_total<kScanWaves>(x, part);
+    all = block_total<kScanWaves>(y, part + kScanWaves);
+}
+
+// For each of the thread's ids: take(id, bit, set bits before it in the pool).
+template <typename F>
+__device__ __forceinline__ void each_id(const PagesArgs& a, int group, int before, F take) {
+    const int lane = threadIdx.x & 63;
+    const int w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    const unsigned long long mine = a.bits[static_cast<size_t>(group) * kWords + lane];
+    const int n = __popcll(mine);
+    const int upto = wave_inclusive_scan(n) - n;
+#pragma unroll
+    for (int k = 0; k < kEach; ++k) {
+        const int word = w * kEach + k;
+        const unsigned lo = __builtin_amdgcn_readlane(static_cast<int>(mine), word);
+        const unsigned hi = __builtin_amdgcn_readlane(static_cast<int>(mine >> 32), word);
+        const unsigned long long m = static_cast<unsigned long long>(hi) << 32 | lo;
+        const int id = group * kIds + word * 64 + lane;
+        if (id < a.NB) {
+            take(id, ((m >> lane) & 1ull) != 0,
+                 before + __builtin_amdgcn_readlane(upto, word) + __popcll(m & ((1ull << lane) - 1ull)));
+        }
+    }
+}
+
+__global__ __launch_bounds__(kScanThreads) void fork_list_kernel(const PagesArgs a) {
+    __shared__ int s_part[2 * kScanWaves];
+    const int tid = threadIdx.x;
+    int before, all;
+    sums_of(a, blockIdx.x, s_part, before, all);
+    const int wanted = a.num_copies[0];
+    const int got = min(wanted, all);
+    auto open_of = [&](int i) { return a.tables_out + static_cast<size_t>(i) * a.MB + (a.ctx_out[i] >> kBlockShift); };
+    each_id(a, blockIdx.x, before, [&](int id, bool free, int k) {
+        if (!free) return;
+        if (k >= got) {
+            a.free_blocks[k - got] = id;
+            return;
+        }
+        int* const entry = open_of(a.copies[k]);
+        const int src = *entry;
+        a.pairs[2 * static_cast<size_t>(k)] = src;
+        a.pairs[2 * static_cast<size_t>(k) + 1] = id;
+        *entry = id;
+        a.refs_out[id] = 1;
+        atomicAdd(a.refs_out + src, -1);
+    });
+    for (int k = got + blockIdx.x * kScanThreads + tid; k < a.S; k += gridDim.x * kScanThreads) {
+        a.pairs[2 * static_cast<size_t>(k)] = -1;
+        a.pairs[2 * static_cast<size_t>(k) + 1] = -1;
+        if (k < wanted) {
+            // (no other thread reads this row)
+            const int i = a.copies[k];
+            atomicAdd(a.refs_out + *open_of(i), -1);
+            a.ctx_out[i] &= ~(kBlockTokens - 1);
+        }
+    }
+    if (blockIdx.x == 0 && tid == 0) {
+        a.num_free[0] = all - got;
+        a.counts[0] = got;
+        a.counts[1] = wanted - got;
+    }
+}
+
+__global__ __launch_bounds__(kScanThreads) void compact_scan_kernel(const PagesArgs a) {
+    __shared__ int s_part[kScanWaves];
+    scan_ids<true>(a, a.refs, blockIdx.x, s_part);
+}
+
+// How many blocks move, of `all` in use: the free ones among the first `all` ids,
+// at most the pairs' room. part: kScanWaves.
+__device__ __forceinline__ int moves_of(const PagesArgs& a, int all, int* part) {
+    const int group = all / kIds;
+    int x = 0;
+    for (int k = threadIdx.x; k < group; k += kScanThreads) x += a.sums[k];
+    if (group < a.groups && threadIdx.x < kWords) {
+        const int n = min(max(all - group * kIds - static_cast<int>(threadIdx.x) * 64, 0), 64);
+        const unsigned long long m = a.bits[static_cast<size_t>(group) * kWords + threadIdx.x];
+        x += __popcll(n == 64 ? m : m & ((1ull << n) - 1ull));
+    }
+    return min(all - block_total<kScanWaves>(x, part), a.rooms);
+}
+
+__global__ __launch_bounds__(kScanThreads) void compact_pairs_kernel(const PagesArgs a) {
+    __shared__ int s_part[3 * kScanWaves];
+    int before, all;
+    sums_of(a, blockIdx.x, s_part, before, all);
+    const int moves = moves_of(a, all, s_part + 2 * kScanWaves);
+    each_id(a, blockIdx.x, before, [&](int id, bool live, int k) {
+        const int at = live ? all - 1 - k : id - k;
+        if (at >= moves) return;
+        (live ? a.from : a.to)[at] = id;
+        if (live) a.order[id] = at;
+    });
+}
+
+__global__ __launch_bounds__(kScanThreads) void compact_apply_kernel(const PagesArgs a) {
+    __shared__ int s_part[3 * kScanWaves];
+    const int tid = threadIdx.x;
+    const int group = min(static_cast<int>(blockIdx.x), a.groups - 1);
+    int before, all;
+    sums_of(a, group, s_part, before, all);
+    const int moves = moves_of(a, all, s_part + 2 * kScanWaves);
+    const int lowest = moves > 0 ? a.from[moves - 1] : a.NB;   // of those that move
+    if (static_cast<int>(blockIdx.x) < a.groups) {
+        each_id(a, group, before, [&](int id, bool live, int k) {
+            const bool goes = live && id >= lowest;
+            const int r = id - k;                              // free ones before this
+            const bool comes = !live && r < moves;
+            a.new_ids[id] = goes ? a.to[a.order[id]] : id;
+            a.refs_out[id] = goes ? 0 : a.refs[comes ? a.from[r] : id];
+            if (id >= lowest) {
+                a.free_blocks[id - all] = id;
+            } else if (!live && !comes) {
+                a.free_blocks[r - moves] = id;
+            }
+        });
+        for (int k = blockIdx.x * kScanThreads + tid; k < a.rooms; k += a.groups * kScanThreads) {
+            a.pairs[2 * static_cast<size_t>(k)] = k < moves ? a.from[k] : -1;
+            a.pairs[2 * static_cast<size_t>(k) + 1] = k < moves ? a.to[k] : -1;
+        }
+        if (blockIdx.x == 0 && tid == 0) {
+            a.num_free[0] = a.NB - all;
+            a.counts[0] = moves;
+            a.counts[1] = all;
+        }
+        return;
+    }
+    const int i = blockIdx.x - a.groups;
+    const int used = blocks_of(a.ctx[i], a.MB);
+    const size_t at = static_cast<size_t>(i) * a.MB;
+    for (int j = tid; j < used; j += kScanThreads) {
+        const int b = a.tables[at + j];
+        int to = b;
+        if (b >= lowest && b < a.NB && ((a.bits[b >> 6] >> (b & 63)) & 1ull) != 0) to = a.to[a.order[b]];
+        a.tables_out[at + j] = to;
+    }
+}
+
+// Offsets of the workspace.
+struct Space {
+    size_t sums, copies_n, bits, rank, copies, from, to, order, bytes;
+};
+
+Space space_of(long long S, long long NB) {
+    const auto up = [](long long n) { return static_cast<size_t>((n + 255) / 256 * 256); };
+    const long long groups = (NB + kIds - 1) / kIds;
+    Space s;
+    s.sums = 0;
+    s.copies_n = s.sums + up(4 * groups);
+    s.bits = s.copies_n + 256;
+    s.rank = s.bits + up(8 * groups * kWords);
+    s.copies = s.rank + up(4 * S);
+    s.from = s.copies + up(4 * S);
+    s.to = s.from + up(4 * (NB / 2));
+    s.order = s.to + up(4 * (NB / 2));
+    s.bytes = s.order + up(4 * NB);
+    return s;
+}
+
+int check_sizes(const char* who, long long S, long long MB, int block_size, long long NB) {
+    if (S < 0 || MB < 0 || NB <= 0 || block_size <= 0) {
+        return fail(SWIFTLLM_ERR_INVALID_PARAMETER,
+                    "%s: num_seqs=%lld max_num_blocks_per_seq=%lld block_size=%d num_blocks=%lld", who, S, MB,
+                    block_size, NB);
+    }
+    if (block_size != kBlockTokens) {
+        return fail(SWIFTLLM_ERR_NOT_SUPPORTED, "%s: block_size=%d (supported: 16)", who, block_size);
+    }
+    // Slots are 32 bits, and so are a table's tokens.
+    if (S > 65535 || MB >= (1 << 27) || NB >= (1 << 27)) {
+        return fail(SWIFTLLM_ERR_NOT_SUPPORTED, "%s: num_seqs=%lld max_num_blocks_per_seq=%lld num_blocks=%lld", who, S,
+                    MB, NB);
+    }
+    return SWIFTLLM_OK;
+}
+
+void set_space(PagesArgs& a, void* workspace, const Space& s) {
+    char* const ws = static_cast<char*>(workspace);
+    a.sums = reinterpret_cast<int*>(ws + s.sums);
+    a.num_copies = reinterpret_cast<int*>(ws + s.copies_n);
+    a.bits = reinterpret_cast<unsigned long long*>(ws + s.bits);
+    a.rank = reinterpret_cast<int*>(ws + s.rank);
+    a.copies = reinterpret_cast<int*>(ws + s.copies);
+    a.from = reinterpret_cast<int*>(ws + s.from);
+    a.to = reinterpret_cast<int*>(ws + s.to);
+    a.order = reinterpret_cast<int*>(ws + s.order);
+}
+
+// Whether one of the first `outputs` spans shares bytes with another span.
+template <size_t N>
+bool tangled(const Bytes (&span)[N], size_t outputs) {
+    for (size_t i = 0; i < outputs; ++i) {
+        for (size_t j = i + 1; j < N; ++j) {
+            if (overlap_any(span[i], {span[j]})) return true;
+        }
+    }
+    return false;
+}
+
+}  // namespace
+}  // namespace swiftllm
+
+using namespace swiftllm;
+
+extern "C" {
+
+size_t swiftllm_hip_pages_workspace_size(int num_seqs, int num_blocks) {
+    if (check_sizes("swiftllm_hip_pages_workspace_size", num_seqs, 0, kBlockTokens, num_blocks) != SWIFTLLM_OK) return 0;
+    ok();
+    return space_of(num_seqs, num_blocks).bytes;
+}
+
+int swiftllm_hip_fork_pages(int32_t* block_tables_out, int32_t* context_lens_out, const int32_t* block_tables,
+                            const int32_t* context_lens, const int32_t* parents, int32_t* ref_counts,
+                            int32_t* free_blocks, int32_t* num_free, const int32_t* taken, int64_t* copy_pairs,
+                            int32_t* counts, void* workspace, size_t workspace_bytes, int num_seqs,
+                            int max_num_blocks_per_seq, int block_size, int num_blocks, hipStream_t stream) {
+    const char* who = "swiftllm_hip_fork_pages";
+    const int S = num_seqs, MB = max_num_blocks_per_seq, NB = num_blocks;
+    int rc = check_sizes(who, S, MB, block_size, NB);
+    if (rc != SWIFTLLM_OK) return rc;
+    if (!ref_counts || !free_blocks || !num_free || !counts || !workspace ||
+        (S > 0 && (!context_lens_out || !context_lens || !parents || !copy_pairs)) ||
+        (S > 0 && MB > 0 && (!block_tables_out || !block_tables))) {
+        return fail(SWIFTLLM_ERR_INVALID_PARAMETER, "%s: null pointer", who);
+    }
+    const Space space = space_of(S, NB);
+    if (workspace_bytes < space.bytes) {
+        return fail(SWIFTLLM_ERR_INVALID_PARAMETER, "%s: workspace of %zu bytes, %zu needed", who, workspace_bytes, space.bytes);
+    }
+    const size_t n = S, word = sizeof(int32_t);
+    const Bytes span[] = {{block_tables_out, word * n * MB}, {context_lens_out, word * n}, {ref_counts, word * NB},
+                          {free_blocks, word * NB}, {num_free, word}, {copy_pairs, 16 * n}, {counts, 2 * word},
+                          {workspace, space.bytes}, {block_tables, word * n * MB}, {context_lens, word * n},
+                          {parents, word * n}, {taken, word}};
+    for (const Bytes& s : span) {
+        if (!aligned(s.p, 4)) return fail(SWIFTLLM_ERR_INVALID_PARAMETER, "%s: misaligned pointer", who);
+    }
+    if (!aligned(workspace, 256) || !aligned(copy_pairs, 8)) {
+        return fail(SWIFTLLM_ERR_INVALID_PARAMETER, "%s: misaligned pointer", who);
+    }
+    if (tangled(span, 8)) return fail(SWIFTLLM_ERR_INVALID_PARAMETER, "%s: an output overlaps another argument", who);
+    rc = require_device();
+    if (rc != SWIFTLLM_OK) return rc;
+    PagesArgs a{};
+    a.tables = block_tables;
+    a.ctx = context_lens;
+    a.parents = parents;
+    a.tables_out = block_tables_out;
+    a.ctx_out = context_lens_out;
+    a.refs_out = ref_counts;
+    a.taken = taken;
+    a.free_blocks = free_blocks;
+    a.num_free = num_free;
+    a.pairs = reinterpret_cast<long long*>(copy_pairs);
+    a.counts = counts;
+    a.S = S;
+    a.MB = MB;
+    a.NB = NB;
+    a.groups = (NB + kIds - 1) / kIds;
+    a.rooms = S;
+    set_space(a, workspace, space);
+    rc = launched(launch(fork_rows_kernel, dim3(std::max(S, 1)), dim3(kRowThreads), 0, stream, a), who);
+    if (rc != SWIFTLLM_OK) return rc;
+    rc = launched(launch(fork_scan_kernel, dim3(a.groups + 1), dim3(kScanThreads), 0, stream, a), who);
+    if (rc != SWIFTLLM_OK) return rc;
+    return launched(launch(fork_list_kernel, dim3(a.groups), dim3(kScanThreads), 0, stream, a), who);
+}
+
+int swiftllm_hip_compact_pages(int32_t* block_tables_out, int32_t* ref_counts_out, const int32_t* block_tables,
+                               const int32_t* context_lens, const int32_t* ref_counts, int32_t* free_blocks,
+                               int32_t* num_free, int64_t* copy_pairs, int32_t* new_ids, int32_t* counts,
+                               void* workspace, size_t workspace_bytes, int num_seqs, int max_num_blocks_per_seq,
+                               int block_size, int num_blocks, int max_moves, hipStream_t stream) {
+    const char* who = "swiftllm_hip_compact_pages";
+    const int S = num_seqs, MB = max_num_blocks_per_seq, NB = num_blocks;
+    int rc = check_sizes(who, S, MB, block_size, NB);
+    if (rc != SWIFTLLM_OK) return rc;
+    if (max_moves < 0 || max_moves > NB) {
+        return fail(SWIFTLLM_ERR_INVALID_PARAMETER, "%s: max_moves=%d of num_blocks=%d", who, max_moves, NB);
+    }
+    if (!ref_counts_out || !ref_counts || !free_blocks || !num_free || !new_ids || !counts || !workspace ||
+        (max_moves > 0 && !copy_pairs) || (S > 0 && !context_lens) ||
+        (S > 0 && MB > 0 && (!block_tables_out || !block_tables))) {
+        return fail(SWIFTLLM_ERR_INVALID_PARAMETER, "%s: null pointer", who);
+    }
+    const Space space = space_of(S, NB);
+    if (workspace_bytes < space.bytes) {
+        return fail(SWIFTLLM_ERR_INVALID_PARAMETER, "%s: workspace of %zu bytes, %zu needed", who, workspace_bytes, space.bytes);
+    }
+    const size_t n = S, word = sizeof(int32_t);
+    const Bytes span[] = {{block_tables_out, word * n * MB}, {ref_counts_out, word * NB}, {free_blocks, word * NB},
+                          {num_free, word}, {copy_pairs, 16 * static_cast<size_t>(max_moves)}, {new_ids, word * NB},
+                          {counts, 2 * word}, {workspace, space.bytes}, {context_lens, word * n}, {ref_counts, word * NB},
+                          {block_tables_out == block_tables ? nullptr : block_tables, word * n * MB}};
+    for (const Bytes& s : span) {
+        if (!aligned(s.p, 4)) return fail(SWIFTLLM_ERR_INVALID_PARAMETER, "%s: misaligned pointer", who);
+    }
+    if (!aligned(workspace, 256) || !aligned(copy_pairs, 8)) {
+        return fail(SWIFTLLM_ERR_INVALID_PARAMETER, "%s: misaligned pointer", who);
+    }
+    if (tangled(span, 8)) return fail(SWIFTLLM_ERR_INVALID_PARAMETER, "%s: an output overlaps another argument", who);
+    rc = require_device();
+    if (rc != SWIFTLLM_OK) return rc;
+    PagesArgs a{};
+    a.tables = block_tables;
+    a.ctx = context_lens;
+    a.tables_out = block_tables_out;
+    a.refs = ref_counts;
+    a.refs_out = ref_counts_out;
+    a.free_blocks = free_blocks;
+    a.num_free = num_free;
+    a.pairs = reinterpret_cast<long long*>(copy_pairs);
+    a.new_ids = new_ids;
+    a.counts = counts;
+    a.S = S;
+    a.MB = MB;
+    a.NB = NB;
+    a.groups = (NB + kIds - 1) / kIds;
+    a.rooms = max_moves;
+    set_space(a, workspace, space);
+    rc = launched(launch(compact_scan_kernel, dim3(a.groups), dim3(kScanThreads), 0, stream, a), who);
+    if (rc != SWIFTLLM_OK) return rc;
+    rc = launched(launch(compact_pairs_kernel, dim3(a.groups), dim3(kScanThreads), 0, stream, a), who);
+    if (rc != SWIFTLLM_OK) return rc;
+    return launched(launch(compact_apply_kernel, dim3(a.groups + S), dim3(kScanThreads), 0, stream, a), who);
+}
+
+}  // extern "C"
