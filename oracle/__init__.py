@@ -467,7 +467,8 @@ def beam_select(logits, beam_scores, num_candidates: int, eos_id: int = -1):
                 gap = row - top
             score = c - np.log(np.exp(gap).sum()) + gap
             best = np.lexsort((np.arange(V), -row))[:C]      # of a beam: by logit, then token
-            found += [(-score[v], w, -row[v], v) for v in best.tolist() if score[v] > -np.inf]
+            found += [(-score[v], w, -row[v], v) for v in best.tolist() if score[v] >= -3.4028235677973366e38]
+            # (less rounds to -inf in 32 bits)
         found.sort()
         going = 0
         for k, (s, w, _, v) in enumerate(found[:C]):

@@ -11,7 +11,7 @@
 // and a list that holds their C largest. The threads' own maxima are 256 of them,
 // so the C-th largest of those is a threshold that at least C logits reach, and few
 // more do: only values in threads above it can. It is found bit by bit, a ballot
-// each, which costs an eighth of what the exponentials do. Second kernel, a
+// each. Second kernel, a
 // workgroup per request: the rows' lse, the same threshold over all lists' scores
 // rounded to 32 bits (which keeps their order), and the few that reach it ranked by
 // counting. Lists that ties fill past their room are cut to C one by one.
@@ -38,11 +38,14 @@ constexpr int kThreads = 256;
 constexpr int kWaves = kThreads / 64;
 constexpr int kEach = 32;                  // logits of a thread
 constexpr int kChunk = kThreads * kEach;
+constexpr int kGroup = 8, kGroups = kEach / kGroup;
+static_assert(kGroups == 4 && kEach == 32, "maxima, and a word of bits");
 constexpr int kRoom = 128;                 // entries of a chunk's list
 constexpr int kMostCandidates = 64;
 constexpr int kPickThreads = 1024;
 constexpr int kPickWaves = kPickThreads / 64;
-constexpr int kPickRoom = 512;             // candidates that are ranked
+constexpr int kPickKeys = kPickThreads / 2;
+constexpr int kPickRoom = 1024;            // candidates that are ranked
 constexpr float kLog2e = 1.4426950408889634f;
 static_assert(kMostCandidates <= kRoom && kMostCandidates <= kThreads, "a list holds the candidates");
 
@@ -73,8 +76,8 @@ struct SelectArgs {
 };
 
 struct F32 {};
-template <typename T>    // the upper bits in which keys differ
-constexpr int key_bits = std::is_same<T, BF16>::value ? 16 : std::is_same<T, F16>::value ? 19 : 32;
+template <typename T>    // the upper bits of a key that a line is found by
+constexpr int key_bits = std::is_same<T, BF16>::value ? 16 : 20;
 template <typename T>
 constexpr int vec_of = std::is_same<T, F32>::value ? 4 : 8;    // values of 16 bytes
 
@@ -87,20 +90,33 @@ __device__ __forceinline__ float of_key(unsigned k) {
     return __builtin_bit_cast(float, k ^ ((k >> 31) ? 0x80000000u : 0xffffffffu));
 }
 
-// The n-th largest of 256 keys, four of each lane, that differ in their `bits`
-// upper bits alone: the largest number that n of them reach.
-__device__ __forceinline__ unsigned nth_largest(const unsigned (&k)[4], int n, int bits) {
+// A number that n of 64 M keys reach, M of each lane, and hardly more: the
+// n-th largest of them with its lower bits cleared. One ballot a key and bit: at 20
+// bits a line lies at most 2^-11 of itself low.
+template <int BITS, int M>
+__device__ __forceinline__ unsigned nth_largest(const unsigned (&k)[M], int n) {
     unsigned t = 0;
-    for (int b = 31; b >= 32 - bits; --b) {
-        const unsigned c = t | (1u << b);
+#pragma unroll 1
+    for (unsigned bit = 1u << 31; bit >= 1u << (32 - BITS); bit >>= 1) {
+        const unsigned c = t | bit;
         int reach = 0;
 #pragma unroll
-        for (int i = 0; i < 4; ++i) reach += __popcll(__ballot(k[i] >= c));
+        for (int i = 0; i < M; ++i) reach += __popcll(__ballot(k[i] >= c));
         if (reach >= n) t = c;
     }
-    // A negative value's lower bits are ones in its key.
-    return (t >> 31) || bits == 32 ? t : t | ((1u << (32 - bits)) - 1u);
+    return t;
 }
+
+// The bare instructions: fmaxf quiets its operands first, an operation each. Of
+// values that are no number they make one or pass over it.
+__device__ __forceinline__ float max3(float a, float b, float c) {
+    float r;
+    asm("v_max3_f32 %0, %1, %2, %3" : "=v"(r) : "v"(a), "v"(b), "v"(c));
+    return r;
+}
+
+template <typename T>    // -infinity, as many as fit 32 bits
+constexpr unsigned kNone = std::is_same<T, F32>::value ? 0xff800000u : std::is_same<T, BF16>::value ? 0xff80ff80u : 0xfc00fc00u;
 
 // A value that is no number counts as one that is banned.
 __device__ __forceinline__ float number(float x) { return x != x ? -INFINITY : x; }
@@ -175,26 +191,47 @@ __global__ __launch_bounds__(kThreads) void beam_chunk_kernel(const SelectArgs a
     const char* const base = static_cast<const char*>(a.logits) + static_cast<long long>(row) * a.stride * kSize;
     const int off = static_cast<int>((reinterpret_cast<uintptr_t>(base) & 15u) / kSize);
     const int first = chunk * kChunk - off;
-    auto index = [&](int k) { return first + (k * kThreads + tid) * VEC; };
-    float v[kEach];
+    // All loads are on their way before the first is waited for. (Unpacked each in
+    // its own branch, 64 x 4 rows of 128000 bfloat16 logits took 30 us, not @@.)
+    u4 raw[NV];
 #pragma unroll
     for (int k = 0; k < NV; ++k) {
-        const int i = index(k);
+        const int i = first + (k * kThreads + tid) * VEC;
+        raw[k] = u4{kNone<T>, kNone<T>, kNone<T>, kNone<T>};
         if (i >= 0 && i <= a.V - VEC) {
-            const u4 r = __builtin_nontemporal_load(reinterpret_cast<const u4*>(base + static_cast<long long>(i) * kSize));
-            unpack<T>(r, v + k * VEC);
-        } else {
+            raw[k] = __builtin_nontemporal_load(reinterpret_cast<const u4*>(base + static_cast<long long>(i) * kSize));
+        }
+    }
+    float v[kEach];
 #pragma unroll
-            for (int j = 0; j < VEC; ++j) {
-                v[k * VEC + j] = i + j >= 0 && i + j < a.V ? load_one<T>(base, i + j) : -INFINITY;
+    for (int k = 0; k < NV; ++k) unpack<T>(raw[k], v + k * VEC);
+    if (first < 0 || first + kChunk > a.V) {
+        // Vectors that begin or end outside of the row.
+#pragma unroll
+        for (int k = 0; k < NV; ++k) {
+            const int i = first + (k * kThreads + tid) * VEC;
+            if ((i < 0 && i > -VEC) || (i < a.V && i > a.V - VEC)) {
+#pragma unroll
+                for (int j = 0; j < VEC; ++j) {
+                    if (i + j >= 0 && i + j < a.V) v[k * VEC + j] = load_one<T>(base, i + j);
+                }
             }
         }
     }
-    // (fmaxf passes over what is no number)
-    float most = -INFINITY;
+    // The largest of every kGroup values, and of all.
+    float top[kGroups], most;
+    auto maxima = [&] {
 #pragma unroll
-    for (int k = 0; k < kEach; ++k) most = fmaxf(most, v[k]);
-    s_key[tid] = key_of(most);
+        for (int g = 0; g < kGroups; ++g) {
+            const float* const x = v + g * kGroup;
+            top[g] = max3(x[0], x[1], x[2]);
+#pragma unroll
+            for (int k = 3; k + 1 < kGroup; k += 2) top[g] = max3(top[g], x[k], x[k + 1]);
+            top[g] = max3(top[g], x[kGroup - 1], x[kGroup - 1]);
+        }
+        most = max3(max3(top[0], top[1], top[2]), top[3], top[3]);
+    };
+    maxima();
     const float r = most * kLog2e;
     float sum = 0.0f;
 #pragma unroll
@@ -205,14 +242,14 @@ __global__ __launch_bounds__(kThreads) void beam_chunk_kernel(const SelectArgs a
         // type's range, or an infinite maximum, which has all the weight.
 #pragma unroll
         for (int k = 0; k < kEach; ++k) v[k] = number(v[k]);
-        if (!(sum < INFINITY)) {
-            sum = 0.0f;
+        maxima();
+        sum = 0.0f;
 #pragma unroll
-            for (int k = 0; k < kEach; ++k) {
-                sum += v[k] == most ? 1.0f : __builtin_amdgcn_exp2f((v[k] - most) * kLog2e);
-            }
+        for (int k = 0; k < kEach; ++k) {
+            sum += v[k] == most ? 1.0f : __builtin_amdgcn_exp2f((v[k] - most) * kLog2e);
         }
     }
+    s_key[tid] = key_of(most);
     const float wf = wave_max(most);
     const float ws = wave_sum(weighed(sum, most, wf));
     if (lane == 0) {
@@ -222,37 +259,46 @@ __global__ __launch_bounds__(kThreads) void beam_chunk_kernel(const SelectArgs a
     __syncthreads();
     const u4 ks = *reinterpret_cast<const u4*>(s_key + 4 * lane);
     const unsigned keys[4] = {ks[0], ks[1], ks[2], ks[3]};
-    // What is banned is no candidate.
-    const float line = fmaxf(of_key(nth_largest(keys, a.C, key_bits<T>)), -3.402823466e38f);
+    // What is banned is no candidate. (Some keys are no number's.)
+    const float line = fmaxf(of_key(nth_largest<key_bits<T>>(keys, a.C)), -3.402823466e38f);
+    unsigned mine = 0;     // which of the thread's values reach it
 #pragma unroll
-    for (int k = 0; k < kEach; ++k) {
-        if (v[k] >= line) {
-            const int at = atomicAdd(&s_fill, 1);
-            if (at < kRoom) s_list[at] = Entry{v[k], index(k / VEC) + k % VEC};
+    for (int g = 0; g < kGroups; ++g) {
+        if (__any(top[g] >= line)) {
+#pragma unroll
+            for (int k = g * kGroup; k < (g + 1) * kGroup; ++k) mine |= v[k] >= line ? 1u << k : 0u;
         }
+    }
+    // They are few, and read again rather than held in registers by number.
+    auto token_of = [&](int k) { return first + (k / VEC * kThreads + tid) * VEC + k % VEC; };
+    const int count = __popc(mine);
+    const int upto = wave_inclusive_scan(count);
+    int at = 0;
+    if (lane == 63 && upto > 0) at = atomicAdd(&s_fill, upto);
+    at = __builtin_amdgcn_readlane(at, 63) + upto - count;
+#pragma unroll 1
+    for (unsigned left = mine; left != 0; left &= left - 1, ++at) {
+        const int token = token_of(__ffs(left) - 1);
+        if (at < kRoom) s_list[at] = Entry{load_one<T>(base, token), token};
     }
     __syncthreads();
     int n = s_fill;
     if (n > kRoom) {
-        // Ties: the C largest one by one.
+        // Ties: the C largest one by one, each behind the last.
         n = a.C;
+        unsigned long long last = ~0ull;
+#pragma unroll 1
         for (int c = 0; c < n; ++c) {
             unsigned long long best = 0;
-#pragma unroll
-            for (int k = 0; k < kEach; ++k) {
-                const unsigned i = index(k / VEC) + k % VEC;
-                const unsigned long long key = static_cast<unsigned long long>(key_of(v[k] + 0.0f)) << 32 | (0xffffffffu - i);
-                if (v[k] >= line) best = std::max(best, key);
+#pragma unroll 1
+            for (unsigned left = mine; left != 0; left &= left - 1) {
+                const int token = token_of(__ffs(left) - 1);
+                const unsigned long long key = static_cast<unsigned long long>(key_of(load_one<T>(base, token) + 0.0f)) << 32 |
+                                               (0xffffffffu - static_cast<unsigned>(token));
+                if (key < last) best = std::max(best, key);
             }
-            best = block_max(best, s_best);
-            const int token = static_cast<int>(0xffffffffu - static_cast<unsigned>(best));
-#pragma unroll
-            for (int k = 0; k < kEach; ++k) {
-                if (index(k / VEC) + k % VEC == token) {
-                    s_list[c] = Entry{v[k], token};
-                    v[k] = -INFINITY;
-                }
-            }
+            last = block_max(best, s_best);
+            if (tid == 0) s_list[c] = Entry{of_key(static_cast<unsigned>(last >> 32)), static_cast<int>(0xffffffffu - static_cast<unsigned>(last))};
         }
         __syncthreads();
     }
@@ -289,9 +335,9 @@ __device__ __forceinline__ double wave_sum64(double x) {
 __global__ __launch_bounds__(kPickThreads) void beam_pick_kernel(const SelectArgs a) {
     __shared__ double s_base[kMostCandidates];     // of a beam: its score less log sum exp(x - top)
     __shared__ float s_top[kMostCandidates];
-    __shared__ __align__(16) unsigned s_key[kPickThreads / 4];
+    __shared__ __align__(16) unsigned s_key[kPickKeys];
     __shared__ Cand s_cand[kPickRoom];
-    __shared__ Cand s_best[kPickThreads / 64];
+    __shared__ Cand s_best[kPickWaves];
     __shared__ Cand s_order[kMostCandidates];
     __shared__ int s_fill;
     __shared__ float s_line;
@@ -336,21 +382,20 @@ __global__ __launch_bounds__(kPickThreads) void beam_pick_kernel(const SelectArg
                 const Entry e = a.lists[slot * kRoom + k];
                 // (beside an infinite logit only others of its kind have a share)
                 const double score = e.x == s_top[b] ? base : base + (e.x - top);
-                if (score > -INFINITY) take(Cand{score, e.x, b, e.token});
+                if (static_cast<float>(score) > -INFINITY) take(Cand{score, e.x, b, e.token});
             }
         }
     };
     float most = -INFINITY;
     each([&](const Cand& c) { most = fmaxf(most, static_cast<float>(c.score)); });
     most = fmaxf(most, __shfl_xor(most, 1));
-    most = fmaxf(most, __shfl_xor(most, 2));
-    if ((tid & 3) == 0) s_key[tid >> 2] = key_of(most);
+    if ((tid & 1) == 0) s_key[tid >> 1] = key_of(most);
     __syncthreads();
     if (w == 0) {
-        const u4 ks = *reinterpret_cast<const u4*>(s_key + 4 * lane);
-        const unsigned keys[4] = {ks[0], ks[1], ks[2], ks[3]};
-        const unsigned t = nth_largest(keys, a.C, 32);
-        if (lane == 0) s_line = of_key(t);
+        const u4 k0 = *reinterpret_cast<const u4*>(s_key + 8 * lane), k1 = *reinterpret_cast<const u4*>(s_key + 8 * lane + 4);
+        const unsigned keys[8] = {k0[0], k0[1], k0[2], k0[3], k1[0], k1[1], k1[2], k1[3]};
+        const unsigned t = nth_largest<20>(keys, a.C);
+        if (lane == 0) s_line = fmaxf(of_key(t), -3.402823466e38f);
     }
     __syncthreads();
     const float line = s_line;
