@@ -42,10 +42,9 @@ constexpr int kGroup = 8, kGroups = kEach / kGroup;
 static_assert(kGroups == 4 && kEach == 32, "maxima, and a word of bits");
 constexpr int kRoom = 128;                 // entries of a chunk's list
 constexpr int kMostCandidates = 64;
-constexpr int kPickThreads = 1024;
-constexpr int kPickWaves = kPickThreads / 64;
-constexpr int kPickKeys = kPickThreads / 2;
+constexpr int kPickLists = 1024;           // lists that reach the first line
 constexpr int kPickRoom = 1024;            // candidates that are ranked
+constexpr int kFewEnough = 160;            // by one line
 constexpr float kLog2e = 1.4426950408889634f;
 static_assert(kMostCandidates <= kRoom && kMostCandidates <= kThreads, "a list holds the candidates");
 
@@ -332,73 +331,127 @@ __device__ __forceinline__ double wave_sum64(double x) {
     return x;
 }
 
-__global__ __launch_bounds__(kPickThreads) void beam_pick_kernel(const SelectArgs a) {
+// SMALL: every 16 threads have a list of their own, whose entries are on their way
+// before anything else is known. Otherwise the lists' maxima give a first line, and
+// only lists that reach it are read.
+template <int THREADS, bool SMALL>
+__global__ __launch_bounds__(THREADS) void beam_pick_kernel(const SelectArgs a) {
+    constexpr int WAVES = THREADS / 64;
+    constexpr int KEYS = THREADS / 128;            // a lane's, of every two threads' maxima
     __shared__ double s_base[kMostCandidates];     // of a beam: its score less log sum exp(x - top)
     __shared__ float s_top[kMostCandidates];
-    __shared__ __align__(16) unsigned s_key[kPickKeys];
+    __shared__ __align__(16) unsigned s_key[THREADS / 2];
     __shared__ Cand s_cand[kPickRoom];
-    __shared__ Cand s_best[kPickWaves];
+    __shared__ Cand s_best[WAVES];
     __shared__ Cand s_order[kMostCandidates];
-    __shared__ int s_fill;
+    __shared__ int s_list[SMALL ? 1 : kPickLists];
+    __shared__ int s_fill, s_lists;
     __shared__ float s_line;
     const int tid = threadIdx.x, lane = tid & 63;
     const int w = __builtin_amdgcn_readfirstlane(tid >> 6);
     const int r = blockIdx.x;
-    if (tid == 0) s_fill = 0;
-    for (int b = w; b < a.W; b += kPickWaves) {
+    const int lists = a.W * a.chunks;
+    const size_t slot0 = static_cast<size_t>(r) * lists;
+    if (tid == 0) s_fill = s_lists = 0;
+    // (entries past a list's fill are read and not used)
+    constexpr int kKept = kRoom / 16, kFirst = 2;
+    Entry kept[SMALL ? kKept : 1];
+    int fill = 0;
+    if (SMALL && tid >> 4 < lists) {
+        fill = a.fill[slot0 + (tid >> 4)];
+#pragma unroll
+        for (int k = 0; k < kFirst; ++k) kept[k] = a.lists[(slot0 + (tid >> 4)) * kRoom + (tid & 15) + 16 * k];
+    }
+    for (int b = w; b < a.W; b += WAVES) {
         const size_t row = static_cast<size_t>(r) * a.W + b;
         const float score = a.scores[row];
+        const float2* const sums = a.sums + row * a.chunks;
+        const float2 mine = lane < a.chunks ? sums[lane] : float2{-INFINITY, 0.0f};
         double base = -INFINITY;
         float top = 0.0f;
         if (score > -INFINITY) {
-            const float2* const sums = a.sums + row * a.chunks;
-            float F = -INFINITY;
-            for (int c = lane; c < a.chunks; c += 64) F = fmaxf(F, sums[c].x);
-            F = wave_max(F);
-            double S = 0.0;
-            for (int c = lane; c < a.chunks; c += 64) {
-                const float2 x = sums[c];
-                S += x.x == F ? static_cast<double>(x.y) : x.y * exp(static_cast<double>(x.x) - F);
-            }
-            S = wave_sum64(S);
-            base = score - log(S);
-            top = F;
+            top = mine.x;
+            for (int c = lane + 64; c < a.chunks; c += 64) top = fmaxf(top, sums[c].x);
+            top = wave_max(top);
+            double S = weighed(mine.y, mine.x, top);
+            for (int c = lane + 64; c < a.chunks; c += 64) S += weighed(sums[c].y, sums[c].x, top);
+            base = score - log(wave_sum64(S));
         }
         if (lane == 0) {
             s_base[b] = base;
             s_top[b] = top;
         }
     }
+    if constexpr (SMALL) {
+#pragma unroll
+        for (int k = kFirst; k < kKept; ++k) {
+            if (16 * k < fill) kept[k] = a.lists[(slot0 + (tid >> 4)) * kRoom + (tid & 15) + 16 * k];
+        }
+    }
     __syncthreads();
-    // A list per 16 lanes.
-    const int lists = a.W * a.chunks;
-    auto each = [&](auto take) {
-        for (int i = tid >> 4; i < lists; i += kPickThreads / 16) {
+    // (beside an infinite logit only others of its kind have a share)
+    auto score_of = [&](int b, float x) { return x == s_top[b] ? s_base[b] : s_base[b] + (x - static_cast<double>(s_top[b])); };
+    // A line that C candidates reach, of every two threads' maxima.
+    auto find_line = [&](float most) {
+        most = fmaxf(most, __shfl_xor(most, 1));
+        if ((tid & 1) == 0) s_key[tid >> 1] = key_of(most);
+        __syncthreads();
+        if (w == 0) {
+            unsigned keys[KEYS];
+#pragma unroll
+            for (int k = 0; k < KEYS; ++k) keys[k] = s_key[64 * k + lane];
+            const unsigned t = nth_largest<20>(keys, a.C);
+            if (lane == 0) s_line = fmaxf(of_key(t), -3.402823466e38f);
+        }
+        __syncthreads();
+        return s_line;
+    };
+    int use = lists;
+    bool some = false;     // the lists named in s_list
+    if constexpr (!SMALL) {
+        // (a beam without a score has no sums)
+        auto list_max = [&](int i) {
             const int b = i / a.chunks;
-            const size_t slot = static_cast<size_t>(r) * lists + i;
-            const int n = a.fill[slot];
-            const double base = s_base[b], top = s_top[b];
-            for (int k = tid & 15; k < n; k += 16) {
-                const Entry e = a.lists[slot * kRoom + k];
-                // (beside an infinite logit only others of its kind have a share)
-                const double score = e.x == s_top[b] ? base : base + (e.x - top);
+            return s_base[b] > -INFINITY ? static_cast<float>(score_of(b, a.sums[slot0 + i].x)) : -INFINITY;
+        };
+        float most = -INFINITY;
+        for (int i = tid; i < lists; i += THREADS) most = fmaxf(most, list_max(i));
+        const float line = find_line(most);
+        for (int i = tid; i < lists; i += THREADS) {
+            if (list_max(i) >= line) {
+                const int at = atomicAdd(&s_lists, 1);
+                if (at < kPickLists) s_list[at] = i;
+            }
+        }
+        __syncthreads();
+        some = s_lists <= kPickLists;
+        if (some) use = s_lists;
+    }
+    auto each = [&](auto take) {
+        if constexpr (SMALL) {
+            const int b = (tid >> 4) / a.chunks;
+#pragma unroll
+            for (int k = 0; k < kKept; ++k) {
+                if ((tid & 15) + 16 * k >= fill) break;
+                const double score = score_of(b, kept[k].x);
+                if (static_cast<float>(score) > -INFINITY) take(Cand{score, kept[k].x, b, kept[k].token});
+            }
+            return;
+        }
+        for (int k = tid >> 4; k < use; k += THREADS / 16) {
+            const int i = some ? s_list[k] : k;
+            const int b = i / a.chunks;
+            const int n = a.fill[slot0 + i];
+            for (int z = tid & 15; z < n; z += 16) {
+                const Entry e = a.lists[(slot0 + i) * kRoom + z];
+                const double score = score_of(b, e.x);
                 if (static_cast<float>(score) > -INFINITY) take(Cand{score, e.x, b, e.token});
             }
         }
     };
     float most = -INFINITY;
     each([&](const Cand& c) { most = fmaxf(most, static_cast<float>(c.score)); });
-    most = fmaxf(most, __shfl_xor(most, 1));
-    if ((tid & 1) == 0) s_key[tid >> 1] = key_of(most);
-    __syncthreads();
-    if (w == 0) {
-        const u4 k0 = *reinterpret_cast<const u4*>(s_key + 8 * lane), k1 = *reinterpret_cast<const u4*>(s_key + 8 * lane + 4);
-        const unsigned keys[8] = {k0[0], k0[1], k0[2], k0[3], k1[0], k1[1], k1[2], k1[3]};
-        const unsigned t = nth_largest<20>(keys, a.C);
-        if (lane == 0) s_line = fmaxf(of_key(t), -3.402823466e38f);
-    }
-    __syncthreads();
-    const float line = s_line;
+    const float line = find_line(most);
     each([&](const Cand& c) {
         if (static_cast<float>(c.score) >= line) {
             const int at = atomicAdd(&s_fill, 1);
@@ -407,12 +460,25 @@ __global__ __launch_bounds__(kPickThreads) void beam_pick_kernel(const SelectArg
     });
     __syncthreads();
     int n = s_fill;
+    if (THREADS == kPickRoom && n > kFewEnough && n <= kPickRoom) {
+        // A closer line among these: they are ranked by n^2 comparisons.
+        const Cand mine = tid < n ? s_cand[tid] : Cand{-INFINITY, 0.0f, 0, -1};
+        const float closer = find_line(static_cast<float>(mine.score));
+        if (tid == 0) s_fill = 0;
+        __syncthreads();
+        if (static_cast<float>(mine.score) >= closer) s_cand[atomicAdd(&s_fill, 1)] = mine;
+        __syncthreads();
+        n = s_fill;
+    }
     if (n <= kPickRoom) {
-        for (int i = tid; i < n; i += kPickThreads) {
+        // Eight threads compare a candidate with every eighth.
+        for (int i = tid >> 3; i < n; i += THREADS / 8) {
             const Cand mine = s_cand[i];
             int rank = 0;
-            for (int j = 0; j < n; ++j) rank += before(s_cand[j], mine);
-            if (rank < a.C) s_order[rank] = mine;
+            for (int j = tid & 7; j < n; j += 8) rank += before(s_cand[j], mine);
+#pragma unroll
+            for (int d = 1; d < 8; d <<= 1) rank += __shfl_xor(rank, d);
+            if ((tid & 7) == 0 && rank < a.C) s_order[rank] = mine;
         }
         n = min(n, a.C);
     } else {
@@ -433,7 +499,7 @@ __global__ __launch_bounds__(kPickThreads) void beam_pick_kernel(const SelectArg
             if (lane == 0) s_best[w] = best;
             __syncthreads();
             if (tid == 0) {
-                for (int i = 1; i < kPickWaves; ++i) {
+                for (int i = 1; i < WAVES; ++i) {
                     if (before(s_best[i], best)) best = s_best[i];
                 }
                 s_order[k] = best;
@@ -583,7 +649,9 @@ int swiftllm_hip_beam_select(const void* logits, const float* beam_scores, float
     static const K kernels[3] = {beam_chunk_kernel<F16>, beam_chunk_kernel<BF16>, beam_chunk_kernel<F32>};
     rc = launched(launch(kernels[dtype], dim3(static_cast<unsigned>(rows * space.chunks)), dim3(kThreads), 0, stream, a), who);
     if (rc != SWIFTLLM_OK) return rc;
-    return launched(launch(beam_pick_kernel, dim3(static_cast<unsigned>(R)), dim3(kPickThreads), 0, stream, a), who);
+    const long long lists = W * space.chunks;
+    const K pick = lists <= 16 ? beam_pick_kernel<256, true> : lists <= 64 ? beam_pick_kernel<1024, true> : beam_pick_kernel<1024, false>;
+    return launched(launch(pick, dim3(static_cast<unsigned>(R)), dim3(lists <= 16 ? 256 : 1024), 0, stream, a), who);
 }
 
 }  // extern "C"
