@@ -493,7 +493,7 @@ def _own_shared(s: dict) -> dict:
     plan = _kept(s, "plan", lambda: step.plan_shared_size(*sizes))
     ws = _kept(s, "ws", lambda: step.shared_decode_workspace_size(*sizes))
     step.plan_shared(_ptr(plan), plan.numel(), _ptr(s["shared"]), _ptr(s["bt"]), _ptr(s["ctx"]),
-                     _ptr(s["goff"]), s["N"], *sizes, num_blocks=s["NB"])
+                     _ptr(s["goff"]), s["N"], *sizes)
     score = step.ScoreParams(scale=s["scale"], softcap=case["cap"], alibi_slopes=_ptr(s["slopes"]))
     for x, out in zip(s["layers"], s["out"]):
         step.shared_decode(_ptr(out), _ptr(ws), ws.numel(), _ptr(plan), plan.numel(), _ptr(x["q"]),
