@@ -619,7 +619,9 @@ size_t swiftllm_hip_beam_select_workspace_size(int num_requests,
  * refers to then, in ascending order (room for num_blocks; entries behind stay),
  * and counts[2] = copies, rows cut. taken (NULL: none): the first taken[0] of
  * free_blocks as they come in were taken since (counts of
- * swiftllm_hip_plan_step) and get their first reference here. Entries of a row
+ * swiftllm_hip_plan_step) and get their first reference here. new_lens [num_seqs]
+ * (NULL: not wanted): 1 for rows that go on, 0 for those that ended or were cut,
+ * which the next swiftllm_hip_plan_step takes. Entries of a row
  * behind its context stay as they were; ids outside [0, num_blocks) are carried
  * along and not counted. No output may overlap another argument. */
 int swiftllm_hip_fork_pages(
@@ -627,9 +629,9 @@ int swiftllm_hip_fork_pages(
     const int32_t* block_tables, const int32_t* context_lens,
     const int32_t* parents, int32_t* ref_counts, int32_t* free_blocks,
     int32_t* num_free, const int32_t* taken, int64_t* copy_pairs,
-    int32_t* counts, void* workspace, size_t workspace_bytes, int num_seqs,
-    int max_num_blocks_per_seq, int block_size, int num_blocks,
-    hipStream_t stream);
+    int32_t* new_lens, int32_t* counts, void* workspace,
+    size_t workspace_bytes, int num_seqs, int max_num_blocks_per_seq,
+    int block_size, int num_blocks, hipStream_t stream);
 
 /* Brings a pool together: the highest block that something refers to moves to
  * the lowest that nothing does, and so on while it lies above it, at most
@@ -648,6 +650,52 @@ int swiftllm_hip_compact_pages(
     int64_t* copy_pairs, int32_t* new_ids, int32_t* counts, void* workspace,
     size_t workspace_bytes, int num_seqs, int max_num_blocks_per_seq,
     int block_size, int num_blocks, int max_moves, hipStream_t stream);
+
+/* The plan of a step's attention over shared blocks, once for all of its layers.
+ * Group g is the sequences group_offsets[g] .. group_offsets[g + 1] - 1 (device
+ * memory, num_groups + 1 entries ascending within [0, num_seqs]; otherwise no
+ * group shares anything); a sequence of no group shares nothing. Writes
+ * shared_blocks[g], the leading blocks that every sequence of the group with a
+ * context uses, and all of them the same (0 where none has a context), and the
+ * plan: swiftllm_hip_plan_shared_size() bytes, 256-byte aligned, for
+ * swiftllm_hip_shared_decode calls with the same sizes, which take the contexts
+ * and what is shared from it. */
+int swiftllm_hip_plan_shared(void* plan, size_t plan_bytes,
+                             int32_t* shared_blocks,
+                             const int32_t* block_tables,
+                             const int32_t* context_lens,
+                             const int32_t* group_offsets, int num_groups,
+                             int num_seqs, int num_heads, int num_kv_heads,
+                             int head_dim, int block_size,
+                             int max_num_blocks_per_seq, hipStream_t stream);
+
+/* Bytes of a plan; 0 where swiftllm_hip_plan_shared would refuse the sizes. */
+size_t swiftllm_hip_plan_shared_size(int num_seqs, int num_heads,
+                                     int num_kv_heads, int head_dim,
+                                     int block_size,
+                                     int max_num_blocks_per_seq);
+
+/* swiftllm_hip_scored_decode without windows, where sequences share blocks: the
+ * blocks that a group shares are read once for all of its sequences. Contexts are
+ * the plan's; block_tables are those that it was made from. A plan of other sizes
+ * writes nothing. Values that are not finite and unknown blocks are as there;
+ * weights are rounded to dtype, as in swiftllm_hip_scored_prefill. The caches are
+ * 16-byte aligned; output overlaps no other argument. `workspace`: plain scratch,
+ * 256-byte aligned, of swiftllm_hip_shared_decode_workspace_size() bytes; calls
+ * that share one must be ordered on one stream. */
+int swiftllm_hip_shared_decode(
+    void* output, void* workspace, size_t workspace_bytes, const void* plan,
+    size_t plan_bytes, const void* query, const void* key_cache,
+    const void* value_cache, const int32_t* block_tables,
+    const int32_t* query_offsets, const float* alibi_slopes, float scale,
+    float softcap, int dtype, int num_tokens, int num_seqs, int num_heads,
+    int num_kv_heads, int head_dim, int block_size, int max_num_blocks_per_seq,
+    int num_blocks, hipStream_t stream);
+
+/* Bytes of workspace it needs for these sizes; 0 where it would refuse them. */
+size_t swiftllm_hip_shared_decode_workspace_size(
+    int num_seqs, int num_heads, int num_kv_heads, int head_dim,
+    int block_size, int max_num_blocks_per_seq);
 
 /* Bytes of workspace (plain scratch, 256-byte aligned) that
  * swiftllm_hip_fork_pages and swiftllm_hip_compact_pages need; 0 where they

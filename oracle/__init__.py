@@ -562,3 +562,21 @@ def compact_pages(block_tables, context_lens, ref_counts, free_blocks, max_moves
     pairs = np.full((max_moves, 2), -1, np.int64)
     pairs[:len(moves)] = np.array(moves, np.int64).reshape(-1, 2)
     return tables, refs, free, len(left), pairs, ids, np.array([len(moves), len(used)], np.int32)
+
+
+def shared_blocks(block_tables, context_lens, group_offsets):
+    """The leading blocks that all sequences of a group with a context use, and
+    alike: what swiftllm_hip_plan_shared documents."""
+    bt = np.asarray(block_tables)
+    S, MB = bt.shape
+    off = [int(o) for o in group_offsets]
+    if any(not 0 <= b <= e <= S for b, e in zip(off, off[1:])):
+        return np.zeros(len(off) - 1, np.int32)
+    out = []
+    for b, e in zip(off, off[1:]):
+        rows = [bt[s, :min(-(-int(context_lens[s]) // 16), MB)].tolist() for s in range(b, e) if context_lens[s] > 0]
+        n = 0
+        while rows and all(len(r) > n and r[n] == rows[0][n] for r in rows):
+            n += 1
+        out.append(n)
+    return np.array(out, np.int32)

@@ -297,7 +297,7 @@ extern "C" {
         block_tables_out: *mut i32, context_lens_out: *mut i32, block_tables: *const i32,
         context_lens: *const i32, parents: *const i32, ref_counts: *mut i32,
         free_blocks: *mut i32, num_free: *mut i32, taken: *const i32, copy_pairs: *mut i64,
-        counts: *mut i32, workspace: *mut c_void, workspace_bytes: usize, num_seqs: c_int,
+        new_lens: *mut i32, counts: *mut i32, workspace: *mut c_void, workspace_bytes: usize, num_seqs: c_int,
         max_num_blocks_per_seq: c_int, block_size: c_int, num_blocks: c_int,
         stream: hipStream_t,
     ) -> c_int;
@@ -310,6 +310,30 @@ extern "C" {
         max_moves: c_int, stream: hipStream_t,
     ) -> c_int;
     pub fn swiftllm_hip_pages_workspace_size(num_seqs: c_int, num_blocks: c_int) -> usize;
+    pub fn swiftllm_hip_plan_shared(
+        plan: *mut c_void, plan_bytes: usize, shared_blocks: *mut i32,
+        block_tables: *const i32, context_lens: *const i32, group_offsets: *const i32,
+        num_groups: c_int, num_seqs: c_int, num_heads: c_int, num_kv_heads: c_int,
+        head_dim: c_int, block_size: c_int, max_num_blocks_per_seq: c_int,
+        stream: hipStream_t,
+    ) -> c_int;
+    pub fn swiftllm_hip_plan_shared_size(
+        num_seqs: c_int, num_heads: c_int, num_kv_heads: c_int, head_dim: c_int,
+        block_size: c_int, max_num_blocks_per_seq: c_int,
+    ) -> usize;
+    pub fn swiftllm_hip_shared_decode(
+        output: *mut c_void, workspace: *mut c_void, workspace_bytes: usize,
+        plan: *const c_void, plan_bytes: usize, query: *const c_void,
+        key_cache: *const c_void, value_cache: *const c_void, block_tables: *const i32,
+        query_offsets: *const i32, alibi_slopes: *const c_float, scale: c_float,
+        softcap: c_float, dtype: c_int, num_tokens: c_int, num_seqs: c_int,
+        num_heads: c_int, num_kv_heads: c_int, head_dim: c_int, block_size: c_int,
+        max_num_blocks_per_seq: c_int, num_blocks: c_int, stream: hipStream_t,
+    ) -> c_int;
+    pub fn swiftllm_hip_shared_decode_workspace_size(
+        num_seqs: c_int, num_heads: c_int, num_kv_heads: c_int, head_dim: c_int,
+        block_size: c_int, max_num_blocks_per_seq: c_int,
+    ) -> usize;
 
     // -- host metadata: kv_cache.rs:186-216, 250-286 ------------------------------
     pub fn swiftllm_hip_slot_mapping(

@@ -108,10 +108,17 @@ SIGNATURES = {
         i32, [vp, vp, vp, vp, vp, vp, vp, vp, vp, sz, i32, i32, i32, i32, i32, i64, i32, vp]),
     "swiftllm_hip_beam_select_workspace_size": (sz, [i32, i32, i32, i32]),
     "swiftllm_hip_fork_pages": (
-        i32, [vp, vp, vp, vp, vp, vp, vp, vp, vp, vp, vp, vp, sz, i32, i32, i32, i32, vp]),
+        i32, [vp, vp, vp, vp, vp, vp, vp, vp, vp, vp, vp, vp, vp, sz, i32, i32, i32, i32, vp]),
     "swiftllm_hip_compact_pages": (
         i32, [vp, vp, vp, vp, vp, vp, vp, vp, vp, vp, vp, sz, i32, i32, i32, i32, i32, vp]),
     "swiftllm_hip_pages_workspace_size": (sz, [i32, i32]),
+    "swiftllm_hip_plan_shared": (
+        i32, [vp, sz, vp, vp, vp, vp, i32, i32, i32, i32, i32, i32, i32, vp]),
+    "swiftllm_hip_plan_shared_size": (sz, [i32, i32, i32, i32, i32, i32]),
+    "swiftllm_hip_shared_decode": (
+        i32, [vp, vp, sz, vp, sz, vp, vp, vp, vp, vp, vp, f32, f32, i32, i32, i32, i32, i32, i32,
+              i32, i32, i32, vp]),
+    "swiftllm_hip_shared_decode_workspace_size": (sz, [i32, i32, i32, i32, i32, i32]),
     "swiftllm_hip_slot_mapping": (i32, [vp, sz, sz, sz, sz, vp]),
     "swiftllm_hip_pack_block_tables": (i32, [vp, vp, vp, sz, sz, sz, vp, vp]),
 }

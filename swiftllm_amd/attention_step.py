@@ -5,6 +5,9 @@
     scored_decode       paged attention of one new token, its scores shaped: soft cap,
                         distance bias (ALiBi), sliding window, prefix
     scored_prefill      the same of packed prompts or chunks of them
+    plan_shared, shared_decode
+                        scored_decode of sequences whose tables begin alike, their
+                        common blocks read once
 
 Reference (paths relative to the swiftllm repository): the host routines and
 options these stand for are
@@ -216,6 +219,61 @@ def scored_prefill(output: Ptr, query: Ptr, key_cache: Ptr, value_cache: Ptr, bl
         num_kv_heads, head_dim, block_size, max_num_blocks_per_seq, num_blocks, _s(stream)))
 
 
+# ---------------------------------------------------------------------------
+# Sequences that share blocks
+# ---------------------------------------------------------------------------
+def plan_shared_size(num_seqs: int, num_heads: int, num_kv_heads: int, head_dim: int,
+                     block_size: int, max_num_blocks_per_seq: int) -> int:
+    n = _lib.lib().swiftllm_hip_plan_shared_size(
+        num_seqs, num_heads, num_kv_heads, head_dim, block_size, max_num_blocks_per_seq)
+    if n == 0:
+        check_status(_lib.lib().swiftllm_hip_last_error() or CudaError.code)
+    return int(n)
+
+
+def plan_shared(plan: Ptr, plan_bytes: int, shared_blocks: Ptr, block_tables: Ptr,
+                context_lens: Ptr, group_offsets: Ptr, num_groups: int, num_seqs: int,
+                num_heads: int, num_kv_heads: int, head_dim: int, block_size: int,
+                max_num_blocks_per_seq: int, stream: Optional[Stream] = None) -> None:
+    """The plan of a step's shared_decode calls (swiftllm_hip_plan_shared): the
+    sequences group_offsets[g] .. group_offsets[g + 1] - 1 are a group, and
+    shared_blocks[g] becomes the leading blocks that all of them have in common.
+    `plan` holds plan_shared_size(...) bytes and serves every layer of these sizes."""
+    check_status(_lib.lib().swiftllm_hip_plan_shared(
+        _p(plan), plan_bytes, _p(shared_blocks), _p(block_tables), _p(context_lens),
+        _p(group_offsets), num_groups, num_seqs, num_heads, num_kv_heads, head_dim, block_size,
+        max_num_blocks_per_seq, _s(stream)))
+
+
+def shared_decode_workspace_size(num_seqs: int, num_heads: int, num_kv_heads: int, head_dim: int,
+                                 block_size: int, max_num_blocks_per_seq: int) -> int:
+    n = _lib.lib().swiftllm_hip_shared_decode_workspace_size(
+        num_seqs, num_heads, num_kv_heads, head_dim, block_size, max_num_blocks_per_seq)
+    if n == 0:
+        check_status(_lib.lib().swiftllm_hip_last_error() or CudaError.code)
+    return int(n)
+
+
+def shared_decode(output: Ptr, workspace: Ptr, workspace_bytes: int, plan: Ptr, plan_bytes: int,
+                  query: Ptr, key_cache: Ptr, value_cache: Ptr, block_tables: Ptr,
+                  score: ScoreParams, num_seqs: int, num_heads: int, num_kv_heads: int,
+                  head_dim: int, block_size: int, max_num_blocks_per_seq: int, dtype: str = "f16",
+                  num_blocks: int = 0, query_offsets: Ptr = None, num_tokens: int = 0,
+                  stream: Optional[Stream] = None) -> None:
+    """scored_decode where the blocks that a group shares are read once for all of
+    its sequences (swiftllm_hip_shared_decode); contexts and groups are the
+    plan's. Without a window (under one, little of a long prefix is seen:
+    scored_decode); score.prefix_lens has no effect then."""
+    if score.window:
+        raise NotSupported(f"window {score.window} over shared blocks")
+    check_status(_lib.lib().swiftllm_hip_shared_decode(
+        _p(output), _p(workspace), workspace_bytes, _p(plan), plan_bytes, _p(query),
+        _p(key_cache), _p(value_cache), _p(block_tables), _p(query_offsets),
+        _p(score.alibi_slopes), score.scale, score.softcap, _dtype(dtype), num_tokens, num_seqs,
+        num_heads, num_kv_heads, head_dim, block_size, max_num_blocks_per_seq, num_blocks,
+        _s(stream)))
+
+
 class AttentionStep:
     """A layer's share of a serving step: rotary positions and the cache write,
     then attention with shaped scores, over the arrays that plan() makes once
@@ -230,13 +288,19 @@ class AttentionStep:
     num_seqs and num_tokens are capacities: sequences past a batch have
     cached and new lengths of 0, rows past its tokens are left as they are.
     The rows of a step whose every sequence brings at most one token go through
-    scored_decode (decode=True), all others through scored_prefill."""
+    scored_decode (decode=True), all others through scored_prefill.
+
+    num_groups > 0: plan() also takes group_offsets, the groups of sequences whose
+    tables begin alike (beams, chats on one prompt), and a decode step reads what
+    each group shares once (plan_shared, shared_decode)."""
 
     def __init__(self, num_seqs: int, num_tokens: int, max_num_blocks_per_seq: int,
                  num_heads: int, num_kv_heads: int, head_dim: int, score: ScoreParams,
                  inv_freq: np.ndarray, attn_factor: float = 1.0, interleaved: bool = False,
-                 dtype: str = "f16", block_size: int = 16):
+                 dtype: str = "f16", block_size: int = 16, num_groups: int = 0):
         _dtype(dtype)
+        if num_groups and score.window:
+            raise NotSupported(f"window {score.window} over shared blocks")
         inv = np.ascontiguousarray(inv_freq, dtype=np.float64)
         if inv.ndim != 1 or 2 * inv.size > head_dim:
             raise InvalidParameter(f"inv_freq of shape {inv.shape} for head_dim {head_dim}")
@@ -256,16 +320,34 @@ class AttentionStep:
         self.counts = DeviceArray((3,), np.int32)
         self.query = DeviceArray((max(num_tokens, 1), num_heads, head_dim), np.uint16)
         self._tables: Ptr = None
+        self.num_groups, self._grouped = num_groups, False
+        if num_groups:
+            sizes = self._sizes()
+            self.shared_plan = DeviceArray((plan_shared_size(*sizes),), np.uint8)
+            self.shared_blocks = DeviceArray((num_groups,), np.int32)
+            self.shared_workspace = DeviceArray((shared_decode_workspace_size(*sizes),), np.uint8)
+
+    def _sizes(self) -> tuple:
+        return (self.num_seqs, self.num_heads, self.num_kv_heads, self.head_dim, self.block_size,
+                self.max_num_blocks_per_seq)
 
     def plan(self, block_tables: Ptr, cached_lens: Ptr, new_lens: Ptr, free_blocks: Ptr,
              num_free: Ptr, free_capacity: int, num_blocks: int = 0,
-             stream: Optional[Stream] = None) -> None:
-        """plan_step into this object's arrays; block_tables is completed in place."""
+             stream: Optional[Stream] = None, group_offsets: Ptr = None) -> None:
+        """plan_step into this object's arrays; block_tables is completed in place.
+        With group_offsets [num_groups + 1], plan_shared of those groups too."""
+        if group_offsets is not None and not self.num_groups:
+            raise InvalidParameter("group_offsets for a step without num_groups")
         plan_step(block_tables, cached_lens, new_lens, free_blocks, num_free, free_capacity,
                   self.num_seqs, self.max_num_blocks_per_seq, self.block_size, self.num_tokens,
                   self.context_lens, self.query_offsets, self.positions, self.slot_mapping,
                   self.counts, num_blocks=num_blocks, stream=stream)
         self._tables = block_tables
+        self._grouped = group_offsets is not None
+        if self._grouped:
+            plan_shared(self.shared_plan, self.shared_plan.nbytes, self.shared_blocks, block_tables,
+                        self.context_lens, group_offsets, self.num_groups, *self._sizes(),
+                        stream=stream)
 
     def layer(self, query: Ptr, key: Ptr, value: Ptr, key_cache: Ptr, value_cache: Ptr,
               output: Ptr, query_stride: Optional[int] = None, key_stride: Optional[int] = None,
@@ -285,7 +367,14 @@ class AttentionStep:
                          attn_factor=self.attn_factor, interleaved=self.interleaved,
                          query_stride=query_stride, key_stride=key_stride,
                          value_stride=value_stride, num_blocks=num_blocks, stream=stream)
-        if decode:
+        if decode and self._grouped:
+            shared_decode(output, self.shared_workspace, self.shared_workspace.nbytes,
+                          self.shared_plan, self.shared_plan.nbytes, self.query, key_cache,
+                          value_cache, self._tables, self.score, *self._sizes(),
+                          dtype=self.dtype, num_blocks=num_blocks,
+                          query_offsets=self.query_offsets, num_tokens=self.num_tokens,
+                          stream=stream)
+        elif decode:
             scored_decode(output, self.workspace, self.workspace.nbytes, self.query, key_cache,
                           value_cache, self._tables, self.context_lens, self.score, self.num_seqs,
                           H, Hkv, D, self.block_size, self.max_num_blocks_per_seq,

@@ -26,7 +26,8 @@ ARCH = "gfx950"
 
 SOURCES = ["abi.cpp", "paged_attention.hip", "prefill.hip", "cache_ops.hip", "block_copy.hip", "moe.hip",
            "moe_experts.hip", "checks.hip", "step_plan.hip", "rotary.hip",
-           "scored_decode.hip", "scored_prefill.hip", "pages.hip", "beam_select.hip"]
+           "scored_decode.hip", "scored_prefill.hip", "pages.hip", "beam_select.hip",
+           "shared_plan.hip", "shared_decode.hip"]
 
 # The measurement kernels bench.py times beside the path (include/swiftllm_ceilings.h)
 # are a library of their own, outside the drop-in interface.

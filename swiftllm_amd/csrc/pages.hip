@@ -52,6 +52,7 @@ struct PagesArgs {
     int* free_blocks;
     int* num_free;         // [1]
     long long* pairs;      // [rooms][2]
+    int* new_lens;         // [S] or null
     int* new_ids;
     int* counts;           // [2]
     // workspace
@@ -129,6 +130,7 @@ __global__ __launch_bounds__(kRowThreads) void fork_rows_kernel(const PagesArgs 
     if (tid == 0) {
         a.rank[i] = n;
         a.ctx_out[i] = ctx;
+        if (a.new_lens != nullptr) a.new_lens[i] = p >= 0;
     }
 }
 
@@ -267,6 +269,7 @@ __global__ __launch_bounds__(kScanThreads) void fork_list_kernel(const PagesArgs
             const int i = a.copies[k];
             atomicAdd(a.refs_out + *open_of(i), -1);
             a.ctx_out[i] &= ~(kBlockTokens - 1);
+            if (a.new_lens != nullptr) a.new_lens[i] = 0;
         }
     }
     if (blockIdx.x == 0 && tid == 0) {
@@ -428,7 +431,7 @@ size_t swiftllm_hip_pages_workspace_size(int num_seqs, int num_blocks) {
 int swiftllm_hip_fork_pages(int32_t* block_tables_out, int32_t* context_lens_out, const int32_t* block_tables,
                             const int32_t* context_lens, const int32_t* parents, int32_t* ref_counts,
                             int32_t* free_blocks, int32_t* num_free, const int32_t* taken, int64_t* copy_pairs,
-                            int32_t* counts, void* workspace, size_t workspace_bytes, int num_seqs,
+                            int32_t* new_lens, int32_t* counts, void* workspace, size_t workspace_bytes, int num_seqs,
                             int max_num_blocks_per_seq, int block_size, int num_blocks, hipStream_t stream) {
     const char* who = "swiftllm_hip_fork_pages";
     const int S = num_seqs, MB = max_num_blocks_per_seq, NB = num_blocks;
@@ -446,7 +449,7 @@ int swiftllm_hip_fork_pages(int32_t* block_tables_out, int32_t* context_lens_out
     const size_t n = S, word = sizeof(int32_t);
     const Bytes span[] = {{block_tables_out, word * n * MB}, {context_lens_out, word * n}, {ref_counts, word * NB},
                           {free_blocks, word * NB}, {num_free, word}, {copy_pairs, 16 * n}, {counts, 2 * word},
-                          {workspace, space.bytes}, {block_tables, word * n * MB}, {context_lens, word * n},
+                          {workspace, space.bytes}, {new_lens, word * n}, {block_tables, word * n * MB}, {context_lens, word * n},
                           {parents, word * n}, {taken, word}};
     for (const Bytes& s : span) {
         if (!aligned(s.p, 4)) return fail(SWIFTLLM_ERR_INVALID_PARAMETER, "%s: misaligned pointer", who);
@@ -454,7 +457,7 @@ int swiftllm_hip_fork_pages(int32_t* block_tables_out, int32_t* context_lens_out
     if (!aligned(workspace, 256) || !aligned(copy_pairs, 8)) {
         return fail(SWIFTLLM_ERR_INVALID_PARAMETER, "%s: misaligned pointer", who);
     }
-    if (tangled(span, 8)) return fail(SWIFTLLM_ERR_INVALID_PARAMETER, "%s: an output overlaps another argument", who);
+    if (tangled(span, 9)) return fail(SWIFTLLM_ERR_INVALID_PARAMETER, "%s: an output overlaps another argument", who);
     rc = require_device();
     if (rc != SWIFTLLM_OK) return rc;
     PagesArgs a{};
@@ -468,6 +471,7 @@ int swiftllm_hip_fork_pages(int32_t* block_tables_out, int32_t* context_lens_out
     a.free_blocks = free_blocks;
     a.num_free = num_free;
     a.pairs = reinterpret_cast<long long*>(copy_pairs);
+    a.new_lens = new_lens;
     a.counts = counts;
     a.S = S;
     a.MB = MB;

@@ -1,0 +1,625 @@
+// Paged attention of one new token per sequence over blocks that sequences share
+// (gfx950), with a soft cap and a distance bias (scored_core.hpp): what
+// scored_decode computes, each group's shared blocks read once for all of its
+// sequences. The query of sequence s is its last token, at position L_s - 1.
+//
+// softmax over all keys in parts: a walk over the keys [j0, j1) leaves, for every
+// query row, m = max score, l = sum exp2(score - m) and o = sum exp2(score - m) v / l;
+// rows are joined as sum of exp2(m - M) l o over sum of exp2(m - M) l.
+//
+// Work. The plan's list (shared_plan.hpp) is cut into equal ranges, one workgroup
+// per range and chunk of heads. A walk's rows are the query heads of up to
+// 4 x 32 / gw sequences, gw = min(G, 32) heads each, 32 rows to a wave: one
+// sequence's own blocks keep one wave at its products, shared blocks up to four.
+// K and V go through LDS in stages of 64 keys as in scored_prefill, whose products
+// these are: S^T = K Q^T, O^T = V P^T, 32x32x16.
+//
+// Bound: HBM, one read of the shared K and V for each tile of 128 rows and one of
+// every sequence's own: a CU's share of HBM brings a stage in 1.4 us, and a wave's
+// products and weights of one take 0.9 us.
+
+#include <algorithm>
+#include <cmath>
+
+#include "scored_tiles.hpp"
+#include "shared_plan.hpp"
+
+namespace swiftllm {
+namespace {
+
+using namespace scored;
+using namespace shared;
+
+struct SharedArgs {
+    uint16_t* out;           // [rows][H][D]
+    const uint16_t* q;
+    const uint16_t* kc;
+    const uint16_t* vc;
+    const int* bt;
+    const int* qoff;         // [S + 1] or null: row s
+    const Head* head;
+    const Walk* walks;
+    const int* starts;
+    const Seq* seqs;
+    float2* frag_ml;         // [HC][rows]
+    float* frag_o;           // [HC][rows][D]
+    long long frag_rows;
+    Shape shape;             // scale > 0
+    unsigned q_and, q_xor;   // on the query's bits, two values each: its sign, or zero
+    int T;                   // rows, where qoff is given
+    int S, H, Hkv, D;
+    int G;                   // query heads per kv head
+    int nhc;                 // chunks of gw of them
+    int gw;
+    int tpw;                 // sequences of a wave's rows
+    int MB;
+    int num_blocks;
+    bool q16, out8;          // q 16-byte, out 8-byte aligned
+};
+
+constexpr int kWaves = kTileWaves;
+
+// The row of a sequence's query and output; negative: it has none.
+__device__ __forceinline__ int row_of(const SharedArgs& a, int s) {
+    if (a.qoff == nullptr) return s;
+    const int b = as_const(a.qoff)[s], e = as_const(a.qoff)[s + 1];
+    return b >= 0 && e > b && e <= a.T ? e - 1 : -1;
+}
+
+// Whether the plan was made for these sizes: what it names lies inside the arguments.
+__device__ __forceinline__ bool plan_fits(const SharedArgs& a) {
+    const const_int* const h = as_const(reinterpret_cast<const int*>(a.head));
+    return h[0] == kMagic && h[1] == a.S && h[2] == a.MB && h[3] == a.H && h[4] == a.Hkv && h[5] == a.D;
+}
+
+template <typename T, int D, bool CAP, bool BIAS>
+__global__ __launch_bounds__(64 * kWaves) __attribute__((amdgpu_waves_per_eu(2)))
+void shared_decode_kernel(const SharedArgs a) {
+    constexpr int NJ = D / 16;   // 16-wide k steps of QK^T
+    constexpr int ND = D / 32;   // 32-row pieces of the output
+    using St = Stage<D>;
+    __shared__ __align__(16) uint16_t s_k[2][St::kK];
+    __shared__ __align__(16) uint16_t s_v[2][St::kV];
+    __shared__ __align__(16) unsigned s_bad[2][4];   // keys of a stage's blocks whose values were not finite
+    if (!plan_fits(a)) return;
+    const const_int* const head = as_const(reinterpret_cast<const int*>(a.head));
+    const int total = head[7], len = head[8];
+    const int start = blockIdx.y * len;
+    if (start >= total) return;
+    const int end = min(start + len, total);
+    const int w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    const int kvh = blockIdx.x / a.nhc;
+    const int hc = blockIdx.x - kvh * a.nhc;
+    int v = as_const(a.starts)[blockIdx.y];
+    for (int at = start; at < end; ++v) {
+        if (at > start) __syncthreads();   // the stages are free for the next walk
+        // (the lane behind an empty asm: kept over the walks, what follows from it
+        // would not leave them enough registers)
+        int lane = threadIdx.x & 63;
+        asm volatile("" : "+v"(lane));
+        const int r = lane & 31;
+        const int h = lane >> 5;
+        // K operand, as in scored_prefill: a lane's eight scores of a block are of
+        // eight consecutive tokens.
+        const int g4 = lane >> 4;
+        const int j = lane & 15;
+        const int swapped = ((j & 1) << 1) | ((j >> 1) & 1);
+        const int koff = (g4 & 1) * St::kOdd + (8 * (g4 >> 1) + (j >> 2)) * kBlockTokens + 4 * swapped;
+        const const_int* const wp = as_const(reinterpret_cast<const int*>(a.walks + v));
+        const int table = wp[0], first = wp[1], blocks = wp[2], seq = wp[3], count = wp[4], begin = wp[5], cost = wp[6], frow = wp[7];
+        // This range's blocks of the walk: i0 .. i1 - 1.
+        const int stop = begin + cost, e = min(end, stop);
+        const int i0 = min(max(at - begin - kWalkCost, 0), blocks);
+        const int i1 = min(max(e - begin - kWalkCost, 0), blocks);
+        at = e;
+        // Query row r of the wave: sequence r / gw, head r % gw.
+        const int rt = r / a.gw;
+        const int rh = r - rt * a.gw;
+        const int g = hc * kWaveRows + rh;
+        const int hd = kvh * a.G + min(g, a.G - 1);
+        const int place = w * a.tpw + rt;
+        const int s = seq + min(place, count - 1);
+        const Seq sq = a.seqs[s];
+        const int qrow = row_of(a, s);
+        const bool ok = rt < a.tpw && place < count && g < a.G && sq.L > 0 && qrow >= 0;
+        const int L = ok ? sq.L : 0x7fffffff;               // (a row without a query is looked at by nobody)
+        int least = L;                                      // of the tile's
+        for (int i = lane; i < count; i += 64) {
+            const int x = a.seqs[seq + i].L;
+            if (x > 0) least = min(least, x);
+        }
+        least = 0x7fffffff - wave_max(0x7fffffff - least);
+        const bool works = __any(ok);
+        const float slope = BIAS ? a.shape.slopes[hd] * kLog2e : 0.0f;
+        f16x acc[ND];
+        float zero = 0.0f;
+        asm volatile("" : "+v"(zero));
+#pragma unroll
+        for (int i = 0; i < ND; ++i) {
+#pragma unroll
+            for (int z = 0; z < 16; ++z) acc[i][z] = zero;
+        }
+        float m = -INFINITY, l = 0.0f;
+        const int nsteps = (i1 - i0 + 3) >> 2;
+        if (nsteps > 0) {
+            const int* const ids_of = a.bt + static_cast<size_t>(table) * a.MB + first;
+            // Ids of 16 stages, four lanes each.
+            auto chunk_ids = [&](int c) { return ids_of[min(i0 + 64 * c + lane, i1 - 1)]; };
+            const int ids_first = chunk_ids(0);
+            int ids_next = chunk_ids(1);
+            // Q^T operand: lane (r, h) holds q[r][16 J + 8 h .. + 7].
+            s8 q[NJ];
+            {
+                const uint16_t* p = a.q + (static_cast<size_t>(max(qrow, 0)) * a.H + hd) * D + 8 * h;
+                const unsigned keep = ok ? a.q_and : 0u;
+                const unsigned flip = ok ? a.q_xor : 0u;
+#pragma unroll
+                for (int J = 0; J < NJ; ++J) {
+                    u4 x;
+                    if (a.q16) {
+                        x = *reinterpret_cast<const u4*>(p + 16 * J);
+                    } else {
+                        x = __builtin_bit_cast(u4, join8(*reinterpret_cast<const s4*>(p + 16 * J),
+                                                         *reinterpret_cast<const s4*>(p + 16 * J + 4)));
+                    }
+                    q[J] = __builtin_bit_cast(s8, (x & keep) ^ flip);
+                }
+            }
+            // The chunk at hand, unknown blocks as block 0 and their bits in `known` clear.
+            int ids;
+            unsigned long long known;
+            auto take_chunk = [&](int x, int c) {
+                const bool k = block_known(x, a.num_blocks) && i0 + 64 * c + lane < i1;
+                known = __ballot(k);
+                ids = k ? x : 0;
+            };
+            take_chunk(ids_first, 0);
+            // Tile of this wave in stage t (16 stages per load of ids) and, in ok4,
+            // which of the stage's four blocks there are.
+            auto tile_of = [&](int t, int& ok4) {
+                const int x = 4 * (t & 15);
+                ok4 = static_cast<int>((known >> x) & 15ull);
+                return kv_tile_offset(__builtin_amdgcn_readlane(ids, x + w), kvh, a.Hkv, D);
+            };
+            auto bytes_of = [&](int t) { return t < nsteps ? D * kBlockTokens * 2 : 0; };
+            auto base_of = [&](int t) { return (first + i0 + 4 * t) * kBlockTokens; };
+            // This wave's block of stage t has landed in its V buffer: true if some
+            // row of the tile may not see the stage whole.
+            auto landed = [&](int t, int ok4) {
+                if (t >= nsteps || (ok4 == 15 && base_of(t) + kStage <= least)) return false;
+                const unsigned bad = clean_v<T, D>(s_v[t & 1], w, lane);
+                if (lane == 0) s_bad[t & 1][w] = bad;
+                return true;
+            };
+            int ok_t, ok_1;                  // of stages t and t + 1
+            const size_t off = tile_of(0, ok_t);
+            stage_k<D>(a.kc, s_k[0], w, off, bytes_of(0), lane);
+            stage_v<D>(a.vc, s_v[0], w, off, bytes_of(0), lane);
+            size_t off_1 = tile_of(1, ok_1);
+            stage_k<D>(a.kc, s_k[1], w, off_1, bytes_of(1), lane);
+            wait_vm<0>();
+            bool cleaned = landed(0, ok_t);  // stage t
+            __syncthreads();
+            f16x sc[2];
+            qk_pair<T, D>(sc[0], s_k[0] + koff, q);
+            qk_pair<T, D>(sc[1], s_k[0] + koff + St::kPair, q);
+            __syncthreads();
+            const float scale = a.shape.scale;
+            const float cap = a.shape.cap;
+            auto cap_part = [&](float x) { return __builtin_amdgcn_rcpf(__builtin_amdgcn_exp2f(x * scale) + 1.0f); };
+            // Scores are what is made of them times mul, plus add; with a cap they
+            // fall as its part grows.
+            constexpr float kHidden = CAP && !BIAS ? INFINITY : -INFINITY;
+            const float mul = CAP ? -2.0f * cap : scale;
+            const float add = CAP ? cap : 0.0f;
+            float rise[16];   // of the bias over a pair's scores
+#pragma unroll
+            for (int i = 0; i < 16; ++i) rise[i] = BIAS ? slope * static_cast<float>(16 * (i >> 3) + (i & 7)) : 0.0f;
+            auto most = [](float x, float y) { return CAP && !BIAS ? fminf(x, y) : fmaxf(x, y); };
+            if constexpr (CAP) {
+#pragma unroll
+                for (int i = 0; i < 32; ++i) sc[i >> 4][i & 15] = cap_part(sc[i >> 4][i & 15]);
+            }
+            for (int t = 0; t < nsteps; ++t) {
+                int ok_2;
+                stage_v<D>(a.vc, s_v[(t + 1) & 1], w, off_1, bytes_of(t + 1), lane);
+                off_1 = tile_of(t + 2, ok_2);
+                stage_k<D>(a.kc, s_k[t & 1], w, off_1, bytes_of(t + 2), lane);
+                const int base = base_of(t);
+                if (works) {
+                    // Score i of pair p: key base + 32 p + 16 (i / 8) + 8 h + i % 8; bit
+                    // 16 p + i of `seen` whether this row sees it.
+                    const bool whole = ok_t == 15 && !__any(base + kStage > L);
+                    unsigned seen = ~0u;
+                    if (!whole) {
+                        const int to = L - (base + 8 * h);
+                        seen = 0;
+#pragma unroll
+                        for (int b = 0; b < 4; ++b) {
+                            if ((ok_t >> b) & 1) seen |= low8(to - 16 * b) << (8 * b);
+                        }
+                    }
+                    // What a pair's scores lack: the bias of its first key.
+                    float lack[2] = {add, add};
+                    if constexpr (BIAS) {
+                        const float d0 = static_cast<float>(base + 8 * h - (L - 1));
+                        lack[0] = __builtin_fmaf(slope, d0, add);
+                        lack[1] = __builtin_fmaf(slope, d0 + 32.0f, add);
+#pragma unroll
+                        for (int i = 0; i < 32; ++i) {
+                            sc[i >> 4][i & 15] = __builtin_fmaf(sc[i >> 4][i & 15], mul, rise[i & 15]);
+                        }
+                    }
+                    if (!whole) {
+#pragma unroll
+                        for (int i = 0; i < 32; ++i) {
+                            const int keep = __builtin_amdgcn_sbfe(static_cast<int>(seen), i, 1);  // 0 or -1
+                            const float x = sc[i >> 4][i & 15];   // (a bit cast of the element itself takes element 0)
+                            const int y = __builtin_bit_cast(int, x);
+                            sc[i >> 4][i & 15] = __builtin_bit_cast(float, (y & keep) | (__builtin_bit_cast(int, kHidden) & ~keep));
+                        }
+                    }
+                    auto most_of = [&](const f16x& x) {
+                        float y = most(most(x[0], x[1]), x[2]);
+#pragma unroll
+                        for (int i = 3; i < 15; i += 2) y = most(most(y, x[i]), x[i + 1]);
+                        return most(y, x[15]);
+                    };
+                    float bm;
+                    if constexpr (BIAS) {
+                        bm = fmaxf(most_of(sc[0]) + lack[0], most_of(sc[1]) + lack[1]);
+                    } else {
+                        bm = __builtin_fmaf(most(most_of(sc[0]), most_of(sc[1])), mul, add);
+                    }
+                    {
+                        const auto y = __builtin_amdgcn_permlane32_swap(__builtin_bit_cast(unsigned, bm), __builtin_bit_cast(unsigned, bm), false, false);
+                        bm = fmaxf(__builtin_bit_cast(float, static_cast<unsigned>(y[0])), __builtin_bit_cast(float, static_cast<unsigned>(y[1])));
+                    }
+                    if (__any(bm > m + kLag)) {
+                        const float m_new = fmaxf(m, bm);
+                        const float alpha = m_new == -INFINITY ? 1.0f : __builtin_amdgcn_exp2f(m - m_new);
+#pragma unroll
+                        for (int i = 0; i < ND; ++i) acc[i] *= alpha;
+                        l *= alpha;
+                        m = m_new;
+                    }
+                    const float c = ((m == -INFINITY) ? 0.0f : m) - weight_exp<T>;
+                    const float lack_c[2] = {lack[0] - c, lack[1] - c};
+                    if (cleaned) {
+                        const u4 bad = *reinterpret_cast<const u4*>(s_bad[t & 1]);
+                        unsigned keys = 0;   // this lane's, as `seen`
+#pragma unroll
+                        for (int b = 0; b < 4; ++b) keys |= ((bad[b] >> (8 * h)) & 0xffu) << (8 * b);
+                        if (seen & keys) l = __builtin_nanf("");
+                    }
+                    // Weights, O^T += V P^T, and the next stage's scores, in the order
+                    // that scored_prefill takes.
+                    const uint16_t* const next = s_k[(t + 1) & 1] + koff;
+                    const uint16_t* const vl = s_v[t & 1] + 8 * lane;
+                    u4 pw[4];
+                    auto weights = [&](int k) {   // the k-th pair of them
+                        const int b = k >> 2, i = k & 3;
+                        float p[2];
+#pragma unroll
+                        for (int z = 0; z < 2; ++z) {
+                            const float x = sc[b >> 1][8 * (b & 1) + 2 * i + z];
+                            p[z] = __builtin_amdgcn_exp2f(BIAS ? x + lack_c[b >> 1] : __builtin_fmaf(x, mul, lack_c[0]));
+                        }
+                        pw[b][i] = T::down2(p[0], p[1]);
+                        l = add_pair(T{}, pw[b][i], l);
+                    };
+                    constexpr int kScores = 2 * ND, kBack = 2 * ND + 2 * NJ, kProducts = 4 * ND + 2 * NJ;
+                    constexpr int kAhead = 2;
+                    auto operand = [&](int n) {
+                        if (n >= kScores && n < kBack) {
+                            const int k = n - kScores;
+                            return k_rows(next + k / NJ * St::kPair + 256 * (k % NJ));
+                        }
+                        const int k = n < kScores ? n : n - 2 * NJ;
+                        return *reinterpret_cast<const s8*>(vl + k / ND * St::kTile + 512 * (k % ND));
+                    };
+                    s8 ring[kAhead];
+#pragma unroll
+                    for (int n = 0; n < kAhead; ++n) ring[n] = operand(n);
+#pragma unroll
+                    for (int k = 0; k < 4; ++k) weights(k);
+                    __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+                    for (int n = 0; n < kProducts; ++n) {
+                        const s8 x = ring[n % kAhead];
+                        if (n + kAhead < kProducts) ring[n % kAhead] = operand(n + kAhead);
+                        if (n >= kScores && n < kBack) {
+                            const int k = n - kScores;
+                            sc[k / NJ] = T::mfma32(x, q[k % NJ], k % NJ == 0 ? f16x{} : sc[k / NJ]);
+                        } else {
+                            const int k = n < kScores ? n : n - 2 * NJ;
+                            acc[k % ND] = T::mfma32(x, __builtin_bit_cast(s8, pw[k / ND]), acc[k % ND]);
+                        }
+                        if (n < kScores) {
+#pragma unroll
+                            for (int i = 4 + n * 4 / ND; i < 4 + (n + 1) * 4 / ND; ++i) weights(i);
+                        } else if (n < kScores + 4) {
+                            weights(12 + n - kScores);
+                        } else if (CAP && n >= kScores + NJ) {
+                            constexpr int kSlots = 2 * ND + NJ;
+                            const int k = n - kScores - NJ;
+#pragma unroll
+                            for (int i = k * 32 / kSlots; i < (k + 1) * 32 / kSlots; ++i) sc[i >> 4][i & 15] = cap_part(sc[i >> 4][i & 15]);
+                        }
+                        __builtin_amdgcn_sched_barrier(0);
+                    }
+                }
+                wait_vm<0>();
+                cleaned = landed(t + 1, ok_1);
+                ok_t = ok_1;
+                ok_1 = ok_2;
+                if (((t + 3) & 15) == 0) {
+                    take_chunk(ids_next, (t + 3) >> 4);
+                    ids_next = chunk_ids(((t + 3) >> 4) + 1);
+                }
+                __syncthreads();
+            }
+        }
+        // The rows' results: outputs that are done, or fragments. Lane (r, h) has
+        // values 32 i + 8 k + 4 h .. + 3 of row r.
+        {
+            const auto y = __builtin_amdgcn_permlane32_swap(__builtin_bit_cast(unsigned, l), __builtin_bit_cast(unsigned, l), false, false);
+            const float sum = __builtin_bit_cast(float, static_cast<unsigned>(y[0])) + __builtin_bit_cast(float, static_cast<unsigned>(y[1]));
+            const float inv = sum == 0.0f ? 0.0f : 1.0f / sum;
+            if (frow < 0) {
+                // (a sequence without a context has zeros)
+                if (rt < a.tpw && place < count && g < a.G && qrow >= 0) {
+                    uint16_t* const p = a.out + (static_cast<size_t>(qrow) * a.H + hd) * D + 4 * h;
+#pragma unroll
+                    for (int i = 0; i < ND; ++i) {
+#pragma unroll
+                        for (int k = 0; k < 4; ++k) {
+                            const u2 o = u2{T::down2(acc[i][4 * k] * inv, acc[i][4 * k + 1] * inv),
+                                            T::down2(acc[i][4 * k + 2] * inv, acc[i][4 * k + 3] * inv)};
+                            uint16_t* const x = p + 32 * i + 8 * k;
+                            if (a.out8) {
+                                *reinterpret_cast<u2*>(x) = o;
+                            } else {
+                                x[0] = o[0] & 0xffffu;
+                                x[1] = o[0] >> 16;
+                                x[2] = o[1] & 0xffffu;
+                                x[3] = o[1] >> 16;
+                            }
+                        }
+                    }
+                }
+            } else if (rt < a.tpw && place < count) {
+                const long long f = static_cast<long long>(blockIdx.x) * a.frag_rows + frow +
+                                    static_cast<long long>(static_cast<int>(blockIdx.y) - begin / len) * count * a.gw + place * a.gw + rh;
+                if (h == 0) a.frag_ml[f] = float2{m, sum};
+                float* const p = a.frag_o + f * D + 4 * h;
+#pragma unroll
+                for (int i = 0; i < ND; ++i) {
+#pragma unroll
+                    for (int k = 0; k < 4; ++k) {
+                        *reinterpret_cast<f4*>(p + 32 * i + 8 * k) =
+                            f4{acc[i][4 * k] * inv, acc[i][4 * k + 1] * inv, acc[i][4 * k + 2] * inv, acc[i][4 * k + 3] * inv};
+                    }
+                }
+            }
+        }
+    }
+}
+
+// Joins the fragments of a sequence's rows: a wave per query head. A lane holds the
+// maximum and the sum of a fragment, and the first rows are on their way before
+// those are there.
+constexpr int kJoinRows = 8;
+constexpr int kJoinWaves = 4;
+
+template <typename T, int D>
+__global__ __launch_bounds__(64 * kJoinWaves) void shared_join_kernel(const SharedArgs a) {
+    constexpr int DL = D / 64;
+    const int lane = threadIdx.x & 63;
+    const int hd = blockIdx.y * kJoinWaves + __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    if (hd >= a.H || !plan_fits(a)) return;
+    const int s = blockIdx.x;
+    const const_int* const sq = as_const(reinterpret_cast<const int*>(a.seqs + s));
+    const int own = sq[1], tile = sq[2], index = sq[3];
+    const int len = as_const(reinterpret_cast<const int*>(a.head))[8];
+    const int kvh = hd / a.G;
+    const int hg = hd - kvh * a.G;
+    const int hc = hg / kWaveRows;
+    const int rh = hg - hc * kWaveRows;
+    // Fragments 0 .. n0 - 1 are of the shared blocks, the others of its own.
+    int n0 = 0, n1 = 0, f0 = 0, f1 = 0, step = 0;
+    if (tile >= 0) {
+        const const_int* const wp = as_const(reinterpret_cast<const int*>(a.walks + tile));
+        step = wp[4] * a.gw;
+        n0 = (wp[5] + wp[6] - 1) / len - wp[5] / len + 1;
+        f0 = wp[7] + index * a.gw + rh;
+    }
+    if (own >= 0) {
+        const const_int* const wp = as_const(reinterpret_cast<const int*>(a.walks + own));
+        if (wp[7] < 0) return;      // its row is written
+        n1 = (wp[5] + wp[6] - 1) / len - wp[5] / len + 1;
+        f1 = wp[7] + rh;
+    }
+    const long long sub = static_cast<long long>(kvh * a.nhc + hc) * a.frag_rows;
+    const int count = n0 + n1;
+    auto place = [&](int i) { return sub + (i < n0 ? f0 + i * step : f1 + (i - n0) * a.gw); };
+    float m = -INFINITY, l = 0.0f, o[DL];
+#pragma unroll
+    for (int j = 0; j < DL; ++j) o[j] = 0.0f;
+    for (int c = 0; c < count; c += 64) {
+        const int n = min(count - c, 64);
+        float v[kJoinRows][DL];
+        auto rows = [&](int i) {
+#pragma unroll
+            for (int k = 0; k < kJoinRows; ++k) {
+                if (i + k >= n) break;
+                const float* const p = a.frag_o + place(c + i + k) * D + lane * DL;
+#pragma unroll
+                for (int j = 0; j < DL; ++j) v[k][j] = p[j];
+            }
+        };
+        rows(0);
+        const float2 ml = a.frag_ml[place(c + min(lane, n - 1))];
+        const float fm = lane < n ? ml.x : -INFINITY;
+        const float fl = lane < n ? ml.y : 0.0f;
+        const float top = fmaxf(m, wave_max(fm));
+        const float keep = m == -INFINITY ? 1.0f : __builtin_amdgcn_exp2f(m - top);
+        // An empty fragment has a sum of 0; one of NaN scores alone has NaN.
+        const float weight = (fm == -INFINITY ? 1.0f : __builtin_amdgcn_exp2f(fm - top)) * fl;
+        l = l * keep + wave_sum(weight);
+#pragma unroll
+        for (int j = 0; j < DL; ++j) o[j] *= keep;
+        m = top;
+        for (int i = 0; i < n; i += kJoinRows) {
+            if (i > 0) rows(i);
+#pragma unroll
+            for (int k = 0; k < kJoinRows; ++k) {
+                const float x = __builtin_bit_cast(float, __builtin_amdgcn_readlane(__builtin_bit_cast(int, weight), (i + k) & 63));
+                if (i + k < n) {
+#pragma unroll
+                    for (int j = 0; j < DL; ++j) o[j] += x * v[k][j];
+                }
+            }
+        }
+    }
+    const int row = row_of(a, s);
+    if (row < 0) return;
+    const float inv = l == 0.0f ? 0.0f : 1.0f / l;
+    uint16_t* const p = a.out + (static_cast<size_t>(row) * a.H + hd) * D + lane * DL;
+#pragma unroll
+    for (int j = 0; j < DL; ++j) p[j] = T::down(o[j] * inv);
+}
+
+struct Space {
+    size_t o, bytes;
+};
+Space space_of(const Layout& l, int HC, int D) {
+    const auto up = [](long long n) { return static_cast<size_t>((n + 255) / 256 * 256); };
+    Space s;
+    s.o = up(8LL * l.rows * HC);
+    s.bytes = s.o + up(4LL * l.rows * HC * D);
+    return s;
+}
+
+}  // namespace
+}  // namespace swiftllm
+
+using namespace swiftllm;
+
+extern "C" {
+
+size_t swiftllm_hip_shared_decode_workspace_size(int num_seqs, int num_heads, int num_kv_heads, int head_dim,
+                                                 int block_size, int max_num_blocks_per_seq) {
+    if (shared::check_sizes("swiftllm_hip_shared_decode_workspace_size", num_seqs, num_heads, num_kv_heads, head_dim,
+                            block_size, max_num_blocks_per_seq) != SWIFTLLM_OK) {
+        return 0;
+    }
+    ok();
+    return space_of(shared::layout_of(num_seqs, num_heads, num_kv_heads), shared::heads_of(num_heads, num_kv_heads).HC, head_dim).bytes;
+}
+
+int swiftllm_hip_shared_decode(void* output, void* workspace, size_t workspace_bytes, const void* plan, size_t plan_bytes,
+                               const void* query, const void* key_cache, const void* value_cache,
+                               const int32_t* block_tables, const int32_t* query_offsets, const float* alibi_slopes,
+                               float scale, float softcap, int dtype, int num_tokens, int num_seqs, int num_heads,
+                               int num_kv_heads, int head_dim, int block_size, int max_num_blocks_per_seq, int num_blocks,
+                               hipStream_t stream) {
+    const char* who = "swiftllm_hip_shared_decode";
+    int rc = shared::check_sizes(who, num_seqs, num_heads, num_kv_heads, head_dim, block_size, max_num_blocks_per_seq);
+    if (rc != SWIFTLLM_OK) return rc;
+    if (dtype != SWIFTLLM_HIP_F16 && dtype != SWIFTLLM_HIP_BF16) {
+        return fail(SWIFTLLM_ERR_NOT_SUPPORTED, "%s: dtype=%d (supported: 0 fp16, 1 bf16)", who, dtype);
+    }
+    SharedArgs a{};
+    if (!scored::make_shape(a.shape, std::fabs(scale), softcap, 0, nullptr, alibi_slopes)) {
+        return fail(SWIFTLLM_ERR_INVALID_PARAMETER, "%s: scale=%g softcap=%g", who, scale, softcap);
+    }
+    if (softcap > scored::kMostCap) {
+        return fail(SWIFTLLM_ERR_NOT_SUPPORTED, "%s: softcap=%g (at most %g)", who, softcap, scored::kMostCap);
+    }
+    if (query_offsets && num_tokens < 0) {
+        return fail(SWIFTLLM_ERR_INVALID_PARAMETER, "%s: num_tokens=%d", who, num_tokens);
+    }
+    if (num_seqs > 0 && (!output || !query || !key_cache || !value_cache || !plan || !workspace ||
+                         (max_num_blocks_per_seq > 0 && !block_tables))) {
+        return fail(SWIFTLLM_ERR_INVALID_PARAMETER, "%s: null pointer", who);
+    }
+    if (!aligned(output, 2) || !aligned(query, 8) || !aligned(key_cache, 16) || !aligned(value_cache, 16) ||
+        !aligned(block_tables, 4) || !aligned(query_offsets, 4) || !aligned(alibi_slopes, 4) || !aligned(plan, 256) ||
+        !aligned(workspace, 256)) {
+        return fail(SWIFTLLM_ERR_INVALID_PARAMETER, "%s: misaligned pointer", who);
+    }
+    const shared::Heads h = shared::heads_of(num_heads, num_kv_heads);
+    const shared::Layout l = shared::layout_of(num_seqs, num_heads, num_kv_heads);
+    const Space space = space_of(l, h.HC, head_dim);
+    if (num_seqs > 0 && (workspace_bytes < space.bytes || plan_bytes < l.bytes)) {
+        return fail(SWIFTLLM_ERR_INVALID_PARAMETER, "%s: workspace of %zu bytes, %zu needed; plan of %zu, %zu needed", who,
+                    workspace_bytes, space.bytes, plan_bytes, l.bytes);
+    }
+    // Queries of one workgroup's rows are read by those of other ranges and heads'
+    // outputs are written meanwhile: no output may lie on an input.
+    if (num_seqs > 0) {
+        const size_t n = num_seqs, rows = query_offsets ? static_cast<size_t>(num_tokens) : n;
+        const Bytes out{output, rows * num_heads * head_dim * 2}, q{query, out.n}, ws{workspace, space.bytes};
+        const Bytes kc{key_cache, cache_bytes(num_blocks, num_kv_heads, head_dim)}, vc{value_cache, kc.n};
+        const Bytes bt{block_tables, 4 * n * max_num_blocks_per_seq}, off{query_offsets, 4 * (n + 1)};
+        const Bytes slopes{alibi_slopes, 4 * static_cast<size_t>(num_heads)}, pl{plan, l.bytes};
+        if (overlap_any(out, {q, kc, vc, bt, off, slopes, pl}) || overlap_any(ws, {out, q, kc, vc, bt, off, slopes, pl})) {
+            return fail(SWIFTLLM_ERR_INVALID_PARAMETER, "%s: output or workspace overlaps another argument", who);
+        }
+    }
+    rc = require_device();
+    if (rc != SWIFTLLM_OK) return rc;
+    if (num_seqs == 0) return ok();
+    // The sign of the scale goes into the query, and a scale of zero makes it zero: the
+    // kernel's scale is positive, so that raw products order as scores.
+    a.q_and = scale == 0.0f ? 0u : 0xffffffffu;
+    a.q_xor = scale < 0.0f ? 0x80008000u : 0u;
+    if (scale == 0.0f) a.shape.scale = 1.0f;
+    a.out = static_cast<uint16_t*>(output);
+    a.q = static_cast<const uint16_t*>(query);
+    a.kc = static_cast<const uint16_t*>(key_cache);
+    a.vc = static_cast<const uint16_t*>(value_cache);
+    a.bt = block_tables;
+    a.qoff = query_offsets;
+    const char* const p = static_cast<const char*>(plan);
+    a.head = reinterpret_cast<const shared::Head*>(p);
+    a.walks = reinterpret_cast<const shared::Walk*>(p + l.walks);
+    a.starts = reinterpret_cast<const int*>(p + l.starts);
+    a.seqs = reinterpret_cast<const shared::Seq*>(p + l.seqs);
+    char* const ws = static_cast<char*>(workspace);
+    a.frag_ml = reinterpret_cast<float2*>(ws);
+    a.frag_o = reinterpret_cast<float*>(ws + space.o);
+    a.frag_rows = l.rows;
+    a.T = num_tokens;
+    a.S = num_seqs;
+    a.H = num_heads;
+    a.Hkv = num_kv_heads;
+    a.D = head_dim;
+    a.G = h.G;
+    a.nhc = h.nhc;
+    a.gw = h.gw;
+    a.tpw = h.tpw;
+    a.MB = max_num_blocks_per_seq;
+    a.num_blocks = num_blocks;
+    a.q16 = aligned(query, 16);
+    a.out8 = aligned(output, 8);
+    using K = void (*)(SharedArgs);
+#define SHARED_DECODE(T_) \
+    {{{shared_decode_kernel<T_, 64, false, false>, shared_decode_kernel<T_, 64, false, true>}, \
+      {shared_decode_kernel<T_, 64, true, false>, shared_decode_kernel<T_, 64, true, true>}}, \
+     {{shared_decode_kernel<T_, 128, false, false>, shared_decode_kernel<T_, 128, false, true>}, \
+      {shared_decode_kernel<T_, 128, true, false>, shared_decode_kernel<T_, 128, true, true>}}}
+    static const K kernels[2][2][2][2] = {SHARED_DECODE(F16), SHARED_DECODE(BF16)};
+#undef SHARED_DECODE
+    static const K joins[2][2] = {{shared_join_kernel<F16, 64>, shared_join_kernel<F16, 128>},
+                                  {shared_join_kernel<BF16, 64>, shared_join_kernel<BF16, 128>}};
+    const int t = dtype == SWIFTLLM_HIP_BF16;
+    rc = launched(launch(kernels[t][head_dim == 128][softcap > 0.0f][alibi_slopes != nullptr], dim3(h.HC, l.ranges),
+                         dim3(64 * kTileWaves), 0, stream, a), who);
+    if (rc != SWIFTLLM_OK) return rc;
+    return launched(launch(joins[t][head_dim == 128], dim3(num_seqs, (num_heads + kJoinWaves - 1) / kJoinWaves),
+                           dim3(64 * kJoinWaves), 0, stream, a), who);
+}
+
+}  // extern "C"

@@ -1,0 +1,334 @@
+// The plan of attention over blocks that sequences share (gfx950): what a group's
+// tables have in common, and the list of walks (shared_plan.hpp) that the layers of
+// a step then take without looking at the tables again but for their ids.
+//
+// Of a group with n >= 2 sequences that have a context, the leading table entries
+// that all of them use, and alike, are shared: sh blocks, where that saves
+// (n - 1) sh >= kLeastSaved. Rows of a group without a context count for nothing.
+//
+// Bound: latency. A step of 128 sequences of 256 blocks compares 131 KB, once for
+// all layers. Two launches: a workgroup per sequence compares its row with its
+// group's first live one; one workgroup makes the list, in scans over the sequences.
+// Nothing is kept from one call for the next.
+
+#include "shared_plan.hpp"
+
+namespace swiftllm {
+namespace {
+
+using namespace shared;
+
+constexpr int kMatchThreads = 256;
+constexpr int kListThreads = 1024;
+constexpr int kListWaves = kListThreads / 64;
+constexpr int kWindow = 4096;       // groups whose minima fit LDS
+
+struct PlanSharedArgs {
+    const int* bt;
+    const int* ctx;
+    const int* offsets;     // [N + 1]
+    int* shared;            // [N]
+    Head* head;
+    Walk* walks;
+    int* starts;            // [ranges]: the walk that a range begins in
+    Seq* seqs;
+    int4* infos;            // [S]: group, its first live row, leading blocks alike with it, blocks shared
+    int2* costs;            // [S]: walks and cost before it
+    int S, N, MB, H, Hkv, D;
+    int gw, per_tile, ranges;
+};
+
+__device__ __forceinline__ int used_blocks(const PlanSharedArgs& a, int s) {
+    const int L = min(max(a.ctx[s], 0), a.MB * kBlockTokens);
+    return (L + kBlockTokens - 1) >> kBlockShift;
+}
+
+__global__ __launch_bounds__(kMatchThreads) void shared_match_kernel(const PlanSharedArgs a) {
+    __shared__ int s_least[kMatchThreads / 64];
+    const int s = blockIdx.x, tid = threadIdx.x;
+    // The least of the threads' numbers, in all of them.
+    auto least = [&](int x) {
+        // (wave_max is of numbers >= 0)
+        const int w = 0x7fffffff - wave_max(0x7fffffff - x);
+        __syncthreads();
+        if ((tid & 63) == 0) s_least[tid >> 6] = w;
+        __syncthreads();
+        int m = s_least[0];
+        for (int i = 1; i < kMatchThreads / 64; ++i) m = min(m, s_least[i]);
+        return m;
+    };
+    // The last group that begins at s or before. (Offsets out of order, which the
+    // list's kernel refuses, give some number of a group here.)
+    int lo = 0, hi = a.N;
+    while (lo < hi) {
+        const int mid = (lo + hi) >> 1;
+        if (a.offsets[mid] <= s) lo = mid + 1; else hi = mid;
+    }
+    const int g = lo - 1;
+    int4 info = int4{-1, -1, 0, 0};
+    if (g >= 0 && g < a.N && a.offsets[g + 1] > s) {
+        info.x = g;
+        const int b = max(a.offsets[g], 0), e = min(a.offsets[g + 1], a.S);
+        int lead = 0x7fffffff;
+        for (int i = b; i < e && lead == 0x7fffffff; i += kMatchThreads) {
+            lead = least(i + tid < e && a.ctx[i + tid] > 0 ? i + tid : 0x7fffffff);
+        }
+        if (lead < a.S) {
+            info.y = lead;
+            const int n = min(used_blocks(a, lead), used_blocks(a, s));
+            const int* const x = a.bt + static_cast<size_t>(lead) * a.MB;
+            const int* const y = a.bt + static_cast<size_t>(s) * a.MB;
+            info.z = n;
+            constexpr int kTake = 4;
+            for (int j0 = 0; j0 < n; j0 += kTake * kMatchThreads) {
+                int first = n;
+#pragma unroll
+                for (int k = kTake - 1; k >= 0; --k) {
+                    const int j = j0 + k * kMatchThreads + tid;
+                    if (j < n && x[j] != y[j]) first = j;
+                }
+                first = least(first);
+                if (first < n) {
+                    info.z = first;
+                    break;
+                }
+            }
+        }
+    }
+    if (tid == 0) a.infos[s] = info;
+}
+
+// Exclusive prefixes of x and y over the workgroup's threads, and their totals.
+__device__ __forceinline__ void scan2(int x, int y, int& before_x, int& before_y, int& all_x, int& all_y, int (*part)[kListWaves]) {
+    const int lane = threadIdx.x & 63, w = threadIdx.x >> 6;
+    const int ix = wave_inclusive_scan(x), iy = wave_inclusive_scan(y);
+    __syncthreads();
+    if (lane == 63) {
+        part[0][w] = ix;
+        part[1][w] = iy;
+    }
+    __syncthreads();
+    before_x = ix - x;
+    before_y = iy - y;
+    all_x = all_y = 0;
+    for (int i = 0; i < kListWaves; ++i) {
+        if (i < w) {
+            before_x += part[0][i];
+            before_y += part[1][i];
+        }
+        all_x += part[0][i];
+        all_y += part[1][i];
+    }
+}
+
+__global__ __launch_bounds__(kListThreads) void shared_list_kernel(const PlanSharedArgs a) {
+    __shared__ int s_least[kWindow], s_live[kWindow];
+    __shared__ int s_part[2][kListWaves];
+    __shared__ int s_bad;
+    const int tid = threadIdx.x;
+    if (tid == 0) s_bad = 0;
+    __syncthreads();
+    for (int i = tid; i < a.N; i += kListThreads) {
+        const int b = a.offsets[i], e = a.offsets[i + 1];
+        if (b < 0 || e < b || e > a.S) s_bad = 1;
+    }
+    __syncthreads();
+    const bool bad = s_bad != 0;
+    // What every group shares, and of that what is worth it, a window of groups at a time.
+    for (int g0 = 0; g0 < max(a.N, 1); g0 += kWindow) {
+        for (int i = tid; i < kWindow; i += kListThreads) {
+            s_least[i] = 0x7fffffff;
+            s_live[i] = 0;
+        }
+        __syncthreads();
+        auto mine = [&](int s, int4& info) {
+            info = a.infos[s];
+            return info.x >= g0 && info.x < g0 + kWindow;
+        };
+        for (int s = tid; s < a.S; s += kListThreads) {
+            int4 info;
+            if (mine(s, info) && a.ctx[s] > 0) {
+                atomicMin(&s_least[info.x - g0], info.z);
+                atomicAdd(&s_live[info.x - g0], 1);
+            }
+        }
+        __syncthreads();
+        for (int s = tid; s < a.S; s += kListThreads) {
+            int4 info;
+            if (mine(s, info)) {
+                const int live = s_live[info.x - g0], sh = s_least[info.x - g0];
+                const bool worth = !bad && live > 1 && static_cast<long long>(live - 1) * sh >= kLeastSaved;
+                a.infos[s].w = worth ? sh : 0;
+            }
+        }
+        for (int i = tid; i < min(a.N - g0, kWindow); i += kListThreads) {
+            a.shared[g0 + i] = bad || s_live[i] == 0 ? 0 : s_least[i];
+        }
+        __syncthreads();
+    }
+    // A sequence's walks: a tile's, where it is the first of one, and its own.
+    auto walks_of = [&](int s, int4& info, int& tile_cost, int& own_blocks, int& own_cost) {
+        info = a.infos[s];
+        const int used = used_blocks(a, s);
+        tile_cost = info.w > 0 && (s - a.offsets[info.x]) % a.per_tile == 0 ? info.w + kWalkCost : 0;
+        const int done = used > 0 ? info.w : 0;     // by the tile
+        own_blocks = used - done;
+        own_cost = own_blocks > 0 || done == 0 ? own_blocks + kWalkCost : 0;
+    };
+    int walks = 0, total = 0;
+    for (int s0 = 0; s0 < a.S; s0 += kListThreads) {
+        const int s = s0 + tid;
+        int4 info;
+        int tile = 0, blocks = 0, own = 0;
+        if (s < a.S) walks_of(s, info, tile, blocks, own);
+        int bx, by, ax, ay;
+        scan2((tile > 0) + (own > 0), tile + own, bx, by, ax, ay, s_part);
+        if (s < a.S) a.costs[s] = int2{walks + bx, total + by};
+        walks += ax;
+        total += ay;
+    }
+    const int len = max((total + a.ranges - 1) / a.ranges, kLeastRange);
+    __syncthreads();      // the costs are there for all
+    int rows = 0;
+    for (int s0 = 0; s0 < a.S; s0 += kListThreads) {
+        const int s = s0 + tid;
+        int4 info;
+        int tile = 0, blocks = 0, own = 0, tile_rows = 0, own_rows = 0, count = 0;
+        int2 at = int2{0, 0};
+        // Ranges that [b, b + cost) touches.
+        auto pieces = [&](int b, int cost) { return (b + cost - 1) / len - b / len + 1; };
+        if (s < a.S) {
+            walks_of(s, info, tile, blocks, own);
+            at = a.costs[s];
+            if (tile > 0) {
+                count = min(a.per_tile, a.offsets[info.x + 1] - s);
+                tile_rows = count * a.gw * pieces(at.y, tile);
+            }
+            const bool joins = info.w > 0 && a.ctx[s] > 0;
+            if (own > 0 && (joins || pieces(at.y + tile, own) > 1)) own_rows = a.gw * pieces(at.y + tile, own);
+        }
+        int bx, none, ax, all_none;
+        scan2(tile_rows + own_rows, 0, bx, none, ax, all_none, s_part);
+        if (s < a.S) {
+            const int f = rows + bx;
+            auto put = [&](int v, const Walk& w) {
+                a.walks[v] = w;
+                for (int r = (w.begin + len - 1) / len; r * len < w.begin + w.cost; ++r) a.starts[r] = v;
+            };
+            if (tile > 0) put(at.x, Walk{info.y, 0, info.w, s, count, at.y, tile, f});
+            if (own > 0) {
+                put(at.x + (tile > 0), Walk{s, a.ctx[s] > 0 ? info.w : 0, blocks, s, 1, at.y + tile, own, own_rows > 0 ? f + tile_rows : -1});
+            }
+            Seq q{min(max(a.ctx[s], 0), a.MB * kBlockTokens), own > 0 ? at.x + (tile > 0) : -1, -1, 0};
+            if (info.w > 0 && a.ctx[s] > 0) {
+                q.index = (s - a.offsets[info.x]) % a.per_tile;
+                q.tile = a.costs[s - q.index].x;
+            }
+            a.seqs[s] = q;
+        }
+        rows += ax;
+    }
+    if (tid == 0) *a.head = Head{kMagic, a.S, a.MB, a.H, a.Hkv, a.D, walks, total, len, rows};
+}
+
+}  // namespace
+
+namespace shared {
+
+int check_sizes(const char* who, long long S, long long H, long long Hkv, long long D, long long BS, long long MB) {
+    if (S < 0 || H <= 0 || Hkv <= 0 || D <= 0 || BS <= 0 || MB < 0) {
+        return fail(SWIFTLLM_ERR_INVALID_PARAMETER,
+                    "%s: num_seqs=%lld num_heads=%lld num_kv_heads=%lld head_dim=%lld block_size=%lld "
+                    "max_num_blocks_per_seq=%lld", who, S, H, Hkv, D, BS, MB);
+    }
+    if (H % Hkv != 0) {
+        return fail(SWIFTLLM_ERR_INVALID_PARAMETER, "%s: num_heads %lld not a multiple of num_kv_heads %lld", who, H, Hkv);
+    }
+    if ((D != 64 && D != 128) || BS != kBlockTokens) {
+        return fail(SWIFTLLM_ERR_NOT_SUPPORTED, "%s: head_dim=%lld block_size=%lld (supported: 64/128, 16)", who, D, BS);
+    }
+    // Token positions and the list's cost are 32-bit sums, and a fragment's row times
+    // its values is too.
+    if (S > 65535 || H > 65535 || MB >= (1 << 27) || 2 * S * (MB + kWalkCost) >= (1LL << 30)) {
+        return fail(SWIFTLLM_ERR_NOT_SUPPORTED, "%s: num_seqs=%lld num_heads=%lld max_num_blocks_per_seq=%lld", who, S, H, MB);
+    }
+    return SWIFTLLM_OK;
+}
+
+}  // namespace shared
+}  // namespace swiftllm
+
+using namespace swiftllm;
+
+extern "C" {
+
+size_t swiftllm_hip_plan_shared_size(int num_seqs, int num_heads, int num_kv_heads, int head_dim, int block_size,
+                                     int max_num_blocks_per_seq) {
+    if (shared::check_sizes("swiftllm_hip_plan_shared_size", num_seqs, num_heads, num_kv_heads, head_dim, block_size,
+                            max_num_blocks_per_seq) != SWIFTLLM_OK) {
+        return 0;
+    }
+    ok();
+    return shared::layout_of(num_seqs, num_heads, num_kv_heads).bytes;
+}
+
+int swiftllm_hip_plan_shared(void* plan, size_t plan_bytes, int32_t* shared_blocks, const int32_t* block_tables,
+                             const int32_t* context_lens, const int32_t* group_offsets, int num_groups, int num_seqs,
+                             int num_heads, int num_kv_heads, int head_dim, int block_size, int max_num_blocks_per_seq,
+                             hipStream_t stream) {
+    const char* who = "swiftllm_hip_plan_shared";
+    int rc = shared::check_sizes(who, num_seqs, num_heads, num_kv_heads, head_dim, block_size, max_num_blocks_per_seq);
+    if (rc != SWIFTLLM_OK) return rc;
+    if (num_groups < 0) return fail(SWIFTLLM_ERR_INVALID_PARAMETER, "%s: num_groups=%d", who, num_groups);
+    if (num_groups > 65535) return fail(SWIFTLLM_ERR_NOT_SUPPORTED, "%s: num_groups=%d", who, num_groups);
+    if (!plan || (num_groups > 0 && (!shared_blocks || !group_offsets)) || (num_seqs > 0 && !context_lens) ||
+        (num_seqs > 0 && max_num_blocks_per_seq > 0 && !block_tables)) {
+        return fail(SWIFTLLM_ERR_INVALID_PARAMETER, "%s: null pointer", who);
+    }
+    if (!aligned(plan, 256) || !aligned(shared_blocks, 4) || !aligned(block_tables, 4) || !aligned(context_lens, 4) ||
+        !aligned(group_offsets, 4)) {
+        return fail(SWIFTLLM_ERR_INVALID_PARAMETER, "%s: misaligned pointer", who);
+    }
+    const shared::Layout l = shared::layout_of(num_seqs, num_heads, num_kv_heads);
+    if (plan_bytes < l.bytes) {
+        return fail(SWIFTLLM_ERR_INVALID_PARAMETER, "%s: plan of %zu bytes, %zu needed", who, plan_bytes, l.bytes);
+    }
+    const size_t n = num_seqs;
+    const Bytes bt{block_tables, 4 * n * max_num_blocks_per_seq}, ctx{context_lens, 4 * n};
+    const Bytes off{group_offsets, num_groups > 0 ? 4 * (static_cast<size_t>(num_groups) + 1) : 0};
+    const Bytes sh{shared_blocks, 4 * static_cast<size_t>(num_groups)}, out{plan, l.bytes};
+    if (overlap_any(out, {sh, bt, ctx, off}) || overlap_any(sh, {bt, ctx, off})) {
+        return fail(SWIFTLLM_ERR_INVALID_PARAMETER, "%s: an output overlaps another argument", who);
+    }
+    rc = require_device();
+    if (rc != SWIFTLLM_OK) return rc;
+    const shared::Heads h = shared::heads_of(num_heads, num_kv_heads);
+    char* const p = static_cast<char*>(plan);
+    PlanSharedArgs a{};
+    a.bt = block_tables;
+    a.ctx = context_lens;
+    a.offsets = group_offsets;
+    a.shared = shared_blocks;
+    a.head = reinterpret_cast<shared::Head*>(p);
+    a.walks = reinterpret_cast<shared::Walk*>(p + l.walks);
+    a.starts = reinterpret_cast<int*>(p + l.starts);
+    a.seqs = reinterpret_cast<shared::Seq*>(p + l.seqs);
+    a.infos = reinterpret_cast<int4*>(p + l.infos);
+    a.costs = reinterpret_cast<int2*>(p + l.costs);
+    a.S = num_seqs;
+    a.N = num_groups;
+    a.MB = max_num_blocks_per_seq;
+    a.H = num_heads;
+    a.Hkv = num_kv_heads;
+    a.D = head_dim;
+    a.gw = h.gw;
+    a.per_tile = h.per_tile;
+    a.ranges = l.ranges;
+    if (num_seqs > 0) {
+        rc = launched(launch(shared_match_kernel, dim3(num_seqs), dim3(kMatchThreads), 0, stream, a), who);
+        if (rc != SWIFTLLM_OK) return rc;
+    }
+    return launched(launch(shared_list_kernel, dim3(1), dim3(kListThreads), 0, stream, a), who);
+}
+
+}  // extern "C"

@@ -34,18 +34,19 @@ def fork_pages(block_tables_out: Ptr, context_lens_out: Ptr, block_tables: Ptr, 
                parents: Ptr, ref_counts: Ptr, free_blocks: Ptr, num_free: Ptr, copy_pairs: Ptr,
                counts: Ptr, workspace: Ptr, workspace_bytes: int, num_seqs: int,
                max_num_blocks_per_seq: int, block_size: int, num_blocks: int, taken: Ptr = None,
-               stream: Optional[Stream] = None) -> None:
+               new_lens: Ptr = None, stream: Optional[Stream] = None) -> None:
     """Row i of the new tables goes on from row parents[i] of the old ones, -1
     from none (swiftllm_hip_fork_pages). ref_counts, free_blocks and num_free are
     brought up to date in place; copy_pairs int64 [num_seqs, 2] is for
     paged_attention.copy_blocks, -1 behind the last pair; counts int32 [2] =
     (copies, rows cut short because no block was free). taken: the counts of the
     plan_step since the last fork, whose blocks get their first reference here.
+    new_lens int32 [num_seqs]: 1 for rows that go on, for the next plan_step.
     With parents[i] = i for every row but those that end, this frees pages."""
     check_status(_lib.lib().swiftllm_hip_fork_pages(
         _p(block_tables_out), _p(context_lens_out), _p(block_tables), _p(context_lens),
         _p(parents), _p(ref_counts), _p(free_blocks), _p(num_free), _p(taken), _p(copy_pairs),
-        _p(counts), _p(workspace), workspace_bytes, num_seqs, max_num_blocks_per_seq, block_size,
+        _p(new_lens), _p(counts), _p(workspace), workspace_bytes, num_seqs, max_num_blocks_per_seq, block_size,
         num_blocks, _s(stream)))
 
 

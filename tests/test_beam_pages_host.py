@@ -52,8 +52,8 @@ def test_select_refuses(kw, code):
 def _fork(**kw):
     a = dict(block_tables_out=P, context_lens_out=2 * P, block_tables=3 * P, context_lens=4 * P,
              parents=5 * P, ref_counts=6 * P, free_blocks=7 * P, num_free=8 * P, taken=0,
-             copy_pairs=9 * P, counts=10 * P, workspace=11 * P, workspace_bytes=1 << 40, num_seqs=4,
-             max_num_blocks_per_seq=8, block_size=16, num_blocks=100)
+             copy_pairs=9 * P, new_lens=0, counts=10 * P, workspace=11 * P, workspace_bytes=1 << 40,
+             num_seqs=4, max_num_blocks_per_seq=8, block_size=16, num_blocks=100)
     a.update(kw)
     return _lib.lib().swiftllm_hip_fork_pages(*a.values(), None)
 
@@ -91,6 +91,8 @@ SIZES = [
     (dict(block_tables_out=3 * P), INVALID),            # tables are not forked in place
     (dict(context_lens_out=4 * P), INVALID),
     (dict(taken=7 * P + 8), INVALID),
+    (dict(new_lens=5 * P), INVALID),
+    (dict(new_lens=12 * P + 1), INVALID),
     (dict(counts=6 * P + 396), INVALID),
 ])
 def test_fork_refuses(kw, code):

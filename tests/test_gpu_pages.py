@@ -23,6 +23,7 @@ class Pool:
         self.d = {}
         self.pairs, self.counts = DeviceArray((S, 2), np.int64), DeviceArray((2,), np.int32)
         self.ctx_out, self.parents = DeviceArray((S,), np.int32), DeviceArray((S,), np.int32)
+        self.new = DeviceArray((S,), np.int32)
         self.refs_out, self.ids = DeviceArray((NB,), np.int32), DeviceArray((NB,), np.int32)
         self.ws = DeviceArray((pages.pages_workspace_size(S, NB),), np.uint8)
         self.ws.fill_byte(0xFF)
@@ -53,7 +54,7 @@ class Pool:
         d = self.d
         pages.fork_pages(d["other"], self.ctx_out, d["tables"], d["ctx"], self.parents, d["refs"], d["free"], d["n"],
                          self.pairs, self.counts, self.ws, self.ws.nbytes, self.S, self.MB, 16, self.NB,
-                         taken=d["taken"] if taken else None, stream=stream)
+                         taken=d["taken"] if taken else None, new_lens=self.new if taken else None, stream=stream)
 
     def fork(self, parents, taken=None):
         """A fork, checked; the new tables are the pool's then."""
@@ -73,6 +74,11 @@ class Pool:
                int(self.d["n"].numpy()[0]), self.pairs.numpy(), self.counts.numpy())
         for name, g, w in zip(("tables", "contexts", "references", "free", "num_free", "pairs", "counts"), got, want):
             assert np.array_equal(g, w), name
+        if taken is not None:
+            p = np.asarray(parents)
+            new = (p >= 0) & (p < self.S)
+            new[new] &= want[1][new] == np.maximum(h["ctx"][p[new]], 0)     # not cut
+            assert np.array_equal(self.new.numpy(), new.astype(np.int32))
         h["other"], h["tables"], h["ctx"] = h["tables"], want[0], want[1]
         h["refs"], h["free"], h["n"][0] = want[2], want[3], want[4]
         self.d["other"], self.d["tables"] = self.d["tables"], self.d["other"]
@@ -150,7 +156,9 @@ def test_fork_without_room(dev, spare):
     _, counts = p.fork(np.zeros(8, int))
     assert counts.tolist() == [min(spare, 7), 7 - min(spare, 7)]
     assert sorted(p.h["ctx"].tolist()) == [32] * (7 - min(spare, 7)) + [40] * (1 + min(spare, 7))
-    p.fork(np.arange(8))
+    p.fork(np.arange(8), taken=0)
+    p = Pool(4, 4, 4).lone(np.random.default_rng(1), [40, 0, 0, 0])
+    p.fork([0, 0, 0, -1], taken=0)
 
 
 def test_fork_of_odd_rows(dev):
