@@ -8,11 +8,14 @@
 // rows are joined as sum of exp2(m - M) l o over sum of exp2(m - M) l.
 //
 // Work. The plan's list (shared_plan.hpp) is cut into equal ranges, one workgroup
-// per range and chunk of heads. A walk's rows are the query heads of up to
-// 4 x 32 / gw sequences, gw = min(G, 32) heads each, 32 rows to a wave: one
-// sequence's own blocks keep one wave at its products, shared blocks up to four.
-// K and V go through LDS in stages of 64 keys as in scored_prefill, whose products
-// these are: S^T = K Q^T, O^T = V P^T, 32x32x16.
+// per range and chunk of heads. A wide walk's rows are the query heads of up to
+// 4 x 32 / gw sequences, gw = min(G, 32) heads each, 32 rows to a wave; its K and V
+// go through LDS in stages of 64 keys as in scored_prefill, whose products these
+// are: S^T = K Q^T, O^T = V P^T, 32x32x16. A narrow walk, of at most 16 rows or of
+// one sequence, is one wave's as in scored_decode (scored_walk.hpp): no wave waits
+// for another, and eight of them a CU keep 128 KB on the way. (One sequence's own
+// blocks by a whole workgroup through LDS: 128 chats of 1-1000 own tokens behind
+// 8192 shared ones, 32/8 heads x 128, 91 us a layer, not @@; 16 x 8 beams 73, not @@.)
 //
 // Bound: HBM, one read of the shared K and V for each tile of 128 rows and one of
 // every sequence's own: a CU's share of HBM brings a stage in 1.4 us, and a wave's
@@ -22,6 +25,7 @@
 #include <cmath>
 
 #include "scored_tiles.hpp"
+#include "scored_walk.hpp"
 #include "shared_plan.hpp"
 
 namespace swiftllm {
@@ -39,7 +43,8 @@ struct SharedArgs {
     const int* qoff;         // [S + 1] or null: row s
     const Head* head;
     const Walk* walks;
-    const int* starts;
+    const Start* wide;
+    const Start* narrow;
     const Seq* seqs;
     float2* frag_ml;         // [HC][rows]
     float* frag_o;           // [HC][rows][D]
@@ -72,6 +77,120 @@ __device__ __forceinline__ bool plan_fits(const SharedArgs& a) {
     return h[0] == kMagic && h[1] == a.S && h[2] == a.MB && h[3] == a.H && h[4] == a.Hkv && h[5] == a.D;
 }
 
+__device__ __forceinline__ Walk walk_at(const Walk* p) {
+    const const_int* const x = as_const(reinterpret_cast<const int*>(p));
+    return Walk{x[0], x[1], x[2], x[3], x[4], x[5], x[6], x[7]};
+}
+
+// Four outputs of a row.
+template <typename T>
+__device__ __forceinline__ void put_out(uint16_t* p, f4 o, bool out8) {
+    const u2 x = u2{T::down2(o[0], o[1]), T::down2(o[2], o[3])};
+    if (out8) {
+        *reinterpret_cast<u2*>(p) = x;
+    } else {
+        p[0] = x[0] & 0xffffu;
+        p[1] = x[0] >> 16;
+        p[2] = x[1] & 0xffffu;
+        p[3] = x[1] >> 16;
+    }
+}
+
+// Blocks i0 .. i1 - 1 of a narrow walk, by one wave, for the heads hb .. hb + 15 of
+// its chunk. Lane (r, kg) has query row r: sequence r / gw, head hb + r % gw.
+template <typename T, int D, bool BIAS>
+__device__ __forceinline__ void narrow_piece(const SharedArgs& a, const Walk& walk, int kvh, int hc, int hb, int i0, int i1, int range, int lane) {
+    constexpr int NJ = D / 16;
+    const int r = lane & 15;
+    const int kg = lane >> 4;
+    const int gn = min(a.gw - hb, kNarrowRows);              // heads at hand
+    const int rt = r / gn;
+    const int rh = hb + r - rt * gn;
+    const int g = hc * kWaveRows + rh;
+    const int hd = kvh * a.G + min(g, a.G - 1);
+    const int s = walk.seq + min(rt, walk.count - 1);
+    const Seq sq = a.seqs[s];
+    const int qrow = row_of(a, s);
+    const bool row = rt < walk.count;                        // there is a row for it
+    const bool ok = row && g < a.G && sq.L > 0 && qrow >= 0;
+    const int* const ids_of = a.bt + static_cast<size_t>(walk.row) * a.MB + walk.first;
+    const int count = i1 - i0;
+    // Lane l has the id of block i0 + 64 c + l.
+    auto ids_from = [&](int c) { return ids_of[min(i0 + 64 * c + lane, i1 - 1)]; };
+    int ids = ids_from(0);
+    s8 q[NJ / 2];
+    const uint16_t* const qp = a.q + (static_cast<size_t>(max(qrow, 0)) * a.H + hd) * D + 4 * kg;
+    const unsigned keep = ok ? a.q_and : 0u, flip = ok ? a.q_xor : 0u;
+#pragma unroll
+    for (int J = 0; J < NJ; J += 2) {
+        const s8 x = join8(*reinterpret_cast<const s4*>(qp + 16 * J), *reinterpret_cast<const s4*>(qp + 16 * J + 16));
+        q[J / 2] = __builtin_bit_cast(s8, (__builtin_bit_cast(u4, x) & keep) ^ flip);
+    }
+    const float slope = BIAS && ok ? a.shape.slopes[hd] * kLog2e : 0.0f;
+    s4 ident;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) ident[i] = 4 * kg + i == r ? static_cast<short>(T::one()) : 0;
+    const int loff = kv_elem_offset(r, 4 * kg);
+    State<D> st;
+    st.m = -INFINITY;
+    st.l = 0.0f;
+#pragma unroll
+    for (int J = 0; J < NJ; ++J) st.acc[J] = f4{0, 0, 0, 0};
+    // The keys of an own walk end with its sequence; shared blocks are seen whole.
+    const int L = __builtin_amdgcn_readfirstlane(walk.count > 1 ? 0x7fffffff : sq.L);
+    auto load = [&](int k, s4 (&kk)[NJ], s4 (&vv)[NJ], int& base, unsigned& seen) {
+        if (k > 0 && (k & 63) == 0) ids = ids_from(k >> 6);
+        const int b = __builtin_amdgcn_readlane(ids, k & 63);
+        const bool known = block_known(b, a.num_blocks);
+        base = (walk.first + i0 + k) * kBlockTokens;
+        seen = known ? low_bits(L - base) : 0u;
+        // A block outside the pool is read as block 0 and hidden.
+        const size_t tile = kv_tile_offset(known ? b : 0, kvh, a.Hkv, D) + loff;
+#pragma unroll
+        for (int J = 0; J < NJ; ++J) kk[J] = load4(a.kc + tile + kv_elem_offset(16 * J, 0));
+#pragma unroll
+        for (int J = 0; J < NJ; ++J) vv[J] = load4(a.vc + tile + kv_elem_offset(16 * J, 0));
+    };
+    const int last = sq.L - 1;      // the position that a bias's distances are from
+    auto take = [&](s4 (&kk)[NJ], s4 (&vv)[NJ], int base, unsigned seen) {
+        attend<T, D>(st, seen, base - last, kg, kk, vv, q, ident, a.shape, slope);
+    };
+    // Two blocks in flight; no load of the loop depends on a condition.
+    s4 kA[NJ], vA[NJ], kB[NJ], vB[NJ];
+    int bA, bB;
+    unsigned sA, sB;
+    load(0, kA, vA, bA, sA);
+    int k = 0;
+    for (; k + 2 < count; k += 2) {
+        load(k + 1, kB, vB, bB, sB);
+        take(kA, vA, bA, sA);
+        load(k + 2, kA, vA, bA, sA);
+        take(kB, vB, bB, sB);
+    }
+    if (k + 1 < count) {
+        load(k + 1, kB, vB, bB, sB);
+        take(kA, vA, bA, sA);
+        take(kB, vB, bB, sB);
+    } else {
+        take(kA, vA, bA, sA);
+    }
+    const float sum = sum_over_groups(st.l);
+    const float inv = sum == 0.0f ? 0.0f : 1.0f / sum;
+    if (walk.frow < 0) {
+        if (!ok) return;
+        uint16_t* const p = a.out + (static_cast<size_t>(qrow) * a.H + hd) * D + 4 * kg;
+#pragma unroll
+        for (int J = 0; J < NJ; ++J) put_out<T>(p + 16 * J, st.acc[J] * inv, a.out8);
+    } else if (row) {
+        const long long f = static_cast<long long>(blockIdx.x) * a.frag_rows + walk.frow +
+                            static_cast<long long>(range - walk.at / walk.len) * walk.count * a.gw + rt * a.gw + rh;
+        if (kg == 0) a.frag_ml[f] = float2{st.m, sum};
+        float* const p = a.frag_o + f * D + 4 * kg;
+#pragma unroll
+        for (int J = 0; J < NJ; ++J) *reinterpret_cast<f4*>(p + 16 * J) = st.acc[J] * inv;
+    }
+}
+
 template <typename T, int D, bool CAP, bool BIAS>
 __global__ __launch_bounds__(64 * kWaves) __attribute__((amdgpu_waves_per_eu(2)))
 void shared_decode_kernel(const SharedArgs a) {
@@ -81,18 +200,28 @@ void shared_decode_kernel(const SharedArgs a) {
     __shared__ __align__(16) uint16_t s_k[2][St::kK];
     __shared__ __align__(16) uint16_t s_v[2][St::kV];
     __shared__ __align__(16) unsigned s_bad[2][4];   // keys of a stage's blocks whose values were not finite
-    if (!plan_fits(a)) return;
     const const_int* const head = as_const(reinterpret_cast<const int*>(a.head));
-    const int total = head[7], len = head[8];
+    const int wide = head[6], walks = head[7], wide_cost = head[8], total = head[9], len = head[10];
+    if (!plan_fits(a)) return;
     const int start = blockIdx.y * len;
     if (start >= total) return;
     const int end = min(start + len, total);
     const int w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const int kvh = blockIdx.x / a.nhc;
     const int hc = blockIdx.x - kvh * a.nhc;
-    int v = as_const(a.starts)[blockIdx.y];
-    for (int at = start; at < end; ++v) {
-        if (at > start) __syncthreads();   // the stages are free for the next walk
+    if (start < wide_cost) {
+    const Start* const s0 = a.wide + blockIdx.y;
+    Walk walk = walk_at(&s0->walk);
+    int v = as_const(&s0->v)[0];
+    bool again = false;
+    for (;;) {
+        // This range's blocks of the walk: i0 .. i1 - 1.
+        const int i0 = max(start - walk.at, 0);
+        const int i1 = min(end - walk.at, walk.blocks);
+        const Walk next = ++v < wide ? walk_at(a.walks + v) : walk;
+        if (i0 < i1) {
+        if (again) __syncthreads();   // the stages are free for the next walk
+        again = true;
         // (the lane behind an empty asm: kept over the walks, what follows from it
         // would not leave them enough registers)
         int lane = threadIdx.x & 63;
@@ -105,13 +234,7 @@ void shared_decode_kernel(const SharedArgs a) {
         const int j = lane & 15;
         const int swapped = ((j & 1) << 1) | ((j >> 1) & 1);
         const int koff = (g4 & 1) * St::kOdd + (8 * (g4 >> 1) + (j >> 2)) * kBlockTokens + 4 * swapped;
-        const const_int* const wp = as_const(reinterpret_cast<const int*>(a.walks + v));
-        const int table = wp[0], first = wp[1], blocks = wp[2], seq = wp[3], count = wp[4], begin = wp[5], cost = wp[6], frow = wp[7];
-        // This range's blocks of the walk: i0 .. i1 - 1.
-        const int stop = begin + cost, e = min(end, stop);
-        const int i0 = min(max(at - begin - kWalkCost, 0), blocks);
-        const int i1 = min(max(e - begin - kWalkCost, 0), blocks);
-        at = e;
+        const int first = walk.first, seq = walk.seq, count = walk.count;
         // Query row r of the wave: sequence r / gw, head r % gw.
         const int rt = r / a.gw;
         const int rh = r - rt * a.gw;
@@ -122,13 +245,6 @@ void shared_decode_kernel(const SharedArgs a) {
         const Seq sq = a.seqs[s];
         const int qrow = row_of(a, s);
         const bool ok = rt < a.tpw && place < count && g < a.G && sq.L > 0 && qrow >= 0;
-        const int L = ok ? sq.L : 0x7fffffff;               // (a row without a query is looked at by nobody)
-        int least = L;                                      // of the tile's
-        for (int i = lane; i < count; i += 64) {
-            const int x = a.seqs[seq + i].L;
-            if (x > 0) least = min(least, x);
-        }
-        least = 0x7fffffff - wave_max(0x7fffffff - least);
         const bool works = __any(ok);
         const float slope = BIAS ? a.shape.slopes[hd] * kLog2e : 0.0f;
         f16x acc[ND];
@@ -141,8 +257,8 @@ void shared_decode_kernel(const SharedArgs a) {
         }
         float m = -INFINITY, l = 0.0f;
         const int nsteps = (i1 - i0 + 3) >> 2;
-        if (nsteps > 0) {
-            const int* const ids_of = a.bt + static_cast<size_t>(table) * a.MB + first;
+        {
+            const int* const ids_of = a.bt + static_cast<size_t>(walk.row) * a.MB + first;
             // Ids of 16 stages, four lanes each.
             auto chunk_ids = [&](int c) { return ids_of[min(i0 + 64 * c + lane, i1 - 1)]; };
             const int ids_first = chunk_ids(0);
@@ -183,10 +299,10 @@ void shared_decode_kernel(const SharedArgs a) {
             };
             auto bytes_of = [&](int t) { return t < nsteps ? D * kBlockTokens * 2 : 0; };
             auto base_of = [&](int t) { return (first + i0 + 4 * t) * kBlockTokens; };
-            // This wave's block of stage t has landed in its V buffer: true if some
-            // row of the tile may not see the stage whole.
+            // This wave's block of stage t has landed in its V buffer: true if the
+            // stage is not seen whole.
             auto landed = [&](int t, int ok4) {
-                if (t >= nsteps || (ok4 == 15 && base_of(t) + kStage <= least)) return false;
+                if (t >= nsteps || ok4 == 15) return false;
                 const unsigned bad = clean_v<T, D>(s_v[t & 1], w, lane);
                 if (lane == 0) s_bad[t & 1][w] = bad;
                 return true;
@@ -228,21 +344,20 @@ void shared_decode_kernel(const SharedArgs a) {
                 const int base = base_of(t);
                 if (works) {
                     // Score i of pair p: key base + 32 p + 16 (i / 8) + 8 h + i % 8; bit
-                    // 16 p + i of `seen` whether this row sees it.
-                    const bool whole = ok_t == 15 && !__any(base + kStage > L);
+                    // 16 p + i of `seen` whether it is there.
+                    const bool whole = ok_t == 15;
                     unsigned seen = ~0u;
                     if (!whole) {
-                        const int to = L - (base + 8 * h);
                         seen = 0;
 #pragma unroll
                         for (int b = 0; b < 4; ++b) {
-                            if ((ok_t >> b) & 1) seen |= low8(to - 16 * b) << (8 * b);
+                            if ((ok_t >> b) & 1) seen |= 0xffu << (8 * b);
                         }
                     }
                     // What a pair's scores lack: the bias of its first key.
                     float lack[2] = {add, add};
                     if constexpr (BIAS) {
-                        const float d0 = static_cast<float>(base + 8 * h - (L - 1));
+                        const float d0 = static_cast<float>(base + 8 * h - (sq.L - 1));
                         lack[0] = __builtin_fmaf(slope, d0, add);
                         lack[1] = __builtin_fmaf(slope, d0 + 32.0f, add);
 #pragma unroll
@@ -360,37 +475,15 @@ void shared_decode_kernel(const SharedArgs a) {
                 __syncthreads();
             }
         }
-        // The rows' results: outputs that are done, or fragments. Lane (r, h) has
-        // values 32 i + 8 k + 4 h .. + 3 of row r.
+        // The rows' fragments: they share, and go on. Lane (r, h) has values
+        // 32 i + 8 k + 4 h .. + 3 of row r.
         {
             const auto y = __builtin_amdgcn_permlane32_swap(__builtin_bit_cast(unsigned, l), __builtin_bit_cast(unsigned, l), false, false);
             const float sum = __builtin_bit_cast(float, static_cast<unsigned>(y[0])) + __builtin_bit_cast(float, static_cast<unsigned>(y[1]));
             const float inv = sum == 0.0f ? 0.0f : 1.0f / sum;
-            if (frow < 0) {
-                // (a sequence without a context has zeros)
-                if (rt < a.tpw && place < count && g < a.G && qrow >= 0) {
-                    uint16_t* const p = a.out + (static_cast<size_t>(qrow) * a.H + hd) * D + 4 * h;
-#pragma unroll
-                    for (int i = 0; i < ND; ++i) {
-#pragma unroll
-                        for (int k = 0; k < 4; ++k) {
-                            const u2 o = u2{T::down2(acc[i][4 * k] * inv, acc[i][4 * k + 1] * inv),
-                                            T::down2(acc[i][4 * k + 2] * inv, acc[i][4 * k + 3] * inv)};
-                            uint16_t* const x = p + 32 * i + 8 * k;
-                            if (a.out8) {
-                                *reinterpret_cast<u2*>(x) = o;
-                            } else {
-                                x[0] = o[0] & 0xffffu;
-                                x[1] = o[0] >> 16;
-                                x[2] = o[1] & 0xffffu;
-                                x[3] = o[1] >> 16;
-                            }
-                        }
-                    }
-                }
-            } else if (rt < a.tpw && place < count) {
-                const long long f = static_cast<long long>(blockIdx.x) * a.frag_rows + frow +
-                                    static_cast<long long>(static_cast<int>(blockIdx.y) - begin / len) * count * a.gw + place * a.gw + rh;
+            if (rt < a.tpw && place < count) {
+                const long long f = static_cast<long long>(blockIdx.x) * a.frag_rows + walk.frow +
+                                    static_cast<long long>(static_cast<int>(blockIdx.y) - walk.at / walk.len) * count * a.gw + place * a.gw + rh;
                 if (h == 0) a.frag_ml[f] = float2{m, sum};
                 float* const p = a.frag_o + f * D + 4 * h;
 #pragma unroll
@@ -403,6 +496,39 @@ void shared_decode_kernel(const SharedArgs a) {
                 }
             }
         }
+        }
+        if (v >= wide || next.at - kWideCost >= end) break;
+        walk = next;
+    }
+    }
+    // This wave's quarter of what is narrow.
+    const int range = kTileWaves * static_cast<int>(blockIdx.y) + w;
+    const int wlen = len / kTileWaves;
+    const int b = range * wlen, e = min(b + wlen, total);
+    if (e <= wide_cost || b >= total) return;
+    Walk walk;
+    int v;
+    if (b <= wide_cost) {
+        v = wide;
+        walk = walk_at(a.walks + v);
+    } else {
+        const Start* const s0 = a.narrow + range;
+        walk = walk_at(&s0->walk);
+        v = as_const(&s0->v)[0];
+    }
+    for (;;) {
+        const int i0 = max(b - walk.at, 0);
+        const int i1 = min(e - walk.at, walk.blocks);
+        const Walk next = ++v < walks ? walk_at(a.walks + v) : walk;
+        if (i0 < i1) {
+            for (int hb = 0; hb < a.gw; hb += kNarrowRows) {
+                int lane = threadIdx.x & 63;
+                asm volatile("" : "+v"(lane));
+                narrow_piece<T, D, BIAS>(a, walk, kvh, hc, hb, i0, i1, range, lane);
+            }
+        }
+        if (v >= walks || next.at - kNarrowCost >= e) break;
+        walk = next;
     }
 }
 
@@ -421,24 +547,24 @@ __global__ __launch_bounds__(64 * kJoinWaves) void shared_join_kernel(const Shar
     const int s = blockIdx.x;
     const const_int* const sq = as_const(reinterpret_cast<const int*>(a.seqs + s));
     const int own = sq[1], tile = sq[2], index = sq[3];
-    const int len = as_const(reinterpret_cast<const int*>(a.head))[8];
     const int kvh = hd / a.G;
     const int hg = hd - kvh * a.G;
     const int hc = hg / kWaveRows;
     const int rh = hg - hc * kWaveRows;
     // Fragments 0 .. n0 - 1 are of the shared blocks, the others of its own.
     int n0 = 0, n1 = 0, f0 = 0, f1 = 0, step = 0;
+    auto pieces = [](const Walk& x) { return (x.at + x.blocks - 1) / x.len - x.at / x.len + 1; };
     if (tile >= 0) {
-        const const_int* const wp = as_const(reinterpret_cast<const int*>(a.walks + tile));
-        step = wp[4] * a.gw;
-        n0 = (wp[5] + wp[6] - 1) / len - wp[5] / len + 1;
-        f0 = wp[7] + index * a.gw + rh;
+        const Walk x = walk_at(a.walks + tile);
+        step = x.count * a.gw;
+        n0 = pieces(x);
+        f0 = x.frow + index * a.gw + rh;
     }
     if (own >= 0) {
-        const const_int* const wp = as_const(reinterpret_cast<const int*>(a.walks + own));
-        if (wp[7] < 0) return;      // its row is written
-        n1 = (wp[5] + wp[6] - 1) / len - wp[5] / len + 1;
-        f1 = wp[7] + rh;
+        const Walk x = walk_at(a.walks + own);
+        if (x.frow < 0) return;      // its row is written
+        n1 = pieces(x);
+        f1 = x.frow + rh;
     }
     const long long sub = static_cast<long long>(kvh * a.nhc + hc) * a.frag_rows;
     const int count = n0 + n1;
@@ -585,7 +711,8 @@ int swiftllm_hip_shared_decode(void* output, void* workspace, size_t workspace_b
     const char* const p = static_cast<const char*>(plan);
     a.head = reinterpret_cast<const shared::Head*>(p);
     a.walks = reinterpret_cast<const shared::Walk*>(p + l.walks);
-    a.starts = reinterpret_cast<const int*>(p + l.starts);
+    a.wide = reinterpret_cast<const shared::Start*>(p + l.wide_starts);
+    a.narrow = reinterpret_cast<const shared::Start*>(p + l.narrow_starts);
     a.seqs = reinterpret_cast<const shared::Seq*>(p + l.seqs);
     char* const ws = static_cast<char*>(workspace);
     a.frag_ml = reinterpret_cast<float2*>(ws);

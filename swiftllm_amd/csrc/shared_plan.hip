@@ -3,8 +3,9 @@
 // a step then take without looking at the tables again but for their ids.
 //
 // Of a group with n >= 2 sequences that have a context, the leading table entries
-// that all of them use, and alike, are shared: sh blocks, where that saves
-// (n - 1) sh >= kLeastSaved. Rows of a group without a context count for nothing.
+// that all of them use, and alike, are shared; a walk takes those that all of them
+// have filled, sh blocks, where that saves (n - 1) sh >= kLeastSaved, so that no
+// row sees part of one. Rows of a group without a context count for nothing.
 //
 // Bound: latency. A step of 128 sequences of 256 blocks compares 131 KB, once for
 // all layers. Two launches: a workgroup per sequence compares its row with its
@@ -21,7 +22,7 @@ using namespace shared;
 constexpr int kMatchThreads = 256;
 constexpr int kListThreads = 1024;
 constexpr int kListWaves = kListThreads / 64;
-constexpr int kWindow = 4096;       // groups whose minima fit LDS
+constexpr int kWindow = 2048;       // groups whose minima are in LDS at a time
 
 struct PlanSharedArgs {
     const int* bt;
@@ -29,11 +30,12 @@ struct PlanSharedArgs {
     const int* offsets;     // [N + 1]
     int* shared;            // [N]
     Head* head;
+    Start* wide;            // [ranges]
+    Start* narrow;          // [ranges * 4]
     Walk* walks;
-    int* starts;            // [ranges]: the walk that a range begins in
     Seq* seqs;
     int4* infos;            // [S]: group, its first live row, leading blocks alike with it, blocks shared
-    int2* costs;            // [S]: walks and cost before it
+    int4* costs;            // [S]: wide walks and their cost, narrow ones and theirs before it
     int S, N, MB, H, Hkv, D;
     int gw, per_tile, ranges;
 };
@@ -122,7 +124,7 @@ __device__ __forceinline__ void scan2(int x, int y, int& before_x, int& before_y
 }
 
 __global__ __launch_bounds__(kListThreads) void shared_list_kernel(const PlanSharedArgs a) {
-    __shared__ int s_least[kWindow], s_live[kWindow];
+    __shared__ int s_least[kWindow], s_full[kWindow], s_live[kWindow];
     __shared__ int s_part[2][kListWaves];
     __shared__ int s_bad;
     const int tid = threadIdx.x;
@@ -136,8 +138,8 @@ __global__ __launch_bounds__(kListThreads) void shared_list_kernel(const PlanSha
     const bool bad = s_bad != 0;
     // What every group shares, and of that what is worth it, a window of groups at a time.
     for (int g0 = 0; g0 < max(a.N, 1); g0 += kWindow) {
-        for (int i = tid; i < kWindow; i += kListThreads) {
-            s_least[i] = 0x7fffffff;
+        for (int i = tid; i < min(max(a.N - g0, 0), kWindow); i += kListThreads) {
+            s_least[i] = s_full[i] = 0x7fffffff;
             s_live[i] = 0;
         }
         __syncthreads();
@@ -149,6 +151,7 @@ __global__ __launch_bounds__(kListThreads) void shared_list_kernel(const PlanSha
             int4 info;
             if (mine(s, info) && a.ctx[s] > 0) {
                 atomicMin(&s_least[info.x - g0], info.z);
+                atomicMin(&s_full[info.x - g0], a.ctx[s] >> kBlockShift);
                 atomicAdd(&s_live[info.x - g0], 1);
             }
         }
@@ -156,7 +159,7 @@ __global__ __launch_bounds__(kListThreads) void shared_list_kernel(const PlanSha
         for (int s = tid; s < a.S; s += kListThreads) {
             int4 info;
             if (mine(s, info)) {
-                const int live = s_live[info.x - g0], sh = s_least[info.x - g0];
+                const int live = s_live[info.x - g0], sh = min(s_least[info.x - g0], s_full[info.x - g0]);
                 const bool worth = !bad && live > 1 && static_cast<long long>(live - 1) * sh >= kLeastSaved;
                 a.infos[s].w = worth ? sh : 0;
             }
@@ -167,68 +170,100 @@ __global__ __launch_bounds__(kListThreads) void shared_list_kernel(const PlanSha
         __syncthreads();
     }
     // A sequence's walks: a tile's, where it is the first of one, and its own.
-    auto walks_of = [&](int s, int4& info, int& tile_cost, int& own_blocks, int& own_cost) {
-        info = a.infos[s];
-        const int used = used_blocks(a, s);
-        tile_cost = info.w > 0 && (s - a.offsets[info.x]) % a.per_tile == 0 ? info.w + kWalkCost : 0;
-        const int done = used > 0 ? info.w : 0;     // by the tile
-        own_blocks = used - done;
-        own_cost = own_blocks > 0 || done == 0 ? own_blocks + kWalkCost : 0;
+    struct Mine {
+        int4 info;
+        int L, count, own;                    // of the tile; own blocks
+        int wide, narrow, wide_cost, tile_cost, own_cost;   // walks, and what they cost
     };
-    int walks = 0, total = 0;
+    auto walks_of = [&](int s) {
+        Mine m{};
+        if (s >= a.S) return m;
+        m.info = a.infos[s];
+        m.L = min(max(a.ctx[s], 0), a.MB * kBlockTokens);
+        m.own = ((m.L + kBlockTokens - 1) >> kBlockShift) - (m.L > 0 ? m.info.w : 0);
+        m.own_cost = m.own > 0 ? m.own + kNarrowCost : 0;
+        if (m.info.w > 0 && (s - a.offsets[m.info.x]) % a.per_tile == 0) {
+            m.count = min(a.per_tile, a.offsets[m.info.x + 1] - s);
+            m.wide = m.count * a.gw > kNarrowRows;
+        }
+        m.wide_cost = m.wide ? m.info.w + kWideCost : 0;
+        m.tile_cost = m.count > 0 && !m.wide ? m.info.w + kNarrowCost : 0;
+        m.narrow = (m.tile_cost > 0) + (m.own_cost > 0);
+        return m;
+    };
+    int wide = 0, narrow = 0, wide_cost = 0, narrow_cost = 0;
     for (int s0 = 0; s0 < a.S; s0 += kListThreads) {
         const int s = s0 + tid;
-        int4 info;
-        int tile = 0, blocks = 0, own = 0;
-        if (s < a.S) walks_of(s, info, tile, blocks, own);
-        int bx, by, ax, ay;
-        scan2((tile > 0) + (own > 0), tile + own, bx, by, ax, ay, s_part);
-        if (s < a.S) a.costs[s] = int2{walks + bx, total + by};
-        walks += ax;
-        total += ay;
+        const Mine m = walks_of(s);
+        int4 before, all;
+        scan2(m.wide, m.wide_cost, before.x, before.y, all.x, all.y, s_part);
+        scan2(m.narrow, m.tile_cost + m.own_cost, before.z, before.w, all.z, all.w, s_part);
+        if (s < a.S) a.costs[s] = int4{wide + before.x, wide_cost + before.y, narrow + before.z, narrow_cost + before.w};
+        wide += all.x;
+        wide_cost += all.y;
+        narrow += all.z;
+        narrow_cost += all.w;
     }
-    const int len = max((total + a.ranges - 1) / a.ranges, kLeastRange);
+    const int total = wide_cost + narrow_cost;
+    const int wlen = max((total + kTileWaves * a.ranges - 1) / (kTileWaves * a.ranges), kLeastRange / kTileWaves);
+    const int len = kTileWaves * wlen;
     __syncthreads();      // the costs are there for all
     int rows = 0;
     for (int s0 = 0; s0 < a.S; s0 += kListThreads) {
         const int s = s0 + tid;
-        int4 info;
-        int tile = 0, blocks = 0, own = 0, tile_rows = 0, own_rows = 0, count = 0;
-        int2 at = int2{0, 0};
-        // Ranges that [b, b + cost) touches.
-        auto pieces = [&](int b, int cost) { return (b + cost - 1) / len - b / len + 1; };
-        if (s < a.S) {
-            walks_of(s, info, tile, blocks, own);
-            at = a.costs[s];
-            if (tile > 0) {
-                count = min(a.per_tile, a.offsets[info.x + 1] - s);
-                tile_rows = count * a.gw * pieces(at.y, tile);
-            }
-            const bool joins = info.w > 0 && a.ctx[s] > 0;
-            if (own > 0 && (joins || pieces(at.y + tile, own) > 1)) own_rows = a.gw * pieces(at.y + tile, own);
+        const Mine m = walks_of(s);
+        const int4 at = s < a.S ? a.costs[s] : int4{0, 0, 0, 0};
+        // Ranges of n that blocks b .. b + k - 1 of the list lie in.
+        auto pieces = [](int b, int k, int n) { return (b + k - 1) / n - b / n + 1; };
+        const bool joins = m.info.w > 0 && m.L > 0;
+        const int tile_at = m.wide ? at.y + kWideCost : wide_cost + at.w + kNarrowCost;
+        const int own_at = wide_cost + at.w + m.tile_cost + kNarrowCost;
+        int tile_rows = 0, own_rows = 0;
+        if (m.count > 0) tile_rows = m.count * a.gw * pieces(tile_at, m.info.w, m.wide ? len : wlen);
+        if (m.own > 0) {
+            const int n = pieces(own_at, m.own, wlen);
+            if (joins || n > 1) own_rows = a.gw * n;
         }
         int bx, none, ax, all_none;
         scan2(tile_rows + own_rows, 0, bx, none, ax, all_none, s_part);
         if (s < a.S) {
             const int f = rows + bx;
-            auto put = [&](int v, const Walk& w) {
+            // A walk, and the ranges of n that begin in it or in what it costs before.
+            auto put = [&](int v, const Walk& w, int cost, Start* starts) {
                 a.walks[v] = w;
-                for (int r = (w.begin + len - 1) / len; r * len < w.begin + w.cost; ++r) a.starts[r] = v;
+                for (int r = (w.at - cost + w.len - 1) / w.len; r * w.len < w.at + w.blocks; ++r) {
+                    Start& x = starts[r];
+                    x.walk = w;
+                    x.v = v;
+                }
             };
-            if (tile > 0) put(at.x, Walk{info.y, 0, info.w, s, count, at.y, tile, f});
-            if (own > 0) {
-                put(at.x + (tile > 0), Walk{s, a.ctx[s] > 0 ? info.w : 0, blocks, s, 1, at.y + tile, own, own_rows > 0 ? f + tile_rows : -1});
+            const int v = wide + at.z;
+            if (m.count > 0) {
+                const Walk w{m.info.y, 0, m.info.w, s, m.count, tile_at, m.wide ? len : wlen, f};
+                if (m.wide) {
+                    put(at.x, w, kWideCost, a.wide);
+                } else {
+                    put(v, w, kNarrowCost, a.narrow);
+                }
             }
-            Seq q{min(max(a.ctx[s], 0), a.MB * kBlockTokens), own > 0 ? at.x + (tile > 0) : -1, -1, 0};
-            if (info.w > 0 && a.ctx[s] > 0) {
-                q.index = (s - a.offsets[info.x]) % a.per_tile;
-                q.tile = a.costs[s - q.index].x;
+            const int own_v = v + (m.tile_cost > 0);
+            if (m.own > 0) {
+                put(own_v, Walk{s, m.L > 0 ? m.info.w : 0, m.own, s, 1, own_at, wlen, own_rows > 0 ? f + tile_rows : -1}, kNarrowCost, a.narrow);
+            }
+            Seq q{m.L, m.own > 0 ? own_v : -1, -1, 0};
+            if (joins) {
+                // Its tile begins with another sequence of the group, or with itself.
+                const int b = a.offsets[m.info.x];
+                q.index = (s - b) % a.per_tile;
+                const int t = s - q.index;
+                const bool is_wide = min(a.per_tile, a.offsets[m.info.x + 1] - t) * a.gw > kNarrowRows;
+                q.tile = is_wide ? a.costs[t].x : wide + a.costs[t].z;
             }
             a.seqs[s] = q;
         }
         rows += ax;
     }
-    if (tid == 0) *a.head = Head{kMagic, a.S, a.MB, a.H, a.Hkv, a.D, walks, total, len, rows};
+    if (tid == 0) *a.head = Head{kMagic, a.S, a.MB, a.H, a.Hkv, a.D, wide, wide + narrow, wide_cost, total, len};
 }
 
 }  // namespace
@@ -249,7 +284,7 @@ int check_sizes(const char* who, long long S, long long H, long long Hkv, long l
     }
     // Token positions and the list's cost are 32-bit sums, and a fragment's row times
     // its values is too.
-    if (S > 65535 || H > 65535 || MB >= (1 << 27) || 2 * S * (MB + kWalkCost) >= (1LL << 30)) {
+    if (S > 65535 || H > 65535 || MB >= (1 << 27) || 2 * S * (MB + kWideCost) >= (1LL << 30)) {
         return fail(SWIFTLLM_ERR_NOT_SUPPORTED, "%s: num_seqs=%lld num_heads=%lld max_num_blocks_per_seq=%lld", who, S, H, MB);
     }
     return SWIFTLLM_OK;
@@ -311,10 +346,11 @@ int swiftllm_hip_plan_shared(void* plan, size_t plan_bytes, int32_t* shared_bloc
     a.shared = shared_blocks;
     a.head = reinterpret_cast<shared::Head*>(p);
     a.walks = reinterpret_cast<shared::Walk*>(p + l.walks);
-    a.starts = reinterpret_cast<int*>(p + l.starts);
+    a.wide = reinterpret_cast<shared::Start*>(p + l.wide_starts);
+    a.narrow = reinterpret_cast<shared::Start*>(p + l.narrow_starts);
     a.seqs = reinterpret_cast<shared::Seq*>(p + l.seqs);
     a.infos = reinterpret_cast<int4*>(p + l.infos);
-    a.costs = reinterpret_cast<int2*>(p + l.costs);
+    a.costs = reinterpret_cast<int4*>(p + l.costs);
     a.S = num_seqs;
     a.N = num_groups;
     a.MB = max_num_blocks_per_seq;

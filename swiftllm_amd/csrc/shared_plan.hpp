@@ -3,10 +3,12 @@
 //
 // The work of a step is a list of walks: of a group's shared blocks by the queries
 // of up to `per_tile` of its sequences, and of each sequence's other blocks by its
-// own. The list is cut into equal ranges of its cost, one per workgroup and chunk
-// of heads, and a piece of a walk that its rows are not done with leaves one
-// fragment (maximum, sum, output) a row. Fragments of a walk lie behind each other,
-// from row `frow` on.
+// own. Walks of more than 16 query rows are wide, a workgroup's, and come first;
+// the others are narrow, a wave's. The list is cut into equal ranges of its cost,
+// one per workgroup and chunk of heads, of which each wave has a quarter of what is
+// narrow. Every piece of a walk that does not end its rows leaves one fragment
+// (maximum, sum, output) a row; those of a walk lie behind each other from row
+// `frow` on.
 #pragma once
 
 #include <algorithm>
@@ -17,28 +19,21 @@ namespace swiftllm {
 namespace shared {
 
 constexpr int kMagic = 0x53484152;
-constexpr int kWaveRows = 32;       // query rows of a wave: tokens x heads
+constexpr int kWaveRows = 32;       // query rows of a wave of a wide walk: tokens x heads
 constexpr int kTileWaves = 4;
 constexpr int kTileRows = kWaveRows * kTileWaves;
+constexpr int kNarrowRows = 16;
 
-// Blocks that starting and ending a walk costs, and one that a tile's rows cost beside.
-constexpr int kWalkCost = 4;
+// Blocks that starting and ending a walk costs.
+constexpr int kWideCost = 8;
+constexpr int kNarrowCost = 2;
 // Workgroups the list is cut for: two for each of the 256 CUs of an MI355X, as the
-// tiles' registers allow.
+// wide walks' registers allow.
 constexpr int kResident = 2 * 256;
-// Shortest range, in blocks: a stage and what a walk costs.
-constexpr int kLeastRange = 8;
+// Shortest range, in blocks: four of each wave.
+constexpr int kLeastRange = 16;
 // Blocks that reading shared ones once has to save.
 constexpr int kLeastSaved = 16;
-
-struct Head {
-    int magic, S, MB, heads, kv_heads, head_dim;
-    int walks;      // in the list
-    int total;      // its cost
-    int len;        // of a range
-    int rows;       // fragments
-    int pad[6];
-};
 
 struct Walk {
     int row;        // whose table names the blocks
@@ -46,9 +41,26 @@ struct Walk {
     int blocks;     //   and how many
     int seq;        // the first of its sequences
     int count;      //   and how many: more than one shares
-    int begin;      // in the list
-    int cost;
-    int frow;       // its first fragment, in rows of a chunk of heads; -1: one piece that is done
+    int at;         // its first block's place in the list
+    int len;        // of the ranges that cut it
+    int frow;       // its first fragment, in rows of a chunk of heads; -1: one piece that ends its row
+};
+
+// Where a range begins: a walk, and its number.
+struct Start {
+    Walk walk;
+    int v;
+    int pad[7];
+};
+
+struct Head {
+    int magic, S, MB, heads, kv_heads, head_dim;
+    int wide;       // walks
+    int walks;      //   in all
+    int wide_cost;  // the list's wide part
+    int total;
+    int len;        // of a workgroup's range, four times a wave's
+    int pad[5];
 };
 
 struct Seq {
@@ -75,27 +87,26 @@ inline Heads heads_of(int H, int Hkv) {
 
 struct Layout {
     int ranges;
-    int most_walks;
-    size_t walks, starts, seqs, infos, costs, bytes;
+    size_t wide_starts, narrow_starts, walks, seqs, infos, costs, bytes;
     long long rows;        // fragments of a chunk of heads, at most
 };
 
 // Walks: one per sequence and, of those that share, one per tile, which has two of
-// them at least. Rows: each walk has at most as many pieces as ranges touch it, and
-// all of them together at most `ranges` more than there are walks.
+// them at least. Rows: a walk has one piece and one more for every end of a range in
+// it, of at most a tile's rows or, at a wave's, a sequence's heads.
 inline Layout layout_of(long long S, int H, int Hkv) {
     const auto up = [](long long n) { return static_cast<size_t>((n + 255) / 256 * 256); };
     const Heads h = heads_of(H, Hkv);
     Layout l;
     l.ranges = std::max(kResident / h.HC, 1);
-    l.most_walks = static_cast<int>(2 * S);
-    l.walks = 256;
-    l.starts = l.walks + up(static_cast<long long>(sizeof(Walk)) * l.most_walks);
-    l.seqs = l.starts + up(4LL * l.ranges);
+    l.wide_starts = 256;
+    l.narrow_starts = l.wide_starts + up(static_cast<long long>(sizeof(Start)) * l.ranges);
+    l.walks = l.narrow_starts + up(static_cast<long long>(sizeof(Start)) * l.ranges * kTileWaves);
+    l.seqs = l.walks + up(static_cast<long long>(sizeof(Walk)) * (2 * S + 1));
     l.infos = l.seqs + up(static_cast<long long>(sizeof(Seq)) * S);
     l.costs = l.infos + up(16 * S);
-    l.bytes = l.costs + up(8 * S);
-    l.rows = 2 * S * h.gw + l.ranges * static_cast<long long>(kTileRows + h.gw);
+    l.bytes = l.costs + up(16 * S);
+    l.rows = 2 * S * h.gw + static_cast<long long>(l.ranges) * (kTileRows + kTileWaves * std::max(h.gw, kNarrowRows));
     return l;
 }
 
