@@ -99,7 +99,7 @@ __device__ __forceinline__ void put_out(uint16_t* p, f4 o, bool out8) {
 // Blocks i0 .. i1 - 1 of a narrow walk, by one wave, for the heads hb .. hb + 15 of
 // its chunk. Lane (r, kg) has query row r: sequence r / gw, head hb + r % gw.
 template <typename T, int D, bool BIAS>
-__device__ __forceinline__ void narrow_piece(const SharedArgs& a, const Walk& walk, int kvh, int hc, int hb, int i0, int i1, int range, int lane) {
+__device__ __forceinline__ void narrow_piece(const SharedArgs& a, const Walk& walk, int kvh, int hc, int hb, int i0, int i1, int range, int wlen, int lane) {
     constexpr int NJ = D / 16;
     const int r = lane & 15;
     const int kg = lane >> 4;
@@ -183,11 +183,32 @@ __device__ __forceinline__ void narrow_piece(const SharedArgs& a, const Walk& wa
         for (int J = 0; J < NJ; ++J) put_out<T>(p + 16 * J, st.acc[J] * inv, a.out8);
     } else if (row) {
         const long long f = static_cast<long long>(blockIdx.x) * a.frag_rows + walk.frow +
-                            static_cast<long long>(range - walk.at / walk.len) * walk.count * a.gw + rt * a.gw + rh;
+                            static_cast<long long>(range - walk.at / wlen) * walk.count * a.gw + rt * a.gw + rh;
         if (kg == 0) a.frag_ml[f] = float2{st.m, sum};
         float* const p = a.frag_o + f * D + 4 * kg;
 #pragma unroll
         for (int J = 0; J < NJ; ++J) *reinterpret_cast<f4*>(p + 16 * J) = st.acc[J] * inv;
+    }
+}
+
+// The ring of steps, two blocks each, that a workgroup's loads fill ahead of its
+// products.
+constexpr int kRing = 4;
+
+// 16 bytes a lane, from byte v + s of the buffer to LDS from m0 on, lanes side by
+// side. In assembly, so that the compiler does not wait for all of them before any
+// read of LDS: every read of what they bring comes behind wait_vm and a barrier.
+// There is no register that they write; m0 holds nothing of the compiler's from one
+// instruction to the next. once: what no other walk reads streams past the caches
+// (8 x 32 rows on 16384 tokens, 32/8 heads x 128, 106 us, not 126; four tiles on the
+// same 8192 tokens so 80, not 74).
+__device__ __forceinline__ void load_lds16(u4 rsrc, unsigned lds, unsigned v, unsigned s, bool once) {
+    if (once) {
+        asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tbuffer_load_dwordx4 %1, %2, %3 offen nt lds" ::"s"(lds), "v"(v), "s"(rsrc), "s"(s)
+                     : "memory");
+    } else {
+        asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tbuffer_load_dwordx4 %1, %2, %3 offen lds" ::"s"(lds), "v"(v), "s"(rsrc), "s"(s)
+                     : "memory");
     }
 }
 
@@ -197,9 +218,9 @@ void shared_decode_kernel(const SharedArgs a) {
     constexpr int NJ = D / 16;   // 16-wide k steps of QK^T
     constexpr int ND = D / 32;   // 32-row pieces of the output
     using St = Stage<D>;
-    __shared__ __align__(16) uint16_t s_k[2][St::kK];
-    __shared__ __align__(16) uint16_t s_v[2][St::kV];
-    __shared__ __align__(16) unsigned s_bad[2][4];   // keys of a stage's blocks whose values were not finite
+    constexpr int kStep = St::kPair + 2 * St::kTile;     // halves of a step: two blocks' K, then their V
+    __shared__ __align__(16) uint16_t s_ring[kRing * kStep];
+    __shared__ unsigned s_bad[kRing][2];                 // keys of a step's blocks whose values were not finite
     const const_int* const head = as_const(reinterpret_cast<const int*>(a.head));
     const int wide = head[6], walks = head[7], wide_cost = head[8], total = head[9], len = head[10];
     if (!plan_fits(a)) return;
@@ -210,18 +231,17 @@ void shared_decode_kernel(const SharedArgs a) {
     const int kvh = blockIdx.x / a.nhc;
     const int hc = blockIdx.x - kvh * a.nhc;
     if (start < wide_cost) {
+    auto k_of = [&](int t) { return s_ring + (t & (kRing - 1)) * kStep; };
+    auto v_of = [&](int t) { return k_of(t) + St::kPair; };
     const Start* const s0 = a.wide + blockIdx.y;
     Walk walk = walk_at(&s0->walk);
     int v = as_const(&s0->v)[0];
-    bool again = false;
     for (;;) {
         // This range's blocks of the walk: i0 .. i1 - 1.
         const int i0 = max(start - walk.at, 0);
         const int i1 = min(end - walk.at, walk.blocks);
         const Walk next = ++v < wide ? walk_at(a.walks + v) : walk;
         if (i0 < i1) {
-        if (again) __syncthreads();   // the stages are free for the next walk
-        again = true;
         // (the lane behind an empty asm: kept over the walks, what follows from it
         // would not leave them enough registers)
         int lane = threadIdx.x & 63;
@@ -247,6 +267,61 @@ void shared_decode_kernel(const SharedArgs a) {
         const bool ok = rt < a.tpw && place < count && g < a.G && sq.L > 0 && qrow >= 0;
         const bool works = __any(ok);
         const float slope = BIAS ? a.shape.slopes[hd] * kLog2e : 0.0f;
+        const int* const ids_of = a.bt + static_cast<size_t>(walk.row) * a.MB + first;
+        const int nsteps = (i1 - i0 + 1) >> 1;
+        // Ids of a step's blocks, by scalar loads a step ahead of their use.
+        auto ids_at = [&](int t) {
+            return int2{as_const(ids_of)[min(i0 + 2 * t, i1 - 1)], as_const(ids_of)[min(i0 + 2 * t + 1, i1 - 1)]};
+        };
+        // Waves 0 and 1 load a step's K, a block each, the others its V. Which of its
+        // blocks there are goes into `there`, two bits a step of the ring; others are
+        // read as block 0 and hidden. (Behind the last step there is nothing to load.)
+        const int mine = w & 1;
+        const bool is_k = w < 2;
+        const uint16_t* const cache = is_k ? a.kc : a.vc;
+        const unsigned lane_at = is_k ? 16u * lane : 32u * (lane & 31) + 16u * (lane >> 5);
+        const unsigned lds_at = static_cast<unsigned>(reinterpret_cast<uintptr_t>(to_lds(
+            s_ring + (is_k ? mine * St::kOdd : St::kPair + mine * St::kTile))));
+        unsigned there = 0;
+        auto fetch = [&](int t, int2 ids) {
+            const int slot = t & (kRing - 1);
+            const bool k0 = block_known(ids.x, a.num_blocks) && i0 + 2 * t < i1;
+            const bool k1 = block_known(ids.y, a.num_blocks) && i0 + 2 * t + 1 < i1;
+            there = (there & ~(3u << (2 * slot))) | (k0 ? 1u << (2 * slot) : 0u) | (k1 ? 2u << (2 * slot) : 0u);
+            const int id = mine ? (k1 ? ids.y : 0) : (k0 ? ids.x : 0);
+            const uintptr_t p = reinterpret_cast<uintptr_t>(cache + kv_tile_offset(id, kvh, a.Hkv, D));
+            const u4 rsrc = u4{static_cast<unsigned>(p), static_cast<unsigned>(p >> 32) & 0xffffu,
+                               t < nsteps ? D * kBlockTokens * 2u : 0u, static_cast<unsigned>(kRsrcWord3)};
+            const unsigned lds = lds_at + slot * 2 * kStep;
+            if (walk.once) {
+#pragma unroll
+                for (int i = 0; i < D / 32; ++i) load_lds16(rsrc, lds + 1024u * i, lane_at, 1024u * i, true);
+            } else {
+#pragma unroll
+                for (int i = 0; i < D / 32; ++i) load_lds16(rsrc, lds + 1024u * i, lane_at, 1024u * i, false);
+            }
+        };
+#pragma unroll
+        for (int t = 0; t < kRing - 1; ++t) fetch(t, ids_at(t));
+        int2 ahead = ids_at(kRing - 1);
+        // Q^T operand: lane (r, h) holds q[r][16 J + 8 h .. + 7].
+        s8 q[NJ];
+        {
+            const uint16_t* p = a.q + (static_cast<size_t>(max(qrow, 0)) * a.H + hd) * D + 8 * h;
+            const unsigned keep = ok ? a.q_and : 0u;
+            const unsigned flip = ok ? a.q_xor : 0u;
+#pragma unroll
+            for (int J = 0; J < NJ; ++J) {
+                u4 x;
+                if (a.q16) {
+                    x = *reinterpret_cast<const u4*>(p + 16 * J);
+                } else {
+                    x = __builtin_bit_cast(u4, join8(*reinterpret_cast<const s4*>(p + 16 * J),
+                                                     *reinterpret_cast<const s4*>(p + 16 * J + 4)));
+                }
+                q[J] = __builtin_bit_cast(s8, (x & keep) ^ flip);
+            }
+        }
         f16x acc[ND];
         float zero = 0.0f;
         asm volatile("" : "+v"(zero));
@@ -256,254 +331,132 @@ void shared_decode_kernel(const SharedArgs a) {
             for (int z = 0; z < 16; ++z) acc[i][z] = zero;
         }
         float m = -INFINITY, l = 0.0f;
-        const int nsteps = (i1 - i0 + 3) >> 2;
-        {
-            const int* const ids_of = a.bt + static_cast<size_t>(walk.row) * a.MB + first;
-            // Ids of 16 stages, four lanes each.
-            auto chunk_ids = [&](int c) { return ids_of[min(i0 + 64 * c + lane, i1 - 1)]; };
-            const int ids_first = chunk_ids(0);
-            int ids_next = chunk_ids(1);
-            // Q^T operand: lane (r, h) holds q[r][16 J + 8 h .. + 7].
-            s8 q[NJ];
-            {
-                const uint16_t* p = a.q + (static_cast<size_t>(max(qrow, 0)) * a.H + hd) * D + 8 * h;
-                const unsigned keep = ok ? a.q_and : 0u;
-                const unsigned flip = ok ? a.q_xor : 0u;
-#pragma unroll
-                for (int J = 0; J < NJ; ++J) {
-                    u4 x;
-                    if (a.q16) {
-                        x = *reinterpret_cast<const u4*>(p + 16 * J);
-                    } else {
-                        x = __builtin_bit_cast(u4, join8(*reinterpret_cast<const s4*>(p + 16 * J),
-                                                         *reinterpret_cast<const s4*>(p + 16 * J + 4)));
-                    }
-                    q[J] = __builtin_bit_cast(s8, (x & keep) ^ flip);
-                }
+        const float scale = a.shape.scale;
+        const float cap = a.shape.cap;
+        // Scores are what is made of them times mul, plus add; with a cap they fall as
+        // its part grows.
+        constexpr float kHidden = CAP && !BIAS ? INFINITY : -INFINITY;
+        const float mul = CAP ? -2.0f * cap : scale;
+        const float add = CAP ? cap : 0.0f;
+        auto most = [](float x, float y) { return CAP && !BIAS ? fminf(x, y) : fmaxf(x, y); };
+        wait_vm<0>();      // (with the queries' loads the count of the ring's is not known)
+        for (int t = 0; t < nsteps; ++t) {
+            // This wave's part of step t is there: those of the next two may be on
+            // their way.
+            wait_vm<2 * (D / 32)>();
+            const unsigned here = (there >> (2 * (t & (kRing - 1)))) & 3u;
+            if (here != 3u && !is_k) {
+                const unsigned bad = clean_v<T, D>(v_of(t), mine, lane);
+                if (lane == 0) s_bad[t & (kRing - 1)][mine] = bad;
             }
-            // The chunk at hand, unknown blocks as block 0 and their bits in `known` clear.
-            int ids;
-            unsigned long long known;
-            auto take_chunk = [&](int x, int c) {
-                const bool k = block_known(x, a.num_blocks) && i0 + 64 * c + lane < i1;
-                known = __ballot(k);
-                ids = k ? x : 0;
-            };
-            take_chunk(ids_first, 0);
-            // Tile of this wave in stage t (16 stages per load of ids) and, in ok4,
-            // which of the stage's four blocks there are.
-            auto tile_of = [&](int t, int& ok4) {
-                const int x = 4 * (t & 15);
-                ok4 = static_cast<int>((known >> x) & 15ull);
-                return kv_tile_offset(__builtin_amdgcn_readlane(ids, x + w), kvh, a.Hkv, D);
-            };
-            auto bytes_of = [&](int t) { return t < nsteps ? D * kBlockTokens * 2 : 0; };
-            auto base_of = [&](int t) { return (first + i0 + 4 * t) * kBlockTokens; };
-            // This wave's block of stage t has landed in its V buffer: true if the
-            // stage is not seen whole.
-            auto landed = [&](int t, int ok4) {
-                if (t >= nsteps || ok4 == 15) return false;
-                const unsigned bad = clean_v<T, D>(s_v[t & 1], w, lane);
-                if (lane == 0) s_bad[t & 1][w] = bad;
-                return true;
-            };
-            int ok_t, ok_1;                  // of stages t and t + 1
-            const size_t off = tile_of(0, ok_t);
-            stage_k<D>(a.kc, s_k[0], w, off, bytes_of(0), lane);
-            stage_v<D>(a.vc, s_v[0], w, off, bytes_of(0), lane);
-            size_t off_1 = tile_of(1, ok_1);
-            stage_k<D>(a.kc, s_k[1], w, off_1, bytes_of(1), lane);
-            wait_vm<0>();
-            bool cleaned = landed(0, ok_t);  // stage t
-            __syncthreads();
-            f16x sc[2];
-            qk_pair<T, D>(sc[0], s_k[0] + koff, q);
-            qk_pair<T, D>(sc[1], s_k[0] + koff + St::kPair, q);
-            __syncthreads();
-            const float scale = a.shape.scale;
-            const float cap = a.shape.cap;
-            auto cap_part = [&](float x) { return __builtin_amdgcn_rcpf(__builtin_amdgcn_exp2f(x * scale) + 1.0f); };
-            // Scores are what is made of them times mul, plus add; with a cap they
-            // fall as its part grows.
-            constexpr float kHidden = CAP && !BIAS ? INFINITY : -INFINITY;
-            const float mul = CAP ? -2.0f * cap : scale;
-            const float add = CAP ? cap : 0.0f;
-            float rise[16];   // of the bias over a pair's scores
+            __syncthreads();   // and everybody's, and step t - 1 is done with
+            const uint16_t* const kl = k_of(t) + koff;
+            const uint16_t* const vl = v_of(t) + 8 * lane;
+            // Operands are read all at once, and the next loads asked for meanwhile.
+            s8 op[NJ];
 #pragma unroll
-            for (int i = 0; i < 16; ++i) rise[i] = BIAS ? slope * static_cast<float>(16 * (i >> 3) + (i & 7)) : 0.0f;
-            auto most = [](float x, float y) { return CAP && !BIAS ? fminf(x, y) : fmaxf(x, y); };
+            for (int J = 0; J < NJ; ++J) op[J] = k_rows(kl + 256 * J);
+            __builtin_amdgcn_sched_barrier(0);
+            fetch(t + kRing - 1, ahead);
+            ahead = ids_at(t + kRing);
+            if (!works) continue;
+            // Score i: key base + 16 (i / 8) + 8 h + i % 8 of the step.
+            f16x sc = f16x{};
+#pragma unroll
+            for (int J = 0; J < NJ; ++J) sc = T::mfma32(op[J], q[J], sc);
+            __builtin_amdgcn_sched_barrier(0);
+            s8 val[2 * ND];
+#pragma unroll
+            for (int k = 0; k < 2 * ND; ++k) val[k] = *reinterpret_cast<const s8*>(vl + k / ND * St::kTile + 512 * (k % ND));
+            __builtin_amdgcn_sched_barrier(0);
             if constexpr (CAP) {
 #pragma unroll
-                for (int i = 0; i < 32; ++i) sc[i >> 4][i & 15] = cap_part(sc[i >> 4][i & 15]);
+                for (int i = 0; i < 16; ++i) sc[i] = __builtin_amdgcn_rcpf(__builtin_amdgcn_exp2f(sc[i] * scale) + 1.0f);
             }
-            for (int t = 0; t < nsteps; ++t) {
-                int ok_2;
-                stage_v<D>(a.vc, s_v[(t + 1) & 1], w, off_1, bytes_of(t + 1), lane);
-                off_1 = tile_of(t + 2, ok_2);
-                stage_k<D>(a.kc, s_k[t & 1], w, off_1, bytes_of(t + 2), lane);
-                const int base = base_of(t);
-                if (works) {
-                    // Score i of pair p: key base + 32 p + 16 (i / 8) + 8 h + i % 8; bit
-                    // 16 p + i of `seen` whether it is there.
-                    const bool whole = ok_t == 15;
-                    unsigned seen = ~0u;
-                    if (!whole) {
-                        seen = 0;
+            // What a score lacks: the bias of the step's first key.
+            float lack = add;
+            if constexpr (BIAS) {
+                const int base = (first + i0 + 2 * t) * kBlockTokens;
+                lack = __builtin_fmaf(slope, static_cast<float>(base + 8 * h - (sq.L - 1)), add);
 #pragma unroll
-                        for (int b = 0; b < 4; ++b) {
-                            if ((ok_t >> b) & 1) seen |= 0xffu << (8 * b);
-                        }
-                    }
-                    // What a pair's scores lack: the bias of its first key.
-                    float lack[2] = {add, add};
-                    if constexpr (BIAS) {
-                        const float d0 = static_cast<float>(base + 8 * h - (sq.L - 1));
-                        lack[0] = __builtin_fmaf(slope, d0, add);
-                        lack[1] = __builtin_fmaf(slope, d0 + 32.0f, add);
+                for (int i = 0; i < 16; ++i) sc[i] = __builtin_fmaf(sc[i], mul, slope * static_cast<float>(16 * (i >> 3) + (i & 7)));
+            }
+            if (here != 3u) {
 #pragma unroll
-                        for (int i = 0; i < 32; ++i) {
-                            sc[i >> 4][i & 15] = __builtin_fmaf(sc[i >> 4][i & 15], mul, rise[i & 15]);
-                        }
-                    }
-                    if (!whole) {
-#pragma unroll
-                        for (int i = 0; i < 32; ++i) {
-                            const int keep = __builtin_amdgcn_sbfe(static_cast<int>(seen), i, 1);  // 0 or -1
-                            const float x = sc[i >> 4][i & 15];   // (a bit cast of the element itself takes element 0)
-                            const int y = __builtin_bit_cast(int, x);
-                            sc[i >> 4][i & 15] = __builtin_bit_cast(float, (y & keep) | (__builtin_bit_cast(int, kHidden) & ~keep));
-                        }
-                    }
-                    auto most_of = [&](const f16x& x) {
-                        float y = most(most(x[0], x[1]), x[2]);
-#pragma unroll
-                        for (int i = 3; i < 15; i += 2) y = most(most(y, x[i]), x[i + 1]);
-                        return most(y, x[15]);
-                    };
-                    float bm;
-                    if constexpr (BIAS) {
-                        bm = fmaxf(most_of(sc[0]) + lack[0], most_of(sc[1]) + lack[1]);
-                    } else {
-                        bm = __builtin_fmaf(most(most_of(sc[0]), most_of(sc[1])), mul, add);
-                    }
-                    {
-                        const auto y = __builtin_amdgcn_permlane32_swap(__builtin_bit_cast(unsigned, bm), __builtin_bit_cast(unsigned, bm), false, false);
-                        bm = fmaxf(__builtin_bit_cast(float, static_cast<unsigned>(y[0])), __builtin_bit_cast(float, static_cast<unsigned>(y[1])));
-                    }
-                    if (__any(bm > m + kLag)) {
-                        const float m_new = fmaxf(m, bm);
-                        const float alpha = m_new == -INFINITY ? 1.0f : __builtin_amdgcn_exp2f(m - m_new);
-#pragma unroll
-                        for (int i = 0; i < ND; ++i) acc[i] *= alpha;
-                        l *= alpha;
-                        m = m_new;
-                    }
-                    const float c = ((m == -INFINITY) ? 0.0f : m) - weight_exp<T>;
-                    const float lack_c[2] = {lack[0] - c, lack[1] - c};
-                    if (cleaned) {
-                        const u4 bad = *reinterpret_cast<const u4*>(s_bad[t & 1]);
-                        unsigned keys = 0;   // this lane's, as `seen`
-#pragma unroll
-                        for (int b = 0; b < 4; ++b) keys |= ((bad[b] >> (8 * h)) & 0xffu) << (8 * b);
-                        if (seen & keys) l = __builtin_nanf("");
-                    }
-                    // Weights, O^T += V P^T, and the next stage's scores, in the order
-                    // that scored_prefill takes.
-                    const uint16_t* const next = s_k[(t + 1) & 1] + koff;
-                    const uint16_t* const vl = s_v[t & 1] + 8 * lane;
-                    u4 pw[4];
-                    auto weights = [&](int k) {   // the k-th pair of them
-                        const int b = k >> 2, i = k & 3;
-                        float p[2];
-#pragma unroll
-                        for (int z = 0; z < 2; ++z) {
-                            const float x = sc[b >> 1][8 * (b & 1) + 2 * i + z];
-                            p[z] = __builtin_amdgcn_exp2f(BIAS ? x + lack_c[b >> 1] : __builtin_fmaf(x, mul, lack_c[0]));
-                        }
-                        pw[b][i] = T::down2(p[0], p[1]);
-                        l = add_pair(T{}, pw[b][i], l);
-                    };
-                    constexpr int kScores = 2 * ND, kBack = 2 * ND + 2 * NJ, kProducts = 4 * ND + 2 * NJ;
-                    constexpr int kAhead = 2;
-                    auto operand = [&](int n) {
-                        if (n >= kScores && n < kBack) {
-                            const int k = n - kScores;
-                            return k_rows(next + k / NJ * St::kPair + 256 * (k % NJ));
-                        }
-                        const int k = n < kScores ? n : n - 2 * NJ;
-                        return *reinterpret_cast<const s8*>(vl + k / ND * St::kTile + 512 * (k % ND));
-                    };
-                    s8 ring[kAhead];
-#pragma unroll
-                    for (int n = 0; n < kAhead; ++n) ring[n] = operand(n);
-#pragma unroll
-                    for (int k = 0; k < 4; ++k) weights(k);
-                    __builtin_amdgcn_sched_barrier(0);
-#pragma unroll
-                    for (int n = 0; n < kProducts; ++n) {
-                        const s8 x = ring[n % kAhead];
-                        if (n + kAhead < kProducts) ring[n % kAhead] = operand(n + kAhead);
-                        if (n >= kScores && n < kBack) {
-                            const int k = n - kScores;
-                            sc[k / NJ] = T::mfma32(x, q[k % NJ], k % NJ == 0 ? f16x{} : sc[k / NJ]);
-                        } else {
-                            const int k = n < kScores ? n : n - 2 * NJ;
-                            acc[k % ND] = T::mfma32(x, __builtin_bit_cast(s8, pw[k / ND]), acc[k % ND]);
-                        }
-                        if (n < kScores) {
-#pragma unroll
-                            for (int i = 4 + n * 4 / ND; i < 4 + (n + 1) * 4 / ND; ++i) weights(i);
-                        } else if (n < kScores + 4) {
-                            weights(12 + n - kScores);
-                        } else if (CAP && n >= kScores + NJ) {
-                            constexpr int kSlots = 2 * ND + NJ;
-                            const int k = n - kScores - NJ;
-#pragma unroll
-                            for (int i = k * 32 / kSlots; i < (k + 1) * 32 / kSlots; ++i) sc[i >> 4][i & 15] = cap_part(sc[i >> 4][i & 15]);
-                        }
-                        __builtin_amdgcn_sched_barrier(0);
-                    }
+                for (int i = 0; i < 16; ++i) {
+                    if (!((here >> (i >> 3)) & 1u)) sc[i] = kHidden;
                 }
-                wait_vm<0>();
-                cleaned = landed(t + 1, ok_1);
-                ok_t = ok_1;
-                ok_1 = ok_2;
-                if (((t + 3) & 15) == 0) {
-                    take_chunk(ids_next, (t + 3) >> 4);
-                    ids_next = chunk_ids(((t + 3) >> 4) + 1);
+            }
+            float bm = most(most(sc[0], sc[1]), sc[2]);
+#pragma unroll
+            for (int i = 3; i < 15; i += 2) bm = most(most(bm, sc[i]), sc[i + 1]);
+            bm = most(bm, sc[15]);
+            bm = BIAS ? bm + lack : __builtin_fmaf(bm, mul, add);
+            {
+                const auto y = __builtin_amdgcn_permlane32_swap(__builtin_bit_cast(unsigned, bm), __builtin_bit_cast(unsigned, bm), false, false);
+                bm = fmaxf(__builtin_bit_cast(float, static_cast<unsigned>(y[0])), __builtin_bit_cast(float, static_cast<unsigned>(y[1])));
+            }
+            if (__any(bm > m + kLag)) {
+                const float m_new = fmaxf(m, bm);
+                const float alpha = m_new == -INFINITY ? 1.0f : __builtin_amdgcn_exp2f(m - m_new);
+#pragma unroll
+                for (int i = 0; i < ND; ++i) acc[i] *= alpha;
+                l *= alpha;
+                m = m_new;
+            }
+            const float lack_c = lack - (((m == -INFINITY) ? 0.0f : m) - weight_exp<T>);
+            if (here != 3u) {
+                const unsigned* const bad = s_bad[t & (kRing - 1)];
+                const unsigned keys = ((here & 1u) ? (bad[0] >> (8 * h)) & 0xffu : 0u) | ((here & 2u) ? (bad[1] >> (8 * h)) & 0xffu : 0u);
+                if (keys) l = __builtin_nanf("");
+            }
+            u4 pw[2];
+#pragma unroll
+            for (int k = 0; k < 8; ++k) {
+                float p[2];
+#pragma unroll
+                for (int z = 0; z < 2; ++z) {
+                    const float x = sc[2 * k + z];
+                    p[z] = __builtin_amdgcn_exp2f(BIAS ? x + lack_c : __builtin_fmaf(x, mul, lack_c));
                 }
-                __syncthreads();
+                const unsigned both = T::down2(p[0], p[1]);
+                pw[k >> 2][k & 3] = both;
+                l = add_pair(T{}, both, l);
+            }
+#pragma unroll
+            for (int k = 0; k < 2 * ND; ++k) {
+                acc[k % ND] = T::mfma32(val[k], __builtin_bit_cast(s8, pw[k / ND]), acc[k % ND]);
             }
         }
+        wait_vm<0>();
         // The rows' fragments: they share, and go on. Lane (r, h) has values
         // 32 i + 8 k + 4 h .. + 3 of row r.
-        {
+        if (rt < a.tpw && place < count) {
             const auto y = __builtin_amdgcn_permlane32_swap(__builtin_bit_cast(unsigned, l), __builtin_bit_cast(unsigned, l), false, false);
             const float sum = __builtin_bit_cast(float, static_cast<unsigned>(y[0])) + __builtin_bit_cast(float, static_cast<unsigned>(y[1]));
             const float inv = sum == 0.0f ? 0.0f : 1.0f / sum;
-            if (rt < a.tpw && place < count) {
-                const long long f = static_cast<long long>(blockIdx.x) * a.frag_rows + walk.frow +
-                                    static_cast<long long>(static_cast<int>(blockIdx.y) - walk.at / walk.len) * count * a.gw + place * a.gw + rh;
-                if (h == 0) a.frag_ml[f] = float2{m, sum};
-                float* const p = a.frag_o + f * D + 4 * h;
+            const long long f = static_cast<long long>(blockIdx.x) * a.frag_rows + walk.frow +
+                                static_cast<long long>(static_cast<int>(blockIdx.y) - walk.at / len) * count * a.gw + place * a.gw + rh;
+            if (h == 0) a.frag_ml[f] = float2{m, sum};
+            float* const p = a.frag_o + f * D + 4 * h;
 #pragma unroll
-                for (int i = 0; i < ND; ++i) {
+            for (int i = 0; i < ND; ++i) {
 #pragma unroll
-                    for (int k = 0; k < 4; ++k) {
-                        *reinterpret_cast<f4*>(p + 32 * i + 8 * k) =
-                            f4{acc[i][4 * k] * inv, acc[i][4 * k + 1] * inv, acc[i][4 * k + 2] * inv, acc[i][4 * k + 3] * inv};
-                    }
+                for (int k = 0; k < 4; ++k) {
+                    *reinterpret_cast<f4*>(p + 32 * i + 8 * k) =
+                        f4{acc[i][4 * k] * inv, acc[i][4 * k + 1] * inv, acc[i][4 * k + 2] * inv, acc[i][4 * k + 3] * inv};
                 }
             }
         }
+        __syncthreads();       // the ring is free
         }
         if (v >= wide || next.at - kWideCost >= end) break;
         walk = next;
     }
     }
-    // This wave's quarter of what is narrow.
-    const int range = kTileWaves * static_cast<int>(blockIdx.y) + w;
-    const int wlen = len / kTileWaves;
+    // This wave's part of what is narrow.
+    const int range = kWaves * static_cast<int>(blockIdx.y) + w;
+    const int wlen = len / kWaves;
     const int b = range * wlen, e = min(b + wlen, total);
     if (e <= wide_cost || b >= total) return;
     Walk walk;
@@ -524,7 +477,7 @@ void shared_decode_kernel(const SharedArgs a) {
             for (int hb = 0; hb < a.gw; hb += kNarrowRows) {
                 int lane = threadIdx.x & 63;
                 asm volatile("" : "+v"(lane));
-                narrow_piece<T, D, BIAS>(a, walk, kvh, hc, hb, i0, i1, range, lane);
+                narrow_piece<T, D, BIAS>(a, walk, kvh, hc, hb, i0, i1, range, wlen, lane);
             }
         }
         if (v >= walks || next.at - kNarrowCost >= e) break;
@@ -553,17 +506,21 @@ __global__ __launch_bounds__(64 * kJoinWaves) void shared_join_kernel(const Shar
     const int rh = hg - hc * kWaveRows;
     // Fragments 0 .. n0 - 1 are of the shared blocks, the others of its own.
     int n0 = 0, n1 = 0, f0 = 0, f1 = 0, step = 0;
-    auto pieces = [](const Walk& x) { return (x.at + x.blocks - 1) / x.len - x.at / x.len + 1; };
+    const const_int* const head = as_const(reinterpret_cast<const int*>(a.head));
+    auto pieces = [&](const Walk& x, int v) {
+        const int n = v < head[6] ? head[10] : head[10] / kTileWaves;    // a wide walk's ranges, and a narrow one's
+        return (x.at + x.blocks - 1) / n - x.at / n + 1;
+    };
     if (tile >= 0) {
         const Walk x = walk_at(a.walks + tile);
         step = x.count * a.gw;
-        n0 = pieces(x);
+        n0 = pieces(x, tile);
         f0 = x.frow + index * a.gw + rh;
     }
     if (own >= 0) {
         const Walk x = walk_at(a.walks + own);
         if (x.frow < 0) return;      // its row is written
-        n1 = pieces(x);
+        n1 = pieces(x, own);
         f1 = x.frow + rh;
     }
     const long long sub = static_cast<long long>(kvh * a.nhc + hc) * a.frag_rows;
@@ -743,7 +700,7 @@ int swiftllm_hip_shared_decode(void* output, void* workspace, size_t workspace_b
                                   {shared_join_kernel<BF16, 64>, shared_join_kernel<BF16, 128>}};
     const int t = dtype == SWIFTLLM_HIP_BF16;
     rc = launched(launch(kernels[t][head_dim == 128][softcap > 0.0f][alibi_slopes != nullptr], dim3(h.HC, l.ranges),
-                         dim3(64 * kTileWaves), 0, stream, a), who);
+                         dim3(64 * kWaves), 0, stream, a), who);
     if (rc != SWIFTLLM_OK) return rc;
     return launched(launch(joins[t][head_dim == 128], dim3(num_seqs, (num_heads + kJoinWaves - 1) / kJoinWaves),
                            dim3(64 * kJoinWaves), 0, stream, a), who);

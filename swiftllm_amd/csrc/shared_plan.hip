@@ -31,7 +31,7 @@ struct PlanSharedArgs {
     int* shared;            // [N]
     Head* head;
     Start* wide;            // [ranges]
-    Start* narrow;          // [ranges * 4]
+    Start* narrow;          // [ranges * kTileWaves]
     Walk* walks;
     Seq* seqs;
     int4* infos;            // [S]: group, its first live row, leading blocks alike with it, blocks shared
@@ -205,7 +205,7 @@ __global__ __launch_bounds__(kListThreads) void shared_list_kernel(const PlanSha
         narrow_cost += all.w;
     }
     const int total = wide_cost + narrow_cost;
-    const int wlen = max((total + kTileWaves * a.ranges - 1) / (kTileWaves * a.ranges), kLeastRange / kTileWaves);
+    const int wlen = max((total + kTileWaves * a.ranges - 1) / (kTileWaves * a.ranges), kLeastRange);
     const int len = kTileWaves * wlen;
     __syncthreads();      // the costs are there for all
     int rows = 0;
@@ -229,9 +229,9 @@ __global__ __launch_bounds__(kListThreads) void shared_list_kernel(const PlanSha
         if (s < a.S) {
             const int f = rows + bx;
             // A walk, and the ranges of n that begin in it or in what it costs before.
-            auto put = [&](int v, const Walk& w, int cost, Start* starts) {
+            auto put = [&](int v, const Walk& w, int cost, int n, Start* starts) {
                 a.walks[v] = w;
-                for (int r = (w.at - cost + w.len - 1) / w.len; r * w.len < w.at + w.blocks; ++r) {
+                for (int r = (w.at - cost + n - 1) / n; r * n < w.at + w.blocks; ++r) {
                     Start& x = starts[r];
                     x.walk = w;
                     x.v = v;
@@ -239,16 +239,17 @@ __global__ __launch_bounds__(kListThreads) void shared_list_kernel(const PlanSha
             };
             const int v = wide + at.z;
             if (m.count > 0) {
-                const Walk w{m.info.y, 0, m.info.w, s, m.count, tile_at, m.wide ? len : wlen, f};
+                const bool once = a.offsets[m.info.x + 1] - a.offsets[m.info.x] <= a.per_tile;
+                const Walk w{m.info.y, 0, m.info.w, s, m.count, tile_at, once, f};
                 if (m.wide) {
-                    put(at.x, w, kWideCost, a.wide);
+                    put(at.x, w, kWideCost, len, a.wide);
                 } else {
-                    put(v, w, kNarrowCost, a.narrow);
+                    put(v, w, kNarrowCost, wlen, a.narrow);
                 }
             }
             const int own_v = v + (m.tile_cost > 0);
             if (m.own > 0) {
-                put(own_v, Walk{s, m.L > 0 ? m.info.w : 0, m.own, s, 1, own_at, wlen, own_rows > 0 ? f + tile_rows : -1}, kNarrowCost, a.narrow);
+                put(own_v, Walk{s, m.L > 0 ? m.info.w : 0, m.own, s, 1, own_at, 1, own_rows > 0 ? f + tile_rows : -1}, kNarrowCost, wlen, a.narrow);
             }
             Seq q{m.L, m.own > 0 ? own_v : -1, -1, 0};
             if (joins) {

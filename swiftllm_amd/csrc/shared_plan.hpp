@@ -3,10 +3,10 @@
 //
 // The work of a step is a list of walks: of a group's shared blocks by the queries
 // of up to `per_tile` of its sequences, and of each sequence's other blocks by its
-// own. Walks of more than 16 query rows are wide, a workgroup's, and come first;
-// the others are narrow, a wave's. The list is cut into equal ranges of its cost,
-// one per workgroup and chunk of heads, of which each wave has a quarter of what is
-// narrow. Every piece of a walk that does not end its rows leaves one fragment
+// own. Shared ones of more than 16 query rows are wide, a workgroup's, and come
+// first; the others are narrow, a wave's. The list is cut into equal ranges of its cost,
+// one per workgroup and chunk of heads, of which each wave has an equal part of what
+// is narrow. Every piece of a walk that does not end its rows leaves one fragment
 // (maximum, sum, output) a row; those of a walk lie behind each other from row
 // `frow` on.
 #pragma once
@@ -27,11 +27,11 @@ constexpr int kNarrowRows = 16;
 // Blocks that starting and ending a walk costs.
 constexpr int kWideCost = 8;
 constexpr int kNarrowCost = 2;
-// Workgroups the list is cut for: two for each of the 256 CUs of an MI355X, as the
-// wide walks' registers allow.
+// Workgroups the list is cut for: two for each of the 256 CUs of an MI355X, whose
+// LDS their rings of steps take.
 constexpr int kResident = 2 * 256;
-// Shortest range, in blocks: four of each wave.
-constexpr int kLeastRange = 16;
+// Shortest part of a wave in what is narrow, in blocks.
+constexpr int kLeastRange = 4;
 // Blocks that reading shared ones once has to save.
 constexpr int kLeastSaved = 16;
 
@@ -42,7 +42,7 @@ struct Walk {
     int seq;        // the first of its sequences
     int count;      //   and how many: more than one shares
     int at;         // its first block's place in the list
-    int len;        // of the ranges that cut it
+    int once;       // no other walk reads its blocks
     int frow;       // its first fragment, in rows of a chunk of heads; -1: one piece that ends its row
 };
 
@@ -59,7 +59,7 @@ struct Head {
     int walks;      //   in all
     int wide_cost;  // the list's wide part
     int total;
-    int len;        // of a workgroup's range, four times a wave's
+    int len;        // of a workgroup's range, kTileWaves times a wave's
     int pad[5];
 };
 
