@@ -85,7 +85,8 @@ __device__ __forceinline__ Walk walk_at(const Walk* p) {
 // Four outputs of a row.
 template <typename T>
 __device__ __forceinline__ void put_out(uint16_t* p, f4 o, bool out8) {
-    const u2 x = u2{T::down2(o[0], o[1]), T::down2(o[2], o[3])};
+    u2 x = u2{T::down2(o[0], o[1]), T::down2(o[2], o[3])};
+    asm volatile("" : "+v"(x));     // rounded once, the same for any address
     if (out8) {
         *reinterpret_cast<u2*>(p) = x;
     } else {
@@ -96,53 +97,64 @@ __device__ __forceinline__ void put_out(uint16_t* p, f4 o, bool out8) {
     }
 }
 
-// Blocks i0 .. i1 - 1 of a narrow walk, by one wave, for the heads hb .. hb + 15 of
-// its chunk. Lane (r, kg) has query row r: sequence r / gw, head hb + r % gw.
-template <typename T, int D, bool BIAS>
-__device__ __forceinline__ void narrow_piece(const SharedArgs& a, const Walk& walk, int kvh, int hc, int hb, int i0, int i1, int range, int wlen, int lane) {
+// A wave's walk for 16 query rows: blocks i0, i0 + STEP .. below i1 of the walk, for
+// the heads hb .. hb + 15 of its chunk. Lane (r, kg) has query row r: sequence r / gn,
+// head hb + r % gn, gn of them at hand.
+template <int D>
+struct Rows {
+    State<D> st;
+    int qrow, hd;
+    int place;       // among the rows of the walk
+    bool row, ok;    // there is a row for it, and a query in it
+};
+
+template <typename T, int D, bool BIAS, int STEP>
+__device__ __forceinline__ void narrow_walk(const SharedArgs& a, const Walk& walk, int kvh, int hc, int hb, int i0, int i1, int lane, Rows<D>& o) {
     constexpr int NJ = D / 16;
     const int r = lane & 15;
     const int kg = lane >> 4;
-    const int gn = min(a.gw - hb, kNarrowRows);              // heads at hand
+    const int gn = min(a.gw - hb, kNarrowRows);
     const int rt = r / gn;
     const int rh = hb + r - rt * gn;
     const int g = hc * kWaveRows + rh;
-    const int hd = kvh * a.G + min(g, a.G - 1);
     const int s = walk.seq + min(rt, walk.count - 1);
     const Seq sq = a.seqs[s];
-    const int qrow = row_of(a, s);
-    const bool row = rt < walk.count;                        // there is a row for it
-    const bool ok = row && g < a.G && sq.L > 0 && qrow >= 0;
+    o.hd = kvh * a.G + min(g, a.G - 1);
+    o.qrow = row_of(a, s);
+    o.place = rt * a.gw + rh;
+    o.row = rt < walk.count;
+    o.ok = o.row && g < a.G && sq.L > 0 && o.qrow >= 0;
+    State<D>& st = o.st;
+    st.m = -INFINITY;
+    st.l = 0.0f;
+#pragma unroll
+    for (int J = 0; J < NJ; ++J) st.acc[J] = f4{0, 0, 0, 0};
+    const int count = i1 > i0 ? (i1 - i0 + STEP - 1) / STEP : 0;
+    if (count == 0) return;
     const int* const ids_of = a.bt + static_cast<size_t>(walk.row) * a.MB + walk.first;
-    const int count = i1 - i0;
-    // Lane l has the id of block i0 + 64 c + l.
-    auto ids_from = [&](int c) { return ids_of[min(i0 + 64 * c + lane, i1 - 1)]; };
+    // Lane l has the id of the wave's block 64 c + l.
+    auto ids_from = [&](int c) { return ids_of[min(i0 + STEP * (64 * c + lane), i1 - 1)]; };
     int ids = ids_from(0);
     s8 q[NJ / 2];
-    const uint16_t* const qp = a.q + (static_cast<size_t>(max(qrow, 0)) * a.H + hd) * D + 4 * kg;
-    const unsigned keep = ok ? a.q_and : 0u, flip = ok ? a.q_xor : 0u;
+    const uint16_t* const qp = a.q + (static_cast<size_t>(max(o.qrow, 0)) * a.H + o.hd) * D + 4 * kg;
+    const unsigned keep = o.ok ? a.q_and : 0u, flip = o.ok ? a.q_xor : 0u;
 #pragma unroll
     for (int J = 0; J < NJ; J += 2) {
         const s8 x = join8(*reinterpret_cast<const s4*>(qp + 16 * J), *reinterpret_cast<const s4*>(qp + 16 * J + 16));
         q[J / 2] = __builtin_bit_cast(s8, (__builtin_bit_cast(u4, x) & keep) ^ flip);
     }
-    const float slope = BIAS && ok ? a.shape.slopes[hd] * kLog2e : 0.0f;
+    const float slope = BIAS && o.ok ? a.shape.slopes[o.hd] * kLog2e : 0.0f;
     s4 ident;
 #pragma unroll
     for (int i = 0; i < 4; ++i) ident[i] = 4 * kg + i == r ? static_cast<short>(T::one()) : 0;
     const int loff = kv_elem_offset(r, 4 * kg);
-    State<D> st;
-    st.m = -INFINITY;
-    st.l = 0.0f;
-#pragma unroll
-    for (int J = 0; J < NJ; ++J) st.acc[J] = f4{0, 0, 0, 0};
     // The keys of an own walk end with its sequence; shared blocks are seen whole.
     const int L = __builtin_amdgcn_readfirstlane(walk.count > 1 ? 0x7fffffff : sq.L);
     auto load = [&](int k, s4 (&kk)[NJ], s4 (&vv)[NJ], int& base, unsigned& seen) {
         if (k > 0 && (k & 63) == 0) ids = ids_from(k >> 6);
         const int b = __builtin_amdgcn_readlane(ids, k & 63);
         const bool known = block_known(b, a.num_blocks);
-        base = (walk.first + i0 + k) * kBlockTokens;
+        base = (walk.first + i0 + STEP * k) * kBlockTokens;
         seen = known ? low_bits(L - base) : 0u;
         // A block outside the pool is read as block 0 and hidden.
         const size_t tile = kv_tile_offset(known ? b : 0, kvh, a.Hkv, D) + loff;
@@ -174,20 +186,83 @@ __device__ __forceinline__ void narrow_piece(const SharedArgs& a, const Walk& wa
     } else {
         take(kA, vA, bA, sA);
     }
-    const float sum = sum_over_groups(st.l);
+}
+
+// Blocks i0 .. i1 - 1 of a narrow walk, by one wave.
+template <typename T, int D, bool BIAS>
+__device__ __forceinline__ void narrow_piece(const SharedArgs& a, const Walk& walk, int kvh, int hc, int hb, int i0, int i1, int range, int wlen, int lane) {
+    constexpr int NJ = D / 16;
+    const int kg = lane >> 4;
+    Rows<D> o;
+    narrow_walk<T, D, BIAS, 1>(a, walk, kvh, hc, hb, i0, i1, lane, o);
+    const float sum = sum_over_groups(o.st.l);
     const float inv = sum == 0.0f ? 0.0f : 1.0f / sum;
     if (walk.frow < 0) {
-        if (!ok) return;
-        uint16_t* const p = a.out + (static_cast<size_t>(qrow) * a.H + hd) * D + 4 * kg;
+        if (!o.ok) return;
+        uint16_t* const p = a.out + (static_cast<size_t>(o.qrow) * a.H + o.hd) * D + 4 * kg;
 #pragma unroll
-        for (int J = 0; J < NJ; ++J) put_out<T>(p + 16 * J, st.acc[J] * inv, a.out8);
-    } else if (row) {
+        for (int J = 0; J < NJ; ++J) put_out<T>(p + 16 * J, o.st.acc[J] * inv, a.out8);
+    } else if (o.row) {
         const long long f = static_cast<long long>(blockIdx.x) * a.frag_rows + walk.frow +
-                            static_cast<long long>(range - walk.at / wlen) * walk.count * a.gw + rt * a.gw + rh;
-        if (kg == 0) a.frag_ml[f] = float2{st.m, sum};
+                            static_cast<long long>(range - walk.at / wlen) * walk.count * a.gw + o.place;
+        if (kg == 0) a.frag_ml[f] = float2{o.st.m, sum};
         float* const p = a.frag_o + f * D + 4 * kg;
 #pragma unroll
-        for (int J = 0; J < NJ; ++J) *reinterpret_cast<f4*>(p + 16 * J) = st.acc[J] * inv;
+        for (int J = 0; J < NJ; ++J) *reinterpret_cast<f4*>(p + 16 * J) = o.st.acc[J] * inv;
+    }
+}
+
+// Every sequence whole, in one launch: a workgroup per sequence and 16 heads of a
+// chunk, its waves take the blocks in turn.
+template <typename T, int D, bool BIAS>
+__global__ __launch_bounds__(64 * kWaves) void shared_whole_kernel(const SharedArgs a) {
+    constexpr int NJ = D / 16;
+    __shared__ float s_m[kWaves][16], s_l[kWaves][16];
+    __shared__ __align__(16) float s_o[kWaves][16][D];
+    if (!plan_fits(a)) return;
+    const int s = blockIdx.y;
+    const int parts = (a.gw + kNarrowRows - 1) / kNarrowRows;
+    const int hb = static_cast<int>(blockIdx.x) % parts * kNarrowRows;
+    const int sub = blockIdx.x / parts;
+    const int kvh = sub / a.nhc;
+    const int hc = sub - kvh * a.nhc;
+    const int tid = threadIdx.x, lane = tid & 63;
+    const int w = __builtin_amdgcn_readfirstlane(tid >> 6);
+    const int L = as_const(reinterpret_cast<const int*>(a.seqs + s))[0];
+    const int row = row_of(a, s);
+    if (row < 0) return;
+    const int blocks = (L + kBlockTokens - 1) >> kBlockShift;
+    const Walk walk{s, 0, blocks, s, 1, 0, 1, -1};
+    Rows<D> o;
+    narrow_walk<T, D, BIAS, kWaves>(a, walk, kvh, hc, hb, w, blocks, lane, o);
+    const int r = lane & 15, kg = lane >> 4;
+    const float l = sum_over_groups(o.st.l);
+    if (kg == 0) {
+        s_m[w][r] = o.st.m;
+        s_l[w][r] = l;
+    }
+#pragma unroll
+    for (int J = 0; J < NJ; ++J) *reinterpret_cast<f4*>(&s_o[w][r][16 * J + 4 * kg]) = o.st.acc[J];
+    __syncthreads();
+    const int heads = min(min(a.gw - hb, kNarrowRows), a.G - hc * kWaveRows - hb);
+    for (int i = tid; i < heads * (D / 4); i += 64 * kWaves) {
+        const int g = i / (D / 4);
+        const int d = 4 * (i - g * (D / 4));
+        float m = -INFINITY;
+#pragma unroll
+        for (int x = 0; x < kWaves; ++x) m = fmaxf(m, s_m[x][g]);
+        f4 num = f4{0, 0, 0, 0};
+        float den = 0.0f;
+#pragma unroll
+        for (int x = 0; x < kWaves; ++x) {
+            // A wave that saw no key has zeros; one of NaN scores alone a NaN sum.
+            const float f = s_m[x][g] == -INFINITY ? 1.0f : __builtin_amdgcn_exp2f(s_m[x][g] - m);
+            num += f * *reinterpret_cast<const f4*>(&s_o[x][g][d]);
+            den += f * s_l[x][g];
+        }
+        const float inv = den == 0.0f ? 0.0f : 1.0f / den;
+        const int hd = kvh * a.G + hc * kWaveRows + hb + g;
+        put_out<T>(a.out + (static_cast<size_t>(row) * a.H + hd) * D + d, num * inv, a.out8);
     }
 }
 
@@ -485,18 +560,28 @@ void shared_decode_kernel(const SharedArgs a) {
     }
 }
 
-// Joins the fragments of a sequence's rows: a wave per query head. A lane holds the
-// maximum and the sum of a fragment, and the first rows are on their way before
-// those are there.
+// Joins the fragments of a sequence's rows: WAVES waves a query head, which take them
+// in turn. A lane holds the maximum and the sum of a fragment, and the first rows are
+// on their way before those are there: a join is bound by latency.
 constexpr int kJoinRows = 8;
-constexpr int kJoinWaves = 4;
+constexpr int kJoinWaves = 4;       // of a workgroup
+constexpr int kFewRows = 2048;
 
-template <typename T, int D>
+// Tables and bytes of K and V up to which every sequence is taken whole.
+constexpr int kMostWhole = 96;
+constexpr double kWholeBytes = 24e6;
+
+template <typename T, int D, int WAVES>
 __global__ __launch_bounds__(64 * kJoinWaves) void shared_join_kernel(const SharedArgs a) {
     constexpr int DL = D / 64;
+    constexpr int kHeads = kJoinWaves / WAVES;
+    __shared__ float s_o[WAVES > 1 ? kJoinWaves : 1][D];
+    __shared__ float s_ml[WAVES > 1 ? kJoinWaves : 1][2];
     const int lane = threadIdx.x & 63;
-    const int hd = blockIdx.y * kJoinWaves + __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-    if (hd >= a.H || !plan_fits(a)) return;
+    const int w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    const int hd = blockIdx.y * kHeads + w / WAVES;
+    const int turn = w % WAVES;
+    if (hd >= a.H || !plan_fits(a)) return;      // (with several waves a head, one head a workgroup)
     const int s = blockIdx.x;
     const const_int* const sq = as_const(reinterpret_cast<const int*>(a.seqs + s));
     const int own = sq[1], tile = sq[2], index = sq[3];
@@ -524,8 +609,12 @@ __global__ __launch_bounds__(64 * kJoinWaves) void shared_join_kernel(const Shar
         f1 = x.frow + rh;
     }
     const long long sub = static_cast<long long>(kvh * a.nhc + hc) * a.frag_rows;
-    const int count = n0 + n1;
-    auto place = [&](int i) { return sub + (i < n0 ? f0 + i * step : f1 + (i - n0) * a.gw); };
+    // This wave's i-th fragment.
+    const int count = max((n0 + n1 - turn + WAVES - 1) / WAVES, 0);
+    auto place = [&](int i) {
+        const int x = turn + WAVES * i;
+        return sub + (x < n0 ? f0 + x * step : f1 + (x - n0) * a.gw);
+    };
     float m = -INFINITY, l = 0.0f, o[DL];
 #pragma unroll
     for (int j = 0; j < DL; ++j) o[j] = 0.0f;
@@ -563,6 +652,29 @@ __global__ __launch_bounds__(64 * kJoinWaves) void shared_join_kernel(const Shar
                     for (int j = 0; j < DL; ++j) o[j] += x * v[k][j];
                 }
             }
+        }
+    }
+    if constexpr (WAVES > 1) {
+#pragma unroll
+        for (int j = 0; j < DL; ++j) s_o[w][lane * DL + j] = o[j];
+        if (lane == 0) {
+            s_ml[w][0] = m;
+            s_ml[w][1] = l;
+        }
+        __syncthreads();
+        if (turn > 0) return;
+        m = -INFINITY;
+        l = 0.0f;
+#pragma unroll
+        for (int x = 0; x < WAVES; ++x) m = fmaxf(m, s_ml[x][0]);
+#pragma unroll
+        for (int j = 0; j < DL; ++j) o[j] = 0.0f;
+#pragma unroll
+        for (int x = 0; x < WAVES; ++x) {
+            const float f = s_ml[x][0] == -INFINITY ? 1.0f : __builtin_amdgcn_exp2f(s_ml[x][0] - m);
+            l += f * s_ml[x][1];
+#pragma unroll
+            for (int j = 0; j < DL; ++j) o[j] += f * s_o[x][lane * DL + j];
         }
     }
     const int row = row_of(a, s);
@@ -696,13 +808,26 @@ int swiftllm_hip_shared_decode(void* output, void* workspace, size_t workspace_b
       {shared_decode_kernel<T_, 128, true, false>, shared_decode_kernel<T_, 128, true, true>}}}
     static const K kernels[2][2][2][2] = {SHARED_DECODE(F16), SHARED_DECODE(BF16)};
 #undef SHARED_DECODE
-    static const K joins[2][2] = {{shared_join_kernel<F16, 64>, shared_join_kernel<F16, 128>},
-                                  {shared_join_kernel<BF16, 64>, shared_join_kernel<BF16, 128>}};
+    static const K joins[2][2][2] = {
+        {{shared_join_kernel<F16, 64, 1>, shared_join_kernel<F16, 64, 4>}, {shared_join_kernel<F16, 128, 1>, shared_join_kernel<F16, 128, 4>}},
+        {{shared_join_kernel<BF16, 64, 1>, shared_join_kernel<BF16, 64, 4>}, {shared_join_kernel<BF16, 128, 1>, shared_join_kernel<BF16, 128, 4>}}};
     const int t = dtype == SWIFTLLM_HIP_BF16;
+    // Short tables of few sequences are read whole by each: less than a second launch
+    // would cost. (The host knows the tables, not the contexts.)
+    const int parts = (h.gw + kNarrowRows - 1) / kNarrowRows;
+    const double whole = 1.0 * num_seqs * h.HC * parts * max_num_blocks_per_seq * (4.0 * kBlockTokens * head_dim);
+    if (max_num_blocks_per_seq <= kMostWhole && whole <= kWholeBytes && num_seqs <= 65535) {
+        static const K whole_kernel[2][2][2] = {
+            {{shared_whole_kernel<F16, 64, false>, shared_whole_kernel<F16, 64, true>}, {shared_whole_kernel<F16, 128, false>, shared_whole_kernel<F16, 128, true>}},
+            {{shared_whole_kernel<BF16, 64, false>, shared_whole_kernel<BF16, 64, true>}, {shared_whole_kernel<BF16, 128, false>, shared_whole_kernel<BF16, 128, true>}}};
+        return launched(launch(whole_kernel[t][head_dim == 128][alibi_slopes != nullptr], dim3(h.HC * parts, num_seqs), dim3(64 * kWaves), 0, stream, a), who);
+    }
     rc = launched(launch(kernels[t][head_dim == 128][softcap > 0.0f][alibi_slopes != nullptr], dim3(h.HC, l.ranges),
                          dim3(64 * kWaves), 0, stream, a), who);
     if (rc != SWIFTLLM_OK) return rc;
-    return launched(launch(joins[t][head_dim == 128], dim3(num_seqs, (num_heads + kJoinWaves - 1) / kJoinWaves),
+    // Few rows may have many fragments each, and leave the GPU to four waves of each.
+    const bool few = static_cast<long long>(num_seqs) * num_heads < kFewRows;
+    return launched(launch(joins[t][head_dim == 128][few], dim3(num_seqs, few ? num_heads : (num_heads + kJoinWaves - 1) / kJoinWaves),
                            dim3(64 * kJoinWaves), 0, stream, a), who);
 }
 

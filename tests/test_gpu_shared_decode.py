@@ -18,12 +18,13 @@ class Shared:
     """groups: of each, (tokens of whole shared blocks, the contexts of its sequences)."""
 
     def __init__(self, rng, groups, H, Hkv, D, dtype, cap=0.0, alibi=False, MB=None, scale=None, spare=3, qstd=3.0,
-                 lone=0):
+                 lone=0, tight=False):
         ctx = [c for _, cs in groups for c in cs]
         self.ctx = np.array(ctx + [int(rng.integers(0, 50)) for _ in range(lone)], np.int32)
         self.S, self.H, self.Hkv, self.D, self.dtype = len(self.ctx), H, Hkv, D, dtype
         used = [-(-max(int(c), 0) // 16) for c in self.ctx]
-        self.MB = max(used + [1]) if MB is None else MB
+        # (tables of up to 96 blocks are taken whole where they are few: tight ones)
+        self.MB = max(used + [1 if tight else 97]) if MB is None else MB
         common = [p // 16 for p, _ in groups]
         need = sum(common) + sum(used) + 1
         self.NB = need + spare
@@ -107,6 +108,13 @@ class Shared:
         return got
 
 
+def whole(s):
+    """Whether every sequence is read whole, by the launcher's rule."""
+    G = s.H // s.Hkv
+    parts = -(-min(G, 32) // 16)
+    return s.MB <= 96 and s.S * s.Hkv * -(-G // 32) * parts * s.MB * 64 * s.D <= 24e6
+
+
 HEADS = [(8, 8, 64), (32, 8, 128), (16, 2, 128), (6, 2, 64), (5, 1, 128), (1, 1, 64), (40, 1, 64), (96, 2, 128)]
 
 
@@ -119,6 +127,25 @@ def test_heads(dev, H, Hkv, D, dtype):
     Shared(rng, groups, H, Hkv, D, dtype, lone=2).run().check()
 
 
+@pytest.mark.parametrize("dtype", ["f16", "bf16"])
+@pytest.mark.parametrize("H,Hkv,D", HEADS)
+def test_heads_whole(dev, H, Hkv, D, dtype):
+    """Short tables, each sequence read whole; those without a context, odd block ids, an output at any address."""
+    rng = np.random.default_rng(H + D)
+    groups = [(160, [165, 170, 0]), (64, [70, 64, 100, 1, 16]), (0, [33])]
+    for cap, alibi in ((0.0, False), (25.0, True)):
+        s = Shared(rng, groups, H, Hkv, D, dtype, cap=cap, alibi=alibi, lone=2, tight=True)
+        assert whole(s)
+        s.bt[1, 3], s.bt[5, 5] = -3, s.NB
+        s.bt[0, 3] = s.bt[2, 3] = -3
+        s.upload()
+        s.run().check()
+        out = DeviceArray((s.q.size + 3,), np.uint16)
+        s.run_decode(out=out.ptr + 2)
+        synchronize()
+        assert np.array_equal(out.numpy()[1:-2].reshape(s.q.shape), s.out.numpy()[:s.S])
+
+
 @pytest.mark.parametrize("cap,alibi", [(0.0, False), (20.0, False), (0.0, True), (30.0, True)])
 @pytest.mark.parametrize("H,Hkv,D,dtype", [(8, 2, 128, "bf16"), (16, 2, 64, "f16"), (4, 4, 128, "f16"), (8, 1, 64, "bf16")])
 def test_scores(dev, H, Hkv, D, dtype, cap, alibi):
@@ -128,14 +155,18 @@ def test_scores(dev, H, Hkv, D, dtype, cap, alibi):
 
 
 @pytest.mark.parametrize("extra", [0, 1, 15, 16, 17, 63, 64, 65, 127, 128, 129])
-def test_lengths_around_stages(dev, extra):
-    """Shared and own parts that end inside a block and a stage, and at their edges."""
+@pytest.mark.parametrize("tight", [False, True])
+@pytest.mark.parametrize("H", [8, 24])
+def test_lengths_around_stages(dev, extra, tight, H):
+    """Shared and own parts that end inside a block and a step, and at their edges."""
     rng = np.random.default_rng(extra)
     groups = [(p, [p + extra, p + extra + 1, p + max(extra - 1, 0)]) for p in (16, 48, 64, 80, 128, 272)]
-    Shared(rng, groups, 8, 2, 128, "f16").run().check()
+    s = Shared(rng, groups, H, 2, 128, "f16", tight=tight)
+    assert whole(s) == tight
+    s.run().check()
 
 
-@pytest.mark.parametrize("each", [1, 2, 7, 8, 9, 31, 32, 33, 70])
+@pytest.mark.parametrize("each", [1, 2, 7, 8, 9, 31, 32, 33, 70, 131])
 @pytest.mark.parametrize("H,Hkv,D", [(8, 2, 128), (8, 8, 64), (6, 2, 64)])
 def test_group_sizes(dev, each, H, Hkv, D):
     """Tiles that fill their waves' rows, and that do not."""
@@ -280,10 +311,11 @@ def test_scales(dev, scale, cap):
     Shared(rng, [(160, [200, 210]), (0, [64])], 8, 2, 64, "bf16", cap=cap, scale=scale, qstd=1.0).run().check()
 
 
-def test_packed_rows(dev):
+@pytest.mark.parametrize("tight", [False, True])
+def test_packed_rows(dev, tight):
     """Rows of a step: the last of each sequence's; sequences without rows, and rows of none."""
     rng = np.random.default_rng(12)
-    s = Shared(rng, [(160, [170, 180, 190, 200])], 8, 2, 64, "f16")
+    s = Shared(rng, [(160, [170, 180, 190, 200])], 8, 2, 64, "f16", tight=tight)
     off = np.array([0, 1, 1, 4, 5], np.int32)     # rows 0, none, 1-3, 4; row 5 of none
     q = normal(rng, (6, 8, 64), "f16", 3.0)
     s.q = np.stack([q[0], np.zeros_like(q[0]), q[3], q[4]])
@@ -321,10 +353,11 @@ def test_odd_addresses(dev):
     assert (np.abs(got - want) <= bound).all()
 
 
-def test_plan_of_other_sizes_writes_nothing(dev):
+@pytest.mark.parametrize("tight", [False, True])
+def test_plan_of_other_sizes_writes_nothing(dev, tight):
     rng = np.random.default_rng(14)
-    s = Shared(rng, [(160, [170, 180])], 8, 2, 64, "f16")
-    t = Shared(rng, [(160, [170, 180])], 4, 2, 64, "f16")
+    s = Shared(rng, [(160, [170, 180])], 8, 2, 64, "f16", tight=tight)
+    t = Shared(rng, [(160, [170, 180])], 4, 2, 64, "f16", tight=tight)
     t.run_plan()
     s.plan.upload(t.plan.numpy())
     s.run_decode()
@@ -390,6 +423,6 @@ def test_random_sweep(dev):
             n = int(np.exp(rng.uniform(0, np.log(40))))
             groups.append((p, [0 if rng.random() < 0.1 else p + int(rng.integers(0, 150)) - int(rng.integers(0, 2)) * 16 for _ in range(n)]))
         dtype = ["f16", "bf16"][rng.integers(2)]
-        kw = dict(cap=float(rng.choice([0, 0, 25])), alibi=bool(rng.random() < 0.3), lone=int(rng.integers(0, 3)))
+        kw = dict(cap=float(rng.choice([0, 0, 25])), alibi=bool(rng.random() < 0.3), lone=int(rng.integers(0, 3)), tight=bool(rng.random() < 0.3))
         print(H, Hkv, D, dtype, [(p, len(c)) for p, c in groups], kw, flush=True)
         Shared(rng, groups, H, Hkv, D, dtype, **kw).run().check()
