@@ -657,6 +657,8 @@ int swiftllm_hip_compact_pages(
  * group shares anything); a sequence of no group shares nothing. Writes
  * shared_blocks[g], the leading blocks that every sequence of the group with a
  * context uses, and all of them the same (0 where none has a context), and the
+ * plan. It reads a group's blocks once where that saves min_saved blocks of a kv
+ * head or more; below 0 where it is the faster way by the library's own rule. The
  * plan: swiftllm_hip_plan_shared_size() bytes, 256-byte aligned, for
  * swiftllm_hip_shared_decode calls with the same sizes, which take the contexts
  * and what is shared from it. */
@@ -667,7 +669,8 @@ int swiftllm_hip_plan_shared(void* plan, size_t plan_bytes,
                              const int32_t* group_offsets, int num_groups,
                              int num_seqs, int num_heads, int num_kv_heads,
                              int head_dim, int block_size,
-                             int max_num_blocks_per_seq, hipStream_t stream);
+                             int max_num_blocks_per_seq, int min_saved,
+                             hipStream_t stream);
 
 /* Bytes of a plan; 0 where swiftllm_hip_plan_shared would refuse the sizes. */
 size_t swiftllm_hip_plan_shared_size(int num_seqs, int num_heads,

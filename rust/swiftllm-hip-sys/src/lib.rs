@@ -315,7 +315,7 @@ extern "C" {
         block_tables: *const i32, context_lens: *const i32, group_offsets: *const i32,
         num_groups: c_int, num_seqs: c_int, num_heads: c_int, num_kv_heads: c_int,
         head_dim: c_int, block_size: c_int, max_num_blocks_per_seq: c_int,
-        stream: hipStream_t,
+        min_saved: c_int, stream: hipStream_t,
     ) -> c_int;
     pub fn swiftllm_hip_plan_shared_size(
         num_seqs: c_int, num_heads: c_int, num_kv_heads: c_int, head_dim: c_int,

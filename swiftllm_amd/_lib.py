@@ -113,7 +113,7 @@ SIGNATURES = {
         i32, [vp, vp, vp, vp, vp, vp, vp, vp, vp, vp, vp, sz, i32, i32, i32, i32, i32, vp]),
     "swiftllm_hip_pages_workspace_size": (sz, [i32, i32]),
     "swiftllm_hip_plan_shared": (
-        i32, [vp, sz, vp, vp, vp, vp, i32, i32, i32, i32, i32, i32, i32, vp]),
+        i32, [vp, sz, vp, vp, vp, vp, i32, i32, i32, i32, i32, i32, i32, i32, vp]),
     "swiftllm_hip_plan_shared_size": (sz, [i32, i32, i32, i32, i32, i32]),
     "swiftllm_hip_shared_decode": (
         i32, [vp, vp, sz, vp, sz, vp, vp, vp, vp, vp, vp, f32, f32, i32, i32, i32, i32, i32, i32,

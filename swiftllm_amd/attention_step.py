@@ -234,15 +234,17 @@ def plan_shared_size(num_seqs: int, num_heads: int, num_kv_heads: int, head_dim:
 def plan_shared(plan: Ptr, plan_bytes: int, shared_blocks: Ptr, block_tables: Ptr,
                 context_lens: Ptr, group_offsets: Ptr, num_groups: int, num_seqs: int,
                 num_heads: int, num_kv_heads: int, head_dim: int, block_size: int,
-                max_num_blocks_per_seq: int, stream: Optional[Stream] = None) -> None:
+                max_num_blocks_per_seq: int, min_saved: int = -1,
+                stream: Optional[Stream] = None) -> None:
     """The plan of a step's shared_decode calls (swiftllm_hip_plan_shared): the
     sequences group_offsets[g] .. group_offsets[g + 1] - 1 are a group, and
     shared_blocks[g] becomes the leading blocks that all of them have in common.
-    `plan` holds plan_shared_size(...) bytes and serves every layer of these sizes."""
+    `plan` holds plan_shared_size(...) bytes and serves every layer of these sizes.
+    min_saved: blocks that reading a group's once has to save; -1: the library's rule."""
     check_status(_lib.lib().swiftllm_hip_plan_shared(
         _p(plan), plan_bytes, _p(shared_blocks), _p(block_tables), _p(context_lens),
         _p(group_offsets), num_groups, num_seqs, num_heads, num_kv_heads, head_dim, block_size,
-        max_num_blocks_per_seq, _s(stream)))
+        max_num_blocks_per_seq, min_saved, _s(stream)))
 
 
 def shared_decode_workspace_size(num_seqs: int, num_heads: int, num_kv_heads: int, head_dim: int,

@@ -568,8 +568,8 @@ constexpr int kJoinWaves = 4;       // of a workgroup
 constexpr int kFewRows = 2048;
 
 // Tables and bytes of K and V up to which every sequence is taken whole.
-constexpr int kMostWhole = 96;
-constexpr double kWholeBytes = 24e6;
+constexpr int kMostWhole = 48;
+constexpr double kWholeBytes = 64e6;
 
 template <typename T, int D, int WAVES>
 __global__ __launch_bounds__(64 * kJoinWaves) void shared_join_kernel(const SharedArgs a) {

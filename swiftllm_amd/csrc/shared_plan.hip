@@ -4,8 +4,8 @@
 //
 // Of a group with n >= 2 sequences that have a context, the leading table entries
 // that all of them use, and alike, are shared; a walk takes those that all of them
-// have filled, sh blocks, where that saves (n - 1) sh >= kLeastSaved, so that no
-// row sees part of one. Rows of a group without a context count for nothing.
+// have filled, sh blocks, so that no row sees part of one, where the (n - 1) sh that
+// it saves are worth it. Rows of a group without a context count for nothing.
 //
 // Bound: latency. A step of 128 sequences of 256 blocks compares 131 KB, once for
 // all layers. Two launches: a workgroup per sequence compares its row with its
@@ -20,8 +20,10 @@ namespace {
 using namespace shared;
 
 constexpr int kMatchThreads = 256;
-constexpr int kListThreads = 1024;
+constexpr int kMostCounted = 1024;
+constexpr int kListThreads = 512;
 constexpr int kListWaves = kListThreads / 64;
+constexpr int kTries = 16;          // lengths of a range that are tried
 constexpr int kWindow = 2048;       // groups whose minima are in LDS at a time
 
 struct PlanSharedArgs {
@@ -35,9 +37,10 @@ struct PlanSharedArgs {
     Walk* walks;
     Seq* seqs;
     int4* infos;            // [S]: group, its first live row, leading blocks alike with it, blocks shared
-    int4* costs;            // [S]: wide walks and their cost, narrow ones and theirs before it
+    int4* costs;            // [S][2]: aligned, other wide and narrow walks and their costs before it
     int S, N, MB, H, Hkv, D;
-    int gw, per_tile, ranges;
+    int HC, gw, per_tile, ranges;
+    int min_saved;
 };
 
 __device__ __forceinline__ int used_blocks(const PlanSharedArgs& a, int s) {
@@ -59,12 +62,23 @@ __global__ __launch_bounds__(kMatchThreads) void shared_match_kernel(const PlanS
         for (int i = 1; i < kMatchThreads / 64; ++i) m = min(m, s_least[i]);
         return m;
     };
-    // The last group that begins at s or before. (Offsets out of order, which the
-    // list's kernel refuses, give some number of a group here.)
-    int lo = 0, hi = a.N;
-    while (lo < hi) {
-        const int mid = (lo + hi) >> 1;
-        if (a.offsets[mid] <= s) lo = mid + 1; else hi = mid;
+    // The last group that begins at s or before: by counting those that do, all at
+    // once, or among many by bisection. (Offsets out of order, which the list's kernel
+    // refuses, give some number of a group here.)
+    int lo = 0;
+    if (a.N <= kMostCounted) {
+        for (int i = tid; i < a.N; i += kMatchThreads) lo += a.offsets[i] <= s;
+        lo = wave_total(lo);
+        if ((tid & 63) == 0) s_least[tid >> 6] = lo;
+        __syncthreads();
+        lo = 0;
+        for (int i = 0; i < kMatchThreads / 64; ++i) lo += s_least[i];
+    } else {
+        int hi = a.N;
+        while (lo < hi) {
+            const int mid = (lo + hi) >> 1;
+            if (a.offsets[mid] <= s) lo = mid + 1; else hi = mid;
+        }
     }
     const int g = lo - 1;
     int4 info = int4{-1, -1, 0, 0};
@@ -123,19 +137,41 @@ __device__ __forceinline__ void scan2(int x, int y, int& before_x, int& before_y
     }
 }
 
+// ONE: at most as many sequences as threads, each of which keeps what it knows of its own.
+template <bool ONE>
 __global__ __launch_bounds__(kListThreads) void shared_list_kernel(const PlanSharedArgs a) {
     __shared__ int s_least[kWindow], s_full[kWindow], s_live[kWindow];
     __shared__ int s_part[2][kListWaves];
-    __shared__ int s_bad;
+    __shared__ int s_pad[kTries];
+    __shared__ int s_tile[ONE ? kListThreads : 1];    // the walk of the tile that begins with a sequence
+    __shared__ int s_bad, s_saved;
     const int tid = threadIdx.x;
-    if (tid == 0) s_bad = 0;
+    if (tid == 0) s_bad = s_saved = 0;
+    if (tid < kTries) s_pad[tid] = 0;
+    struct Row {
+        int4 info;       // w: blocks shared
+        int ctx;
+        int off, end;    // its group
+    };
+    auto load_row = [&](int s) {
+        Row r{int4{-1, -1, 0, 0}, 0, 0, 0};
+        if (s < a.S) {
+            r.info = a.infos[s];
+            r.ctx = a.ctx[s];
+            if (r.info.x >= 0) {
+                r.off = a.offsets[r.info.x];
+                r.end = a.offsets[r.info.x + 1];
+            }
+        }
+        return r;
+    };
+    Row mine = load_row(ONE ? tid : a.S);
+    auto row_of = [&](int s) { return ONE ? mine : load_row(s); };
     __syncthreads();
     for (int i = tid; i < a.N; i += kListThreads) {
         const int b = a.offsets[i], e = a.offsets[i + 1];
         if (b < 0 || e < b || e > a.S) s_bad = 1;
     }
-    __syncthreads();
-    const bool bad = s_bad != 0;
     // What every group shares, and of that what is worth it, a window of groups at a time.
     for (int g0 = 0; g0 < max(a.N, 1); g0 += kWindow) {
         for (int i = tid; i < min(max(a.N - g0, 0), kWindow); i += kListThreads) {
@@ -143,25 +179,29 @@ __global__ __launch_bounds__(kListThreads) void shared_list_kernel(const PlanSha
             s_live[i] = 0;
         }
         __syncthreads();
-        auto mine = [&](int s, int4& info) {
-            info = a.infos[s];
-            return info.x >= g0 && info.x < g0 + kWindow;
-        };
+        const bool bad = s_bad != 0;
         for (int s = tid; s < a.S; s += kListThreads) {
-            int4 info;
-            if (mine(s, info) && a.ctx[s] > 0) {
-                atomicMin(&s_least[info.x - g0], info.z);
-                atomicMin(&s_full[info.x - g0], a.ctx[s] >> kBlockShift);
-                atomicAdd(&s_live[info.x - g0], 1);
+            const Row r = row_of(s);
+            const int g = r.info.x - g0;
+            if (r.info.x >= 0 && g >= 0 && g < kWindow && r.ctx > 0) {
+                atomicMin(&s_least[g], r.info.z);
+                atomicMin(&s_full[g], r.ctx >> kBlockShift);
+                atomicAdd(&s_live[g], 1);
             }
         }
         __syncthreads();
         for (int s = tid; s < a.S; s += kListThreads) {
-            int4 info;
-            if (mine(s, info)) {
-                const int live = s_live[info.x - g0], sh = min(s_least[info.x - g0], s_full[info.x - g0]);
-                const bool worth = !bad && live > 1 && static_cast<long long>(live - 1) * sh >= kLeastSaved;
-                a.infos[s].w = worth ? sh : 0;
+            const Row r = row_of(s);
+            const int g = r.info.x - g0;
+            if (r.info.x >= 0 && g >= 0 && g < kWindow) {
+                const int live = s_live[g], sh = min(s_least[g], s_full[g]);
+                const bool worth = !bad && live > 1 && static_cast<long long>(live - 1) * sh >= (a.min_saved < 0 ? kLeastSaved : max(a.min_saved, 1));
+                if (worth && r.info.y == s) atomicAdd(&s_saved, (live - 1) * sh);
+                if (ONE) {
+                    mine.info.w = worth ? sh : 0;
+                } else {
+                    a.infos[s].w = worth ? sh : 0;
+                }
             }
         }
         for (int i = tid; i < min(a.N - g0, kWindow); i += kListThreads) {
@@ -169,102 +209,174 @@ __global__ __launch_bounds__(kListThreads) void shared_list_kernel(const PlanSha
         }
         __syncthreads();
     }
+    // All of it together has to be worth the joins.
+    const bool share = a.min_saved >= 0 || static_cast<long long>(s_saved) * a.HC * a.D >= kLeastSavedAll;
     // A sequence's walks: a tile's, where it is the first of one, and its own.
     struct Mine {
-        int4 info;
-        int L, count, own;                    // of the tile; own blocks
-        int wide, narrow, wide_cost, tile_cost, own_cost;   // walks, and what they cost
+        int sh, L, count, own;                // blocks shared; sequences of the tile; own blocks
+        int wide, tile_cost, own_cost;        // (a walk's cost of 0: there is none)
+        int group;                            // sequences of its group
+        int lead;
     };
     auto walks_of = [&](int s) {
         Mine m{};
         if (s >= a.S) return m;
-        m.info = a.infos[s];
-        m.L = min(max(a.ctx[s], 0), a.MB * kBlockTokens);
-        m.own = ((m.L + kBlockTokens - 1) >> kBlockShift) - (m.L > 0 ? m.info.w : 0);
+        const Row r = row_of(s);
+        m.sh = share ? r.info.w : 0;
+        m.lead = r.info.y;
+        m.L = min(max(r.ctx, 0), a.MB * kBlockTokens);
+        m.own = ((m.L + kBlockTokens - 1) >> kBlockShift) - (m.L > 0 ? m.sh : 0);
         m.own_cost = m.own > 0 ? m.own + kNarrowCost : 0;
-        if (m.info.w > 0 && (s - a.offsets[m.info.x]) % a.per_tile == 0) {
-            m.count = min(a.per_tile, a.offsets[m.info.x + 1] - s);
+        m.group = r.end - r.off;
+        if (m.sh > 0 && (s - r.off) % a.per_tile == 0) {
+            m.count = min(a.per_tile, r.end - s);
             m.wide = m.count * a.gw > kNarrowRows;
+            m.tile_cost = m.sh + (m.wide ? kWideCost : kNarrowCost);
         }
-        m.wide_cost = m.wide ? m.info.w + kWideCost : 0;
-        m.tile_cost = m.count > 0 && !m.wide ? m.info.w + kNarrowCost : 0;
-        m.narrow = (m.tile_cost > 0) + (m.own_cost > 0);
         return m;
     };
-    int wide = 0, narrow = 0, wide_cost = 0, narrow_cost = 0;
-    for (int s0 = 0; s0 < a.S; s0 += kListThreads) {
-        const int s = s0 + tid;
+    int sum = 0;
+    for (int s = tid; s < a.S; s += kListThreads) {
         const Mine m = walks_of(s);
-        int4 before, all;
-        scan2(m.wide, m.wide_cost, before.x, before.y, all.x, all.y, s_part);
-        scan2(m.narrow, m.tile_cost + m.own_cost, before.z, before.w, all.z, all.w, s_part);
-        if (s < a.S) a.costs[s] = int4{wide + before.x, wide_cost + before.y, narrow + before.z, narrow_cost + before.w};
-        wide += all.x;
-        wide_cost += all.y;
-        narrow += all.z;
-        narrow_cost += all.w;
+        sum += m.tile_cost + m.own_cost;
     }
-    const int total = wide_cost + narrow_cost;
-    const int wlen = max((total + kTileWaves * a.ranges - 1) / (kTileWaves * a.ranges), kLeastRange);
-    const int len = kTileWaves * wlen;
-    __syncthreads();      // the costs are there for all
+    int none, all, all_none, base;
+    scan2(sum, 0, base, none, all, all_none, s_part);
+    // Where several tiles share blocks, each begins and ends with a range, so that
+    // they come by the same blocks at the same time, in one L2. What that leaves empty
+    // makes the ranges longer, by a sixteenth of the first length and more.
+    const int wlen0 = max((all + kTileWaves * a.ranges - 1) / (kTileWaves * a.ranges), kLeastRange);
+    auto try_len = [&](int k) { return kTileWaves * (wlen0 + k * max(wlen0 / 16, 1)); };
+    auto padded = [&](const Mine& m, int len) {
+        const bool aligned = m.wide && m.group > a.per_tile && m.tile_cost > 2 * len;
+        return aligned ? (m.tile_cost + len - 1) / len * len : 0;
+    };
+    for (int s = tid; s < a.S; s += kListThreads) {
+        const Mine m = walks_of(s);
+        if (m.wide && m.group > a.per_tile) {
+            for (int k = 0; k < kTries; ++k) {
+                const int n = padded(m, try_len(k));
+                if (n > 0) atomicAdd(&s_pad[k], n - m.tile_cost);
+            }
+        }
+    }
+    __syncthreads();
+    int len = try_len(0);
+    bool align = false;
+    for (int k = kTries - 1; k >= 0; --k) {
+        if (static_cast<long long>(all) + s_pad[k] <= static_cast<long long>(a.ranges) * try_len(k)) {
+            len = try_len(k);
+            align = true;
+        }
+    }
+    const int wlen = len / kTileWaves;
+    // Aligned tiles first, other wide ones, then the narrow ones.
+    auto cost_of = [&](const Mine& m, int& aligned, int& wide, int& narrow) {
+        const int n = align ? padded(m, len) : 0;
+        aligned = n;
+        wide = m.wide && n == 0 ? m.tile_cost : 0;
+        narrow = m.wide ? 0 : m.tile_cost;
+    };
+    int walks[3] = {0, 0, 0}, costs[3] = {0, 0, 0};     // of the chunks before
+    int at_walks[3], at_costs[3];                       // of this thread's sequence, and in all at the end
+    auto scan_row = [&](int s, const Mine& m) {
+        int aligned, wide, narrow;
+        cost_of(m, aligned, wide, narrow);
+        const int n[3] = {aligned > 0, wide > 0, (narrow > 0) + (m.own_cost > 0)};
+        const int c[3] = {aligned, wide, narrow + m.own_cost};
+#pragma unroll
+        for (int x = 0; x < 3; ++x) {
+            int bn, bc, an, ac;
+            scan2(n[x], c[x], bn, bc, an, ac, s_part);
+            at_walks[x] = walks[x] + bn;
+            at_costs[x] = costs[x] + bc;
+            walks[x] += an;
+            costs[x] += ac;
+        }
+        if (!ONE && s < a.S) {
+            a.costs[2 * static_cast<size_t>(s)] = int4{at_walks[0], at_costs[0], at_walks[1], at_costs[1]};
+            a.costs[2 * static_cast<size_t>(s) + 1] = int4{at_walks[2], at_costs[2], 0, 0};
+        }
+    };
+    for (int s0 = 0; s0 < (ONE ? 1 : a.S); s0 += kListThreads) scan_row(s0 + tid, walks_of(s0 + tid));
+    const int wide_walks = walks[0] + walks[1];
+    const int wide_cost = costs[0] + costs[1];
+    const int total = wide_cost + costs[2];
+    // A tile's walk, from the sums before its first sequence.
+    auto tile_walk = [&](const Mine& m, const int (&n)[3]) {
+        int aligned, wide, narrow;
+        cost_of(m, aligned, wide, narrow);
+        return aligned > 0 ? n[0] : wide > 0 ? walks[0] + n[1] : wide_walks + n[2];
+    };
+    if (ONE) s_tile[tid] = tile_walk(walks_of(tid), at_walks);
+    __syncthreads();      // that, or the costs, is there for all
     int rows = 0;
     for (int s0 = 0; s0 < a.S; s0 += kListThreads) {
         const int s = s0 + tid;
         const Mine m = walks_of(s);
-        const int4 at = s < a.S ? a.costs[s] : int4{0, 0, 0, 0};
+        if (!ONE && s < a.S) {
+            const int4 x = a.costs[2 * static_cast<size_t>(s)], y = a.costs[2 * static_cast<size_t>(s) + 1];
+            at_walks[0] = x.x;
+            at_costs[0] = x.y;
+            at_walks[1] = x.z;
+            at_costs[1] = x.w;
+            at_walks[2] = y.x;
+            at_costs[2] = y.y;
+        }
+        int aligned, wide, narrow;
+        cost_of(m, aligned, wide, narrow);
         // Ranges of n that blocks b .. b + k - 1 of the list lie in.
         auto pieces = [](int b, int k, int n) { return (b + k - 1) / n - b / n + 1; };
-        const bool joins = m.info.w > 0 && m.L > 0;
-        const int tile_at = m.wide ? at.y + kWideCost : wide_cost + at.w + kNarrowCost;
-        const int own_at = wide_cost + at.w + m.tile_cost + kNarrowCost;
+        const bool joins = m.sh > 0 && m.L > 0;
+        const int tile_at = aligned > 0 ? at_costs[0] + kWideCost : wide > 0 ? costs[0] + at_costs[1] + kWideCost : wide_cost + at_costs[2] + kNarrowCost;
+        const int own_at = wide_cost + at_costs[2] + narrow + kNarrowCost;
         int tile_rows = 0, own_rows = 0;
-        if (m.count > 0) tile_rows = m.count * a.gw * pieces(tile_at, m.info.w, m.wide ? len : wlen);
+        if (m.count > 0) tile_rows = m.count * a.gw * pieces(tile_at, m.sh, m.wide ? len : wlen);
         if (m.own > 0) {
             const int n = pieces(own_at, m.own, wlen);
             if (joins || n > 1) own_rows = a.gw * n;
         }
-        int bx, none, ax, all_none;
+        int bx, ax;
         scan2(tile_rows + own_rows, 0, bx, none, ax, all_none, s_part);
         if (s < a.S) {
             const int f = rows + bx;
-            // A walk, and the ranges of n that begin in it or in what it costs before.
-            auto put = [&](int v, const Walk& w, int cost, int n, Start* starts) {
+            // A walk, and the ranges of n that begin in it or in what it costs.
+            auto put = [&](int v, const Walk& w, int from, int to, int n, Start* starts) {
                 a.walks[v] = w;
-                for (int r = (w.at - cost + n - 1) / n; r * n < w.at + w.blocks; ++r) {
+                for (int r = (from + n - 1) / n; r * n < to; ++r) {
                     Start& x = starts[r];
                     x.walk = w;
                     x.v = v;
                 }
             };
-            const int v = wide + at.z;
             if (m.count > 0) {
-                const bool once = a.offsets[m.info.x + 1] - a.offsets[m.info.x] <= a.per_tile;
-                const Walk w{m.info.y, 0, m.info.w, s, m.count, tile_at, once, f};
-                if (m.wide) {
-                    put(at.x, w, kWideCost, len, a.wide);
-                } else {
-                    put(v, w, kNarrowCost, wlen, a.narrow);
-                }
+                const Walk w{m.lead, 0, m.sh, s, m.count, tile_at, m.group <= a.per_tile, f};
+                const int from = tile_at - (m.wide ? kWideCost : kNarrowCost);
+                put(tile_walk(m, at_walks), w, from, aligned > 0 ? from + aligned : tile_at + m.sh, m.wide ? len : wlen, m.wide ? a.wide : a.narrow);
             }
-            const int own_v = v + (m.tile_cost > 0);
+            const int own_v = wide_walks + at_walks[2] + (narrow > 0);
             if (m.own > 0) {
-                put(own_v, Walk{s, m.L > 0 ? m.info.w : 0, m.own, s, 1, own_at, 1, own_rows > 0 ? f + tile_rows : -1}, kNarrowCost, wlen, a.narrow);
+                put(own_v, Walk{s, m.L > 0 ? m.sh : 0, m.own, s, 1, own_at, 1, own_rows > 0 ? f + tile_rows : -1}, own_at - kNarrowCost, own_at + m.own, wlen, a.narrow);
             }
             Seq q{m.L, m.own > 0 ? own_v : -1, -1, 0};
             if (joins) {
                 // Its tile begins with another sequence of the group, or with itself.
-                const int b = a.offsets[m.info.x];
-                q.index = (s - b) % a.per_tile;
+                const Row r = row_of(s);
+                q.index = (s - r.off) % a.per_tile;
                 const int t = s - q.index;
-                const bool is_wide = min(a.per_tile, a.offsets[m.info.x + 1] - t) * a.gw > kNarrowRows;
-                q.tile = is_wide ? a.costs[t].x : wide + a.costs[t].z;
+                if (ONE) {
+                    q.tile = s_tile[t];
+                } else {
+                    const int4 x = a.costs[2 * static_cast<size_t>(t)], y = a.costs[2 * static_cast<size_t>(t) + 1];
+                    const int n[3] = {x.x, x.z, y.x};
+                    q.tile = tile_walk(walks_of(t), n);
+                }
             }
             a.seqs[s] = q;
         }
         rows += ax;
     }
-    if (tid == 0) *a.head = Head{kMagic, a.S, a.MB, a.H, a.Hkv, a.D, wide, wide + narrow, wide_cost, total, len};
+    if (tid == 0) *a.head = Head{kMagic, a.S, a.MB, a.H, a.Hkv, a.D, wide_walks, wide_walks + walks[2], wide_cost, total, len};
 }
 
 }  // namespace
@@ -311,7 +423,7 @@ size_t swiftllm_hip_plan_shared_size(int num_seqs, int num_heads, int num_kv_hea
 int swiftllm_hip_plan_shared(void* plan, size_t plan_bytes, int32_t* shared_blocks, const int32_t* block_tables,
                              const int32_t* context_lens, const int32_t* group_offsets, int num_groups, int num_seqs,
                              int num_heads, int num_kv_heads, int head_dim, int block_size, int max_num_blocks_per_seq,
-                             hipStream_t stream) {
+                             int min_saved, hipStream_t stream) {
     const char* who = "swiftllm_hip_plan_shared";
     int rc = shared::check_sizes(who, num_seqs, num_heads, num_kv_heads, head_dim, block_size, max_num_blocks_per_seq);
     if (rc != SWIFTLLM_OK) return rc;
@@ -358,14 +470,16 @@ int swiftllm_hip_plan_shared(void* plan, size_t plan_bytes, int32_t* shared_bloc
     a.H = num_heads;
     a.Hkv = num_kv_heads;
     a.D = head_dim;
+    a.HC = h.HC;
     a.gw = h.gw;
     a.per_tile = h.per_tile;
     a.ranges = l.ranges;
+    a.min_saved = min_saved;
     if (num_seqs > 0) {
         rc = launched(launch(shared_match_kernel, dim3(num_seqs), dim3(kMatchThreads), 0, stream, a), who);
         if (rc != SWIFTLLM_OK) return rc;
     }
-    return launched(launch(shared_list_kernel, dim3(1), dim3(kListThreads), 0, stream, a), who);
+    return launched(launch(num_seqs <= kListThreads ? shared_list_kernel<true> : shared_list_kernel<false>, dim3(1), dim3(kListThreads), 0, stream, a), who);
 }
 
 }  // extern "C"

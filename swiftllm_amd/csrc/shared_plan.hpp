@@ -32,8 +32,10 @@ constexpr int kNarrowCost = 2;
 constexpr int kResident = 2 * 256;
 // Shortest part of a wave in what is narrow, in blocks.
 constexpr int kLeastRange = 4;
-// Blocks that reading shared ones once has to save.
+// Blocks of a group that reading shared ones once has to save, and values of a head of
+// all of them (blocks x chunks of heads x head_dim).
 constexpr int kLeastSaved = 16;
+constexpr long long kLeastSavedAll = 2500 * 128;
 
 struct Walk {
     int row;        // whose table names the blocks
@@ -105,7 +107,7 @@ inline Layout layout_of(long long S, int H, int Hkv) {
     l.seqs = l.walks + up(static_cast<long long>(sizeof(Walk)) * (2 * S + 1));
     l.infos = l.seqs + up(static_cast<long long>(sizeof(Seq)) * S);
     l.costs = l.infos + up(16 * S);
-    l.bytes = l.costs + up(16 * S);
+    l.bytes = l.costs + up(32 * S);
     l.rows = 2 * S * h.gw + static_cast<long long>(l.ranges) * (kTileRows + kTileWaves * std::max(h.gw, kNarrowRows));
     return l;
 }

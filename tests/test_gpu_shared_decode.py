@@ -18,7 +18,8 @@ class Shared:
     """groups: of each, (tokens of whole shared blocks, the contexts of its sequences)."""
 
     def __init__(self, rng, groups, H, Hkv, D, dtype, cap=0.0, alibi=False, MB=None, scale=None, spare=3, qstd=3.0,
-                 lone=0, tight=False):
+                 lone=0, tight=False, min_saved=0):
+        self.min_saved = min_saved      # what is alike is shared, but where a test asks for the rule
         ctx = [c for _, cs in groups for c in cs]
         self.ctx = np.array(ctx + [int(rng.integers(0, 50)) for _ in range(lone)], np.int32)
         self.S, self.H, self.Hkv, self.D, self.dtype = len(self.ctx), H, Hkv, D, dtype
@@ -76,7 +77,7 @@ class Shared:
 
     def run_plan(self, stream=None):
         step.plan_shared(self.plan, self.plan.nbytes, self.sh, self.d["bt"], self.d["ctx"], self.d["off"], self.N,
-                         *self.sizes, stream=stream)
+                         *self.sizes, min_saved=self.min_saved, stream=stream)
 
     def run_decode(self, stream=None, bounded=True, out=None, **kw):
         p = step.ScoreParams(self.score["scale"], self.score["softcap"], alibi_slopes=self.d["slopes"])
@@ -183,6 +184,24 @@ def test_sequences_without_context(dev):
     assert (got[s.ctx <= 0] == 0).all()
 
 
+@pytest.mark.parametrize("min_saved", [-1, 0, 1, 400, 10 ** 6])
+@pytest.mark.parametrize("H,Hkv", [(16, 8), (4, 4)])
+def test_what_is_worth_sharing(dev, H, Hkv, min_saved):
+    """By the rule, by a number of blocks, never: the same outputs. Several tiles of a
+    group that begin with ranges, beside others that do not."""
+    rng = np.random.default_rng(H)
+    groups = [(1600, [1610 + i % 90 for i in range(70)]), (32, [40, 50]), (320, [333, 321, 400])]
+    Shared(rng, groups, H, Hkv, 64, "f16", min_saved=min_saved).run().check()
+
+
+@pytest.mark.parametrize("each", [33, 64, 100, 129])
+def test_aligned_tiles(dev, each):
+    """Groups of several tiles whose walks begin and end with ranges."""
+    rng = np.random.default_rng(each)
+    groups = [(9600, [9600 + i % 70 for i in range(each)]), (64, [70, 80, 90]), (4800, [4810] * (each + 1))]
+    Shared(rng, groups, 8, 2, 64, "bf16", lone=2).run().check()
+
+
 def test_nothing_shared_and_everything(dev):
     rng = np.random.default_rng(2)
     s = Shared(rng, [(0, [100, 200, 300])], 8, 2, 128, "f16").run()
@@ -230,14 +249,15 @@ def test_groups_that_leave_sequences_out(dev, off):
     s.check()
 
 
-def test_many_small_groups(dev):
-    """More groups than a window of the list's kernel holds."""
+@pytest.mark.parametrize("n", [300, 1100, 4200])
+def test_many_small_groups(dev, n):
+    """More sequences than the list's kernel has threads, and more groups than its window holds."""
     rng = np.random.default_rng(6)
-    groups = [(32, [33 + int(rng.integers(0, 20)) for _ in range(2)]) for _ in range(4200)]
+    groups = [(32, [33 + int(rng.integers(0, 20)) for _ in range(2)]) for _ in range(n)]
     s = Shared(rng, groups, 2, 1, 64, "f16")
     s.run()
     synchronize()
-    assert np.array_equal(s.sh.numpy(), np.full(4200, 2))
+    assert np.array_equal(s.sh.numpy(), np.full(n, 2))
     s.check()
 
 

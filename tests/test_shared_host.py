@@ -18,7 +18,7 @@ P = 1 << 32   # never dereferenced: validation fails first
 def _plan(**kw):
     a = dict(plan=P, plan_bytes=1 << 40, shared_blocks=2 * P, block_tables=3 * P, context_lens=4 * P,
              group_offsets=5 * P, num_groups=2, num_seqs=6, num_heads=8, num_kv_heads=2, head_dim=64,
-             block_size=16, max_num_blocks_per_seq=4)
+             block_size=16, max_num_blocks_per_seq=4, min_saved=-1)
     a.update(kw)
     return _lib.lib().swiftllm_hip_plan_shared(*a.values(), None)
 
