@@ -24,6 +24,7 @@ constexpr int kMostCounted = 1024;
 constexpr int kListThreads = 512;
 constexpr int kListWaves = kListThreads / 64;
 constexpr int kTries = 16;          // lengths of a range that are tried
+constexpr int kMostMulti = 512;
 constexpr int kWindow = 2048;       // groups whose minima are in LDS at a time
 
 struct PlanSharedArgs {
@@ -114,26 +115,30 @@ __global__ __launch_bounds__(kMatchThreads) void shared_match_kernel(const PlanS
     if (tid == 0) a.infos[s] = info;
 }
 
-// Exclusive prefixes of x and y over the workgroup's threads, and their totals.
-__device__ __forceinline__ void scan2(int x, int y, int& before_x, int& before_y, int& all_x, int& all_y, int (*part)[kListWaves]) {
+// Exclusive prefixes of the N numbers of x over the workgroup's threads, in x, and
+// their totals.
+template <int N>
+__device__ __forceinline__ void scan(int (&x)[N], int (&all)[N], int (*part)[kListWaves]) {
     const int lane = threadIdx.x & 63, w = threadIdx.x >> 6;
-    const int ix = wave_inclusive_scan(x), iy = wave_inclusive_scan(y);
+    int upto[N];
+#pragma unroll
+    for (int k = 0; k < N; ++k) upto[k] = wave_inclusive_scan(x[k]);
     __syncthreads();
     if (lane == 63) {
-        part[0][w] = ix;
-        part[1][w] = iy;
+#pragma unroll
+        for (int k = 0; k < N; ++k) part[k][w] = upto[k];
     }
     __syncthreads();
-    before_x = ix - x;
-    before_y = iy - y;
-    all_x = all_y = 0;
-    for (int i = 0; i < kListWaves; ++i) {
-        if (i < w) {
-            before_x += part[0][i];
-            before_y += part[1][i];
+#pragma unroll
+    for (int k = 0; k < N; ++k) {
+        x[k] = upto[k] - x[k];
+        all[k] = 0;
+#pragma unroll
+        for (int i = 0; i < kListWaves; ++i) {
+            const int p = part[k][i];
+            if (i < w) x[k] += p;
+            all[k] += p;
         }
-        all_x += part[0][i];
-        all_y += part[1][i];
     }
 }
 
@@ -141,12 +146,13 @@ __device__ __forceinline__ void scan2(int x, int y, int& before_x, int& before_y
 template <bool ONE>
 __global__ __launch_bounds__(kListThreads) void shared_list_kernel(const PlanSharedArgs a) {
     __shared__ int s_least[kWindow], s_full[kWindow], s_live[kWindow];
-    __shared__ int s_part[2][kListWaves];
+    __shared__ int s_part[6][kListWaves];
     __shared__ int s_pad[kTries];
+    __shared__ int s_multi[kMostMulti];               // costs of tiles that share with others
     __shared__ int s_tile[ONE ? kListThreads : 1];    // the walk of the tile that begins with a sequence
-    __shared__ int s_bad, s_saved;
+    __shared__ int s_bad, s_saved, s_tiles;
     const int tid = threadIdx.x;
-    if (tid == 0) s_bad = s_saved = 0;
+    if (tid == 0) s_bad = s_saved = s_tiles = 0;
     if (tid < kTries) s_pad[tid] = 0;
     struct Row {
         int4 info;       // w: blocks shared
@@ -235,35 +241,33 @@ __global__ __launch_bounds__(kListThreads) void shared_list_kernel(const PlanSha
         }
         return m;
     };
-    int sum = 0;
+    int sum[1] = {0}, sums[1];
     for (int s = tid; s < a.S; s += kListThreads) {
         const Mine m = walks_of(s);
-        sum += m.tile_cost + m.own_cost;
+        sum[0] += m.tile_cost + m.own_cost;
+        if (m.wide && m.group > a.per_tile) {
+            const int at = atomicAdd(&s_tiles, 1);
+            if (at < kMostMulti) s_multi[at] = m.tile_cost;
+        }
     }
-    int none, all, all_none, base;
-    scan2(sum, 0, base, none, all, all_none, s_part);
+    scan(sum, sums, s_part);
+    const int all = sums[0];
     // Where several tiles share blocks, each begins and ends with a range, so that
     // they come by the same blocks at the same time, in one L2. What that leaves empty
-    // makes the ranges longer, by a sixteenth of the first length and more.
+    // makes the ranges longer, by a sixteenth of the first length and more. (More than
+    // kMostMulti of them are many for any cut.)
+    const int tiles = s_tiles <= kMostMulti ? s_tiles : 0;
     const int wlen0 = max((all + kTileWaves * a.ranges - 1) / (kTileWaves * a.ranges), kLeastRange);
     auto try_len = [&](int k) { return kTileWaves * (wlen0 + k * max(wlen0 / 16, 1)); };
-    auto padded = [&](const Mine& m, int len) {
-        const bool aligned = m.wide && m.group > a.per_tile && m.tile_cost > 2 * len;
-        return aligned ? (m.tile_cost + len - 1) / len * len : 0;
-    };
-    for (int s = tid; s < a.S; s += kListThreads) {
-        const Mine m = walks_of(s);
-        if (m.wide && m.group > a.per_tile) {
-            for (int k = 0; k < kTries; ++k) {
-                const int n = padded(m, try_len(k));
-                if (n > 0) atomicAdd(&s_pad[k], n - m.tile_cost);
-            }
-        }
+    auto padded = [](int cost, int len) { return cost > 2 * len ? (cost + len - 1) / len * len : cost; };
+    for (int i = tid / kTries; i < tiles; i += kListThreads / kTries) {
+        const int k = tid % kTries;
+        atomicAdd(&s_pad[k], padded(s_multi[i], try_len(k)) - s_multi[i]);
     }
     __syncthreads();
     int len = try_len(0);
     bool align = false;
-    for (int k = kTries - 1; k >= 0; --k) {
+    for (int k = kTries - 1; k >= 0 && tiles > 0; --k) {
         if (static_cast<long long>(all) + s_pad[k] <= static_cast<long long>(a.ranges) * try_len(k)) {
             len = try_len(k);
             align = true;
@@ -272,7 +276,7 @@ __global__ __launch_bounds__(kListThreads) void shared_list_kernel(const PlanSha
     const int wlen = len / kTileWaves;
     // Aligned tiles first, other wide ones, then the narrow ones.
     auto cost_of = [&](const Mine& m, int& aligned, int& wide, int& narrow) {
-        const int n = align ? padded(m, len) : 0;
+        const int n = align && m.wide && m.group > a.per_tile && m.tile_cost > 2 * len ? padded(m.tile_cost, len) : 0;
         aligned = n;
         wide = m.wide && n == 0 ? m.tile_cost : 0;
         narrow = m.wide ? 0 : m.tile_cost;
@@ -282,16 +286,14 @@ __global__ __launch_bounds__(kListThreads) void shared_list_kernel(const PlanSha
     auto scan_row = [&](int s, const Mine& m) {
         int aligned, wide, narrow;
         cost_of(m, aligned, wide, narrow);
-        const int n[3] = {aligned > 0, wide > 0, (narrow > 0) + (m.own_cost > 0)};
-        const int c[3] = {aligned, wide, narrow + m.own_cost};
+        int x[6] = {aligned > 0, aligned, wide > 0, wide, (narrow > 0) + (m.own_cost > 0), narrow + m.own_cost}, sums[6];
+        scan(x, sums, s_part);
 #pragma unroll
-        for (int x = 0; x < 3; ++x) {
-            int bn, bc, an, ac;
-            scan2(n[x], c[x], bn, bc, an, ac, s_part);
-            at_walks[x] = walks[x] + bn;
-            at_costs[x] = costs[x] + bc;
-            walks[x] += an;
-            costs[x] += ac;
+        for (int k = 0; k < 3; ++k) {
+            at_walks[k] = walks[k] + x[2 * k];
+            at_costs[k] = costs[k] + x[2 * k + 1];
+            walks[k] += sums[2 * k];
+            costs[k] += sums[2 * k + 1];
         }
         if (!ONE && s < a.S) {
             a.costs[2 * static_cast<size_t>(s)] = int4{at_walks[0], at_costs[0], at_walks[1], at_costs[1]};
@@ -336,17 +338,17 @@ __global__ __launch_bounds__(kListThreads) void shared_list_kernel(const PlanSha
             const int n = pieces(own_at, m.own, wlen);
             if (joins || n > 1) own_rows = a.gw * n;
         }
-        int bx, ax;
-        scan2(tile_rows + own_rows, 0, bx, none, ax, all_none, s_part);
+        int x[1] = {tile_rows + own_rows}, sums[1];
+        scan(x, sums, s_part);
         if (s < a.S) {
-            const int f = rows + bx;
+            const int f = rows + x[0];
             // A walk, and the ranges of n that begin in it or in what it costs.
             auto put = [&](int v, const Walk& w, int from, int to, int n, Start* starts) {
                 a.walks[v] = w;
                 for (int r = (from + n - 1) / n; r * n < to; ++r) {
-                    Start& x = starts[r];
-                    x.walk = w;
-                    x.v = v;
+                    Start& begin = starts[r];
+                    begin.walk = w;
+                    begin.v = v;
                 }
             };
             if (m.count > 0) {
@@ -367,14 +369,14 @@ __global__ __launch_bounds__(kListThreads) void shared_list_kernel(const PlanSha
                 if (ONE) {
                     q.tile = s_tile[t];
                 } else {
-                    const int4 x = a.costs[2 * static_cast<size_t>(t)], y = a.costs[2 * static_cast<size_t>(t) + 1];
-                    const int n[3] = {x.x, x.z, y.x};
+                    const int4 p = a.costs[2 * static_cast<size_t>(t)], y = a.costs[2 * static_cast<size_t>(t) + 1];
+                    const int n[3] = {p.x, p.z, y.x};
                     q.tile = tile_walk(walks_of(t), n);
                 }
             }
             a.seqs[s] = q;
         }
-        rows += ax;
+        rows += sums[0];
     }
     if (tid == 0) *a.head = Head{kMagic, a.S, a.MB, a.H, a.Hkv, a.D, wide_walks, wide_walks + walks[2], wide_cost, total, len};
 }
