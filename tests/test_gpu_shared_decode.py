@@ -24,7 +24,7 @@ class Shared:
         self.ctx = np.array(ctx + [int(rng.integers(0, 50)) for _ in range(lone)], np.int32)
         self.S, self.H, self.Hkv, self.D, self.dtype = len(self.ctx), H, Hkv, D, dtype
         used = [-(-max(int(c), 0) // 16) for c in self.ctx]
-        # (tables of up to 96 blocks are taken whole where they are few: tight ones)
+        # (tables of up to 48 blocks are taken whole where they are few: tight ones)
         self.MB = max(used + [1 if tight else 97]) if MB is None else MB
         common = [p // 16 for p, _ in groups]
         need = sum(common) + sum(used) + 1
@@ -113,7 +113,7 @@ def whole(s):
     """Whether every sequence is read whole, by the launcher's rule."""
     G = s.H // s.Hkv
     parts = -(-min(G, 32) // 16)
-    return s.MB <= 96 and s.S * s.Hkv * -(-G // 32) * parts * s.MB * 64 * s.D <= 24e6
+    return s.MB <= 48 and s.S * s.Hkv * -(-G // 32) * parts * s.MB * 64 * s.D <= 64e6
 
 
 HEADS = [(8, 8, 64), (32, 8, 128), (16, 2, 128), (6, 2, 64), (5, 1, 128), (1, 1, 64), (40, 1, 64), (96, 2, 128)]
