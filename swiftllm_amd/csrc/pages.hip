@@ -20,11 +20,18 @@
 // afterwards, id - L of them before id; below T the free ones but for the M lowest.
 //
 // Bound: latency. A step of 16 requests of 8 beams in 65536 blocks moves 0.9 MB
-// (0.2 us), 1024 beams in 524288 blocks 12 MB. Three launches each, whose ends are
-// the only order between workgroups: what moves references, what counts the free
-// blocks of every 4096 ids (and keeps them as bits), what lists them. Where a row
-// and its parent have the same block in the same place, as in a prompt that both
+// (0.2 us), 1024 beams in 524288 blocks 12 MB (2.4 us). Three launches each, whose
+// ends are the only order between workgroups: fork_pages moves references, counts the
+// free blocks of every 4096 ids (and keeps them as bits), lists them: 3.6 + 4.6 + 3.7
+// us and 5.9 + 5.7 + 5.2 us at those sizes, each a chain of dependent reads.
+// compact_pages counts the blocks in use, pairs them, renames: 3.2 + 4.1 + 4.2 us for
+// 64 rows over 65536 blocks, 3.7 + 4.7 + 8.8 for 512 rows of 1000 blocks over 524288
+// (18 MB, 3.6 us). A block's place among those in use is a word of bits and the count
+// before it; kept for every block in an array of its own, the last took 10.9. Where a
+// row and its parent have the same block in the same place, as in a prompt that both
 // share, nothing is counted: a search's reordering touches few counters.
+// (Counting all ids in the pairing workgroups, a launch less, took 8.9 us at 65536
+// blocks, the two launches 7.3.)
 
 #include <algorithm>
 
@@ -39,6 +46,8 @@ constexpr int kScanWaves = kScanThreads / 64;
 constexpr int kIds = 4096;               // ids of a workgroup: 64 words of 64 bits
 constexpr int kWords = kIds / 64;
 constexpr int kEach = kIds / kScanThreads;
+constexpr int kSmallTables = 4096;       // entries of all rows, for one workgroup
+constexpr int kRowHalves = 2;            // rows of a workgroup that renames entries
 
 struct PagesArgs {
     const int* tables;
@@ -63,7 +72,8 @@ struct PagesArgs {
     int* copies;           // [S]: rows that take a copy, in order
     int* from;             // [NB / 2]: compact: the blocks that move, highest first,
     int* to;               //   the free ones, lowest first,
-    int* order;            // [NB]: and a moving block's place among them
+    int* starts;           // [groups * kWords]: blocks in use before a word of ids
+    int* found;            // [3]: compact: moves, blocks in use, the lowest that moves
     int S;
     int MB;
     int NB;
@@ -94,18 +104,20 @@ __device__ __forceinline__ int block_total(int x, int* part) {
     return all;
 }
 
-__global__ __launch_bounds__(kRowThreads) void fork_rows_kernel(const PagesArgs a) {
-    __shared__ int s_part[kRowThreads / 64];
-    const int i = blockIdx.x, tid = threadIdx.x;
-    if (a.taken != nullptr) {
-        // Blocks that a plan took: of nobody until now.
-        const int n = min(min(max(a.taken[0], 0), max(a.num_free[0], 0)), a.NB);
-        for (int k = i * kRowThreads + tid; k < n; k += gridDim.x * kRowThreads) {
-            const int b = a.free_blocks[k];
-            if (in_pool(b, a.NB)) atomicAdd(a.refs_out + b, 1);
-        }
+// Blocks that a plan took: of nobody until now.
+__device__ __forceinline__ void fork_taken(const PagesArgs& a, int at, int step) {
+    if (a.taken == nullptr) return;
+    const int n = min(min(max(a.taken[0], 0), max(a.num_free[0], 0)), a.NB);
+    for (int k = at; k < n; k += step) {
+        const int b = a.free_blocks[k];
+        if (in_pool(b, a.NB)) atomicAdd(a.refs_out + b, 1);
     }
-    if (i >= a.S) return;
+}
+
+// Row i by THREADS threads, of which this is t: its table, the references that
+// change, its place among its siblings. part: of a workgroup, THREADS / 64.
+template <int THREADS>
+__device__ __forceinline__ void fork_row(const PagesArgs& a, int i, int t, int* part) {
     const int p = parent_of(a, i);
     const int was = blocks_of(a.ctx[i], a.MB);
     const int ctx = p < 0 ? 0 : max(a.ctx[p], 0);
@@ -113,7 +125,7 @@ __global__ __launch_bounds__(kRowThreads) void fork_rows_kernel(const PagesArgs 
     const int* const old = a.tables + static_cast<size_t>(i) * a.MB;
     const int* const row = a.tables + static_cast<size_t>(max(p, 0)) * a.MB;
     int* const out = a.tables_out + static_cast<size_t>(i) * a.MB;
-    for (int j = tid; j < max(was, is); j += kRowThreads) {
+    for (int j = t; j < max(was, is); j += THREADS) {
         const int x = j < was ? old[j] : -1;
         const int y = j < is ? row[j] : -1;
         if (j < is) out[j] = y;
@@ -124,14 +136,24 @@ __global__ __launch_bounds__(kRowThreads) void fork_rows_kernel(const PagesArgs 
     }
     int n = 0;
     if (p >= 0) {
-        for (int k = tid; k < i; k += kRowThreads) n += a.parents[k] == p;
+        for (int k = t; k < i; k += THREADS) n += a.parents[k] == p;
     }
-    n = block_total<kRowThreads / 64>(n, s_part);
-    if (tid == 0) {
+    if constexpr (THREADS == 64) {
+        n = wave_total(n);
+    } else {
+        n = block_total<THREADS / 64>(n, part);
+    }
+    if (t == 0) {
         a.rank[i] = n;
         a.ctx_out[i] = ctx;
         if (a.new_lens != nullptr) a.new_lens[i] = p >= 0;
     }
+}
+
+__global__ __launch_bounds__(kRowThreads) void fork_rows_kernel(const PagesArgs a) {
+    __shared__ int s_part[kRowThreads / 64];
+    fork_taken(a, blockIdx.x * kRowThreads + threadIdx.x, gridDim.x * kRowThreads);
+    if (static_cast<int>(blockIdx.x) < a.S) fork_row<kRowThreads>(a, blockIdx.x, threadIdx.x, s_part);
 }
 
 // Bit b of word w of the pool: a block that nothing refers to (in use: LIVE).
@@ -164,14 +186,9 @@ __device__ __forceinline__ int open_entry(const PagesArgs& a, int ctx) {
     return (ctx & (kBlockTokens - 1)) != 0 && j < a.MB ? j : -1;
 }
 
-__global__ __launch_bounds__(kScanThreads) void fork_scan_kernel(const PagesArgs a) {
-    __shared__ int s_part[kScanWaves];
+// The rows that take a copy, in order, four rows a thread at a time. part: kScanWaves.
+__device__ __forceinline__ void fork_copies(const PagesArgs& a, int* part) {
     const int tid = threadIdx.x;
-    if (static_cast<int>(blockIdx.x) < a.groups) {
-        scan_ids<false>(a, a.refs_out, blockIdx.x, s_part);
-        return;
-    }
-    // The rows that take a copy, in order, four rows a thread at a time.
     int before = 0;
     for (int s0 = 0; s0 < a.S; s0 += 4 * kScanThreads) {
         bool copy[4];
@@ -188,13 +205,13 @@ __global__ __launch_bounds__(kScanThreads) void fork_scan_kernel(const PagesArgs
             n += copy[k];
         }
         const int incl = wave_inclusive_scan(n);
-        if ((tid & 63) == 63) s_part[tid >> 6] = incl;
+        if ((tid & 63) == 63) part[tid >> 6] = incl;
         __syncthreads();
         int at = before + incl - n;
 #pragma unroll
         for (int w = 0; w < kScanWaves; ++w) {
-            if (w < (tid >> 6)) at += s_part[w];
-            before += s_part[w];
+            if (w < (tid >> 6)) at += part[w];
+            before += part[w];
         }
         __syncthreads();
 #pragma unroll
@@ -203,6 +220,15 @@ __global__ __launch_bounds__(kScanThreads) void fork_scan_kernel(const PagesArgs
         }
     }
     if (tid == 0) a.num_copies[0] = before;
+}
+
+__global__ __launch_bounds__(kScanThreads) void fork_scan_kernel(const PagesArgs a) {
+    __shared__ int s_part[kScanWaves];
+    if (static_cast<int>(blockIdx.x) < a.groups) {
+        scan_ids<false>(a, a.refs_out, blockIdx.x, s_part);
+    } else {
+        fork_copies(a, s_part);
+    }
 }
 
 // What lies before this workgroup's ids, and in all: set bits. part: 2 kScanWaves.
@@ -217,14 +243,23 @@ __device__ __forceinline__ void sums_of(const PagesArgs& a, int group, int* part
     all = block_total<kScanWaves>(y, part + kScanWaves);
 }
 
+// Set bits before each word of a group, of which lane k has word k, `before` of them
+// before the group.
+__device__ __forceinline__ int starts_of(unsigned long long mine, int before) {
+    const int n = __popcll(mine);
+    return before + wave_inclusive_scan(n) - n;
+}
+
+__device__ __forceinline__ unsigned long long word_of(const PagesArgs& a, int group) {
+    return a.bits[static_cast<size_t>(group) * kWords + (threadIdx.x & 63)];
+}
+
 // For each of the thread's ids: take(id, bit, set bits before it in the pool).
+// mine, start: of lane's word, as above.
 template <typename F>
-__device__ __forceinline__ void each_id(const PagesArgs& a, int group, int before, F take) {
+__device__ __forceinline__ void each_id(const PagesArgs& a, int group, unsigned long long mine, int start, F take) {
     const int lane = threadIdx.x & 63;
     const int w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-    const unsigned long long mine = a.bits[static_cast<size_t>(group) * kWords + lane];
-    const int n = __popcll(mine);
-    const int upto = wave_inclusive_scan(n) - n;
 #pragma unroll
     for (int k = 0; k < kEach; ++k) {
         const int word = w * kEach + k;
@@ -234,20 +269,22 @@ __device__ __forceinline__ void each_id(const PagesArgs& a, int group, int befor
         const int id = group * kIds + word * 64 + lane;
         if (id < a.NB) {
             take(id, ((m >> lane) & 1ull) != 0,
-                 before + __builtin_amdgcn_readlane(upto, word) + __popcll(m & ((1ull << lane) - 1ull)));
+                 __builtin_amdgcn_readlane(start, word) + __popcll(m & ((1ull << lane) - 1ull)));
         }
     }
 }
 
-__global__ __launch_bounds__(kScanThreads) void fork_list_kernel(const PagesArgs a) {
-    __shared__ int s_part[2 * kScanWaves];
+// The copies and free blocks of a group's ids, one of `groups` that share the
+// pairs behind the last. part: 2 kScanWaves.
+__device__ __forceinline__ void fork_list(const PagesArgs& a, int group, int groups, int* part) {
     const int tid = threadIdx.x;
     int before, all;
-    sums_of(a, blockIdx.x, s_part, before, all);
+    sums_of(a, group, part, before, all);
     const int wanted = a.num_copies[0];
     const int got = min(wanted, all);
     auto open_of = [&](int i) { return a.tables_out + static_cast<size_t>(i) * a.MB + (a.ctx_out[i] >> kBlockShift); };
-    each_id(a, blockIdx.x, before, [&](int id, bool free, int k) {
+    const unsigned long long mine = word_of(a, group);
+    each_id(a, group, mine, starts_of(mine, before), [&](int id, bool free, int k) {
         if (!free) return;
         if (k >= got) {
             a.free_blocks[k - got] = id;
@@ -261,7 +298,7 @@ __global__ __launch_bounds__(kScanThreads) void fork_list_kernel(const PagesArgs
         a.refs_out[id] = 1;
         atomicAdd(a.refs_out + src, -1);
     });
-    for (int k = got + blockIdx.x * kScanThreads + tid; k < a.S; k += gridDim.x * kScanThreads) {
+    for (int k = got + group * kScanThreads + tid; k < a.S; k += groups * kScanThreads) {
         a.pairs[2 * static_cast<size_t>(k)] = -1;
         a.pairs[2 * static_cast<size_t>(k) + 1] = -1;
         if (k < wanted) {
@@ -272,11 +309,33 @@ __global__ __launch_bounds__(kScanThreads) void fork_list_kernel(const PagesArgs
             if (a.new_lens != nullptr) a.new_lens[i] = 0;
         }
     }
-    if (blockIdx.x == 0 && tid == 0) {
+    if (group == 0 && tid == 0) {
         a.num_free[0] = all - got;
         a.counts[0] = got;
         a.counts[1] = wanted - got;
     }
+}
+
+__global__ __launch_bounds__(kScanThreads) void fork_list_kernel(const PagesArgs a) {
+    __shared__ int s_part[2 * kScanWaves];
+    fork_list(a, blockIdx.x, gridDim.x, s_part);
+}
+
+// All of it by one workgroup, a wave a row, where the pool is one group of ids and
+// the tables are small. (us, three launches and one: 4 rows over 4096 blocks 9.9 and
+// 7.2, 32 rows of 34 blocks 9.7 and 8.4; 4 rows over 8192 10.4 and 9.6, 32 rows of 65
+// blocks over 8192 12.0 and 12.2.)
+__global__ __launch_bounds__(kScanThreads) void fork_small_kernel(const PagesArgs a) {
+    __shared__ int s_part[2 * kScanWaves];
+    const int tid = threadIdx.x;
+    fork_taken(a, tid, kScanThreads);
+    for (int i = tid >> 6; i < a.S; i += kScanWaves) fork_row<64>(a, i, tid & 63, nullptr);
+    __syncthreads();
+    scan_ids<false>(a, a.refs_out, 0, s_part);
+    __syncthreads();
+    fork_copies(a, s_part);
+    __syncthreads();
+    fork_list(a, 0, 1, s_part);
 }
 
 __global__ __launch_bounds__(kScanThreads) void compact_scan_kernel(const PagesArgs a) {
@@ -284,47 +343,50 @@ __global__ __launch_bounds__(kScanThreads) void compact_scan_kernel(const PagesA
     scan_ids<true>(a, a.refs, blockIdx.x, s_part);
 }
 
-// How many blocks move, of `all` in use: the free ones among the first `all` ids,
-// at most the pairs' room. part: kScanWaves.
-__device__ __forceinline__ int moves_of(const PagesArgs& a, int all, int* part) {
-    const int group = all / kIds;
-    int x = 0;
-    for (int k = threadIdx.x; k < group; k += kScanThreads) x += a.sums[k];
-    if (group < a.groups && threadIdx.x < kWords) {
-        const int n = min(max(all - group * kIds - static_cast<int>(threadIdx.x) * 64, 0), 64);
-        const unsigned long long m = a.bits[static_cast<size_t>(group) * kWords + threadIdx.x];
-        x += __popcll(n == 64 ? m : m & ((1ull << n) - 1ull));
-    }
-    return min(all - block_total<kScanWaves>(x, part), a.rooms);
-}
-
+// `live` of the first `all` ids are in use, of `all` in the pool: the others move, at
+// most the pairs' room.
 __global__ __launch_bounds__(kScanThreads) void compact_pairs_kernel(const PagesArgs a) {
     __shared__ int s_part[3 * kScanWaves];
+    const int tid = threadIdx.x;
     int before, all;
     sums_of(a, blockIdx.x, s_part, before, all);
-    const int moves = moves_of(a, all, s_part + 2 * kScanWaves);
-    each_id(a, blockIdx.x, before, [&](int id, bool live, int k) {
-        const int at = live ? all - 1 - k : id - k;
+    const int group = all / kIds;
+    int live = 0;      // of the first `all` ids
+    for (int k = tid; k < group; k += kScanThreads) live += a.sums[k];
+    if (group < a.groups && tid < kWords) {
+        const int n = min(max(all - group * kIds - tid * 64, 0), 64);
+        const unsigned long long m = a.bits[static_cast<size_t>(group) * kWords + tid];
+        live += __popcll(n == 64 ? m : m & ((1ull << n) - 1ull));
+    }
+    live = block_total<kScanWaves>(live, s_part + 2 * kScanWaves);
+    const int moves = min(all - live, a.rooms);
+    if (blockIdx.x == 0 && tid == 0) {
+        a.found[0] = moves;
+        a.found[1] = all;
+        if (moves == 0) a.found[2] = a.NB;
+    }
+    const unsigned long long mine = word_of(a, blockIdx.x);
+    const int start = starts_of(mine, before);
+    if (tid < kWords) a.starts[static_cast<size_t>(blockIdx.x) * kWords + tid] = start;
+    each_id(a, blockIdx.x, mine, start, [&](int id, bool used, int k) {
+        const int at = used ? all - 1 - k : id - k;
         if (at >= moves) return;
-        (live ? a.from : a.to)[at] = id;
-        if (live) a.order[id] = at;
+        (used ? a.from : a.to)[at] = id;
+        if (used && at == moves - 1) a.found[2] = id;
     });
 }
 
 __global__ __launch_bounds__(kScanThreads) void compact_apply_kernel(const PagesArgs a) {
-    __shared__ int s_part[3 * kScanWaves];
     const int tid = threadIdx.x;
-    const int group = min(static_cast<int>(blockIdx.x), a.groups - 1);
-    int before, all;
-    sums_of(a, group, s_part, before, all);
-    const int moves = moves_of(a, all, s_part + 2 * kScanWaves);
-    const int lowest = moves > 0 ? a.from[moves - 1] : a.NB;   // of those that move
+    const int moves = a.found[0], all = a.found[1], lowest = a.found[2];
     if (static_cast<int>(blockIdx.x) < a.groups) {
-        each_id(a, group, before, [&](int id, bool live, int k) {
+        const int group = blockIdx.x;
+        const int start = a.starts[static_cast<size_t>(group) * kWords + (tid & 63)];
+        each_id(a, group, word_of(a, group), start, [&](int id, bool live, int k) {
             const bool goes = live && id >= lowest;
             const int r = id - k;                              // free ones before this
             const bool comes = !live && r < moves;
-            a.new_ids[id] = goes ? a.to[a.order[id]] : id;
+            a.new_ids[id] = goes ? a.to[all - 1 - k] : id;
             a.refs_out[id] = goes ? 0 : a.refs[comes ? a.from[r] : id];
             if (id >= lowest) {
                 a.free_blocks[id - all] = id;
@@ -332,31 +394,37 @@ __global__ __launch_bounds__(kScanThreads) void compact_apply_kernel(const Pages
                 a.free_blocks[r - moves] = id;
             }
         });
-        for (int k = blockIdx.x * kScanThreads + tid; k < a.rooms; k += a.groups * kScanThreads) {
+        for (int k = group * kScanThreads + tid; k < a.rooms; k += a.groups * kScanThreads) {
             a.pairs[2 * static_cast<size_t>(k)] = k < moves ? a.from[k] : -1;
             a.pairs[2 * static_cast<size_t>(k) + 1] = k < moves ? a.to[k] : -1;
         }
-        if (blockIdx.x == 0 && tid == 0) {
+        if (group == 0 && tid == 0) {
             a.num_free[0] = a.NB - all;
             a.counts[0] = moves;
             a.counts[1] = all;
         }
         return;
     }
-    const int i = blockIdx.x - a.groups;
+    constexpr int kHalf = kScanThreads / kRowHalves;
+    const int i = (blockIdx.x - a.groups) * kRowHalves + tid / kHalf;
+    if (i >= a.S) return;
     const int used = blocks_of(a.ctx[i], a.MB);
     const size_t at = static_cast<size_t>(i) * a.MB;
-    for (int j = tid; j < used; j += kScanThreads) {
+    for (int j = tid % kHalf; j < used; j += kHalf) {
         const int b = a.tables[at + j];
         int to = b;
-        if (b >= lowest && b < a.NB && ((a.bits[b >> 6] >> (b & 63)) & 1ull) != 0) to = a.to[a.order[b]];
+        if (b >= lowest && b < a.NB) {
+            const unsigned long long m = a.bits[b >> 6], bit = 1ull << (b & 63);
+            const int k = a.starts[b >> 6] + __popcll(m & (bit - 1ull));
+            if ((m & bit) != 0) to = a.to[all - 1 - k];
+        }
         a.tables_out[at + j] = to;
     }
 }
 
 // Offsets of the workspace.
 struct Space {
-    size_t sums, copies_n, bits, rank, copies, from, to, order, bytes;
+    size_t sums, copies_n, found, bits, rank, copies, from, to, starts, bytes;
 };
 
 Space space_of(long long S, long long NB) {
@@ -365,13 +433,14 @@ Space space_of(long long S, long long NB) {
     Space s;
     s.sums = 0;
     s.copies_n = s.sums + up(4 * groups);
-    s.bits = s.copies_n + 256;
+    s.found = s.copies_n + 256;
+    s.bits = s.found + 256;
     s.rank = s.bits + up(8 * groups * kWords);
     s.copies = s.rank + up(4 * S);
     s.from = s.copies + up(4 * S);
     s.to = s.from + up(4 * (NB / 2));
-    s.order = s.to + up(4 * (NB / 2));
-    s.bytes = s.order + up(4 * NB);
+    s.starts = s.to + up(4 * (NB / 2));
+    s.bytes = s.starts + up(4 * groups * kWords);
     return s;
 }
 
@@ -396,12 +465,13 @@ void set_space(PagesArgs& a, void* workspace, const Space& s) {
     char* const ws = static_cast<char*>(workspace);
     a.sums = reinterpret_cast<int*>(ws + s.sums);
     a.num_copies = reinterpret_cast<int*>(ws + s.copies_n);
+    a.found = reinterpret_cast<int*>(ws + s.found);
     a.bits = reinterpret_cast<unsigned long long*>(ws + s.bits);
     a.rank = reinterpret_cast<int*>(ws + s.rank);
     a.copies = reinterpret_cast<int*>(ws + s.copies);
     a.from = reinterpret_cast<int*>(ws + s.from);
     a.to = reinterpret_cast<int*>(ws + s.to);
-    a.order = reinterpret_cast<int*>(ws + s.order);
+    a.starts = reinterpret_cast<int*>(ws + s.starts);
 }
 
 // Whether one of the first `outputs` spans shares bytes with another span.
@@ -479,6 +549,9 @@ int swiftllm_hip_fork_pages(int32_t* block_tables_out, int32_t* context_lens_out
     a.groups = (NB + kIds - 1) / kIds;
     a.rooms = S;
     set_space(a, workspace, space);
+    if (a.groups == 1 && static_cast<long long>(S) * MB <= kSmallTables) {
+        return launched(launch(fork_small_kernel, dim3(1), dim3(kScanThreads), 0, stream, a), who);
+    }
     rc = launched(launch(fork_rows_kernel, dim3(std::max(S, 1)), dim3(kRowThreads), 0, stream, a), who);
     if (rc != SWIFTLLM_OK) return rc;
     rc = launched(launch(fork_scan_kernel, dim3(a.groups + 1), dim3(kScanThreads), 0, stream, a), who);
@@ -542,7 +615,8 @@ int swiftllm_hip_compact_pages(int32_t* block_tables_out, int32_t* ref_counts_ou
     if (rc != SWIFTLLM_OK) return rc;
     rc = launched(launch(compact_pairs_kernel, dim3(a.groups), dim3(kScanThreads), 0, stream, a), who);
     if (rc != SWIFTLLM_OK) return rc;
-    return launched(launch(compact_apply_kernel, dim3(a.groups + S), dim3(kScanThreads), 0, stream, a), who);
+    const int rows = (S + kRowHalves - 1) / kRowHalves;
+    return launched(launch(compact_apply_kernel, dim3(a.groups + rows), dim3(kScanThreads), 0, stream, a), who);
 }
 
 }  // extern "C"

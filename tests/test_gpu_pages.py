@@ -253,3 +253,17 @@ def test_fork_in_a_graph(dev):
         for k in ("tables", "other", "ctx", "refs", "free", "n"):
             assert np.array_equal(d[k].numpy(), h[k]), k
         assert np.array_equal(p.pairs.numpy(), want[5]) and np.array_equal(p.counts.numpy(), want[6])
+
+
+@pytest.mark.parametrize("NB", [4096, 4097])
+@pytest.mark.parametrize("S,MB", [(1, 4096), (1, 4097), (64, 64), (65, 64), (4096, 1)])
+def test_forks_of_small_pools(dev, S, MB, NB):
+    """At the sizes where one workgroup does all of it and where it does not."""
+    rng = np.random.default_rng(S + MB)
+    free = NB - 200
+    lens = rng.integers(0, 16 * min(MB, max(free // S, 1)) + 1, S)
+    if S > 1000:
+        lens[rng.permutation(S)[:S - 3500]] = 0
+    p = Pool(S, MB, NB).lone(rng, lens)
+    for _ in range(4):
+        p.fork(rng.integers(-1, S, S).astype(np.int32))
