@@ -23,7 +23,11 @@
 // lse by 2e-8 of the distance from the maximum.
 //
 // Bound: HBM for 32-bit logits, for 16-bit ones as much the vector operations, nine
-// per logit of which the exponential is four.
+// per logit of which the exponential is four. 64 x 4 rows of 128000 bfloat16 logits:
+// 16.4 us, 4.0 TB/s; 9 x 32 of 100003 in 32 bits 28 us, 4.1 TB/s; 4 of 32000 5.2 us,
+// as long as a chunk's way through. The second kernel is latency, of one workgroup a
+// request: 4.8 us for 16 lists of 8 candidates, 6.5 for 64, 14 for 416 lists of 64 or
+// more (20 with every pass over the entries in memory, their scores found again).
 
 #include <algorithm>
 #include <cmath>
@@ -42,6 +46,9 @@ constexpr int kGroup = 8, kGroups = kEach / kGroup;
 static_assert(kGroups == 4 && kEach == 32, "maxima, and a word of bits");
 constexpr int kRoom = 128;                 // entries of a chunk's list
 constexpr int kMostCandidates = 64;
+// Up to so many, a chunk's line is the C-th largest of 128 maxima, not 256 (32 of 128
+// lets 37 values pass, 64 would let 89): 64 x 4 bfloat16 rows 16.4 us, not 17.6.
+constexpr int kFewCandidates = 32;
 constexpr int kPickLists = 1024;           // lists that reach the first line
 constexpr int kPickRoom = 1024;            // candidates that are ranked
 constexpr int kFewEnough = 160;            // by one line
@@ -191,7 +198,7 @@ __global__ __launch_bounds__(kThreads) void beam_chunk_kernel(const SelectArgs a
     const int off = static_cast<int>((reinterpret_cast<uintptr_t>(base) & 15u) / kSize);
     const int first = chunk * kChunk - off;
     // All loads are on their way before the first is waited for. (Unpacked each in
-    // its own branch, 64 x 4 rows of 128000 bfloat16 logits took 30 us, not @@.)
+    // its own branch, 64 x 4 rows of 128000 bfloat16 logits took 30 us, not 26.)
     u4 raw[NV];
 #pragma unroll
     for (int k = 0; k < NV; ++k) {
@@ -257,9 +264,16 @@ __global__ __launch_bounds__(kThreads) void beam_chunk_kernel(const SelectArgs a
     }
     __syncthreads();
     const u4 ks = *reinterpret_cast<const u4*>(s_key + 4 * lane);
-    const unsigned keys[4] = {ks[0], ks[1], ks[2], ks[3]};
+    unsigned found;
+    if (a.C <= kFewCandidates) {
+        const unsigned keys[2] = {std::max(ks[0], ks[1]), std::max(ks[2], ks[3])};
+        found = nth_largest<key_bits<T>>(keys, a.C);
+    } else {
+        const unsigned keys[4] = {ks[0], ks[1], ks[2], ks[3]};
+        found = nth_largest<key_bits<T>>(keys, a.C);
+    }
     // What is banned is no candidate. (Some keys are no number's.)
-    const float line = fmaxf(of_key(nth_largest<key_bits<T>>(keys, a.C)), -3.402823466e38f);
+    const float line = fmaxf(of_key(found), -3.402823466e38f);
     unsigned mine = 0;     // which of the thread's values reach it
 #pragma unroll
     for (int g = 0; g < kGroups; ++g) {
@@ -325,12 +339,6 @@ __device__ __forceinline__ bool before(const Cand& p, const Cand& q) {
     return p.token < q.token;
 }
 
-__device__ __forceinline__ double wave_sum64(double x) {
-#pragma unroll
-    for (int d = 1; d < 64; d <<= 1) x += __shfl_xor(x, d);
-    return x;
-}
-
 // SMALL: every 16 threads have a list of their own, whose entries are on their way
 // before anything else is known. Otherwise the lists' maxima give a first line, and
 // only lists that reach it are read.
@@ -346,68 +354,97 @@ __global__ __launch_bounds__(THREADS) void beam_pick_kernel(const SelectArgs a) 
     __shared__ Cand s_order[kMostCandidates];
     __shared__ int s_list[SMALL ? 1 : kPickLists];
     __shared__ int s_fill, s_lists;
-    __shared__ float s_line;
+    __shared__ int s_reach[2][16];
     const int tid = threadIdx.x, lane = tid & 63;
     const int w = __builtin_amdgcn_readfirstlane(tid >> 6);
     const int r = blockIdx.x;
     const int lists = a.W * a.chunks;
     const size_t slot0 = static_cast<size_t>(r) * lists;
     if (tid == 0) s_fill = s_lists = 0;
-    // (entries past a list's fill are read and not used)
-    constexpr int kKept = kRoom / 16, kFirst = 2;
-    Entry kept[SMALL ? kKept : 1];
-    int fill = 0;
+    // A thread's entries, of HELD lists. (Those past a list's fill are read and not used.)
+    constexpr int kKept = kRoom / 16, kFirst = SMALL ? 2 : kKept / 2, HELD = SMALL ? 1 : 2;
+    Entry kept[HELD][kKept];
+    int fill[HELD] = {}, beam[HELD] = {};
+    auto list_of = [&](int i) { return a.lists + (slot0 + i) * kRoom + (tid & 15); };
     if (SMALL && tid >> 4 < lists) {
-        fill = a.fill[slot0 + (tid >> 4)];
+        fill[0] = a.fill[slot0 + (tid >> 4)];
+        beam[0] = (tid >> 4) / a.chunks;
 #pragma unroll
-        for (int k = 0; k < kFirst; ++k) kept[k] = a.lists[(slot0 + (tid >> 4)) * kRoom + (tid & 15) + 16 * k];
+        for (int k = 0; k < kFirst; ++k) kept[0][k] = list_of(tid >> 4)[16 * k];
     }
-    for (int b = w; b < a.W; b += WAVES) {
-        const size_t row = static_cast<size_t>(r) * a.W + b;
+    // The rows' sums, by as many threads as there are chunks.
+    const int span = a.chunks <= 16 ? 16 : 64, at = tid & (span - 1);
+    for (int b0 = 0; b0 < a.W; b0 += THREADS / span) {
+        const int b = b0 + tid / span;
+        const bool real = b < a.W;
+        const size_t row = static_cast<size_t>(r) * a.W + (real ? b : 0);
         const float score = a.scores[row];
         const float2* const sums = a.sums + row * a.chunks;
-        const float2 mine = lane < a.chunks ? sums[lane] : float2{-INFINITY, 0.0f};
-        double base = -INFINITY;
-        float top = 0.0f;
-        if (score > -INFINITY) {
-            top = mine.x;
-            for (int c = lane + 64; c < a.chunks; c += 64) top = fmaxf(top, sums[c].x);
-            top = wave_max(top);
-            double S = weighed(mine.y, mine.x, top);
-            for (int c = lane + 64; c < a.chunks; c += 64) S += weighed(sums[c].y, sums[c].x, top);
-            base = score - log(wave_sum64(S));
+        const float2 mine = at < a.chunks ? sums[at] : float2{-INFINITY, 0.0f};
+        // (a beam without a score has no sums)
+        const bool scored = real && score > -INFINITY;
+        float top = scored ? mine.x : -INFINITY;
+        if (scored) {
+            for (int c = at + 64; c < a.chunks; c += 64) top = fmaxf(top, sums[c].x);
         }
-        if (lane == 0) {
-            s_base[b] = base;
-            s_top[b] = top;
+        for (int d = 1; d < span; d <<= 1) top = fmaxf(top, __shfl_xor(top, d));
+        double S = scored ? weighed(mine.y, mine.x, top) : 0.0f;
+        if (scored) {
+            for (int c = at + 64; c < a.chunks; c += 64) S += weighed(sums[c].y, sums[c].x, top);
+        }
+        for (int d = 1; d < span; d <<= 1) S += __shfl_xor(S, d);
+        if (at == 0 && real) {
+            s_base[b] = scored ? score - log(S) : -INFINITY;
+            s_top[b] = scored ? top : 0.0f;
         }
     }
-    if constexpr (SMALL) {
+    auto rest_of = [&](int h, int i) {
 #pragma unroll
         for (int k = kFirst; k < kKept; ++k) {
-            if (16 * k < fill) kept[k] = a.lists[(slot0 + (tid >> 4)) * kRoom + (tid & 15) + 16 * k];
+            if (16 * k < fill[h]) kept[h][k] = list_of(i)[16 * k];
         }
-    }
+    };
+    if (SMALL) rest_of(0, tid >> 4);
     __syncthreads();
     // (beside an infinite logit only others of its kind have a share)
     auto score_of = [&](int b, float x) { return x == s_top[b] ? s_base[b] : s_base[b] + (x - static_cast<double>(s_top[b])); };
-    // A line that C candidates reach, of every two threads' maxima.
+    // A line that C candidates reach, of every two threads' maxima. Sixteen waves try
+    // as many values of the next four bits, each over all keys.
     auto find_line = [&](float most) {
         most = fmaxf(most, __shfl_xor(most, 1));
         if ((tid & 1) == 0) s_key[tid >> 1] = key_of(most);
         __syncthreads();
-        if (w == 0) {
-            unsigned keys[KEYS];
+        unsigned keys[KEYS];
+        unsigned t = 0;
+        if (WAVES == 16 || w == 0) {
 #pragma unroll
             for (int k = 0; k < KEYS; ++k) keys[k] = s_key[64 * k + lane];
-            const unsigned t = nth_largest<20>(keys, a.C);
-            if (lane == 0) s_line = fmaxf(of_key(t), -3.402823466e38f);
         }
-        __syncthreads();
-        return s_line;
+        if constexpr (WAVES == 16) {
+#pragma unroll
+            for (int k = 0; k < 5; ++k) {
+                const unsigned c = t | static_cast<unsigned>(w) << (28 - 4 * k);
+                int reach = 0;
+#pragma unroll
+                for (int i = 0; i < KEYS; ++i) reach += __popcll(__ballot(keys[i] >= c));
+                if (lane == 0) s_reach[k & 1][w] = reach;
+                __syncthreads();
+                const unsigned long long on = __ballot(lane < 16 && s_reach[k & 1][lane & 15] >= a.C);
+                t |= static_cast<unsigned>(__popcll(on) - 1) << (28 - 4 * k);
+            }
+        } else {
+            if (w == 0) {
+                t = nth_largest<20>(keys, a.C);
+                if (lane == 0) s_reach[0][0] = static_cast<int>(t);
+            }
+            __syncthreads();
+            t = static_cast<unsigned>(s_reach[0][0]);
+        }
+        return fmaxf(of_key(t), -3.402823466e38f);
     };
     int use = lists;
     bool some = false;     // the lists named in s_list
+    float line = 0.0f;
     if constexpr (!SMALL) {
         // (a beam without a score has no sums)
         auto list_max = [&](int i) {
@@ -416,50 +453,102 @@ __global__ __launch_bounds__(THREADS) void beam_pick_kernel(const SelectArgs a) 
         };
         float most = -INFINITY;
         for (int i = tid; i < lists; i += THREADS) most = fmaxf(most, list_max(i));
-        const float line = find_line(most);
+        line = find_line(most);
         for (int i = tid; i < lists; i += THREADS) {
             if (list_max(i) >= line) {
-                const int at = atomicAdd(&s_lists, 1);
-                if (at < kPickLists) s_list[at] = i;
+                const int to = atomicAdd(&s_lists, 1);
+                if (to < kPickLists) s_list[to] = i;
             }
         }
         __syncthreads();
         some = s_lists <= kPickLists;
         if (some) use = s_lists;
+        if (use <= HELD * (THREADS / 16)) {
+#pragma unroll
+            for (int h = 0; h < HELD; ++h) {
+                const int k = (tid >> 4) + h * (THREADS / 16);
+                if (k >= use) break;
+                const int i = some ? s_list[k] : k;
+                fill[h] = a.fill[slot0 + i];
+                beam[h] = i / a.chunks;
+#pragma unroll
+                for (int z = 0; z < kFirst; ++z) kept[h][z] = list_of(i)[16 * z];
+            }
+#pragma unroll
+            for (int h = 0; h < HELD; ++h) {
+                const int k = (tid >> 4) + h * (THREADS / 16);
+                if (k < use) rest_of(h, some ? s_list[k] : k);
+            }
+        }
     }
-    auto each = [&](auto take) {
-        if constexpr (SMALL) {
-            const int b = (tid >> 4) / a.chunks;
+    const bool held = SMALL || use <= HELD * (THREADS / 16);
+    auto cand_of = [&](int b, const Entry& e) { return Cand{score_of(b, e.x), e.x, b, e.token}; };
+    float rounded[HELD][kKept];    // scores, -infinity where there is no entry
+    if (held) {
+#pragma unroll
+        for (int h = 0; h < HELD; ++h) {
 #pragma unroll
             for (int k = 0; k < kKept; ++k) {
-                if ((tid & 15) + 16 * k >= fill) break;
-                const double score = score_of(b, kept[k].x);
-                if (static_cast<float>(score) > -INFINITY) take(Cand{score, kept[k].x, b, kept[k].token});
+                rounded[h][k] = -INFINITY;
+                if ((tid & 15) + 16 * k < fill[h]) rounded[h][k] = static_cast<float>(score_of(beam[h], kept[h][k].x));
+            }
+        }
+    }
+    auto each = [&](auto take) {
+        if (held) {
+#pragma unroll
+            for (int h = 0; h < HELD; ++h) {
+#pragma unroll
+                for (int k = 0; k < kKept; ++k) take(rounded[h][k], beam[h], kept[h][k]);
             }
             return;
         }
         for (int k = tid >> 4; k < use; k += THREADS / 16) {
             const int i = some ? s_list[k] : k;
-            const int b = i / a.chunks;
-            const int n = a.fill[slot0 + i];
-            for (int z = tid & 15; z < n; z += 16) {
-                const Entry e = a.lists[(slot0 + i) * kRoom + z];
-                const double score = score_of(b, e.x);
-                if (static_cast<float>(score) > -INFINITY) take(Cand{score, e.x, b, e.token});
+            const int b = i / a.chunks, n = a.fill[slot0 + i];
+            for (int z = 0; (tid & 15) + z < n; z += 16) {
+                const Entry e = list_of(i)[z];
+                take(static_cast<float>(score_of(b, e.x)), b, e);
             }
         }
     };
-    float most = -INFINITY;
-    each([&](const Cand& c) { most = fmaxf(most, static_cast<float>(c.score)); });
-    const float line = find_line(most);
-    each([&](const Cand& c) {
-        if (static_cast<float>(c.score) >= line) {
-            const int at = atomicAdd(&s_fill, 1);
-            if (at < kPickRoom) s_cand[at] = c;
+    // Those that reach the line, where there is room for all of them; how many.
+    auto collect = [&] {
+        if constexpr (SMALL) {
+            each([&](float score, int b, const Entry& e) {
+                if (score >= line) {
+                    const int to = atomicAdd(&s_fill, 1);
+                    if (to < kPickRoom) s_cand[to] = cand_of(b, e);
+                }
+            });
+            __syncthreads();
+            return s_fill;
         }
-    });
-    __syncthreads();
-    int n = s_fill;
+        int count = 0;
+        each([&](float score, int, const Entry&) { count += score >= line; });
+        const int upto = wave_inclusive_scan(count);
+        int to = 0;
+        if (lane == 63 && upto > 0) to = atomicAdd(&s_fill, upto);
+        to = __builtin_amdgcn_readlane(to, 63) + upto - count;
+        __syncthreads();
+        const int n = s_fill;
+        if (n <= kPickRoom) {
+            each([&](float score, int b, const Entry& e) {
+                if (score >= line) s_cand[to++] = cand_of(b, e);
+            });
+        }
+        __syncthreads();
+        return n;
+    };
+    // The lists' line may be enough: few lie above it unless few lists hold most.
+    int n = SMALL ? kPickRoom + 1 : collect();
+    if (n > kPickRoom) {
+        if (tid == 0) s_fill = 0;
+        float most = -INFINITY;
+        each([&](float score, int, const Entry&) { most = fmaxf(most, score); });
+        line = find_line(most);
+        n = collect();
+    }
     if (THREADS == kPickRoom && n > kFewEnough && n <= kPickRoom) {
         // A closer line among these: they are ranked by n^2 comparisons.
         const Cand mine = tid < n ? s_cand[tid] : Cand{-INFINITY, 0.0f, 0, -1};
@@ -487,7 +576,9 @@ __global__ __launch_bounds__(THREADS) void beam_pick_kernel(const SelectArgs a) 
         n = a.C;
         for (int k = 0; k < n; ++k) {
             Cand best = none;
-            each([&](const Cand& c) {
+            each([&](float score, int b, const Entry& e) {
+                if (!(score > -INFINITY)) return;
+                const Cand c = cand_of(b, e);
                 if (k > 0 && !before(s_order[k - 1], c)) return;
                 if (before(c, best)) best = c;
             });
@@ -515,24 +606,24 @@ __global__ __launch_bounds__(THREADS) void beam_pick_kernel(const SelectArgs a) 
     const int row = real ? r * a.W + c.beam : -1;
     const float score = static_cast<float>(c.score);
     if (lane < a.C) {
-        const size_t at = static_cast<size_t>(r) * a.C + lane;
-        a.cand_scores[at] = score;
-        a.cand_rows[at] = row;
-        a.cand_tokens[at] = c.token;
+        const size_t to = static_cast<size_t>(r) * a.C + lane;
+        a.cand_scores[to] = score;
+        a.cand_rows[to] = row;
+        a.cand_tokens[to] = c.token;
     }
     const unsigned long long on = __ballot(real && c.token != a.eos);
     const int place = __popcll(on & ((1ull << lane) - 1ull));
     const int all = __popcll(on);
-    const size_t at = static_cast<size_t>(r) * a.W;
+    const size_t first = static_cast<size_t>(r) * a.W;
     if (((on >> lane) & 1ull) && place < a.W) {
-        a.next_scores[at + place] = score;
-        a.next_rows[at + place] = row;
-        a.next_tokens[at + place] = c.token;
+        a.next_scores[first + place] = score;
+        a.next_rows[first + place] = row;
+        a.next_tokens[first + place] = c.token;
     }
     if (lane >= all && lane < a.W) {
-        a.next_scores[at + lane] = -INFINITY;
-        a.next_rows[at + lane] = -1;
-        a.next_tokens[at + lane] = -1;
+        a.next_scores[first + lane] = -INFINITY;
+        a.next_rows[first + lane] = -1;
+        a.next_tokens[first + lane] = -1;
     }
 }
 

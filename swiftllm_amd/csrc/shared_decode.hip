@@ -10,16 +10,23 @@
 // Work. The plan's list (shared_plan.hpp) is cut into equal ranges, one workgroup
 // per range and chunk of heads. A wide walk's rows are the query heads of up to
 // 4 x 32 / gw sequences, gw = min(G, 32) heads each, 32 rows to a wave; its K and V
-// go through LDS in stages of 64 keys as in scored_prefill, whose products these
-// are: S^T = K Q^T, O^T = V P^T, 32x32x16. A narrow walk, of at most 16 rows or of
-// one sequence, is one wave's as in scored_decode (scored_walk.hpp): no wave waits
-// for another, and eight of them a CU keep 128 KB on the way. (One sequence's own
-// blocks by a whole workgroup through LDS: 128 chats of 1-1000 own tokens behind
-// 8192 shared ones, 32/8 heads x 128, 91 us a layer, not @@; 16 x 8 beams 73, not @@.)
+// go through LDS, a ring of four steps of 32 keys, of which two to three are on the
+// way while one is used (loads the compiler does not see, counted by hand: with its
+// own waits it let one be), and the products are S^T = K Q^T, O^T = V P^T, 32x32x16,
+// as in scored_prefill. A narrow walk, of at most 16 rows or of one sequence, is one
+// wave's as in scored_decode (scored_walk.hpp): no wave waits for another, and eight
+// of them a CU keep 128 KB on the way. (One sequence's own blocks by a whole workgroup
+// through LDS: 128 chats of 1-1000 own tokens behind 8192 shared ones, 32/8 heads x
+// 128, 87 us a layer, not 82; 16 x 8 beams 73, not 62.)
 //
 // Bound: HBM, one read of the shared K and V for each tile of 128 rows and one of
-// every sequence's own: a CU's share of HBM brings a stage in 1.4 us, and a wave's
-// products and weights of one take 0.9 us.
+// every sequence's own. At 4.92 TB/s, what a large copy reaches: 16 x 8 beams on 1000
+// to 4000 tokens, 32/8 heads x 128 in bfloat16 with a cap, 44.0 us of reads, 52.4 in
+// all; the 128 chats 58.1 and 67.6 (two tiles share L2 for what both read); 4 x 16
+// questions on 30000 tokens, 64/8 heads, with distance biases 137 and 149. What is left
+// over is a range's start (its walk, ids, queries, a first step: 2.5 us), the ranges'
+// unequal ends and the second launch, 4 us. One walk of 128 rows on 131072 tokens takes
+// 117 us (with 64 keys a step and two of them 132, with the compiler's waits 159).
 
 #include <algorithm>
 #include <cmath>
@@ -565,9 +572,14 @@ void shared_decode_kernel(const SharedArgs a) {
 // on their way before those are there: a join is bound by latency.
 constexpr int kJoinRows = 8;
 constexpr int kJoinWaves = 4;       // of a workgroup
+// Rows below which four waves join one. (us a layer of 32/8 heads x 128, with one wave
+// and with four: 4 beams on 1000 tokens 12.9 and 11.6, 4 x 4 on 8192 41.5 and 37.2,
+// 32 on 32768 49.7 and 47.3; 16 x 4 on 600 25.3 and 27.1, 16 x 8 on 2500 53.5 and 59.0.)
 constexpr int kFewRows = 2048;
 
-// Tables and bytes of K and V up to which every sequence is taken whole.
+// Tables and bytes of K and V up to which every sequence is taken whole. (us a layer of
+// 2 x 4 beams, 8 heads x 64, in two launches and in one: 15 blocks each 9.2 and 5.6,
+// 38 blocks 9.3 and 7.8; they meet at about 48.)
 constexpr int kMostWhole = 48;
 constexpr double kWholeBytes = 64e6;
 

@@ -24,7 +24,7 @@ constexpr int kTileWaves = 4;
 constexpr int kTileRows = kWaveRows * kTileWaves;
 constexpr int kNarrowRows = 16;
 
-// Blocks that starting and ending a walk costs.
+// Blocks that starting and ending a walk costs. (16 and 4 or 8 are no faster.)
 constexpr int kWideCost = 8;
 constexpr int kNarrowCost = 2;
 // Workgroups the list is cut for: two for each of the 256 CUs of an MI355X, whose
@@ -33,7 +33,9 @@ constexpr int kResident = 2 * 256;
 // Shortest part of a wave in what is narrow, in blocks.
 constexpr int kLeastRange = 4;
 // Blocks of a group that reading shared ones once has to save, and values of a head of
-// all of them (blocks x chunks of heads x head_dim).
+// all of them (blocks x chunks of heads x head_dim): below, the second launch and its
+// joins cost what is saved. (4 beams on 1000 tokens, 8 kv heads x 128: 12.0 us a layer
+// shared, 11.6 not; 16 x 8 beams on 2500 tokens 53.5 shared, 153 by scored_decode.)
 constexpr int kLeastSaved = 16;
 constexpr long long kLeastSavedAll = 2500 * 128;
 
