@@ -589,7 +589,8 @@ int swiftllm_hip_scored_prefill(
  * is +infinity, its like share the row. beam_width <= num_candidates <= 64;
  * twice the width leaves every beam a candidate that goes on. next_scores may be
  * beam_scores. `workspace`: plain scratch, 256-byte aligned, of
- * swiftllm_hip_beam_select_workspace_size() bytes. */
+ * swiftllm_hip_beam_select_workspace_size() bytes; calls that share one must be
+ * ordered on one stream. */
 int swiftllm_hip_beam_select(
     const void* logits, const float* beam_scores, float* cand_scores,
     int32_t* cand_rows, int32_t* cand_tokens, float* next_scores,
@@ -702,7 +703,7 @@ size_t swiftllm_hip_shared_decode_workspace_size(
 
 /* Bytes of workspace (plain scratch, 256-byte aligned) that
  * swiftllm_hip_fork_pages and swiftllm_hip_compact_pages need; 0 where they
- * would refuse the sizes. */
+ * would refuse the sizes. Calls that share one must be ordered on one stream. */
 size_t swiftllm_hip_pages_workspace_size(int num_seqs, int num_blocks);
 
 /* ------------------------------------------------------------------------ */

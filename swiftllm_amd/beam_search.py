@@ -72,13 +72,17 @@ class BeamSearch:
     next_tokens and scores are the rows' choice, cand_* all of a request's
     candidates, among them those that end with eos_id. A row whose score is -inf
     (a request's other rows at first; one that the caller gives up) ends, and its
-    blocks are free again. A row that ended, or was cut because no block was free,
-    brings no token, and the tokens of the rows behind it move up: row s's is token
-    step.query_offsets[s] of the step. select() takes its logits in row s.
+    blocks are free again. A row that ended, that fork() cut or that plan() refused
+    because no block was free (counts[1], step.counts[2]) brings no token, and the
+    tokens of the rows behind it move up: row s's is token step.query_offsets[s] of the
+    step. select() takes its logits in row s; one without a token has none to give,
+    and its score is the caller's to set to -inf.
 
-    The calls are asynchronous on `stream`, in that order, and start() apart may be
-    captured. fork() changes between two sets of tables: a graph holds an even number
-    of steps."""
+    The calls are asynchronous on `stream`, in that order; all but start() and
+    compact() may be captured. fork() changes between two sets of tables, and what it
+    counts is of the plan() before: a graph holds an even number of steps, and is
+    replayed where it was captured, the same number of steps after a start() or an even
+    number more, not before the first of them."""
 
     def __init__(self, num_requests: int, beam_width: int, vocab: int,
                  max_num_blocks_per_seq: int, num_blocks: int,

@@ -46,7 +46,8 @@ constexpr int kScanWaves = kScanThreads / 64;
 constexpr int kIds = 4096;               // ids of a workgroup: 64 words of 64 bits
 constexpr int kWords = kIds / 64;
 constexpr int kEach = kIds / kScanThreads;
-constexpr int kSmallTables = 4096;       // entries of all rows, for one workgroup
+constexpr int kSmallRows = 64;           // rows and entries of all, for one workgroup
+constexpr int kSmallTables = 4096;
 constexpr int kRowHalves = 2;            // rows of a workgroup that renames entries
 
 struct PagesArgs {
@@ -549,7 +550,7 @@ int swiftllm_hip_fork_pages(int32_t* block_tables_out, int32_t* context_lens_out
     a.groups = (NB + kIds - 1) / kIds;
     a.rooms = S;
     set_space(a, workspace, space);
-    if (a.groups == 1 && static_cast<long long>(S) * MB <= kSmallTables) {
+    if (a.groups == 1 && S <= kSmallRows && static_cast<long long>(S) * MB <= kSmallTables) {
         return launched(launch(fork_small_kernel, dim3(1), dim3(kScanThreads), 0, stream, a), who);
     }
     rc = launched(launch(fork_rows_kernel, dim3(std::max(S, 1)), dim3(kRowThreads), 0, stream, a), who);
