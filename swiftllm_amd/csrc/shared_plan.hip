@@ -241,10 +241,11 @@ __global__ __launch_bounds__(kListThreads) void shared_list_kernel(const PlanSha
         }
         return m;
     };
-    int sum[1] = {0}, sums[1];
+    int sum[2] = {0, 0}, sums[2];
     for (int s = tid; s < a.S; s += kListThreads) {
         const Mine m = walks_of(s);
         sum[0] += m.tile_cost + m.own_cost;
+        sum[1] += m.wide ? m.tile_cost : 0;
         if (m.wide && m.group > a.per_tile) {
             const int at = atomicAdd(&s_tiles, 1);
             if (at < kMostMulti) s_multi[at] = m.tile_cost;
@@ -253,30 +254,31 @@ __global__ __launch_bounds__(kListThreads) void shared_list_kernel(const PlanSha
     scan(sum, sums, s_part);
     const int all = sums[0];
     // Where several tiles share blocks, each begins and ends with a range, so that
-    // they come by the same blocks at the same time, in one L2. What that leaves empty
-    // makes the ranges longer, by a sixteenth of the first length and more. (More than
-    // kMostMulti of them are many for any cut.)
+    // they come by the same blocks at the same time, in one L2. So does all that is
+    // wide: a workgroup would begin with what is narrow when the others have done most
+    // of theirs (4 x 16 questions on 30000 tokens, 64/8 heads x 128, 144 us a layer, not
+    // 138, 16 x 8 beams of 32/8 heads on 2500 53.3, not 52.1). What that leaves empty makes the ranges longer: a sixteenth, or a 64th, of the first length
+    // and more, the least that all fits into. (More than kMostMulti tiles are many for
+    // any cut.)
     const int tiles = s_tiles <= kMostMulti ? s_tiles : 0;
     const int wlen0 = max((all + kTileWaves * a.ranges - 1) / (kTileWaves * a.ranges), kLeastRange);
-    auto try_len = [&](int k) { return kTileWaves * (wlen0 + k * max(wlen0 / 16, 1)); };
+    auto try_len = [&](int k) { return kTileWaves * (wlen0 + k * max(wlen0 / (tiles > 0 ? 16 : 64), 1)); };
     auto padded = [](int cost, int len) { return cost > 2 * len ? (cost + len - 1) / len * len : cost; };
     for (int i = tid / kTries; i < tiles; i += kListThreads / kTries) {
         const int k = tid % kTries;
         atomicAdd(&s_pad[k], padded(s_multi[i], try_len(k)) - s_multi[i]);
     }
     __syncthreads();
-    int len = try_len(0);
-    bool align = false;
-    for (int k = kTries - 1; k >= 0 && tiles > 0; --k) {
-        if (static_cast<long long>(all) + s_pad[k] <= static_cast<long long>(a.ranges) * try_len(k)) {
-            len = try_len(k);
-            align = true;
-        }
-    }
+    // (a lane of every wave tries a length)
+    const int tried = try_len(tid % kTries);
+    const int end = (sums[1] + s_pad[tid % kTries] + tried - 1) / tried * tried;
+    const unsigned long long fits = __ballot(all - sums[1] + static_cast<long long>(end) <= static_cast<long long>(a.ranges) * tried);
+    const bool align = fits != 0;
+    const int len = try_len(align ? __builtin_ctzll(fits) : 0);
     const int wlen = len / kTileWaves;
     // Aligned tiles first, other wide ones, then the narrow ones.
     auto cost_of = [&](const Mine& m, int& aligned, int& wide, int& narrow) {
-        const int n = align && m.wide && m.group > a.per_tile && m.tile_cost > 2 * len ? padded(m.tile_cost, len) : 0;
+        const int n = align && tiles > 0 && m.wide && m.group > a.per_tile && m.tile_cost > 2 * len ? padded(m.tile_cost, len) : 0;
         aligned = n;
         wide = m.wide && n == 0 ? m.tile_cost : 0;
         narrow = m.wide ? 0 : m.tile_cost;
@@ -302,7 +304,8 @@ __global__ __launch_bounds__(kListThreads) void shared_list_kernel(const PlanSha
     };
     for (int s0 = 0; s0 < (ONE ? 1 : a.S); s0 += kListThreads) scan_row(s0 + tid, walks_of(s0 + tid));
     const int wide_walks = walks[0] + walks[1];
-    const int wide_cost = costs[0] + costs[1];
+    const int wide_sum = costs[0] + costs[1];
+    const int wide_cost = align && costs[2] > 0 ? (wide_sum + len - 1) / len * len : wide_sum;
     const int total = wide_cost + costs[2];
     // A tile's walk, from the sums before its first sequence.
     auto tile_walk = [&](const Mine& m, const int (&n)[3]) {
