@@ -257,9 +257,9 @@ __global__ __launch_bounds__(kListThreads) void shared_list_kernel(const PlanSha
     // they come by the same blocks at the same time, in one L2. So does all that is
     // wide: a workgroup would begin with what is narrow when the others have done most
     // of theirs (4 x 16 questions on 30000 tokens, 64/8 heads x 128, 144 us a layer, not
-    // 138, 16 x 8 beams of 32/8 heads on 2500 53.3, not 52.1). What that leaves empty makes the ranges longer: a sixteenth, or a 64th, of the first length
-    // and more, the least that all fits into. (More than kMostMulti tiles are many for
-    // any cut.)
+    // 138; 16 x 8 beams of 32/8 heads on 2500 53.3, not 52.1). What that leaves empty
+    // makes the ranges longer: a sixteenth, or a 64th, of the first length and more, the
+    // least that all fits into. (More than kMostMulti tiles are many for any cut.)
     const int tiles = s_tiles <= kMostMulti ? s_tiles : 0;
     const int wlen0 = max((all + kTileWaves * a.ranges - 1) / (kTileWaves * a.ranges), kLeastRange);
     auto try_len = [&](int k) { return kTileWaves * (wlen0 + k * max(wlen0 / (tiles > 0 ? 16 : 64), 1)); };
