@@ -197,7 +197,7 @@ __device__ __forceinline__ void narrow_walk(const SharedArgs& a, const Walk& wal
 
 // Blocks i0 .. i1 - 1 of a narrow walk, by one wave.
 template <typename T, int D, bool BIAS>
-__device__ __forceinline__ void narrow_piece(const SharedArgs& a, const Walk& walk, int kvh, int hc, int hb, int i0, int i1, int range, int wlen, int lane) {
+__device__ __forceinline__ void narrow_piece(const SharedArgs& a, const Walk& walk, int kvh, int hc, int hb, int i0, int i1, int range, int len, int lane) {
     constexpr int NJ = D / 16;
     const int kg = lane >> 4;
     Rows<D> o;
@@ -211,7 +211,7 @@ __device__ __forceinline__ void narrow_piece(const SharedArgs& a, const Walk& wa
         for (int J = 0; J < NJ; ++J) put_out<T>(p + 16 * J, o.st.acc[J] * inv, a.out8);
     } else if (o.row) {
         const long long f = static_cast<long long>(blockIdx.x) * a.frag_rows + walk.frow +
-                            static_cast<long long>(range - walk.at / wlen) * walk.count * a.gw + o.place;
+                            static_cast<long long>(range - narrow_range(walk.at, len)) * walk.count * a.gw + o.place;
         if (kg == 0) a.frag_ml[f] = float2{o.st.m, sum};
         float* const p = a.frag_o + f * D + 4 * kg;
 #pragma unroll
@@ -518,7 +518,7 @@ void shared_decode_kernel(const SharedArgs a) {
             const float sum = __builtin_bit_cast(float, static_cast<unsigned>(y[0])) + __builtin_bit_cast(float, static_cast<unsigned>(y[1]));
             const float inv = sum == 0.0f ? 0.0f : 1.0f / sum;
             const long long f = static_cast<long long>(blockIdx.x) * a.frag_rows + walk.frow +
-                                static_cast<long long>(static_cast<int>(blockIdx.y) - walk.at / len) * count * a.gw + place * a.gw + rh;
+                                static_cast<long long>(static_cast<int>(blockIdx.y) - wide_range(walk.at, len)) * count * a.gw + place * a.gw + rh;
             if (h == 0) a.frag_ml[f] = float2{m, sum};
             float* const p = a.frag_o + f * D + 4 * h;
 #pragma unroll
@@ -538,8 +538,7 @@ void shared_decode_kernel(const SharedArgs a) {
     }
     // This wave's part of what is narrow.
     const int range = kWaves * static_cast<int>(blockIdx.y) + w;
-    const int wlen = len / kWaves;
-    const int b = range * wlen, e = min(b + wlen, total);
+    const int b = narrow_begin(range, len), e = min(narrow_begin(range + 1, len), total);
     if (e <= wide_cost || b >= total) return;
     Walk walk;
     int v;
@@ -559,7 +558,7 @@ void shared_decode_kernel(const SharedArgs a) {
             for (int hb = 0; hb < a.gw; hb += kNarrowRows) {
                 int lane = threadIdx.x & 63;
                 asm volatile("" : "+v"(lane));
-                narrow_piece<T, D, BIAS>(a, walk, kvh, hc, hb, i0, i1, range, wlen, lane);
+                narrow_piece<T, D, BIAS>(a, walk, kvh, hc, hb, i0, i1, range, len, lane);
             }
         }
         if (v >= walks || next.at - kNarrowCost >= e) break;
@@ -605,8 +604,7 @@ __global__ __launch_bounds__(64 * kJoinWaves) void shared_join_kernel(const Shar
     int n0 = 0, n1 = 0, f0 = 0, f1 = 0, step = 0;
     const const_int* const head = as_const(reinterpret_cast<const int*>(a.head));
     auto pieces = [&](const Walk& x, int v) {
-        const int n = v < head[6] ? head[10] : head[10] / kTileWaves;    // a wide walk's ranges, and a narrow one's
-        return (x.at + x.blocks - 1) / n - x.at / n + 1;
+        return pieces_of(v < head[6], x.at, x.blocks, head[10]);
     };
     if (tile >= 0) {
         const Walk x = walk_at(a.walks + tile);

@@ -150,9 +150,9 @@ __global__ __launch_bounds__(kListThreads) void shared_list_kernel(const PlanSha
     __shared__ int s_pad[kTries];
     __shared__ int s_multi[kMostMulti];               // costs of tiles that share with others
     __shared__ int s_tile[ONE ? kListThreads : 1];    // the walk of the tile that begins with a sequence
-    __shared__ int s_bad, s_saved, s_tiles;
+    __shared__ int s_bad, s_saved, s_tiles, s_most;
     const int tid = threadIdx.x;
-    if (tid == 0) s_bad = s_saved = s_tiles = 0;
+    if (tid == 0) s_bad = s_saved = s_tiles = s_most = 0;
     if (tid < kTries) s_pad[tid] = 0;
     struct Row {
         int4 info;       // w: blocks shared
@@ -249,6 +249,7 @@ __global__ __launch_bounds__(kListThreads) void shared_list_kernel(const PlanSha
         if (m.wide && m.group > a.per_tile) {
             const int at = atomicAdd(&s_tiles, 1);
             if (at < kMostMulti) s_multi[at] = m.tile_cost;
+            atomicMax(&s_most, m.tile_cost);
         }
     }
     scan(sum, sums, s_part);
@@ -258,11 +259,15 @@ __global__ __launch_bounds__(kListThreads) void shared_list_kernel(const PlanSha
     // wide: a workgroup would begin with what is narrow when the others have done most
     // of theirs (4 x 16 questions on 30000 tokens, 64/8 heads x 128, 144 us a layer, not
     // 138; 16 x 8 beams of 32/8 heads on 2500 53.3, not 52.1). What that leaves empty
-    // makes the ranges longer: a sixteenth, or a 64th, of the first length and more, the
-    // least that all fits into. (More than kMostMulti tiles are many for any cut.)
+    // makes the ranges longer: the first length that all fits into, of those that cut the
+    // longest tile evenly, or by 64ths of the first length. (More than kMostMulti tiles
+    // are many for any cut.)
     const int tiles = s_tiles <= kMostMulti ? s_tiles : 0;
-    const int wlen0 = max((all + kTileWaves * a.ranges - 1) / (kTileWaves * a.ranges), kLeastRange);
-    auto try_len = [&](int k) { return kTileWaves * (wlen0 + k * max(wlen0 / (tiles > 0 ? 16 : 64), 1)); };
+    const int len0 = max((all + a.ranges - 1) / a.ranges, kLeastRange);
+    auto try_len = [&](int k) {
+        const int cuts = s_most / len0 - k;
+        return tiles == 0 ? len0 + k * max(len0 / 64, 1) : cuts > 0 ? (s_most + cuts - 1) / cuts : len0 + k * max(len0 / 16, 1);
+    };
     auto padded = [](int cost, int len) { return cost > 2 * len ? (cost + len - 1) / len * len : cost; };
     for (int i = tid / kTries; i < tiles; i += kListThreads / kTries) {
         const int k = tid % kTries;
@@ -275,7 +280,6 @@ __global__ __launch_bounds__(kListThreads) void shared_list_kernel(const PlanSha
     const unsigned long long fits = __ballot(all - sums[1] + static_cast<long long>(end) <= static_cast<long long>(a.ranges) * tried);
     const bool align = fits != 0;
     const int len = try_len(align ? __builtin_ctzll(fits) : 0);
-    const int wlen = len / kTileWaves;
     // Aligned tiles first, other wide ones, then the narrow ones.
     auto cost_of = [&](const Mine& m, int& aligned, int& wide, int& narrow) {
         const int n = align && tiles > 0 && m.wide && m.group > a.per_tile && m.tile_cost > 2 * len ? padded(m.tile_cost, len) : 0;
@@ -330,26 +334,25 @@ __global__ __launch_bounds__(kListThreads) void shared_list_kernel(const PlanSha
         }
         int aligned, wide, narrow;
         cost_of(m, aligned, wide, narrow);
-        // Ranges of n that blocks b .. b + k - 1 of the list lie in.
-        auto pieces = [](int b, int k, int n) { return (b + k - 1) / n - b / n + 1; };
         const bool joins = m.sh > 0 && m.L > 0;
         const int tile_at = aligned > 0 ? at_costs[0] + kWideCost : wide > 0 ? costs[0] + at_costs[1] + kWideCost : wide_cost + at_costs[2] + kNarrowCost;
         const int own_at = wide_cost + at_costs[2] + narrow + kNarrowCost;
         int tile_rows = 0, own_rows = 0;
-        if (m.count > 0) tile_rows = m.count * a.gw * pieces(tile_at, m.sh, m.wide ? len : wlen);
+        if (m.count > 0) tile_rows = m.count * a.gw * pieces_of(m.wide, tile_at, m.sh, len);
         if (m.own > 0) {
-            const int n = pieces(own_at, m.own, wlen);
+            const int n = pieces_of(false, own_at, m.own, len);
             if (joins || n > 1) own_rows = a.gw * n;
         }
         int x[1] = {tile_rows + own_rows}, sums[1];
         scan(x, sums, s_part);
         if (s < a.S) {
             const int f = rows + x[0];
-            // A walk, and the ranges of n that begin in it or in what it costs.
-            auto put = [&](int v, const Walk& w, int from, int to, int n, Start* starts) {
+            // A walk, and the ranges, or waves' parts, that begin in it or in what it costs.
+            auto put = [&](int v, const Walk& w, int from, int to, bool wide) {
                 a.walks[v] = w;
-                for (int r = (from + n - 1) / n; r * n < to; ++r) {
-                    Start& begin = starts[r];
+                const unsigned scale = wide ? 1 : kTileWaves, n = len;
+                for (unsigned r = (scale * from + n - 1) / n; r * n < scale * to; ++r) {
+                    Start& begin = (wide ? a.wide : a.narrow)[r];
                     begin.walk = w;
                     begin.v = v;
                 }
@@ -357,11 +360,11 @@ __global__ __launch_bounds__(kListThreads) void shared_list_kernel(const PlanSha
             if (m.count > 0) {
                 const Walk w{m.lead, 0, m.sh, s, m.count, tile_at, m.group <= a.per_tile, f};
                 const int from = tile_at - (m.wide ? kWideCost : kNarrowCost);
-                put(tile_walk(m, at_walks), w, from, aligned > 0 ? from + aligned : tile_at + m.sh, m.wide ? len : wlen, m.wide ? a.wide : a.narrow);
+                put(tile_walk(m, at_walks), w, from, aligned > 0 ? from + aligned : tile_at + m.sh, m.wide);
             }
             const int own_v = wide_walks + at_walks[2] + (narrow > 0);
             if (m.own > 0) {
-                put(own_v, Walk{s, m.L > 0 ? m.sh : 0, m.own, s, 1, own_at, 1, own_rows > 0 ? f + tile_rows : -1}, own_at - kNarrowCost, own_at + m.own, wlen, a.narrow);
+                put(own_v, Walk{s, m.L > 0 ? m.sh : 0, m.own, s, 1, own_at, 1, own_rows > 0 ? f + tile_rows : -1}, own_at - kNarrowCost, own_at + m.own, false);
             }
             Seq q{m.L, m.own > 0 ? own_v : -1, -1, 0};
             if (joins) {

@@ -30,8 +30,8 @@ constexpr int kNarrowCost = 2;
 // Workgroups the list is cut for: two for each of the 256 CUs of an MI355X, whose
 // LDS their rings of steps take.
 constexpr int kResident = 2 * 256;
-// Shortest part of a wave in what is narrow, in blocks.
-constexpr int kLeastRange = 4;
+// Shortest range, in blocks.
+constexpr int kLeastRange = 16;
 // Blocks of a group that reading shared ones once has to save, and values of a head of
 // all of them (blocks x chunks of heads x head_dim): below, the second launch and its
 // joins cost what is saved. (4 beams on 1000 tokens, 8 kv heads x 128: 12.0 us a layer
@@ -63,7 +63,7 @@ struct Head {
     int walks;      //   in all
     int wide_cost;  // the list's wide part
     int total;
-    int len;        // of a workgroup's range, kTileWaves times a wave's
+    int len;        // of a workgroup's range; a wave's part of what is narrow is a quarter of it
     int pad[5];
 };
 
@@ -73,6 +73,20 @@ struct Seq {
     int tile;       // the walk of its shared blocks, -1: none
     int index;      // its place in that one
 };
+
+// The range of `len` that a wide walk's block at a place of the list lies in; and the
+// wave, counted over ranges, that a narrow walk's does: wave r's begin at r len / 4.
+__device__ __forceinline__ int wide_range(int place, int len) { return place / len; }
+__device__ __forceinline__ int narrow_range(int place, int len) {
+    return static_cast<int>((kTileWaves * static_cast<unsigned>(place) + kTileWaves - 1) / static_cast<unsigned>(len));
+}
+__device__ __forceinline__ int narrow_begin(int range, int len) {
+    return static_cast<int>(static_cast<unsigned>(range) * static_cast<unsigned>(len) / kTileWaves);
+}
+__device__ __forceinline__ int pieces_of(bool wide, int at, int blocks, int len) {
+    return wide ? wide_range(at + blocks - 1, len) - wide_range(at, len) + 1
+                : narrow_range(at + blocks - 1, len) - narrow_range(at, len) + 1;
+}
 
 // How the heads of a kv head lie in a wave's rows.
 struct Heads {
