@@ -30,8 +30,6 @@
 // before it; kept for every block in an array of its own, the last took 10.9. Where a
 // row and its parent have the same block in the same place, as in a prompt that both
 // share, nothing is counted: a search's reordering touches few counters.
-// (Counting all ids in the pairing workgroups, a launch less, took 8.9 us at 65536
-// blocks, the two launches 7.3.)
 
 #include <algorithm>
 
@@ -48,6 +46,7 @@ constexpr int kWords = kIds / 64;
 constexpr int kEach = kIds / kScanThreads;
 constexpr int kSmallRows = 64;           // rows and entries of all, for one workgroup
 constexpr int kSmallTables = 4096;
+constexpr int kFewGroups = 4;            // whose ids every workgroup counts by itself
 constexpr int kRowHalves = 2;            // rows of a workgroup that renames entries
 
 struct PagesArgs {
@@ -344,8 +343,25 @@ __global__ __launch_bounds__(kScanThreads) void compact_scan_kernel(const PagesA
     scan_ids<true>(a, a.refs, blockIdx.x, s_part);
 }
 
-// `live` of the first `all` ids are in use, of `all` in the pool: the others move, at
-// most the pairs' room.
+// The pairs of a group's ids, `before` of those in use before them: `live` of the first
+// `all` ids are in use, of `all` in the pool, so the others move, at most the pairs' room.
+__device__ __forceinline__ void compact_pairs(const PagesArgs& a, int group, unsigned long long mine, int before, int all, int live) {
+    const int moves = min(all - live, a.rooms);
+    if (group == 0 && threadIdx.x == 0) {
+        a.found[0] = moves;
+        a.found[1] = all;
+        if (moves == 0) a.found[2] = a.NB;
+    }
+    const int start = starts_of(mine, before);
+    if (threadIdx.x < kWords) a.starts[static_cast<size_t>(group) * kWords + threadIdx.x] = start;
+    each_id(a, group, mine, start, [&](int id, bool used, int k) {
+        const int at = used ? all - 1 - k : id - k;
+        if (at >= moves) return;
+        (used ? a.from : a.to)[at] = id;
+        if (used && at == moves - 1) a.found[2] = id;
+    });
+}
+
 __global__ __launch_bounds__(kScanThreads) void compact_pairs_kernel(const PagesArgs a) {
     __shared__ int s_part[3 * kScanWaves];
     const int tid = threadIdx.x;
@@ -360,21 +376,62 @@ __global__ __launch_bounds__(kScanThreads) void compact_pairs_kernel(const Pages
         live += __popcll(n == 64 ? m : m & ((1ull << n) - 1ull));
     }
     live = block_total<kScanWaves>(live, s_part + 2 * kScanWaves);
-    const int moves = min(all - live, a.rooms);
-    if (blockIdx.x == 0 && tid == 0) {
-        a.found[0] = moves;
-        a.found[1] = all;
-        if (moves == 0) a.found[2] = a.NB;
+    compact_pairs(a, blockIdx.x, word_of(a, blockIdx.x), before, all, live);
+}
+
+// Both at once, where the groups are few: every workgroup counts all ids by itself, four
+// neighbours of every group a thread. (us of three launches and of two, replayed: 8 rows
+// over 4096 blocks 8.8 and 7.9, 32 over 16384 9.3 and 8.3; 16 groups so, 64 rows over
+// 65536 blocks, 11.3 and 11.4.)
+__global__ __launch_bounds__(kScanThreads) void compact_few_kernel(const PagesArgs a) {
+    typedef int four __attribute__((ext_vector_type(4), aligned(4)));
+    __shared__ int s_part[3 * kScanWaves];
+    __shared__ unsigned long long s_bits[kWords];
+    const int tid = threadIdx.x, lane = tid & 63, group = blockIdx.x;
+    const int w = __builtin_amdgcn_readfirstlane(tid >> 6);
+    four r[kFewGroups];
+#pragma unroll
+    for (int g = 0; g < kFewGroups; ++g) {
+        const int id = g * kIds + 4 * tid;
+        r[g] = four{0, 0, 0, 0};
+        if (id + 4 <= a.NB) {
+            r[g] = *reinterpret_cast<const four*>(a.refs + id);
+        } else {
+#pragma unroll
+            for (int k = 0; k < 3; ++k) {
+                if (id + k < a.NB) r[g][k] = a.refs[id + k];
+            }
+        }
     }
-    const unsigned long long mine = word_of(a, blockIdx.x);
-    const int start = starts_of(mine, before);
-    if (tid < kWords) a.starts[static_cast<size_t>(blockIdx.x) * kWords + tid] = start;
-    each_id(a, blockIdx.x, mine, start, [&](int id, bool used, int k) {
-        const int at = used ? all - 1 - k : id - k;
-        if (at >= moves) return;
-        (used ? a.from : a.to)[at] = id;
-        if (used && at == moves - 1) a.found[2] = id;
-    });
+    int own[kEach];
+#pragma unroll
+    for (int k = 0; k < kEach; ++k) {
+        const int id = group * kIds + (w * kEach + k) * 64 + lane;
+        own[k] = id < a.NB ? a.refs[id] : 0;
+    }
+    unsigned long long mine = 0;     // bit 4 g + k: id g kIds + 4 tid + k is in use
+#pragma unroll
+    for (int g = 0; g < kFewGroups; ++g) {
+#pragma unroll
+        for (int k = 0; k < 4; ++k) mine |= r[g][k] > 0 ? 1ull << (4 * g + k) : 0ull;
+    }
+    static_assert(kFewGroups <= 16 && kIds == 4 * kScanThreads, "a word of bits");
+#pragma unroll
+    for (int k = 0; k < kEach; ++k) {
+        const unsigned long long m = __ballot(own[k] > 0);
+        if (lane == 0) {
+            s_bits[w * kEach + k] = m;
+            a.bits[static_cast<size_t>(group) * kWords + w * kEach + k] = m;
+        }
+    }
+    const int all = block_total<kScanWaves>(__popcll(mine), s_part);
+    const int before = block_total<kScanWaves>(__popcll(mine & ((1ull << (4 * group)) - 1ull)), s_part + kScanWaves);
+    // The thread's ids below `all`: four of every group before that of id `all`, and some there.
+    const int last = all / kIds;
+    const int some = min(max(all - last * kIds - 4 * tid, 0), 4);
+    const unsigned long long lower = last >= 16 ? ~0ull : ((1ull << (4 * last)) - 1ull) | (((1ull << some) - 1ull) << (4 * last));
+    const int live = block_total<kScanWaves>(__popcll(mine & lower), s_part + 2 * kScanWaves);
+    compact_pairs(a, group, s_bits[lane], before, all, live);
 }
 
 __global__ __launch_bounds__(kScanThreads) void compact_apply_kernel(const PagesArgs a) {
@@ -612,9 +669,13 @@ int swiftllm_hip_compact_pages(int32_t* block_tables_out, int32_t* ref_counts_ou
     a.groups = (NB + kIds - 1) / kIds;
     a.rooms = max_moves;
     set_space(a, workspace, space);
-    rc = launched(launch(compact_scan_kernel, dim3(a.groups), dim3(kScanThreads), 0, stream, a), who);
-    if (rc != SWIFTLLM_OK) return rc;
-    rc = launched(launch(compact_pairs_kernel, dim3(a.groups), dim3(kScanThreads), 0, stream, a), who);
+    if (a.groups <= kFewGroups) {
+        rc = launched(launch(compact_few_kernel, dim3(a.groups), dim3(kScanThreads), 0, stream, a), who);
+    } else {
+        rc = launched(launch(compact_scan_kernel, dim3(a.groups), dim3(kScanThreads), 0, stream, a), who);
+        if (rc != SWIFTLLM_OK) return rc;
+        rc = launched(launch(compact_pairs_kernel, dim3(a.groups), dim3(kScanThreads), 0, stream, a), who);
+    }
     if (rc != SWIFTLLM_OK) return rc;
     const int rows = (S + kRowHalves - 1) / kRowHalves;
     return launched(launch(compact_apply_kernel, dim3(a.groups + rows), dim3(kScanThreads), 0, stream, a), who);

@@ -267,3 +267,15 @@ def test_forks_of_small_pools(dev, S, MB, NB):
     p = Pool(S, MB, NB).lone(rng, lens)
     for _ in range(4):
         p.fork(rng.integers(-1, S, S).astype(np.int32))
+
+
+@pytest.mark.parametrize("NB", [1, 2, 3, 5, 4095, 4096, 4097, 65533, 65536, 65537])
+@pytest.mark.parametrize("used", [0.0, 0.3, 0.97, 1.0])
+def test_compactions_by_groups_of_ids(dev, NB, used):
+    """Pools that end inside and at the edges of a group of ids, up to the most that every workgroup counts."""
+    rng = np.random.default_rng(NB + int(10 * used))
+    n = int(used * NB)
+    lens = [16 * (n // 3), 16 * (n - n // 3) - (n > 1)] if n else [0, 0]
+    for moves in (NB, max(NB // 50, 1)):
+        p = Pool(2, max(n, 1), NB).lone(rng, lens)
+        p.compact(moves)
