@@ -7,8 +7,8 @@
 // query row, m = max score, l = sum exp2(score - m) and o = sum exp2(score - m) v / l;
 // rows are joined as sum of exp2(m - M) l o over sum of exp2(m - M) l.
 //
-// Work. The plan's list (shared_plan.hpp) is cut into equal ranges, one workgroup
-// per range and chunk of heads. A wide walk's rows are the query heads of up to
+// Work. The plan's lists (shared_plan.hpp) are cut into ranges, one workgroup per
+// range and chunk of heads. A wide walk's rows are the query heads of up to
 // 4 x 32 / gw sequences, gw = min(G, 32) heads each, 32 rows to a wave; its K and V
 // go through LDS, a ring of four steps of 32 keys, of which two to three are on the
 // way while one is used (loads the compiler does not see, counted by hand: with its
@@ -21,9 +21,9 @@
 //
 // Bound: HBM, one read of the shared K and V for each tile of 128 rows and one of
 // every sequence's own. At 4.92 TB/s, what a large copy reaches: 16 x 8 beams on 1000
-// to 4000 tokens, 32/8 heads x 128 in bfloat16 with a cap, 44.0 us of reads, 52.4 in
-// all; the 128 chats 58.1 and 67.6 (two tiles share L2 for what both read); 4 x 16
-// questions on 30000 tokens, 64/8 heads, with distance biases 137 and 149. What is left
+// to 4000 tokens, 32/8 heads x 128 in bfloat16 with a cap, 44.0 us of reads, 51.3 in
+// all; the 128 chats 58.1 and 67.5 (tiles share L2 for what they read); 4 x 16
+// questions on 30000 tokens, 64/8 heads, with distance biases 137 and 138. What is left
 // over is a range's start (its walk, ids, queries, a first step: 2.5 us), the ranges'
 // unequal ends and the second launch, 4 us. One walk of 128 rows on 131072 tokens takes
 // 117 us (with 64 keys a step and two of them 132, with the compiler's waits 159).
@@ -304,15 +304,15 @@ void shared_decode_kernel(const SharedArgs a) {
     __shared__ __align__(16) uint16_t s_ring[kRing * kStep];
     __shared__ unsigned s_bad[kRing][2];                 // keys of a step's blocks whose values were not finite
     const const_int* const head = as_const(reinterpret_cast<const int*>(a.head));
-    const int wide = head[6], walks = head[7], wide_cost = head[8], total = head[9], len = head[10];
+    const int wide = head[6], walks = head[7], wide_end = head[8], narrow_end = head[9], len = head[10], narrow_len = head[11];
+    const int wide_ranges = head[12];
     if (!plan_fits(a)) return;
-    const int start = blockIdx.y * len;
-    if (start >= total) return;
-    const int end = min(start + len, total);
     const int w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const int kvh = blockIdx.x / a.nhc;
     const int hc = blockIdx.x - kvh * a.nhc;
-    if (start < wide_cost) {
+    if (static_cast<int>(blockIdx.y) < wide_ranges) {
+    const int start = blockIdx.y * len;
+    const int end = min(start + len, wide_end);
     auto k_of = [&](int t) { return s_ring + (t & (kRing - 1)) * kStep; };
     auto v_of = [&](int t) { return k_of(t) + St::kPair; };
     const Start* const s0 = a.wide + blockIdx.y;
@@ -535,21 +535,15 @@ void shared_decode_kernel(const SharedArgs a) {
         if (v >= wide || next.at - kWideCost >= end) break;
         walk = next;
     }
+    return;
     }
     // This wave's part of what is narrow.
-    const int range = kWaves * static_cast<int>(blockIdx.y) + w;
-    const int b = narrow_begin(range, len), e = min(narrow_begin(range + 1, len), total);
-    if (e <= wide_cost || b >= total) return;
-    Walk walk;
-    int v;
-    if (b <= wide_cost) {
-        v = wide;
-        walk = walk_at(a.walks + v);
-    } else {
-        const Start* const s0 = a.narrow + range;
-        walk = walk_at(&s0->walk);
-        v = as_const(&s0->v)[0];
-    }
+    const int range = kWaves * (static_cast<int>(blockIdx.y) - wide_ranges) + w;
+    const int b = narrow_begin(range, narrow_len), e = min(narrow_begin(range + 1, narrow_len), narrow_end);
+    if (b >= narrow_end) return;
+    const Start* const s0 = a.narrow + range;
+    Walk walk = walk_at(&s0->walk);
+    int v = as_const(&s0->v)[0];
     for (;;) {
         const int i0 = max(b - walk.at, 0);
         const int i1 = min(e - walk.at, walk.blocks);
@@ -558,7 +552,7 @@ void shared_decode_kernel(const SharedArgs a) {
             for (int hb = 0; hb < a.gw; hb += kNarrowRows) {
                 int lane = threadIdx.x & 63;
                 asm volatile("" : "+v"(lane));
-                narrow_piece<T, D, BIAS>(a, walk, kvh, hc, hb, i0, i1, range, len, lane);
+                narrow_piece<T, D, BIAS>(a, walk, kvh, hc, hb, i0, i1, range, narrow_len, lane);
             }
         }
         if (v >= walks || next.at - kNarrowCost >= e) break;
@@ -604,7 +598,7 @@ __global__ __launch_bounds__(64 * kJoinWaves) void shared_join_kernel(const Shar
     int n0 = 0, n1 = 0, f0 = 0, f1 = 0, step = 0;
     const const_int* const head = as_const(reinterpret_cast<const int*>(a.head));
     auto pieces = [&](const Walk& x, int v) {
-        return pieces_of(v < head[6], x.at, x.blocks, head[10]);
+        return pieces_of(v < head[6], x.at, x.blocks, v < head[6] ? head[10] : head[11]);
     };
     if (tile >= 0) {
         const Walk x = walk_at(a.walks + tile);

@@ -241,11 +241,14 @@ __global__ __launch_bounds__(kListThreads) void shared_list_kernel(const PlanSha
         }
         return m;
     };
-    int sum[2] = {0, 0}, sums[2];
+    int sum[3] = {0, 0, 0}, sums[3];      // in all; what is wide, and what it takes
     for (int s = tid; s < a.S; s += kListThreads) {
         const Mine m = walks_of(s);
         sum[0] += m.tile_cost + m.own_cost;
-        sum[1] += m.wide ? m.tile_cost : 0;
+        if (m.wide) {
+            sum[1] += m.tile_cost;
+            sum[2] += m.tile_cost + m.tile_cost / 12 * ((m.count * a.gw + kWaveRows - 1) / kWaveRows);
+        }
         if (m.wide && m.group > a.per_tile) {
             const int at = atomicAdd(&s_tiles, 1);
             if (at < kMostMulti) s_multi[at] = m.tile_cost;
@@ -254,19 +257,28 @@ __global__ __launch_bounds__(kListThreads) void shared_list_kernel(const PlanSha
     }
     scan(sum, sums, s_part);
     const int all = sums[0];
+    // The ranges of what is wide. Where that is most of all, its products bound it, and a
+    // block takes a workgroup the longer the more of its waves have rows: it counts for a
+    // twelfth more with each. Where it is not, HBM bounds both alike. (us a pass, counted
+    // so and not: 4 x 16 questions on 30000 tokens, 64/8 heads x 128 with biases, 285 and
+    // 295, 16 x 8 beams on 2500, 32/8 with a cap, 216 and 220; 128 chats on 8192 tokens
+    // 306 and 288.)
+    const int narrow_sum = all - sums[1];
+    int wide_ranges = 0;
+    if (sums[1] > 0) {
+        const float takes = static_cast<float>(sums[1] > narrow_sum ? sums[2] : sums[1]);
+        wide_ranges = static_cast<int>(ceilf(takes / (takes + static_cast<float>(narrow_sum)) * static_cast<float>(a.ranges)));
+        wide_ranges = narrow_sum > 0 ? min(max(wide_ranges, 1), a.ranges - 1) : a.ranges;
+    }
     // Where several tiles share blocks, each begins and ends with a range, so that
-    // they come by the same blocks at the same time, in one L2. So does all that is
-    // wide: a workgroup would begin with what is narrow when the others have done most
-    // of theirs (4 x 16 questions on 30000 tokens, 64/8 heads x 128, 144 us a layer, not
-    // 138; 16 x 8 beams of 32/8 heads on 2500 53.3, not 52.1). What that leaves empty
-    // makes the ranges longer: the first length that all fits into, of those that cut the
-    // longest tile evenly, or by 64ths of the first length. (More than kMostMulti tiles
+    // they come by the same blocks at the same time, in one L2: the first length that
+    // cuts the longest tile evenly and leaves room for all. (More than kMostMulti tiles
     // are many for any cut.)
     const int tiles = s_tiles <= kMostMulti ? s_tiles : 0;
-    const int len0 = max((all + a.ranges - 1) / a.ranges, kLeastRange);
+    const int len0 = wide_ranges > 0 ? max((sums[1] + wide_ranges - 1) / wide_ranges, kLeastRange) : kLeastRange;
     auto try_len = [&](int k) {
         const int cuts = s_most / len0 - k;
-        return tiles == 0 ? len0 + k * max(len0 / 64, 1) : cuts > 0 ? (s_most + cuts - 1) / cuts : len0 + k * max(len0 / 16, 1);
+        return cuts > 0 ? (s_most + cuts - 1) / cuts : len0 + k * max(len0 / 16, 1);
     };
     auto padded = [](int cost, int len) { return cost > 2 * len ? (cost + len - 1) / len * len : cost; };
     for (int i = tid / kTries; i < tiles; i += kListThreads / kTries) {
@@ -276,13 +288,12 @@ __global__ __launch_bounds__(kListThreads) void shared_list_kernel(const PlanSha
     __syncthreads();
     // (a lane of every wave tries a length)
     const int tried = try_len(tid % kTries);
-    const int end = (sums[1] + s_pad[tid % kTries] + tried - 1) / tried * tried;
-    const unsigned long long fits = __ballot(all - sums[1] + static_cast<long long>(end) <= static_cast<long long>(a.ranges) * tried);
+    const unsigned long long fits = __ballot(tiles > 0 && sums[1] + static_cast<long long>(s_pad[tid % kTries]) <= static_cast<long long>(wide_ranges) * tried);
     const bool align = fits != 0;
-    const int len = try_len(align ? __builtin_ctzll(fits) : 0);
+    const int len = align ? try_len(__builtin_ctzll(fits)) : len0;
     // Aligned tiles first, other wide ones, then the narrow ones.
     auto cost_of = [&](const Mine& m, int& aligned, int& wide, int& narrow) {
-        const int n = align && tiles > 0 && m.wide && m.group > a.per_tile && m.tile_cost > 2 * len ? padded(m.tile_cost, len) : 0;
+        const int n = align && m.wide && m.group > a.per_tile && m.tile_cost > 2 * len ? padded(m.tile_cost, len) : 0;
         aligned = n;
         wide = m.wide && n == 0 ? m.tile_cost : 0;
         narrow = m.wide ? 0 : m.tile_cost;
@@ -308,9 +319,9 @@ __global__ __launch_bounds__(kListThreads) void shared_list_kernel(const PlanSha
     };
     for (int s0 = 0; s0 < (ONE ? 1 : a.S); s0 += kListThreads) scan_row(s0 + tid, walks_of(s0 + tid));
     const int wide_walks = walks[0] + walks[1];
-    const int wide_sum = costs[0] + costs[1];
-    const int wide_cost = align && costs[2] > 0 ? (wide_sum + len - 1) / len * len : wide_sum;
-    const int total = wide_cost + costs[2];
+    const int wide_end = costs[0] + costs[1];
+    wide_ranges = (wide_end + len - 1) / len;
+    const int narrow_len = wide_ranges < a.ranges ? max((costs[2] + a.ranges - wide_ranges - 1) / (a.ranges - wide_ranges), kLeastRange) : kLeastRange;
     // A tile's walk, from the sums before its first sequence.
     auto tile_walk = [&](const Mine& m, const int (&n)[3]) {
         int aligned, wide, narrow;
@@ -335,12 +346,12 @@ __global__ __launch_bounds__(kListThreads) void shared_list_kernel(const PlanSha
         int aligned, wide, narrow;
         cost_of(m, aligned, wide, narrow);
         const bool joins = m.sh > 0 && m.L > 0;
-        const int tile_at = aligned > 0 ? at_costs[0] + kWideCost : wide > 0 ? costs[0] + at_costs[1] + kWideCost : wide_cost + at_costs[2] + kNarrowCost;
-        const int own_at = wide_cost + at_costs[2] + narrow + kNarrowCost;
+        const int tile_at = aligned > 0 ? at_costs[0] + kWideCost : wide > 0 ? costs[0] + at_costs[1] + kWideCost : at_costs[2] + kNarrowCost;
+        const int own_at = at_costs[2] + narrow + kNarrowCost;
         int tile_rows = 0, own_rows = 0;
-        if (m.count > 0) tile_rows = m.count * a.gw * pieces_of(m.wide, tile_at, m.sh, len);
+        if (m.count > 0) tile_rows = m.count * a.gw * pieces_of(m.wide, tile_at, m.sh, m.wide ? len : narrow_len);
         if (m.own > 0) {
-            const int n = pieces_of(false, own_at, m.own, len);
+            const int n = pieces_of(false, own_at, m.own, narrow_len);
             if (joins || n > 1) own_rows = a.gw * n;
         }
         int x[1] = {tile_rows + own_rows}, sums[1];
@@ -350,7 +361,7 @@ __global__ __launch_bounds__(kListThreads) void shared_list_kernel(const PlanSha
             // A walk, and the ranges, or waves' parts, that begin in it or in what it costs.
             auto put = [&](int v, const Walk& w, int from, int to, bool wide) {
                 a.walks[v] = w;
-                const unsigned scale = wide ? 1 : kTileWaves, n = len;
+                const unsigned scale = wide ? 1 : kTileWaves, n = wide ? len : narrow_len;
                 for (unsigned r = (scale * from + n - 1) / n; r * n < scale * to; ++r) {
                     Start& begin = (wide ? a.wide : a.narrow)[r];
                     begin.walk = w;
@@ -384,7 +395,7 @@ __global__ __launch_bounds__(kListThreads) void shared_list_kernel(const PlanSha
         }
         rows += sums[0];
     }
-    if (tid == 0) *a.head = Head{kMagic, a.S, a.MB, a.H, a.Hkv, a.D, wide_walks, wide_walks + walks[2], wide_cost, total, len};
+    if (tid == 0) *a.head = Head{kMagic, a.S, a.MB, a.H, a.Hkv, a.D, wide_walks, wide_walks + walks[2], wide_end, costs[2], len, narrow_len, wide_ranges};
 }
 
 }  // namespace

@@ -3,11 +3,12 @@
 //
 // The work of a step is a list of walks: of a group's shared blocks by the queries
 // of up to `per_tile` of its sequences, and of each sequence's other blocks by its
-// own. Shared ones of more than 16 query rows are wide, a workgroup's, and come
-// first; the others are narrow, a wave's. The list is cut into equal ranges of its cost,
-// one per workgroup and chunk of heads, of which each wave has an equal part of what
-// is narrow. Every piece of a walk that does not end its rows leaves one fragment
-// (maximum, sum, output) a row; those of a walk lie behind each other from row
+// own. Shared ones of more than 16 query rows are wide, a workgroup's, and
+// have a list of their own; the others are narrow, a wave's. Both lists are cut into equal
+// ranges of their costs, one per workgroup and chunk of heads; of what is narrow each
+// wave has a quarter of one. (With one list for both, the range in which the wide ones
+// end takes longest.) Every piece of a walk that does not end its rows leaves one
+// fragment (maximum, sum, output) a row; those of a walk lie behind each other from row
 // `frow` on.
 #pragma once
 
@@ -45,7 +46,7 @@ struct Walk {
     int blocks;     //   and how many
     int seq;        // the first of its sequences
     int count;      //   and how many: more than one shares
-    int at;         // its first block's place in the list
+    int at;         // its first block's place in its list
     int once;       // no other walk reads its blocks
     int frow;       // its first fragment, in rows of a chunk of heads; -1: one piece that ends its row
 };
@@ -61,10 +62,12 @@ struct Head {
     int magic, S, MB, heads, kv_heads, head_dim;
     int wide;       // walks
     int walks;      //   in all
-    int wide_cost;  // the list's wide part
-    int total;
-    int len;        // of a workgroup's range; a wave's part of what is narrow is a quarter of it
-    int pad[5];
+    int wide_end;   // of the wide walks' costs,
+    int narrow_end; //   and of the narrow ones'
+    int wide_len;   // of a range of the wide walks
+    int narrow_len; // and of one of the narrow, of which a wave has a quarter
+    int wide_ranges;
+    int pad[3];
 };
 
 struct Seq {
@@ -116,7 +119,7 @@ inline Layout layout_of(long long S, int H, int Hkv) {
     const auto up = [](long long n) { return static_cast<size_t>((n + 255) / 256 * 256); };
     const Heads h = heads_of(H, Hkv);
     Layout l;
-    l.ranges = std::max(kResident / h.HC, 1);
+    l.ranges = std::max(kResident / h.HC, 2);     // (what is wide and what is narrow have ranges of their own)
     l.wide_starts = 256;
     l.narrow_starts = l.wide_starts + up(static_cast<long long>(sizeof(Start)) * l.ranges);
     l.walks = l.narrow_starts + up(static_cast<long long>(sizeof(Start)) * l.ranges * kTileWaves);

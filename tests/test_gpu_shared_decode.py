@@ -446,3 +446,22 @@ def test_random_sweep(dev):
         kw = dict(cap=float(rng.choice([0, 0, 25])), alibi=bool(rng.random() < 0.3), lone=int(rng.integers(0, 3)), tight=bool(rng.random() < 0.3))
         print(H, Hkv, D, dtype, [(p, len(c)) for p, c in groups], kw, flush=True)
         Shared(rng, groups, H, Hkv, D, dtype, **kw).run().check()
+
+
+@pytest.mark.parametrize("Hkv,G", [(300, 1), (520, 1), (130, 2)])
+def test_more_heads_than_workgroups(dev, Hkv, G):
+    """Two ranges for each chunk of heads, one of what is wide and one of what is not."""
+    rng = np.random.default_rng(Hkv)
+    s = Shared(rng, [(336, [340 + i for i in range(20)]), (64, [70, 90])], Hkv * G, Hkv, 64, "f16")
+    s.run().check()
+    s = Shared(rng, [(336, [336] * 20)], Hkv * G, Hkv, 64, "f16")      # nothing but what is wide
+    s.run().check()
+
+
+@pytest.mark.parametrize("each,shared,own", [(24, 800, 3), (24, 48, 900), (3, 640, 400), (130, 1600, 1)])
+def test_shares_of_what_is_wide(dev, each, shared, own):
+    """Mostly wide, mostly narrow, wholly narrow, and tiles that share with others."""
+    rng = np.random.default_rng(each + own)
+    for D, dtype in ((64, "bf16"), (128, "f16")):
+        s = Shared(rng, [(shared, [shared + int(rng.integers(0, own + 1)) for _ in range(each)]) for _ in range(3)], 8, 2, D, dtype)
+        s.run().check()
