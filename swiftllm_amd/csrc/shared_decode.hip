@@ -26,7 +26,8 @@
 // questions on 30000 tokens, 64/8 heads, with distance biases 137 and 138. What is left
 // over is a range's start (its walk, ids, queries, a first step: 2.5 us), the ranges'
 // unequal ends and the second launch, 4 us. One walk of 128 rows on 131072 tokens takes
-// 117 us (with 64 keys a step and two of them 132, with the compiler's waits 159).
+// 121 us (117, and with 64 keys a step and two of them 132, with the compiler's waits
+// 159, before the few other blocks had a range of their own).
 
 #include <algorithm>
 #include <cmath>
