@@ -394,8 +394,10 @@ __global__ __launch_bounds__(THREADS) void beam_pick_kernel(const SelectArgs a) 
         }
         for (int d = 1; d < span; d <<= 1) S += __shfl_xor(S, d);
         if (at == 0 && real) {
-            s_base[b] = scored ? score - log(S) : -INFINITY;
-            s_top[b] = scored ? top : 0.0f;
+            // (a row that allows nothing is one of a beam without a score)
+            const bool some = top > -INFINITY;
+            s_base[b] = some ? score - log(S) : -INFINITY;
+            s_top[b] = some ? top : 0.0f;
         }
     }
     auto rest_of = [&](int h, int i) {
@@ -446,7 +448,7 @@ __global__ __launch_bounds__(THREADS) void beam_pick_kernel(const SelectArgs a) 
     bool some = false;     // the lists named in s_list
     float line = 0.0f;
     if constexpr (!SMALL) {
-        // (a beam without a score has no sums)
+        // (a beam without a score has no sums, or nothing in its lists)
         auto list_max = [&](int i) {
             const int b = i / a.chunks;
             return s_base[b] > -INFINITY ? static_cast<float>(score_of(b, a.sums[slot0 + i].x)) : -INFINITY;
