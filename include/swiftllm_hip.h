@@ -609,10 +609,9 @@ size_t swiftllm_hip_beam_select_workspace_size(int num_requests,
  * block_tables and context_lens (any number that is no row: it ends, with a
  * context of 0). ref_counts[b] is how many rows hold block b, in all tables of
  * the pool; it loses the old rows' holds and gains the new ones'. A partly
- * filled last block is about to be written: of the rows with the same parent,
- * the r-th (from 0) gets a block of its own where r < ref_counts[b] - 1, the
- * holds before any copy, so that one child keeps it unless others hold it. Copies take
- * the lowest blocks that nothing refers to, rows in order; copy_pairs int64
+ * filled last block is about to be written: the rows whose last block it is, of
+ * whatever parents, get a block of their own each, but for the last of them where
+ * ref_counts[b], before any copy, counts nobody else. Copies take the lowest blocks that nothing refers to, rows in order; copy_pairs int64
  * [num_seqs][2] holds their (source, destination) for swiftllm_hip_copy_blocks,
  * which has to run before the next token is written, and -1 behind them. A row
  * that finds none loses its last, partly filled block: its context ends with

@@ -510,16 +510,19 @@ def fork_pages(block_tables_out, block_tables, context_lens, parents, ref_counts
                 count(int(b), 1)
     holds = list(refs)
     spare = [b for b in range(NB) if holds[b] <= 0]
-    pairs, cut, copies, seen = [], 0, 0, {}
-    for i, p in enumerate(parents):
-        older = seen.get(int(p), 0)
-        seen[int(p)] = older + 1
+    opened = [-1] * S     # the block that a row is about to write
+    for i in range(S):
         j = ctx[i] // 16
-        if ctx[i] % 16 == 0 or j >= MB:
+        if ctx[i] % 16 and j < MB and 0 <= tables[i, j] < NB:
+            opened[i] = int(tables[i, j])
+    last = {b: i for i, b in enumerate(opened)}
+    rows = {b: opened.count(b) for b in last}
+    pairs, cut, copies = [], 0, 0
+    for i, b in enumerate(opened):
+        # (the last of them keeps it, where nobody else holds it)
+        if b < 0 or (i == last[b] and rows[b] >= holds[b]):
             continue
-        b = int(tables[i, j])
-        if not 0 <= b < NB or older >= holds[b] - 1:
-            continue
+        j = ctx[i] // 16
         refs[b] -= 1
         if copies < len(spare):
             new = spare[copies]
