@@ -599,7 +599,19 @@ int swiftllm_hip_beam_select(
     int vocab, int num_candidates, long long logits_stride, int eos_id,
     hipStream_t stream);
 
-/* Bytes of workspace it needs for these sizes; 0 where it would refuse them. */
+/* The same for the rows of a step: one that brought no token, query_offsets[row + 1]
+ * <= query_offsets[row] (num_requests * beam_width + 1 entries, as
+ * swiftllm_hip_plan_step writes them; NULL: every row did), has no logits and
+ * counts as one of a beam without a score. */
+int swiftllm_hip_beam_select_rows(
+    const void* logits, const float* beam_scores, const int32_t* query_offsets,
+    float* cand_scores, int32_t* cand_rows, int32_t* cand_tokens,
+    float* next_scores, int32_t* next_rows, int32_t* next_tokens,
+    void* workspace, size_t workspace_bytes, int dtype, int num_requests,
+    int beam_width, int vocab, int num_candidates, long long logits_stride,
+    int eos_id, hipStream_t stream);
+
+/* Bytes of workspace they need for these sizes; 0 where they would refuse them. */
 size_t swiftllm_hip_beam_select_workspace_size(int num_requests,
                                                int beam_width, int vocab,
                                                int num_candidates);

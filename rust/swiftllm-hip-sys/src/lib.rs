@@ -290,6 +290,14 @@ extern "C" {
         vocab: c_int, num_candidates: c_int, logits_stride: c_longlong, eos_id: c_int,
         stream: hipStream_t,
     ) -> c_int;
+    pub fn swiftllm_hip_beam_select_rows(
+        logits: *const c_void, beam_scores: *const c_float, query_offsets: *const i32,
+        cand_scores: *mut c_float, cand_rows: *mut i32, cand_tokens: *mut i32,
+        next_scores: *mut c_float, next_rows: *mut i32, next_tokens: *mut i32,
+        workspace: *mut c_void, workspace_bytes: usize, dtype: c_int, num_requests: c_int,
+        beam_width: c_int, vocab: c_int, num_candidates: c_int, logits_stride: c_longlong,
+        eos_id: c_int, stream: hipStream_t,
+    ) -> c_int;
     pub fn swiftllm_hip_beam_select_workspace_size(
         num_requests: c_int, beam_width: c_int, vocab: c_int, num_candidates: c_int,
     ) -> usize;

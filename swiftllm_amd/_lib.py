@@ -106,6 +106,8 @@ SIGNATURES = {
               i32, i32, vp]),
     "swiftllm_hip_beam_select": (
         i32, [vp, vp, vp, vp, vp, vp, vp, vp, vp, sz, i32, i32, i32, i32, i32, i64, i32, vp]),
+    "swiftllm_hip_beam_select_rows": (
+        i32, [vp, vp, vp, vp, vp, vp, vp, vp, vp, vp, sz, i32, i32, i32, i32, i32, i64, i32, vp]),
     "swiftllm_hip_beam_select_workspace_size": (sz, [i32, i32, i32, i32]),
     "swiftllm_hip_fork_pages": (
         i32, [vp, vp, vp, vp, vp, vp, vp, vp, vp, vp, vp, vp, vp, sz, i32, i32, i32, i32, vp]),

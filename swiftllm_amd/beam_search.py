@@ -39,17 +39,19 @@ def beam_select(logits: Ptr, beam_scores: Ptr, cand_scores: Ptr, cand_rows: Ptr,
                 next_scores: Ptr, next_rows: Ptr, next_tokens: Ptr, workspace: Ptr,
                 workspace_bytes: int, num_requests: int, beam_width: int, vocab: int,
                 num_candidates: int, dtype: str = "f32", logits_stride: Optional[int] = None,
-                eos_id: int = -1, stream: Optional[Stream] = None) -> None:
+                eos_id: int = -1, stream: Optional[Stream] = None, query_offsets: Ptr = None) -> None:
     """The num_candidates largest of beam_scores[row] + log softmax(logits[row])
     over the rows request * beam_width + beam of every request and their tokens,
     in descending order, and the first beam_width of them that do not end with
     eos_id (swiftllm_hip_beam_select): scores float32, rows and tokens int32,
     -inf, -1 and -1 where there is none. next_rows are the parents of
-    pages.fork_pages; next_scores may be beam_scores."""
+    pages.fork_pages; next_scores may be beam_scores. query_offsets int32 [rows + 1],
+    as plan_step writes them: rows without a token in them have no logits, and their
+    beams no score (swiftllm_hip_beam_select_rows)."""
     if dtype not in LOGIT_DTYPES:
         raise NotSupported(f"dtype {dtype!r} (supported: {', '.join(LOGIT_DTYPES)})")
-    check_status(_lib.lib().swiftllm_hip_beam_select(
-        _p(logits), _p(beam_scores), _p(cand_scores), _p(cand_rows), _p(cand_tokens),
+    check_status(_lib.lib().swiftllm_hip_beam_select_rows(
+        _p(logits), _p(beam_scores), _p(query_offsets), _p(cand_scores), _p(cand_rows), _p(cand_tokens),
         _p(next_scores), _p(next_rows), _p(next_tokens), _p(workspace), workspace_bytes,
         LOGIT_DTYPES[dtype], num_requests, beam_width, vocab, num_candidates,
         vocab if logits_stride is None else logits_stride, eos_id, _s(stream)))
@@ -75,8 +77,8 @@ class BeamSearch:
     blocks are free again. A row that ended, that fork() cut or that plan() refused
     because no block was free (counts[1], step.counts[2]) brings no token, and the
     tokens of the rows behind it move up: row s's is token step.query_offsets[s] of the
-    step. select() takes its logits in row s; one without a token has none to give,
-    and its score is the caller's to set to -inf.
+    step. select() takes its logits in row s; one without a token has none to give, and
+    ends there.
 
     The calls are asynchronous on `stream`, in that order; all but start() and
     compact() may be captured. fork() changes between two sets of tables, and what it
@@ -159,13 +161,15 @@ class BeamSearch:
 
     def select(self, logits: Ptr, logits_stride: Optional[int] = None,
                stream: Optional[Stream] = None) -> None:
-        """The best continuations (beam_select) of logits [num_seqs, vocab]; scores
-        become those of the rows that go on."""
+        """The best continuations (beam_select) of logits [num_seqs, vocab], of the rows
+        that brought a token in the plan() before; scores become those of the rows that
+        go on."""
         beam_select(logits, self.scores, self.cand_scores, self.cand_rows, self.cand_tokens,
                     self.scores, self.next_rows, self.next_tokens, self._select_space,
                     self._select_space.nbytes, self.num_requests, self.beam_width, self.vocab,
                     self.num_candidates, dtype=self.dtype, logits_stride=logits_stride,
-                    eos_id=self.eos_id, stream=stream)
+                    eos_id=self.eos_id, stream=stream,
+                    query_offsets=None if self._planned is None else self._planned.query_offsets)
 
     def fork(self, key_caches: Sequence[Ptr], value_caches: Sequence[Ptr], num_kv_heads: int,
              head_dim: int, stream: Optional[Stream] = None) -> None:

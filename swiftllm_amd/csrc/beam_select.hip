@@ -63,6 +63,7 @@ struct Entry {
 struct SelectArgs {
     const void* logits;
     const float* scores;        // [R * W]
+    const int* offsets;         // [R * W + 1] or null: a row whose own are not ascending has no logits
     float* cand_scores;         // [R][C]
     int* cand_rows;
     int* cand_tokens;
@@ -150,6 +151,12 @@ __device__ __forceinline__ float load_one(const void* row, long long i) {
     }
 }
 
+// The score of a row's beam: none where the row has no logits.
+__device__ __forceinline__ float score_of_row(const SelectArgs& a, size_t row) {
+    const float score = a.scores[row];
+    return a.offsets != nullptr && a.offsets[row + 1] <= a.offsets[row] ? -INFINITY : score;
+}
+
 // A sum of exp(x - m) as one of exp(x - top), top >= m.
 __device__ __forceinline__ float weighed(float sum, float m, float top) {
     return m == top ? sum : sum * __builtin_amdgcn_exp2f((m - top) * kLog2e);
@@ -185,8 +192,7 @@ __global__ __launch_bounds__(kThreads) void beam_chunk_kernel(const SelectArgs a
     const int row = blockIdx.x / a.chunks;
     const int chunk = blockIdx.x - row * a.chunks;
     const size_t slot = static_cast<size_t>(row) * a.chunks + chunk;
-    const float score = a.scores[row];
-    if (!(score > -INFINITY)) {
+    if (!(score_of_row(a, row) > -INFINITY)) {
         // Nothing comes of this beam.
         if (tid == 0) a.fill[slot] = 0;
         return;
@@ -378,7 +384,7 @@ __global__ __launch_bounds__(THREADS) void beam_pick_kernel(const SelectArgs a) 
         const int b = b0 + tid / span;
         const bool real = b < a.W;
         const size_t row = static_cast<size_t>(r) * a.W + (real ? b : 0);
-        const float score = a.scores[row];
+        const float score = score_of_row(a, row);
         const float2* const sums = a.sums + row * a.chunks;
         const float2 mine = at < a.chunks ? sums[at] : float2{-INFINITY, 0.0f};
         // (a beam without a score has no sums)
@@ -659,26 +665,10 @@ int check_sizes(const char* who, long long R, long long W, long long V, long lon
     return SWIFTLLM_OK;
 }
 
-}  // namespace
-}  // namespace swiftllm
-
-using namespace swiftllm;
-
-extern "C" {
-
-size_t swiftllm_hip_beam_select_workspace_size(int num_requests, int beam_width, int vocab, int num_candidates) {
-    if (check_sizes("swiftllm_hip_beam_select_workspace_size", num_requests, beam_width, vocab, num_candidates) != SWIFTLLM_OK) {
-        return 0;
-    }
-    ok();
-    return space_of(static_cast<long long>(num_requests) * beam_width, vocab).bytes;
-}
-
-int swiftllm_hip_beam_select(const void* logits, const float* beam_scores, float* cand_scores, int32_t* cand_rows,
-                             int32_t* cand_tokens, float* next_scores, int32_t* next_rows, int32_t* next_tokens,
-                             void* workspace, size_t workspace_bytes, int dtype, int num_requests, int beam_width,
-                             int vocab, int num_candidates, long long logits_stride, int eos_id, hipStream_t stream) {
-    const char* who = "swiftllm_hip_beam_select";
+int select(const char* who, const void* logits, const float* beam_scores, const int32_t* query_offsets, float* cand_scores,
+           int32_t* cand_rows, int32_t* cand_tokens, float* next_scores, int32_t* next_rows, int32_t* next_tokens,
+           void* workspace, size_t workspace_bytes, int dtype, int num_requests, int beam_width, int vocab,
+           int num_candidates, long long logits_stride, int eos_id, hipStream_t stream) {
     const long long R = num_requests, W = beam_width, V = vocab, C = num_candidates;
     int rc = check_sizes(who, R, W, V, C);
     if (rc != SWIFTLLM_OK) return rc;
@@ -698,7 +688,8 @@ int swiftllm_hip_beam_select(const void* logits, const float* beam_scores, float
     const Bytes span[] = {{cand_scores, 4 * static_cast<size_t>(R * C)}, {cand_rows, 4 * static_cast<size_t>(R * C)},
                           {cand_tokens, 4 * static_cast<size_t>(R * C)}, {next_scores, 4 * rows}, {next_rows, 4 * rows},
                           {next_tokens, 4 * rows}, {workspace, space.bytes}, {beam_scores, 4 * rows},
-                          {logits, rows == 0 ? 0 : (static_cast<size_t>(logits_stride) * (rows - 1) + V) * size}};
+                          {logits, rows == 0 ? 0 : (static_cast<size_t>(logits_stride) * (rows - 1) + V) * size},
+                          {query_offsets, 4 * (rows + 1)}};
     for (const Bytes& s : span) {
         if (!aligned(s.p, s.p == logits ? size : 4)) return fail(SWIFTLLM_ERR_INVALID_PARAMETER, "%s: misaligned pointer", who);
     }
@@ -707,7 +698,7 @@ int swiftllm_hip_beam_select(const void* logits, const float* beam_scores, float
         return fail(SWIFTLLM_ERR_INVALID_PARAMETER, "%s: workspace of %zu bytes, %zu needed", who, workspace_bytes, space.bytes);
     }
     for (int i = 0; i < 7; ++i) {
-        for (int j = i + 1; j < 9; ++j) {
+        for (int j = i + 1; j < 10; ++j) {
             // The next step's beams may take the place of this step's: a workgroup
             // has read its request's before it writes them.
             if (i == 3 && j == 7 && next_scores == beam_scores) continue;
@@ -722,6 +713,7 @@ int swiftllm_hip_beam_select(const void* logits, const float* beam_scores, float
     SelectArgs a{};
     a.logits = logits;
     a.scores = beam_scores;
+    a.offsets = query_offsets;
     a.cand_scores = cand_scores;
     a.cand_rows = cand_rows;
     a.cand_tokens = cand_tokens;
@@ -745,6 +737,40 @@ int swiftllm_hip_beam_select(const void* logits, const float* beam_scores, float
     const long long lists = W * space.chunks;
     const K pick = lists <= 16 ? beam_pick_kernel<256, true> : lists <= 64 ? beam_pick_kernel<1024, true> : beam_pick_kernel<1024, false>;
     return launched(launch(pick, dim3(static_cast<unsigned>(R)), dim3(lists <= 16 ? 256 : 1024), 0, stream, a), who);
+}
+
+}  // namespace
+}  // namespace swiftllm
+
+using namespace swiftllm;
+
+extern "C" {
+
+size_t swiftllm_hip_beam_select_workspace_size(int num_requests, int beam_width, int vocab, int num_candidates) {
+    if (check_sizes("swiftllm_hip_beam_select_workspace_size", num_requests, beam_width, vocab, num_candidates) != SWIFTLLM_OK) {
+        return 0;
+    }
+    ok();
+    return space_of(static_cast<long long>(num_requests) * beam_width, vocab).bytes;
+}
+
+int swiftllm_hip_beam_select(const void* logits, const float* beam_scores, float* cand_scores, int32_t* cand_rows,
+                             int32_t* cand_tokens, float* next_scores, int32_t* next_rows, int32_t* next_tokens,
+                             void* workspace, size_t workspace_bytes, int dtype, int num_requests, int beam_width,
+                             int vocab, int num_candidates, long long logits_stride, int eos_id, hipStream_t stream) {
+    return select("swiftllm_hip_beam_select", logits, beam_scores, nullptr, cand_scores, cand_rows, cand_tokens, next_scores,
+                  next_rows, next_tokens, workspace, workspace_bytes, dtype, num_requests, beam_width, vocab, num_candidates,
+                  logits_stride, eos_id, stream);
+}
+
+int swiftllm_hip_beam_select_rows(const void* logits, const float* beam_scores, const int32_t* query_offsets,
+                                  float* cand_scores, int32_t* cand_rows, int32_t* cand_tokens, float* next_scores,
+                                  int32_t* next_rows, int32_t* next_tokens, void* workspace, size_t workspace_bytes,
+                                  int dtype, int num_requests, int beam_width, int vocab, int num_candidates,
+                                  long long logits_stride, int eos_id, hipStream_t stream) {
+    return select("swiftllm_hip_beam_select_rows", logits, beam_scores, query_offsets, cand_scores, cand_rows, cand_tokens,
+                  next_scores, next_rows, next_tokens, workspace, workspace_bytes, dtype, num_requests, beam_width, vocab,
+                  num_candidates, logits_stride, eos_id, stream);
 }
 
 }  // extern "C"
