@@ -322,6 +322,7 @@ class AttentionStep:
         self.counts = DeviceArray((3,), np.int32)
         self.query = DeviceArray((max(num_tokens, 1), num_heads, head_dim), np.uint16)
         self._tables: Ptr = None
+        self.plans = 0      # calls of plan()
         self.num_groups, self._grouped = num_groups, False
         if num_groups:
             sizes = self._sizes()
@@ -344,6 +345,7 @@ class AttentionStep:
                   self.num_seqs, self.max_num_blocks_per_seq, self.block_size, self.num_tokens,
                   self.context_lens, self.query_offsets, self.positions, self.slot_mapping,
                   self.counts, num_blocks=num_blocks, stream=stream)
+        self.plans += 1
         self._tables = block_tables
         self._grouped = group_offsets is not None
         if self._grouped:

@@ -80,6 +80,11 @@ class BeamSearch:
     step. select() takes its logits in row s; one without a token has none to give, and
     ends there.
 
+    From plan() to the next fork() the step's arrays hold what the search goes on from:
+    select() and fork() refuse one that was planned again meanwhile, by another search
+    or otherwise. Searches with one step between them change over after a fork(); one
+    that is captured has a step of its own.
+
     The calls are asynchronous on `stream`, in that order; all but start() and
     compact() may be captured. fork() changes between two sets of tables, and what it
     counts is of the plan() before: a graph holds an even number of steps, and is
@@ -118,7 +123,7 @@ class BeamSearch:
         self.free_blocks, self.num_free = DeviceArray.zeros((num_blocks,), i32), DeviceArray.zeros((1,), i32)
         self.copy_pairs, self.counts = DeviceArray((S, 2), np.int64), DeviceArray((2,), i32)
         self.group_offsets = DeviceArray.from_numpy(np.arange(R + 1, dtype=i32) * W)
-        self._now, self._planned = 0, None
+        self._now, self._planned, self._plan_number = 0, None, 0
 
     @property
     def block_tables(self) -> DeviceArray:
@@ -128,7 +133,14 @@ class BeamSearch:
     @property
     def context_lens(self) -> DeviceArray:
         """[num_seqs]: after plan() with the token that the step brings."""
-        return self._lens[self._now] if self._planned is None else self._planned.context_lens
+        step = self._its_step()
+        return self._lens[self._now] if step is None else step.context_lens
+
+    def _its_step(self) -> Optional[AttentionStep]:
+        """What the last plan() planned, where there was no fork() since."""
+        if self._planned is not None and self._planned.plans != self._plan_number:
+            raise InvalidParameter("the step of the last plan() was planned again before fork()")
+        return self._planned
 
     def start(self, block_tables: np.ndarray, context_lens: np.ndarray) -> None:
         """Tables [num_requests, at most max_num_blocks_per_seq] and lengths of the
@@ -164,18 +176,19 @@ class BeamSearch:
         """The best continuations (beam_select) of logits [num_seqs, vocab], of the rows
         that brought a token in the plan() before; scores become those of the rows that
         go on."""
+        step = self._its_step()
         beam_select(logits, self.scores, self.cand_scores, self.cand_rows, self.cand_tokens,
                     self.scores, self.next_rows, self.next_tokens, self._select_space,
                     self._select_space.nbytes, self.num_requests, self.beam_width, self.vocab,
                     self.num_candidates, dtype=self.dtype, logits_stride=logits_stride,
                     eos_id=self.eos_id, stream=stream,
-                    query_offsets=None if self._planned is None else self._planned.query_offsets)
+                    query_offsets=None if step is None else step.query_offsets)
 
     def fork(self, key_caches: Sequence[Ptr], value_caches: Sequence[Ptr], num_kv_heads: int,
              head_dim: int, stream: Optional[Stream] = None) -> None:
         """The chosen rows' tables (fork_pages), and in every layer's caches the
         copies of the blocks that they are about to write."""
-        now, planned = self._now, self._planned
+        now, planned = self._now, self._its_step()
         fork_pages(self._tables[1 - now], self._lens[1 - now], self._tables[now], self.context_lens,
                    self.next_rows, self.ref_counts, self.free_blocks, self.num_free,
                    self.copy_pairs, self.counts, self._pages_space, self._pages_space.nbytes,
@@ -198,7 +211,7 @@ class BeamSearch:
         step.plan(self.block_tables, self.context_lens, self.new_lens, self.free_blocks,
                   self.num_free, self.num_blocks, num_blocks=self.num_blocks, stream=stream,
                   group_offsets=self.group_offsets if step.num_groups else None)
-        self._planned = step
+        self._planned, self._plan_number = step, step.plans
 
     def compact(self, key_caches: Sequence[Ptr], value_caches: Sequence[Ptr], num_kv_heads: int,
                 head_dim: int, new_ids: DeviceArray, max_moves: int,
