@@ -188,6 +188,7 @@ class BeamSearch:
              head_dim: int, stream: Optional[Stream] = None) -> None:
         """The chosen rows' tables (fork_pages), and in every layer's caches the
         copies of the blocks that they are about to write."""
+        self._check_caches(key_caches, value_caches, num_kv_heads, head_dim)
         now, planned = self._now, self._its_step()
         fork_pages(self._tables[1 - now], self._lens[1 - now], self._tables[now], self.context_lens,
                    self.next_rows, self.ref_counts, self.free_blocks, self.num_free,
@@ -198,6 +199,17 @@ class BeamSearch:
         self._now, self._planned = 1 - now, None
         copy_blocks(key_caches, value_caches, self.copy_pairs, self.num_seqs, num_kv_heads,
                     head_dim, self.block_size, stream=stream)
+
+    @staticmethod
+    def _check_caches(key_caches: Sequence[Ptr], value_caches: Sequence[Ptr], num_kv_heads: int,
+                      head_dim: int) -> None:
+        """What copy_blocks would refuse, before tables change that its copies belong to."""
+        if len(key_caches) != len(value_caches):
+            raise InvalidParameter(f"{len(key_caches)} key caches but {len(value_caches)} value caches")
+        if num_kv_heads <= 0 or head_dim <= 0:
+            raise InvalidParameter(f"num_kv_heads {num_kv_heads} head_dim {head_dim}")
+        if not all(_p(c) for c in (*key_caches, *value_caches)):
+            raise InvalidParameter("null cache")
 
     def plan(self, step: AttentionStep, stream: Optional[Stream] = None) -> None:
         """step.plan() of the rows that go on, by requests where the step has groups."""
@@ -224,6 +236,7 @@ class BeamSearch:
             raise InvalidParameter("compact() between plan() and fork()")
         if max_moves < 0:
             raise InvalidParameter(f"max_moves {max_moves}")
+        self._check_caches(key_caches, value_caches, num_kv_heads, head_dim)
         pairs = DeviceArray((max(max_moves, 1), 2), np.int64)
         refs = DeviceArray((self.num_blocks,), np.int32)
         compact_pages(self.block_tables, refs, self.block_tables, self.context_lens,

@@ -5,7 +5,7 @@ import numpy as np
 import pytest
 
 from swiftllm_amd import paged_attention as pa
-from swiftllm_amd._hip import synchronize
+from swiftllm_amd._hip import DeviceArray, synchronize
 from test_gpu_beam_search import start
 
 pytestmark = pytest.mark.gpu
@@ -45,3 +45,28 @@ def test_two_searches_on_one_step(dev):
     for k, v in before.items():
         assert np.array_equal(getattr(a.search, k).numpy(), v), k
     b.steps(2, taken=taken[b])
+
+
+@pytest.mark.parametrize("bad", ["lists", "null", "heads", "head_dim"])
+def test_caches_that_are_refused(dev, bad):
+    """By fork() and by compact(), with the tables as they were: the same call with the right caches goes on from them."""
+    s = _search()
+    k, v = [c[0] for c in s.caches], [c[1] for c in s.caches]
+    args = dict(lists=(k, v[:1], 2, 64), null=([k[0], None], v, 2, 64), heads=(k, v, 0, 64), head_dim=(k, v, 2, -64))[bad]
+    taken = s.steps(1)
+    s.inputs()
+    s.search.select(s.d_logits)
+    before = _state(s)
+    with pytest.raises(pa.InvalidParameter):
+        s.search.fork(*args)
+    for key, x in _state(s).items():
+        assert np.array_equal(x, before[key]), key
+    s.search.fork(k, v, 2, 64)
+    before = _state(s)
+    with pytest.raises(pa.InvalidParameter):
+        s.search.compact(*args, DeviceArray((80,), np.int32), 80)
+    for key, x in _state(s).items():
+        assert np.array_equal(x, before[key]), key
+    s.layers()
+    synchronize()
+    s.check(taken)
