@@ -122,6 +122,7 @@ class BeamSearch:
         self.ref_counts = DeviceArray.zeros((num_blocks,), i32)
         self.free_blocks, self.num_free = DeviceArray.zeros((num_blocks,), i32), DeviceArray.zeros((1,), i32)
         self.copy_pairs, self.counts = DeviceArray((S, 2), np.int64), DeviceArray((2,), i32)
+        self.compact_counts = DeviceArray.zeros((2,), i32)
         self.group_offsets = DeviceArray.from_numpy(np.arange(R + 1, dtype=i32) * W)
         self._now, self._planned, self._plan_number = 0, None, 0
 
@@ -230,7 +231,8 @@ class BeamSearch:
                 stream: Optional[Stream] = None) -> None:
         """After fork(): the blocks in use to the pool's front, at most max_moves of
         them (compact_pages), in the tables, the references and every layer's caches.
-        new_ids int32 [num_blocks] is for whoever else holds blocks. Waits for the
+        new_ids int32 [num_blocks] is for whoever else holds blocks, compact_counts are
+        (moves, blocks in use); counts stay those of the fork(). Waits for the
         device and allocates: not for a capture."""
         if self._planned is not None:
             raise InvalidParameter("compact() between plan() and fork()")
@@ -240,7 +242,7 @@ class BeamSearch:
         pairs = DeviceArray((max(max_moves, 1), 2), np.int64)
         refs = DeviceArray((self.num_blocks,), np.int32)
         compact_pages(self.block_tables, refs, self.block_tables, self.context_lens,
-                      self.ref_counts, self.free_blocks, self.num_free, pairs, new_ids, self.counts,
+                      self.ref_counts, self.free_blocks, self.num_free, pairs, new_ids, self.compact_counts,
                       self._pages_space, self._pages_space.nbytes, self.num_seqs,
                       self.max_num_blocks_per_seq, self.block_size, self.num_blocks, max_moves,
                       stream=stream)

@@ -70,3 +70,18 @@ def test_caches_that_are_refused(dev, bad):
     s.layers()
     synchronize()
     s.check(taken)
+
+
+def test_compact_keeps_the_counts_of_the_fork(dev):
+    """How many rows fork() cut is there after compact() too, which counts by itself."""
+    s = start(np.random.default_rng(5), [30, 30], 4, 32, 8, 7, 4, 2, 64, "f16")
+    s.inputs()
+    s.forked()
+    synchronize()
+    counts, refs = s.search.counts.numpy(), s.search.ref_counts.numpy()
+    assert counts[1] > 0
+    s.search.compact([c[0] for c in s.caches], [c[1] for c in s.caches], 2, 64, DeviceArray((7,), np.int32), 7)
+    synchronize()
+    assert np.array_equal(s.search.counts.numpy(), counts)
+    used = np.flatnonzero(refs)
+    assert s.search.compact_counts.numpy().tolist() == [(used >= len(used)).sum(), len(used)]
