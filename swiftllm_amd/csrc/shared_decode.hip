@@ -770,7 +770,8 @@ int swiftllm_hip_shared_decode(void* output, void* workspace, size_t workspace_b
     }
     rc = require_device();
     if (rc != SWIFTLLM_OK) return rc;
-    if (num_seqs == 0) return ok();
+    // (lanes without a query read row 0, which is there where any row is)
+    if (num_seqs == 0 || (query_offsets && num_tokens == 0)) return ok();
     // The sign of the scale goes into the query, and a scale of zero makes it zero: the
     // kernel's scale is positive, so that raw products order as scores.
     a.q_and = scale == 0.0f ? 0u : 0xffffffffu;
