@@ -148,7 +148,8 @@ class BeamSearch:
         prompts; requests may share blocks, as prompts that begin alike do. Every
         other block of the pool is free. Synchronous."""
         R, W, BS, MB = self.num_requests, self.beam_width, self.block_size, self.max_num_blocks_per_seq
-        bt, lens = np.asarray(block_tables, np.int32), np.asarray(context_lens, np.int32)
+        # (64 bits until ids and lengths are known to fit 32)
+        bt, lens = np.asarray(block_tables, np.int64), np.asarray(context_lens, np.int64)
         if bt.ndim != 2 or bt.shape[0] != R or bt.shape[1] > MB or lens.shape != (R,):
             raise InvalidParameter(f"block_tables {bt.shape} and context_lens {lens.shape} of {R} requests")
         if (lens < 0).any() or (lens > bt.shape[1] * BS).any():

@@ -85,3 +85,16 @@ def test_compact_keeps_the_counts_of_the_fork(dev):
     assert np.array_equal(s.search.counts.numpy(), counts)
     used = np.flatnonzero(refs)
     assert s.search.compact_counts.numpy().tolist() == [(used >= len(used)).sum(), len(used)]
+
+
+def test_ids_and_lengths_past_32_bits_are_refused(dev):
+    """Numbers that a cast to 32 bits would bring back into range."""
+    s = _search()
+    s.search.start(np.array([[3, 4], [5, 6]]), np.array([20, 32]))
+    for tables, lens in (([[3, 4], [2 ** 32 + 5, 6]], [20, 32]), ([[3, 4], [5, -2 ** 32]], [20, 32]),
+                         ([[3, 4], [5, 6]], [2 ** 32 + 4, 32]), ([[3, 4], [5, 6]], [20, 16 - 2 ** 32])):
+        with pytest.raises(pa.InvalidParameter):
+            s.search.start(np.array(tables), np.array(lens))
+    # (entries behind a prompt may hold anything)
+    s.search.start(np.array([[3, 2 ** 40], [5, 6]]), np.array([16, 32]))
+    assert s.search.ref_counts.numpy()[[3, 5, 6]].tolist() == [1, 1, 1] and int(s.search.num_free.numpy()[0]) == 77
