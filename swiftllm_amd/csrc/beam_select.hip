@@ -151,12 +151,6 @@ __device__ __forceinline__ float load_one(const void* row, long long i) {
     }
 }
 
-// The score of a row's beam: none where the row has no logits.
-__device__ __forceinline__ float score_of_row(const SelectArgs& a, size_t row) {
-    const float score = a.scores[row];
-    return a.offsets != nullptr && a.offsets[row + 1] <= a.offsets[row] ? -INFINITY : score;
-}
-
 // A sum of exp(x - m) as one of exp(x - top), top >= m.
 __device__ __forceinline__ float weighed(float sum, float m, float top) {
     return m == top ? sum : sum * __builtin_amdgcn_exp2f((m - top) * kLog2e);
@@ -192,9 +186,12 @@ __global__ __launch_bounds__(kThreads) void beam_chunk_kernel(const SelectArgs a
     const int row = blockIdx.x / a.chunks;
     const int chunk = blockIdx.x - row * a.chunks;
     const size_t slot = static_cast<size_t>(row) * a.chunks + chunk;
-    if (!(score_of_row(a, row) > -INFINITY)) {
+    if (!(a.scores[row] > -INFINITY) || (a.offsets != nullptr && a.offsets[row + 1] <= a.offsets[row])) {
         // Nothing comes of this beam.
-        if (tid == 0) a.fill[slot] = 0;
+        if (tid == 0) {
+            a.fill[slot] = 0;
+            a.sums[slot] = float2{-INFINITY, 0.0f};
+        }
         return;
     }
     if (tid == 0) s_fill = 0;
@@ -384,20 +381,14 @@ __global__ __launch_bounds__(THREADS) void beam_pick_kernel(const SelectArgs a) 
         const int b = b0 + tid / span;
         const bool real = b < a.W;
         const size_t row = static_cast<size_t>(r) * a.W + (real ? b : 0);
-        const float score = score_of_row(a, row);
+        const float score = a.scores[row];
         const float2* const sums = a.sums + row * a.chunks;
         const float2 mine = at < a.chunks ? sums[at] : float2{-INFINITY, 0.0f};
-        // (a beam without a score has no sums)
-        const bool scored = real && score > -INFINITY;
-        float top = scored ? mine.x : -INFINITY;
-        if (scored) {
-            for (int c = at + 64; c < a.chunks; c += 64) top = fmaxf(top, sums[c].x);
-        }
+        float top = mine.x;
+        for (int c = at + 64; c < a.chunks; c += 64) top = fmaxf(top, sums[c].x);
         for (int d = 1; d < span; d <<= 1) top = fmaxf(top, __shfl_xor(top, d));
-        double S = scored ? weighed(mine.y, mine.x, top) : 0.0f;
-        if (scored) {
-            for (int c = at + 64; c < a.chunks; c += 64) S += weighed(sums[c].y, sums[c].x, top);
-        }
+        double S = weighed(mine.y, mine.x, top);
+        for (int c = at + 64; c < a.chunks; c += 64) S += weighed(sums[c].y, sums[c].x, top);
         for (int d = 1; d < span; d <<= 1) S += __shfl_xor(S, d);
         if (at == 0 && real) {
             // (a row that allows nothing is one of a beam without a score)
@@ -454,7 +445,7 @@ __global__ __launch_bounds__(THREADS) void beam_pick_kernel(const SelectArgs a) 
     bool some = false;     // the lists named in s_list
     float line = 0.0f;
     if constexpr (!SMALL) {
-        // (a beam without a score has no sums, or nothing in its lists)
+        // (the lists of a beam without a score are empty)
         auto list_max = [&](int i) {
             const int b = i / a.chunks;
             return s_base[b] > -INFINITY ? static_cast<float>(score_of(b, a.sums[slot0 + i].x)) : -INFINITY;
