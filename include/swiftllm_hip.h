@@ -576,8 +576,10 @@ int swiftllm_hip_scored_prefill(
 /* A beam search's selection. Row r * beam_width + w of logits (dtype F16, BF16
  * or F32; `vocab` values, logits_stride between rows) belongs to beam w of
  * request r, whose sum of log probabilities is beam_scores[row]. The score of
- * going on with token v is beam_scores[row] + log softmax(logits[row])[v], in
- * 64 bits. Writes, for every request,
+ * going on with token v is beam_scores[row] + log softmax(logits[row])[v], summed
+ * and compared in 64 bits; of the softmax's sum the terms within 8192 logits are of
+ * 32 bits, which moves all scores of a row alike, by less than 2^-17. Beams' scores
+ * closer than that may come in either order. Writes, for every request,
  *   cand_scores, cand_rows, cand_tokens [R, num_candidates]: the largest scores
  *     in descending order (rounded to 32 bits), their rows and tokens; ties go to
  *     the lower beam, then the larger logit, then the lower token

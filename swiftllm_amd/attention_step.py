@@ -265,7 +265,10 @@ def shared_decode(output: Ptr, workspace: Ptr, workspace_bytes: int, plan: Ptr, 
     """scored_decode where the blocks that a group shares are read once for all of
     its sequences (swiftllm_hip_shared_decode); contexts and groups are the
     plan's. Without a window (under one, little of a long prefix is seen:
-    scored_decode); score.prefix_lens has no effect then."""
+    scored_decode); score.prefix_lens has no effect then. Where a group's blocks are
+    read for more than 16 query rows (sequences x heads of a kv head) their softmax
+    weights are rounded to dtype, as in scored_prefill; all others keep two 16-bit
+    parts, as in scored_decode."""
     if score.window:
         raise NotSupported(f"window {score.window} over shared blocks")
     check_status(_lib.lib().swiftllm_hip_shared_decode(
@@ -294,7 +297,10 @@ class AttentionStep:
 
     num_groups > 0: plan() also takes group_offsets, the groups of sequences whose
     tables begin alike (beams, chats on one prompt), and a decode step reads what
-    each group shares once (plan_shared, shared_decode)."""
+    each group shares once (plan_shared, shared_decode), its weights there rounded to
+    dtype. A plan() without group_offsets decodes as a step without groups does, with
+    weights in two parts (error against 64 bits 1.66e-3 and not 1.85e-3 in bfloat16,
+    2.08e-4 and not 2.30e-4 in fp16)."""
 
     def __init__(self, num_seqs: int, num_tokens: int, max_num_blocks_per_seq: int,
                  num_heads: int, num_kv_heads: int, head_dim: int, score: ScoreParams,

@@ -87,9 +87,9 @@ class BeamSearch:
 
     The calls are asynchronous on `stream`, in that order; all but start() and
     compact() may be captured. fork() changes between two sets of tables, and what it
-    counts is of the plan() before: a graph holds an even number of steps, and is
-    replayed where it was captured, the same number of steps after a start() or an even
-    number more, not before the first of them."""
+    counts is of the plan() before: a graph holds an even number of steps, is captured
+    after the first step behind start(), and is replayed as many steps behind a start()
+    as it was captured, or an even number more."""
 
     def __init__(self, num_requests: int, beam_width: int, vocab: int,
                  max_num_blocks_per_seq: int, num_blocks: int,

@@ -5,7 +5,8 @@
 //   score(w, v) = c_w + x_w[v] - lse_w,   lse_w = log sum_v exp x_w[v]
 // Candidates are the C largest scores, compared in 64 bits; ties go to the lower
 // beam, then the larger logit, then the lower token. Within a beam that is the
-// order of (logit, token), so its C first by those hold all of its candidates.
+// order of (logit, token), so its C first by those hold all of its candidates: lse,
+// which moves them alike, decides between beams only.
 //
 // First kernel, a workgroup per kChunk logits of a row: their sum of exponentials
 // and a list that holds their C largest. The threads' own maxima are 256 of them,
@@ -20,13 +21,15 @@
 // maximum: one multiply-add with r, the rounded m L, and the sum times 2^(r - m L),
 // that difference exact. So the roundings are those of the exponents, of exp2 and
 // of the sums: 32 bits up to a chunk's, 64 bits over chunks. L's own error moves
-// lse by 2e-8 of the distance from the maximum.
+// lse by 2e-8 of the distance from the maximum. With d the distance from the maximum in
+// log2 units, whose mean under the softmax is at most log2 V + 2, all of it is less than
+// 2^-24 (2 d + 2 of exp2 + 44 of sums and products) < 2^-17.
 //
-// Bound: HBM for 32-bit logits, for 16-bit ones as much the vector operations, nine
-// per logit of which the exponential is four. 64 x 4 rows of 128000 bfloat16 logits:
-// 16.4 us, 4.0 TB/s; 9 x 32 of 100003 in 32 bits 28 us, 4.1 TB/s; 4 of 32000 5.2 us,
-// as long as a chunk's way through. The second kernel is latency, of one workgroup a
-// request: 4.8 us for 16 lists of 8 candidates, 6.5 for 64, 14 for 416 lists of 64 or
+// Bound: HBM for 32-bit logits, for 16-bit ones as much the vector operations, 13.6
+// per logit as counted, of which the exponential is four. 64 x 4 rows of 128000 bfloat16
+// logits: 16.4 us, 4.0 TB/s; 9 x 32 of 100003 in 32 bits 28 us, 4.1 TB/s; 4 of 32000
+// 5.1 us, as long as a chunk's way through. The second kernel is latency, of one workgroup
+// a request: 5.1 us for 16 lists of 8 candidates, 6.7 for 64, 14 for 416 lists of 64 or
 // more (20 with every pass over the entries in memory, their scores found again).
 
 #include <algorithm>

@@ -21,13 +21,13 @@
 // afterwards, id - L of them before id; below T the free ones but for the M lowest.
 //
 // Bound: latency. A step of 16 requests of 8 beams in 65536 blocks moves 0.9 MB
-// (0.2 us), 1024 beams in 524288 blocks 12 MB (2.4 us). Three launches each, whose
-// ends are the only order between workgroups: fork_pages moves references, counts the
-// free blocks of every 4096 ids (and keeps them as bits), lists them: 3.6 + 4.6 + 3.7
-// us and 5.9 + 5.7 + 5.2 us at those sizes, each a chain of dependent reads.
-// compact_pages counts the blocks in use, pairs them, renames: 3.2 + 4.1 + 4.2 us for
-// 64 rows over 65536 blocks, 3.7 + 4.7 + 8.8 for 512 rows of 1000 blocks over 524288
-// (18 MB, 3.6 us). A block's place among those in use is a word of bits and the count
+// (0.2 us), 1024 beams in 524288 blocks 12 MB (2.4 us). Three launches each (a fork in
+// a small pool one, a compaction of few ids two), whose ends are the only order between
+// workgroups: fork_pages moves references, counts the free blocks of every 4096 ids (and
+// keeps them as bits) beside the copies, lists them: 3.5 + 3.6 + 3.9 us and 6.0 + 4.3 +
+// 6.3 us at those sizes, each a chain of dependent reads. compact_pages counts the blocks
+// in use, pairs them, renames: 3.2 + 3.8 + 3.9 us for 64 rows over 65536 blocks, 3.9 +
+// 4.7 + 8.8 for 512 rows of 1000 blocks over 524288 (18 MB, 3.6 us). A block's place among those in use is a word of bits and the count
 // before it; kept for every block in an array of its own, the last took 10.9. Where a
 // row and its parent have the same block in the same place, as in a prompt that both
 // share, nothing is counted: a search's reordering touches few counters.

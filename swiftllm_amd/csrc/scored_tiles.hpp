@@ -1,6 +1,7 @@
-// Tiles of K and V in LDS for 32x32x16 products (scored_prefill.hip,
-// shared_decode.hip): a stage of 64 keys, four blocks, which the four waves of a
-// workgroup load by one each and all read.
+// Tiles of K and V in LDS for 32x32x16 products, which the four waves of a workgroup
+// load and all read: in scored_prefill.hip a stage of 64 keys, four blocks, by a wave
+// each; in shared_decode.hip a step of two blocks, of which two waves load the K and
+// two the V.
 #pragma once
 
 #include <type_traits>
@@ -14,7 +15,7 @@ constexpr int kStage = 64;             // keys
 
 typedef __attribute__((address_space(3))) s4 lds_s4;
 
-// LDS of one stage, in halves: four K tiles [d][16], then four V tiles in
+// LDS of a stage of four blocks, in halves: four K tiles [d][16], then four V tiles in
 // operand order. The second K tile of a pair sits 128 bytes off, so that the
 // rows an operand read takes from both fall in different banks.
 template <int D>

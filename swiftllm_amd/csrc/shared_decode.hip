@@ -493,6 +493,12 @@ void shared_decode_kernel(const SharedArgs a) {
                 const unsigned keys = ((here & 1u) ? (bad[0] >> (8 * h)) & 0xffu : 0u) | ((here & 2u) ? (bad[1] >> (8 * h)) & 0xffu : 0u);
                 if (keys) l = __builtin_nanf("");
             }
+            // A weight is rounded to the type, as in scored_prefill, and its sum is of the
+            // rounded ones. The second part that a wave's walk keeps of it would be as many
+            // products again: us a pass with one and with two, 16 x 8 beams with a cap 216 and
+            // 217, 128 chats 287 and 305, 4 x 16 questions with biases 284 and 330, for errors
+            // against 64 bits of 1.85e-3 and 1.66e-3 (bfloat16), 2.30e-4 and 2.08e-4 (fp16), of
+            // which the output's own rounding is all but the difference.
             u4 pw[2];
 #pragma unroll
             for (int k = 0; k < 8; ++k) {
@@ -567,8 +573,8 @@ void shared_decode_kernel(const SharedArgs a) {
 constexpr int kJoinRows = 8;
 constexpr int kJoinWaves = 4;       // of a workgroup
 // Rows below which four waves join one. (us a layer of 32/8 heads x 128, with one wave
-// and with four: 4 beams on 1000 tokens 12.9 and 11.6, 4 x 4 on 8192 41.5 and 37.2,
-// 32 on 32768 49.7 and 47.3; 16 x 4 on 600 25.3 and 27.1, 16 x 8 on 2500 53.5 and 59.0.)
+// and with four: 4 beams on 1000 tokens 13.0 and 11.7, 4 x 4 on 8192 41.6 and 37.8,
+// 32 on 32768 47.4 and 45.6; 16 x 4 on 600 25.2 and 26.7, 16 x 8 on 2500 50.3 and 55.8.)
 constexpr int kFewRows = 2048;
 
 // Tables and bytes of K and V up to which every sequence is taken whole. (us a layer of

@@ -36,7 +36,7 @@ constexpr int kLeastRange = 16;
 // Blocks of a group that reading shared ones once has to save, and values of a head of
 // all of them (blocks x chunks of heads x head_dim): below, the second launch and its
 // joins cost what is saved. (4 beams on 1000 tokens, 8 kv heads x 128: 12.0 us a layer
-// shared, 11.6 not; 16 x 8 beams on 2500 tokens 53.5 shared, 153 by scored_decode.)
+// shared, 11.6 not; 16 x 8 beams on 2500 tokens 50.5 shared, 153 by scored_decode.)
 constexpr int kLeastSaved = 16;
 constexpr long long kLeastSavedAll = 2500 * 128;
 
