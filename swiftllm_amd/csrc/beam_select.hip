@@ -28,8 +28,8 @@
 // Bound: HBM for 32-bit logits, for 16-bit ones as much the vector operations, 13.6
 // per logit as counted, of which the exponential is four. 64 x 4 rows of 128000 bfloat16
 // logits: 16.4 us, 4.0 TB/s; 9 x 32 of 100003 in 32 bits 28 us, 4.1 TB/s; 4 of 32000
-// 5.1 us, as long as a chunk's way through. The second kernel is latency, of one workgroup
-// a request: 5.1 us for 16 lists of 8 candidates, 6.7 for 64, 14 for 416 lists of 64 or
+// 5.2 us, as long as a chunk's way through. The second kernel is latency, of one workgroup
+// a request: 5.0 us for 16 lists of 8 candidates, 6.8 for 64, 14 for 416 lists of 64 or
 // more (20 with every pass over the entries in memory, their scores found again).
 
 #include <algorithm>
