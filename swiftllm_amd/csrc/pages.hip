@@ -27,10 +27,11 @@
 // keeps them as bits) beside the copies, lists them: 3.5 + 3.6 + 3.9 us and 6.0 + 4.3 +
 // 6.3 us at those sizes, each a chain of dependent reads. compact_pages counts the blocks
 // in use, pairs them, renames: 3.2 + 3.8 + 3.9 us for 64 rows over 65536 blocks, 3.9 +
-// 4.7 + 8.8 for 512 rows of 1000 blocks over 524288 (18 MB, 3.6 us). A block's place among those in use is a word of bits and the count
-// before it; kept for every block in an array of its own, the last took 10.9. Where a
-// row and its parent have the same block in the same place, as in a prompt that both
-// share, nothing is counted: a search's reordering touches few counters.
+// 4.7 + 8.8 for 512 rows of 1000 blocks over 524288 (18 MB, 3.6 us). A block's place
+// among those in use is a word of bits and the count before it; kept for every block in
+// an array of its own, the last took 10.9. Where a row and its parent have the same
+// block in the same place, as in a prompt that both share, nothing is counted: a
+// search's reordering touches few counters.
 
 #include <algorithm>
 
